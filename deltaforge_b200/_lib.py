@@ -68,6 +68,35 @@ class AttnStepDesc(C.Structure):
     ]  # fmt: skip
 
 
+class RotaryDesc(C.Structure):
+    _fields_ = [
+        ("batch", c_i32), ("tokens", c_i32), ("hq", c_i32), ("hkv", c_i32), ("d", c_i32), ("rotary_dim", c_i32),
+        ("interleaved", c_i32), ("dtype", c_i32), ("q", c_vp), ("k", c_vp), ("v", c_vp),
+        ("q_stride", c_i64 * 3), ("k_stride", c_i64 * 3), ("v_stride", c_i64 * 3),
+        ("pos", c_vp), ("pos_stride", c_i64), ("pos_is_i64", c_i32), ("inv_freq", c_vp), ("freq_is_f64", c_i32), ("factor", c_f32),
+        ("q_out", c_vp), ("k_out", c_vp), ("kcache", c_vp), ("vcache", c_vp), ("kc_stride", c_i64 * 3), ("vc_stride", c_i64 * 3),
+        ("cache_len", c_vp), ("max_seq", c_i32),
+    ]  # fmt: skip
+
+
+class TreeAttnDesc(C.Structure):
+    _fields_ = [
+        ("batch", c_i32), ("nodes", c_i32), ("hq", c_i32), ("hkv", c_i32), ("d", c_i32), ("max_seq", c_i32), ("is_fp16", c_i32),
+        ("q", c_vp), ("kcache", c_vp), ("vcache", c_vp), ("q_stride", c_i64 * 3), ("k_stride", c_i64 * 3), ("v_stride", c_i64 * 3),
+        ("cache_len", c_vp), ("parents", c_vp), ("parents_stride", c_i64), ("scale", c_f32),
+        ("out", c_vp), ("scratch", c_vp), ("scratch_bytes", c_sz),
+    ]  # fmt: skip
+
+
+class DeltaChunkDesc(C.Structure):
+    _fields_ = [
+        ("batch", c_i32), ("tokens", c_i32), ("hk", c_i32), ("hv", c_i32), ("dk", c_i32), ("dv", c_i32),
+        ("q", c_vp), ("k", c_vp), ("v", c_vp), ("q_stride", c_i64 * 3), ("k_stride", c_i64 * 3), ("v_stride", c_i64 * 3),
+        ("g", c_vp), ("beta", c_vp), ("lengths", c_vp), ("parents", c_vp), ("parents_stride", c_i64), ("l2norm", c_i32),
+        ("state", c_vp), ("state_out", c_vp), ("out", c_vp), ("scratch", c_vp), ("scratch_bytes", c_sz),
+    ]  # fmt: skip
+
+
 class Linear(C.Structure):
     _fields_ = [
         ("packed", c_vp), ("scale", c_vp), ("scale_is_bf16", c_i32), ("K", c_i32), ("N", c_i32), ("group", c_i32),
@@ -124,6 +153,11 @@ SIGNATURES = {
     "dfb_attn_decode": (C.c_int, [C.POINTER(AttnDesc), c_vp]),
     "dfb_attn_prep": (C.c_int, [C.POINTER(AttnPrepDesc), c_vp]),
     "dfb_attn_step": (C.c_int, [C.POINTER(AttnStepDesc), c_vp]),
+    "dfb_rotary": (C.c_int, [C.POINTER(RotaryDesc), c_vp]),
+    "dfb_tree_attn_scratch_bytes": (c_sz, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "dfb_tree_attention": (C.c_int, [C.POINTER(TreeAttnDesc), c_vp]),
+    "dfb_delta_chunk_scratch_bytes": (c_sz, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "dfb_delta_chunk": (C.c_int, [C.POINTER(DeltaChunkDesc), c_vp]),
     "dfb_engine_workspace_bytes": (c_sz, [C.POINTER(ModelDesc)]),
     "dfb_engine_num_segments": (C.c_int, [c_vp]),
     "dfb_engine_step_segment": (C.c_int, [c_vp, C.c_int, c_vp]),

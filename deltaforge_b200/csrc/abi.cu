@@ -351,4 +351,162 @@ int dfb_attn_prep(const dfb_attn_prep_desc* d, void* stream) {
   return launch_attn_prep(p, (cudaStream_t)stream);
 }
 
+// ---- several new tokens of a sequence at once ----
+
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+static void copy3(long (&to)[3], const int64_t (&from)[3]) {
+  for (int i = 0; i < 3; ++i) to[i] = (long)from[i];
+}
+static bool multiples(const int64_t (&s)[3], int of) { return s[0] % of == 0 && s[1] % of == 0 && s[2] % of == 0; }
+
+int dfb_rotary(const dfb_rotary_desc* d, void* stream) {
+  if (!d) return bad("dfb_rotary: null descriptor");
+  const bool append = d->kcache != nullptr;
+  if (d->batch < 0 || d->tokens < 0 || d->hq < 1 || d->hkv < 1 || d->d < 1)
+    return bad("dfb_rotary: bad shape batch=%d tokens=%d heads=%d/%d dim=%d", d->batch, d->tokens, d->hq, d->hkv, d->d);
+  if (d->rotary_dim < 2 || d->rotary_dim % 2 || d->rotary_dim > d->d || d->rotary_dim > MAX_ROTARY_DIM)
+    return bad("dfb_rotary: rotary_dim %d must be even, at most the head dim %d and at most %d", d->rotary_dim, d->d, MAX_ROTARY_DIM);
+  if (d->dtype != DFB_BF16 && d->dtype != DFB_FP16 && d->dtype != DFB_FP32) return bad("dfb_rotary: unknown type %d", d->dtype);
+  if ((int64_t)d->batch * d->tokens > 0x7fffffff) return bad("dfb_rotary: %d x %d tokens are too many for one call", d->batch, d->tokens);
+  if (d->batch == 0 || d->tokens == 0) return DFB_OK;
+  if (!d->q || !d->k || !d->pos || !d->inv_freq || !d->q_out) return bad("dfb_rotary: null tensor pointer");
+  if (append && (!d->v || !d->vcache || !d->cache_len)) return bad("dfb_rotary: the appending form needs v, vcache and cache_len");
+  if (!append && !d->k_out) return bad("dfb_rotary: null k_out");
+  RotaryParams p = {};
+  p.batch = d->batch;
+  p.tokens = d->tokens;
+  p.hq = d->hq;
+  p.hkv = d->hkv;
+  p.d = d->d;
+  p.rotary_dim = d->rotary_dim;
+  p.interleaved = d->interleaved != 0;
+  p.dtype = d->dtype;
+  p.q = d->q;
+  p.k = d->k;
+  copy3(p.q_stride, d->q_stride);
+  copy3(p.k_stride, d->k_stride);
+  p.pos = d->pos;
+  p.pos_stride = d->pos_stride;
+  p.pos_is_i64 = d->pos_is_i64;
+  p.inv_freq = d->inv_freq;
+  p.freq_is_f64 = d->freq_is_f64;
+  p.factor = d->factor;
+  p.q_out = d->q_out;
+  if (append) {
+    p.v = d->v;
+    copy3(p.v_stride, d->v_stride);
+    p.kcache = d->kcache;
+    p.vcache = d->vcache;
+    copy3(p.kc_stride, d->kc_stride);
+    copy3(p.vc_stride, d->vc_stride);
+    p.cache_len = d->cache_len;
+    p.max_seq = d->max_seq;
+  } else {
+    p.k_out = d->k_out;
+  }
+  return launch_rotary(p, (cudaStream_t)stream);
+}
+
+size_t dfb_tree_attn_scratch_bytes(int batch, int nodes, int hq, int hkv, int d, int max_seq) {
+  if (batch < 1 || nodes < 1 || hkv < 1 || hq < hkv || max_seq < 1) return 0;
+  const TreePlan plan = tree_plan(batch, nodes, hq, hkv, max_seq);
+  if (plan.splits <= 1) return 0;
+  const size_t rows = (size_t)batch * hq * nodes * plan.splits;
+  return align_up(rows * d * 4, 256) + align_up(rows * 2 * 4, 256);
+}
+
+int dfb_tree_attention(const dfb_tree_attn_desc* d, void* stream) {
+  if (!d) return bad("dfb_tree_attention: null descriptor");
+  if (d->batch < 0 || d->hkv < 1 || d->hq < 1 || d->hq % d->hkv) return bad("%d query heads do not divide into %d KV heads", d->hq, d->hkv);
+  if (d->nodes < 0 || d->nodes > MAX_TREE_NODES) return bad("dfb_tree_attention: a tree has at most %d nodes, got %d", MAX_TREE_NODES, d->nodes);
+  if (d->d != 32 && d->d != 64 && d->d != 128 && d->d != 256) return bad("dfb_tree_attention: head dim %d is not 32, 64, 128 or 256", d->d);
+  if (d->max_seq < 1) return bad("dfb_tree_attention: the cache has no rows");
+  if (d->batch > 65535 || (int64_t)d->hq * d->nodes > 65535) return bad("dfb_tree_attention: batch %d or %d heads are too many", d->batch, d->hq);
+  if (d->batch == 0 || d->nodes == 0) return DFB_OK;
+  if (!d->q || !d->kcache || !d->vcache || !d->cache_len || !d->parents || !d->out) return bad("dfb_tree_attention: null tensor pointer");
+  if (!aligned16(d->kcache) || !aligned16(d->vcache) || !multiples(d->k_stride, 8) || !multiples(d->v_stride, 8))
+    return bad("dfb_tree_attention: cache rows must start on 16-byte boundaries");
+  if (((uintptr_t)d->q & 3) || !multiples(d->q_stride, 2)) return bad("dfb_tree_attention: query rows must start on 4-byte boundaries");
+  const size_t need = dfb_tree_attn_scratch_bytes(d->batch, d->nodes, d->hq, d->hkv, d->d, d->max_seq);
+  if (need && (!d->scratch || d->scratch_bytes < need || !aligned16(d->scratch))) return bad("dfb_tree_attention: aligned scratch of %zu bytes required", need);
+  const TreePlan plan = tree_plan(d->batch, d->nodes, d->hq, d->hkv, d->max_seq);
+  TreeAttnParams p = {};
+  p.batch = d->batch;
+  p.nodes = d->nodes;
+  p.hq = d->hq;
+  p.hkv = d->hkv;
+  p.d = d->d;
+  p.group = d->hq / d->hkv;
+  p.rows = d->nodes * p.group;
+  p.max_seq = d->max_seq;
+  p.is_fp16 = d->is_fp16;
+  p.q = d->q;
+  p.kcache = d->kcache;
+  p.vcache = d->vcache;
+  copy3(p.q_stride, d->q_stride);
+  copy3(p.k_stride, d->k_stride);
+  copy3(p.v_stride, d->v_stride);
+  p.cache_len = d->cache_len;
+  p.parents = d->parents;
+  p.parents_stride = d->parents_stride;
+  p.scale = d->scale;
+  p.out = d->out;
+  p.splits = plan.splits;
+  p.mt = plan.mt;
+  if (need) {
+    p.part_acc = (float*)d->scratch;
+    p.part_ml = (float*)((char*)d->scratch + align_up((size_t)d->batch * d->hq * d->nodes * plan.splits * d->d * 4, 256));
+  }
+  return launch_tree_attention(p, (cudaStream_t)stream);
+}
+
+size_t dfb_delta_chunk_scratch_bytes(int batch, int tokens, int hk, int hv, int dk) {
+  if (batch < 1 || tokens < 1 || hk < 1 || hv < hk || dk < 1) return 0;
+  return delta_chunk_scratch_bytes(batch, tokens, hk, hv, dk);
+}
+
+int dfb_delta_chunk(const dfb_delta_chunk_desc* d, void* stream) {
+  if (!d) return bad("dfb_delta_chunk: null descriptor");
+  if (d->hk < 1 || d->hv < 1 || d->hv % d->hk) return bad("%d value heads do not divide into %d key heads", d->hv, d->hk);
+  if (d->dk < 8 || d->dk > 128 || d->dk % 8 || d->dv < 8 || d->dv % 8)
+    return bad("dfb_delta_chunk: key dim %d (multiple of 8, at most 128) or value dim %d (multiple of 8) unsupported", d->dk, d->dv);
+  const bool tree = d->parents != nullptr;
+  if (tree && d->tokens > MAX_TREE_NODES) return bad("dfb_delta_chunk: a tree has at most %d nodes, got %d", MAX_TREE_NODES, d->tokens);
+  if (tree && d->lengths) return bad("dfb_delta_chunk: a tree takes no lengths (rows without a node say so in parents)");
+  if (d->batch < 0 || d->tokens < 0 || d->batch > 65535 || d->hv > 65535) return bad("dfb_delta_chunk: bad shape batch=%d tokens=%d", d->batch, d->tokens);
+  if (d->batch == 0 || (tree && d->tokens == 0)) return DFB_OK;
+  if (!d->state || (!tree && !d->state_out)) return bad("dfb_delta_chunk: null state pointer");
+  if (d->tokens == 0) return bad("dfb_delta_chunk: no tokens");
+  if (!d->q || !d->k || !d->v || !d->g || !d->beta || !d->out) return bad("dfb_delta_chunk: null tensor pointer");
+  if (!aligned16(d->q) || !aligned16(d->k) || !aligned16(d->v) || !aligned16(d->out) || !multiples(d->q_stride, 8) || !multiples(d->k_stride, 8) ||
+      !multiples(d->v_stride, 8))
+    return bad("dfb_delta_chunk: rows of q, k and v must start on 16-byte boundaries");
+  const size_t need = dfb_delta_chunk_scratch_bytes(d->batch, d->tokens, d->hk, d->hv, d->dk);
+  if (!d->scratch || d->scratch_bytes < need || !aligned16(d->scratch)) return bad("dfb_delta_chunk: aligned scratch of %zu bytes required", need);
+  DeltaChunkParams p = {};
+  p.batch = d->batch;
+  p.tokens = d->tokens;
+  p.hk = d->hk;
+  p.hv = d->hv;
+  p.dk = d->dk;
+  p.dv = d->dv;
+  p.q = (const bf16*)d->q;
+  p.k = (const bf16*)d->k;
+  p.v = (const bf16*)d->v;
+  copy3(p.q_stride, d->q_stride);
+  copy3(p.k_stride, d->k_stride);
+  copy3(p.v_stride, d->v_stride);
+  p.g = d->g;
+  p.beta = d->beta;
+  p.lengths = d->lengths;
+  p.parents = d->parents;
+  p.parents_stride = d->parents_stride;
+  p.l2norm = d->l2norm;
+  p.state = d->state;
+  p.state_out = d->state_out;
+  p.out = (bf16*)d->out;
+  p.scratch = (unsigned char*)d->scratch;
+  return launch_delta_chunk(p, (cudaStream_t)stream);
+}
+
 }  // extern "C"

@@ -297,5 +297,80 @@ int launch_tp_pick(const bf16* logits, int vocab_local, int batch, int tp_rank, 
                    int64_t* tokens, int64_t* hist, const int* pos, int* status, cudaStream_t s);
 int launch_bump(unsigned* counter, cudaStream_t s);
 
+// ---- several new tokens of a sequence at once ----
+
+enum Dtype { DTYPE_BF16 = 0, DTYPE_FP16 = 1, DTYPE_FP32 = 2 };
+
+constexpr int MAX_ROTARY_DIM = 512;
+struct RotaryParams {
+  int batch, tokens, hq, hkv, d, rotary_dim, interleaved, dtype;
+  const void* q;  // [batch, tokens, hq, d]; strides (batch, token, head) in elements, the last dim contiguous
+  const void* k;  // [batch, tokens, hkv, d]
+  const void* v;  // appending form only
+  long q_stride[3], k_stride[3], v_stride[3];
+  const void* pos;  // int32 or int64 [batch, tokens]
+  long pos_stride;
+  int pos_is_i64;
+  const void* inv_freq;  // fp64 or fp32 [rotary_dim / 2]
+  int freq_is_f64;
+  float factor;  // on cos and sin
+  void* q_out;   // [batch, tokens, hq, d] contiguous
+  void* k_out;   // [batch, tokens, hkv, d] contiguous; null in the appending form
+  void* kcache;  // appending form: [batch, hkv, max_seq, d], strides (batch, head, row)
+  void* vcache;
+  long kc_stride[3], vc_stride[3];
+  const int* cache_len;  // [batch]: token t of sequence b goes to row cache_len[b] + t
+  int max_seq;
+  int lanes_per_head;  // set by the launcher
+};
+int launch_rotary(const RotaryParams& p, cudaStream_t stream);
+
+constexpr int MAX_TREE_NODES = 64;
+struct TreeAttnParams {
+  int batch, nodes, hq, hkv, d, group, rows;  // group = hq / hkv, rows = nodes * group
+  int max_seq, is_fp16;
+  const void* q;  // [batch, nodes, hq, d], strides (batch, node, head)
+  const void* kcache;  // [batch, hkv, max_seq, d], strides (batch, head, row)
+  const void* vcache;
+  long q_stride[3], k_stride[3], v_stride[3];
+  const int* cache_len;  // [batch]
+  const int* parents;    // [batch, nodes]
+  long parents_stride;   // 0: one tree for all
+  float scale;
+  void* out;  // [batch, nodes, hq, d] contiguous
+  int splits, mt;
+  float* part_acc;  // [batch, hkv, splits, rows, d]
+  float* part_ml;   // [batch, hkv, splits, rows, 2]
+};
+struct TreePlan {
+  int mt;      // 16-row tiles per CTA
+  int splits;  // key ranges
+};
+TreePlan tree_plan(int batch, int nodes, int hq, int hkv, int max_seq);
+int launch_tree_attention(const TreeAttnParams& p, cudaStream_t stream);
+
+struct DeltaChunkParams {
+  int batch, tokens, hk, hv, dk, dv;
+  const bf16* q;  // [batch, tokens, hk, dk], strides (batch, token, head), the last dim contiguous
+  const bf16* k;
+  const bf16* v;  // [batch, tokens, hv, dv]
+  long q_stride[3], k_stride[3], v_stride[3];
+  const float* g;  // [batch, tokens, hv] contiguous: log decay
+  const float* beta;
+  const int* lengths;  // optional [batch]
+  const int* parents;  // tree form: [batch, tokens]
+  long parents_stride;
+  int l2norm;
+  const float* state;  // [batch, hv, dk, dv]
+  float* state_out;    // the same; null in the tree form
+  bf16* out;           // [batch, tokens, hv, dv] contiguous
+  unsigned char* scratch;
+  // set by the launcher
+  int chunk0, chunks, seg_chunks;  // this segment: chunks chunk0 .. chunk0 + chunks - 1; scratch holds seg_chunks
+  int first, last;                 // first / last segment of the prompt
+};
+size_t delta_chunk_scratch_bytes(int batch, int tokens, int hk, int hv, int dk);
+int launch_delta_chunk(const DeltaChunkParams& p, cudaStream_t stream);
+
 }  // namespace dfb
 

@@ -30,6 +30,7 @@ are coerced with ``.contiguous()``, shapes are not.
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import torch
 from torch import Tensor
@@ -792,3 +793,311 @@ def attn_step(
 @attn_step.register_fake
 def _(proj, q_norm_weight, k_norm_weight, eps, inv_freq, pos, key_cache, value_cache, num_heads, output_gate, swish, splits, cluster_size):
     return proj.new_empty((proj.shape[0], num_heads * key_cache.shape[3]))
+
+
+# --------------------------------------------------------------------------------------
+# Several new tokens of a sequence at once: prompts, and trees of drafted tokens
+# --------------------------------------------------------------------------------------
+#
+# Layout of all four: activations are (batch, tokens, heads, dim), which is what a projection's rows are; any strides with
+# the last dim contiguous are read in place (so a fused projection's row can be passed as views of it, and a
+# (batch, heads, seq, dim) tensor as its transpose). Outputs are new and contiguous.
+
+MAX_TREE_NODES = 64
+_DTYPES = {BF16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _three(t: Tensor):
+    return (C.c_int64 * 3)(t.stride(0), t.stride(1), t.stride(2))
+
+
+def _launch(fn, desc, t: Tensor, op: str) -> None:
+    """Call a C entry point on the current stream of the tensors' device, whichever device is current."""
+    if t.device.index == torch.cuda.current_device():
+        _lib.check(fn(C.byref(desc), _stream(t)), f"dfb200::{op}")
+    else:
+        with torch.cuda.device(t.device):
+            _lib.check(fn(C.byref(desc), _stream(t)), f"dfb200::{op}")
+
+
+def _same_device(op: str, first: Tensor, *rest: Tensor | None) -> None:
+    require_cuda(first, op)
+    for t in rest:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{op}: all tensors must be on {first.device}, got one on {t.device}")
+
+
+def _last_contiguous(op: str, **tensors: Tensor) -> None:
+    for name, t in tensors.items():
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{op}: {name} must have its last dimension contiguous")
+
+
+def _check_cache(op: str, batch: int, heads: int, dim: int, dtype: torch.dtype, key_cache: Tensor, value_cache: Tensor, cache_len: Tensor) -> int:
+    if key_cache.dim() != 4 or key_cache.shape != value_cache.shape:
+        raise ValueError(f"{op}: caches must both be (batch, kv_heads, max_seq, head_dim), got {tuple(key_cache.shape)} and {tuple(value_cache.shape)}")
+    if key_cache.shape[0] != batch or key_cache.shape[1] != heads or key_cache.shape[3] != dim:
+        raise ValueError(f"{op}: caches {tuple(key_cache.shape)} do not match batch {batch}, {heads} KV heads, head dim {dim}")
+    if key_cache.dtype != dtype or value_cache.dtype != dtype:
+        raise ValueError(f"{op}: caches must be {dtype}, got {key_cache.dtype} and {value_cache.dtype}")
+    if tuple(cache_len.shape) != (batch,) or cache_len.dtype != torch.int32 or not cache_len.is_contiguous():
+        raise ValueError(f"{op}: cache_len must be a contiguous int32 tensor of {batch} entries, got {tuple(cache_len.shape)} {cache_len.dtype}")
+    _last_contiguous(op, key_cache=key_cache, value_cache=value_cache)
+    return key_cache.shape[2]
+
+
+def rope_frequencies(
+    rotary_dim: int, theta: float, *, stretch: float = 1.0, method: str = "by_parts", trained_len: int = 32768, slow_turns: float = 1.0,
+    fast_turns: float = 32.0, device: torch.device | str = "cuda",
+) -> tuple[Tensor, float]:  # fmt: skip
+    """Inverse frequencies (fp64, ``rotary_dim / 2``) and the factor on cos and sin for ``rotary_qk`` / ``rotary_append``.
+
+    ``stretch`` > 1 scales them for a context that many times ``trained_len``: ``"linear"`` divides every frequency by
+    it; ``"base"`` raises ``theta`` so that the slowest frequency is divided by it and the fastest stays; ``"by_parts"``
+    divides those that turn less than ``slow_turns`` times over ``trained_len``, keeps those that turn more than ``fast_turns``
+    times, goes linearly in between, and scales cos and sin by ``0.1 ln(stretch) + 1``.
+    """
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and at least 2, got {rotary_dim}")
+    if not stretch >= 1.0:
+        raise ValueError(f"stretch must be at least 1, got {stretch}")
+    if method not in ("linear", "base", "by_parts"):
+        raise ValueError(f"unknown method {method!r}: linear, base or by_parts")
+    if fast_turns <= slow_turns:
+        raise ValueError("fast_turns must be above slow_turns")
+    if method == "base" and rotary_dim > 2:
+        theta = theta * stretch ** (rotary_dim / (rotary_dim - 2))
+    f = theta ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    factor = 1.0
+    if stretch != 1.0 and method == "linear":
+        f = f / stretch
+    elif stretch != 1.0 and method == "by_parts":
+        keep = ((trained_len * f / (2 * math.pi) - slow_turns) / (fast_turns - slow_turns)).clamp(0, 1)
+        f = f * keep + f / stretch * (1 - keep)
+        factor = 0.1 * math.log(stretch) + 1.0
+    return f.to(device), factor
+
+
+def _rotary_desc(op: str, query: Tensor, key: Tensor, positions: Tensor, inv_freq: Tensor, factor: float, interleaved: bool) -> _lib.RotaryDesc:
+    if query.dim() != 4 or key.dim() != 4:
+        raise ValueError(f"{op}: expected query and key (batch, tokens, heads, head_dim), got {tuple(query.shape)} and {tuple(key.shape)}")
+    batch, tokens, hq, d = query.shape
+    if key.shape[0] != batch or key.shape[1] != tokens or key.shape[3] != d:
+        raise ValueError(f"{op}: key {tuple(key.shape)} does not match query {tuple(query.shape)}")
+    if hq < 1 or key.shape[2] < 1:
+        raise ValueError(f"{op}: query and key need at least one head")
+    if query.dtype not in _DTYPES or key.dtype != query.dtype:
+        raise ValueError(f"{op}: query and key must both be bfloat16, float16 or float32, got {query.dtype} and {key.dtype}")
+    if tuple(positions.shape) != (batch, tokens) or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{op}: positions must be int32 or int64 {(batch, tokens)}, got {tuple(positions.shape)} {positions.dtype}")
+    if inv_freq.dim() != 1 or inv_freq.dtype not in (torch.float64, torch.float32) or not inv_freq.is_contiguous():
+        raise ValueError(f"{op}: inv_freq must be a contiguous 1-D float64 or float32 tensor, got {tuple(inv_freq.shape)} {inv_freq.dtype}")
+    rd = 2 * inv_freq.numel()
+    if rd < 2 or rd > d or rd > 512:
+        raise ValueError(f"{op}: rotary_dim {rd} must be at least 2 and at most the head dim {d} and 512")
+    if tokens > 1 and positions.stride(1) != 1:
+        raise ValueError(f"{op}: positions of a sequence must be contiguous")
+    _last_contiguous(op, query=query, key=key)
+    p = _lib.RotaryDesc()
+    p.batch, p.tokens, p.hq, p.hkv, p.d, p.rotary_dim = batch, tokens, hq, key.shape[2], d, rd
+    p.interleaved, p.dtype, p.factor = interleaved, _DTYPES[query.dtype], factor
+    p.q, p.k, p.q_stride, p.k_stride = query.data_ptr(), key.data_ptr(), _three(query), _three(key)
+    p.pos, p.pos_stride, p.pos_is_i64 = positions.data_ptr(), positions.stride(0), positions.dtype == torch.int64
+    p.inv_freq, p.freq_is_f64 = inv_freq.data_ptr(), inv_freq.dtype == torch.float64
+    return p
+
+
+@torch.library.custom_op("dfb200::rotary_qk", mutates_args=())
+def rotary_qk(query: Tensor, key: Tensor, positions: Tensor, inv_freq: Tensor, factor: float, interleaved: bool) -> tuple[Tensor, Tensor]:
+    """Rotate the leading ``2 * len(inv_freq)`` dims of ``query (batch, tokens, heads, head_dim)`` and ``key`` by
+    ``positions (batch, tokens)``: pairs ``(i, i + r/2)``, or ``(2i, 2i + 1)`` when ``interleaved``. Angles are formed in 64
+    bits; cos and sin, times ``factor``, in fp32; the result is rounded once. bf16, fp16 or fp32."""
+    p = _rotary_desc("rotary_qk", query, key, positions, inv_freq, factor, interleaved)
+    _same_device("rotary_qk", query, key, positions, inv_freq)
+    q_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    k_out = torch.empty(key.shape, dtype=key.dtype, device=key.device)
+    if positions.numel():
+        p.q_out, p.k_out = q_out.data_ptr(), k_out.data_ptr()
+        _launch(_lib.load().dfb_rotary, p, query, "rotary_qk")
+    return q_out, k_out
+
+
+@rotary_qk.register_fake
+def _(query, key, positions, inv_freq, factor, interleaved):
+    return query.new_empty(query.shape), key.new_empty(key.shape)
+
+
+@torch.library.custom_op("dfb200::rotary_append", mutates_args=("key_cache", "value_cache"))
+def rotary_append(
+    query: Tensor, key: Tensor, value: Tensor, positions: Tensor, inv_freq: Tensor, factor: float, interleaved: bool,
+    key_cache: Tensor, value_cache: Tensor, cache_len: Tensor,
+) -> Tensor:  # fmt: skip
+    """``rotary_qk``, with the rotated keys and the values written into the caches ``(batch, kv_heads, max_seq, head_dim)``
+    instead of returned: token ``t`` of sequence ``b`` becomes row ``cache_len[b] + t`` (int32, on the device). Rows below 0 or
+    from ``max_seq`` on are not written. Returns the rotated query."""
+    op = "rotary_append"
+    p = _rotary_desc(op, query, key, positions, inv_freq, factor, interleaved)
+    if value.shape != key.shape or value.dtype != key.dtype:
+        raise ValueError(f"{op}: value {tuple(value.shape)} {value.dtype} must match key {tuple(key.shape)} {key.dtype}")
+    p.max_seq = _check_cache(op, key.shape[0], key.shape[2], key.shape[3], key.dtype, key_cache, value_cache, cache_len)
+    _last_contiguous(op, value=value)
+    for t in (key_cache, value_cache):
+        if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+            raise ValueError(f"{op}: the caches are written in place and must not be expanded views")
+    _same_device(op, query, key, value, positions, inv_freq, key_cache, value_cache, cache_len)
+    q_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    if positions.numel():
+        p.v, p.v_stride, p.q_out = value.data_ptr(), _three(value), q_out.data_ptr()
+        p.kcache, p.vcache, p.kc_stride, p.vc_stride = key_cache.data_ptr(), value_cache.data_ptr(), _three(key_cache), _three(value_cache)
+        p.cache_len = cache_len.data_ptr()
+        if p.max_seq:
+            _launch(_lib.load().dfb_rotary, p, query, op)
+    return q_out
+
+
+@rotary_append.register_fake
+def _(query, key, value, positions, inv_freq, factor, interleaved, key_cache, value_cache, cache_len):
+    return query.new_empty(query.shape)
+
+
+def _check_parents(op: str, parents: Tensor, batch: int, nodes: int) -> None:
+    if nodes > MAX_TREE_NODES:
+        raise ValueError(f"{op}: a tree has at most {MAX_TREE_NODES} nodes, got {nodes}")
+    if tuple(parents.shape) not in ((batch, nodes), (nodes,)) or parents.dtype != torch.int32:
+        raise ValueError(f"{op}: parents must be int32 {(batch, nodes)} or {(nodes,)}, got {tuple(parents.shape)} {parents.dtype}")
+    if nodes > 1 and parents.stride(-1) != 1:
+        raise ValueError(f"{op}: parents of a sequence must be contiguous")
+
+
+@torch.library.custom_op("dfb200::tree_attention", mutates_args=())
+def tree_attention(query: Tensor, key_cache: Tensor, value_cache: Tensor, cache_len: Tensor, parents: Tensor, scale: float) -> Tensor:
+    """Attention of a tree of up to 64 drafted tokens over an unexpanded KV cache ``(batch, kv_heads, max_seq, head_dim)``.
+
+    ``query`` is ``(batch, nodes, heads, head_dim)``; node ``i`` of sequence ``b`` holds cache row ``cache_len[b] + i`` and sees
+    the rows before ``cache_len[b]``, its ancestors' and its own. ``parents (batch, nodes)``, or ``(nodes,)`` for one tree for
+    all: the index of a node's parent, which comes before it; -1 where the parent is the last cached token. Any other
+    value marks a row without a node (a padded batch): its output is zero and no node sees it. One node is the decode
+    attention, a chain (``parents = [-1, 0, 1, ...]``) causal attention. bf16 or fp16, head dim 32, 64, 128 or 256."""
+    op = "tree_attention"
+    if query.dim() != 4:
+        raise ValueError(f"{op}: expected query (batch, nodes, heads, head_dim), got {tuple(query.shape)}")
+    batch, nodes, hq, d = query.shape
+    if query.dtype not in (BF16, torch.float16):
+        raise ValueError(f"{op}: query must be bfloat16 or float16, got {query.dtype}")
+    hkv = key_cache.shape[1] if key_cache.dim() == 4 else 0
+    if hkv and hq % hkv:
+        raise ValueError(f"{op}: {hq} query heads do not divide into {hkv} KV heads")
+    if d not in (32, 64, 128, 256):
+        raise ValueError(f"{op}: head dim {d} is not 32, 64, 128 or 256")
+    max_seq = _check_cache(op, batch, hkv, d, query.dtype, key_cache, value_cache, cache_len)
+    if hkv < 1 or hq < 1 or max_seq < 1:
+        raise ValueError(f"{op}: need at least one head and one cache row, got {hq} / {hkv} heads, {max_seq} rows")
+    _check_parents(op, parents, batch, nodes)
+    _last_contiguous(op, query=query)
+    if any(s % 8 for t in (key_cache, value_cache) for s in t.stride()[:3]) or (key_cache.data_ptr() | value_cache.data_ptr()) % 16:
+        raise ValueError(f"{op}: cache rows must start on 16-byte boundaries")
+    if any(s % 2 for s in query.stride()[:3]) or query.data_ptr() % 4:
+        query = query.contiguous()
+    _same_device(op, query, key_cache, value_cache, cache_len, parents)
+    out = torch.empty((batch, nodes, hq, d), dtype=query.dtype, device=query.device)
+    if batch == 0 or nodes == 0:
+        return out
+    lib = _lib.load()
+    nbytes = lib.dfb_tree_attn_scratch_bytes(batch, nodes, hq, hkv, d, max_seq)
+    # from the allocator, not kept: calls on two streams, or two captured graphs, never share it
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
+    a = _lib.TreeAttnDesc()
+    a.batch, a.nodes, a.hq, a.hkv, a.d, a.max_seq, a.is_fp16 = batch, nodes, hq, hkv, d, max_seq, query.dtype == torch.float16
+    a.q, a.kcache, a.vcache = query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr()
+    a.q_stride, a.k_stride, a.v_stride = _three(query), _three(key_cache), _three(value_cache)
+    a.cache_len, a.parents, a.parents_stride = cache_len.data_ptr(), parents.data_ptr(), parents.stride(0) if parents.dim() == 2 else 0
+    a.scale, a.out, a.scratch, a.scratch_bytes = scale, out.data_ptr(), _ptr(scratch), nbytes
+    _launch(lib.dfb_tree_attention, a, query, op)
+    return out
+
+
+@tree_attention.register_fake
+def _(query, key_cache, value_cache, cache_len, parents, scale):
+    return query.new_empty(query.shape)
+
+
+def _delta_tokens(
+    op: str, state: Tensor, query: Tensor, key: Tensor, value: Tensor, g: Tensor, beta: Tensor, lengths: Tensor | None, parents: Tensor | None, l2norm: bool
+) -> tuple[Tensor, Tensor | None]:
+    if state.dim() != 4 or state.dtype != torch.float32:
+        raise ValueError(f"{op}: state must be fp32 (batch, heads, key_dim, value_dim), got {tuple(state.shape)} {state.dtype}")
+    batch, hv, dk, dv = state.shape
+    if query.dim() != 4 or query.shape != key.shape or query.shape[0] != batch or query.shape[3] != dk:
+        raise ValueError(f"{op}: query and key must be (batch, tokens, key_heads, {dk}), got {tuple(query.shape)} and {tuple(key.shape)}")
+    tokens, hk = query.shape[1], query.shape[2]
+    if hk == 0 or hv == 0 or hv % hk:
+        raise ValueError(f"{op}: {hv} value heads do not divide into {hk} key heads")
+    if tuple(value.shape) != (batch, tokens, hv, dv):
+        raise ValueError(f"{op}: value has shape {tuple(value.shape)}, expected {(batch, tokens, hv, dv)}")
+    for name, t in (("g", g), ("beta", beta)):
+        if tuple(t.shape) != (batch, tokens, hv) or not t.is_floating_point():
+            raise ValueError(f"{op}: {name} must be a floating tensor {(batch, tokens, hv)}, got {tuple(t.shape)} {t.dtype}")
+    for name, t in (("query", query), ("key", key), ("value", value)):
+        if t.dtype != BF16:
+            raise ValueError(f"{op}: {name} must be bfloat16, got {t.dtype}")
+    if dk % 8 or dv % 8 or dk < 8 or dk > 128 or dv < 8:
+        raise ValueError(f"{op}: key dim {dk} (a multiple of 8, at most 128) or value dim {dv} (a multiple of 8) unsupported")
+    if lengths is not None and (tuple(lengths.shape) != (batch,) or lengths.dtype != torch.int32 or not lengths.is_contiguous()):
+        raise ValueError(f"{op}: lengths must be a contiguous int32 tensor of {batch} entries, got {tuple(lengths.shape)} {lengths.dtype}")
+    if parents is not None:
+        _check_parents(op, parents, batch, tokens)
+    _last_contiguous(op, query=query, key=key, value=value)
+    _same_device(op, state, query, key, value, g, beta, lengths, parents)
+    # rows that do not start on 16-byte boundaries are copied once
+    query, key, value = (t.contiguous() if t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:3]) else t for t in (query, key, value))
+    state, g, beta = state.contiguous(), g.float().contiguous(), beta.float().contiguous()
+    out = torch.empty((batch, tokens, hv, dv), dtype=BF16, device=state.device)
+    if batch == 0 or tokens == 0:
+        return out, None if parents is not None else state.clone()
+    new_state = torch.empty_like(state) if parents is None else None
+    lib = _lib.load()
+    nbytes = lib.dfb_delta_chunk_scratch_bytes(batch, tokens, hk, hv, dk)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=state.device)  # not kept, as in tree_attention
+    d = _lib.DeltaChunkDesc()
+    d.batch, d.tokens, d.hk, d.hv, d.dk, d.dv = batch, tokens, hk, hv, dk, dv
+    d.q, d.k, d.v, d.q_stride, d.k_stride, d.v_stride = query.data_ptr(), key.data_ptr(), value.data_ptr(), _three(query), _three(key), _three(value)
+    d.g, d.beta, d.lengths, d.l2norm = g.data_ptr(), beta.data_ptr(), _ptr(lengths), l2norm
+    if parents is not None:
+        d.parents, d.parents_stride = parents.data_ptr(), parents.stride(0) if parents.dim() == 2 else 0
+    d.state, d.state_out, d.out, d.scratch, d.scratch_bytes = state.data_ptr(), _ptr(new_state), out.data_ptr(), scratch.data_ptr(), nbytes
+    _launch(lib.dfb_delta_chunk, d, state, op)
+    return out, new_state
+
+
+@torch.library.custom_op("dfb200::delta_rule_chunk", mutates_args=())
+def delta_rule_chunk(
+    state: Tensor, query: Tensor, key: Tensor, value: Tensor, g: Tensor, beta: Tensor, lengths: Tensor | None, qk_l2norm: bool
+) -> tuple[Tensor, Tensor]:
+    """The delta rule over several tokens of each sequence, in chunks of 64: ``delta_rule_step`` token after token.
+
+    ``state (batch, heads, key_dim, value_dim)`` fp32; ``query, key (batch, tokens, key_heads, key_dim)`` and ``value (batch,
+    tokens, heads, value_dim)`` bf16; ``g`` (log decay) and ``beta (batch, tokens, heads)``. ``qk_l2norm`` normalises q and k
+    over the key dim and scales q by ``key_dim ** -0.5``; without it they are used as they are. With ``lengths (batch,)``
+    int32, only the first ``lengths[b]`` tokens of a sequence count: later rows give zeros and leave its state as it is
+    (a padded batch of prompts, or the accepted tokens of a draft). Returns ``(output bf16, new_state)``. Inputs that
+    count are finite: a NaN or an infinity reaches the outputs of its chunk."""
+    return _delta_tokens("delta_rule_chunk", state, query, key, value, g, beta, lengths, None, qk_l2norm)
+
+
+@delta_rule_chunk.register_fake
+def _(state, query, key, value, g, beta, lengths, qk_l2norm):
+    return value.new_empty(value.shape), state.new_empty(state.shape)
+
+
+@torch.library.custom_op("dfb200::delta_rule_tree", mutates_args=())
+def delta_rule_tree(state: Tensor, query: Tensor, key: Tensor, value: Tensor, g: Tensor, beta: Tensor, parents: Tensor, qk_l2norm: bool) -> Tensor:
+    """The delta rule over a tree of up to 64 drafted tokens: node ``i`` continues from the state that the path from the root
+    to its parent leaves. Arguments as in ``delta_rule_chunk``, ``parents`` as in ``tree_attention``. Returns the nodes' outputs
+    (zero for rows without a node); ``state`` stays as it is: once a path is accepted, run its tokens through
+    ``delta_rule_chunk``."""
+    return _delta_tokens("delta_rule_tree", state, query, key, value, g, beta, None, parents, qk_l2norm)[0]
+
+
+@delta_rule_tree.register_fake
+def _(state, query, key, value, g, beta, parents, qk_l2norm):
+    return value.new_empty(value.shape)

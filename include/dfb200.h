@@ -271,6 +271,93 @@ typedef struct dfb_attn_step_desc {
  * 621-676). Takes head_dim 256 and 1, 2 or 4 query heads per KV head. */
 int dfb_attn_step(const dfb_attn_step_desc* desc, void* stream);
 
+/* ---- several new tokens of a sequence at once: prompts and trees of drafted tokens --------------- */
+
+#define DFB_BF16 0
+#define DFB_FP16 1
+#define DFB_FP32 2
+
+typedef struct dfb_rotary_desc {
+  int32_t batch, tokens, hq, hkv, d, rotary_dim;
+  int32_t interleaved; /* pairs (2i, 2i + 1) instead of (i, i + rotary_dim / 2) */
+  int32_t dtype;       /* DFB_BF16, DFB_FP16 or DFB_FP32 */
+  const void* q;       /* [batch, tokens, hq, d]; strides in elements: batch, token, head; the last dim is contiguous */
+  const void* k;       /* [batch, tokens, hkv, d] */
+  const void* v;       /* appending form only: [batch, tokens, hkv, d] */
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const void* pos;     /* int32 or int64 [batch, tokens], pos_stride elements between sequences */
+  int64_t pos_stride;
+  int32_t pos_is_i64;
+  const void* inv_freq; /* [rotary_dim / 2], fp64 or fp32 */
+  int32_t freq_is_f64;
+  float factor;        /* on cos and sin (1, or what a stretched context asks for) */
+  void* q_out;         /* [batch, tokens, hq, d] contiguous */
+  void* k_out;         /* [batch, tokens, hkv, d] contiguous; unused in the appending form */
+  void* kcache;        /* optional [batch, hkv, max_seq, d]: selects the appending form; strides batch, head, row */
+  void* vcache;
+  int64_t kc_stride[3], vc_stride[3];
+  const int32_t* cache_len; /* [batch] on the device: token t of sequence b goes to cache row cache_len[b] + t; rows
+                             * below 0 or from max_seq on are not written */
+  int32_t max_seq;
+} dfb_rotary_desc;
+
+/* Rotary positions of several tokens, angles formed in 64 bits from integer positions; in the appending form rotated
+ * keys and the values are written into the KV cache. The many-token counterpart of GatedAttention.forward's RoPE and
+ * cache update (src/deltaforge/reference.py:638-650); rotary_dim even and at most 512. Outputs must not overlap inputs. */
+int dfb_rotary(const dfb_rotary_desc* desc, void* stream);
+
+typedef struct dfb_tree_attn_desc {
+  int32_t batch, nodes, hq, hkv, d, max_seq; /* d 32, 64, 128 or 256; nodes 1..64 */
+  int32_t is_fp16;     /* q, cache and output are fp16 instead of bf16 */
+  const void* q;       /* [batch, nodes, hq, d], strides batch, node, head (even) */
+  const void* kcache;  /* [batch, hkv, max_seq, d], strides batch, head, row (multiples of 8), 16-byte aligned */
+  const void* vcache;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const int32_t* cache_len; /* [batch] on the device: rows before the tree; node i of sequence b is row cache_len[b] + i */
+  const int32_t* parents;   /* [batch, nodes] on the device: the node's parent, before it in the list; -1: the prefix.
+                             * Any other value: the row holds no node, and its output is zero */
+  int64_t parents_stride;   /* elements between sequences; 0: one tree for all */
+  float scale;
+  void* out;           /* [batch, nodes, hq, d] contiguous */
+  void* scratch;       /* dfb_tree_attn_scratch_bytes() bytes, 16-byte aligned, not shared by calls that may overlap */
+  size_t scratch_bytes;
+} dfb_tree_attn_desc;
+
+size_t dfb_tree_attn_scratch_bytes(int batch, int nodes, int hq, int hkv, int d, int max_seq);
+
+/* Attention of a tree of drafted tokens over the KV cache that holds the accepted prefix and the tree's own rows: the
+ * many-token form of split_kv_decode_attention (src/deltaforge/kernels/flash_decode_splitkv.py:177-256). Cache rows
+ * past the tree are not read; a tree that reaches past max_seq loses the keys it has there. */
+int dfb_tree_attention(const dfb_tree_attn_desc* desc, void* stream);
+
+typedef struct dfb_delta_chunk_desc {
+  int32_t batch, tokens, hk, hv, dk, dv; /* dk, dv multiples of 8, dk <= 128, hv a multiple of hk */
+  const void* q;  /* bf16 [batch, tokens, hk, dk], strides batch, token, head (multiples of 8), 16-byte aligned */
+  const void* k;
+  const void* v;  /* bf16 [batch, tokens, hv, dv] */
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const float* g;    /* [batch, tokens, hv] log decay */
+  const float* beta; /* [batch, tokens, hv] */
+  const int32_t* lengths; /* optional [batch] on the device: tokens of each sequence; rows past them give zeros and leave
+                           * the state as it is */
+  const int32_t* parents; /* tree form (tokens <= 64, no lengths): as in dfb_tree_attn_desc */
+  int64_t parents_stride;
+  int32_t l2norm;    /* normalise q and k over dk (eps 1e-6) and scale q by 1/sqrt(dk); else they are used as they are */
+  const float* state; /* [batch, hv, dk, dv] */
+  float* state_out;   /* the same shape, may be `state`; unused in the tree form */
+  void* out;          /* bf16 [batch, tokens, hv, dv] contiguous, 16-byte aligned */
+  void* scratch;      /* dfb_delta_chunk_scratch_bytes() bytes, 16-byte aligned, not shared by calls that may overlap */
+  size_t scratch_bytes;
+} dfb_delta_chunk_desc;
+
+size_t dfb_delta_chunk_scratch_bytes(int batch, int tokens, int hk, int hv, int dk);
+
+/* The gated delta rule over several tokens of each sequence: delta_rule_step (src/deltaforge/kernels/
+ * gated_delta_step.py:109-177) token after token, computed in chunks of 64; with `parents`, over a tree of drafted
+ * tokens: node i continues from the state its path leaves, and no state is written. Inputs are finite: a NaN or an
+ * infinity reaches the outputs of its whole chunk. */
+int dfb_delta_chunk(const dfb_delta_chunk_desc* desc, void* stream);
+
 /* ---- whole decode step ------------------------------------------------------------------------- */
 
 typedef struct dfb_linear {

@@ -1,0 +1,219 @@
+"""Refusals and host logic of the ops that take several new tokens at once: all of it before any device work."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from deltaforge_b200 import _lib, ops
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def z(*shape, dtype=BF16):
+    return torch.zeros(shape, dtype=dtype)
+
+
+def rotary_args(**over):
+    a = dict(query=z(2, 3, 4, 32), key=z(2, 3, 2, 32), positions=z(2, 3, dtype=torch.int32), inv_freq=z(8, dtype=torch.float64), factor=1.0, interleaved=False)
+    return {**a, **over}
+
+
+def append_args(**over):
+    a = dict(value=z(2, 3, 2, 32), key_cache=z(2, 2, 16, 32), value_cache=z(2, 2, 16, 32), cache_len=z(2, dtype=torch.int32))
+    return {**rotary_args(), **a, **over}
+
+
+@pytest.mark.parametrize(
+    "over,match",
+    [
+        (dict(query=z(2, 3, 32)), "expected query and key"),
+        (dict(key=z(2, 4, 2, 32)), "does not match query"),
+        (dict(key=z(2, 3, 0, 32)), "at least one head"),
+        (dict(key=z(2, 3, 2, 32, dtype=F16)), "must both be"),
+        (dict(query=z(2, 3, 4, 32, dtype=torch.float64), key=z(2, 3, 2, 32, dtype=torch.float64)), "must both be"),
+        (dict(positions=z(2, 3, dtype=F32)), "positions must be int32 or int64"),
+        (dict(positions=z(2, 4, dtype=torch.int32)), "positions must be int32 or int64"),
+        (dict(positions=z(3, 2, dtype=torch.int32).t()), "must be contiguous"),
+        (dict(inv_freq=z(8, dtype=BF16)), "inv_freq must be"),
+        (dict(inv_freq=z(17, dtype=F32)), "rotary_dim 34"),
+        (dict(inv_freq=z(0, dtype=F32)), "rotary_dim 0"),
+        (dict(query=z(2, 3, 32, 4).transpose(2, 3)), "last dimension contiguous"),
+    ],
+)
+def test_rotary_refusals(over, match):
+    with pytest.raises(ValueError, match=match):
+        ops.rotary_qk(**rotary_args(**over))
+
+
+@pytest.mark.parametrize(
+    "over,match",
+    [
+        (dict(value=z(2, 3, 1, 32)), "must match key"),
+        (dict(key_cache=z(2, 2, 16)), "caches must both be"),
+        (dict(value_cache=z(2, 2, 15, 32)), "caches must both be"),
+        (dict(key_cache=z(2, 3, 16, 32), value_cache=z(2, 3, 16, 32)), "do not match batch"),
+        (dict(key_cache=z(2, 2, 16, 32, dtype=F16)), "caches must be"),
+        (dict(cache_len=z(2, dtype=torch.int64)), "cache_len must be"),
+        (dict(cache_len=z(3, dtype=torch.int32)), "cache_len must be"),
+        (dict(key_cache=z(1, 2, 16, 32).expand(2, 2, 16, 32)), "expanded"),
+    ],
+)
+def test_rotary_append_refusals(over, match):
+    with pytest.raises(ValueError, match=match):
+        ops.rotary_append(**append_args(**over))
+
+
+def tree_args(**over):
+    a = dict(query=z(2, 5, 4, 64), key_cache=z(2, 2, 16, 64), value_cache=z(2, 2, 16, 64), cache_len=z(2, dtype=torch.int32), parents=z(2, 5, dtype=torch.int32), scale=0.125)
+    return {**a, **over}
+
+
+@pytest.mark.parametrize(
+    "over,match",
+    [
+        (dict(query=z(2, 5, 64)), "expected query"),
+        (dict(query=z(2, 5, 4, 64, dtype=F32)), "bfloat16 or float16"),
+        (dict(query=z(2, 5, 3, 64)), "do not divide"),
+        (dict(query=z(2, 5, 4, 96), key_cache=z(2, 2, 16, 96), value_cache=z(2, 2, 16, 96)), "head dim 96"),
+        (dict(query=z(2, 5, 4, 64, dtype=F16)), "caches must be"),
+        (dict(key_cache=z(3, 2, 16, 64), value_cache=z(3, 2, 16, 64)), "do not match batch"),
+        (dict(key_cache=z(2, 2, 0, 64), value_cache=z(2, 2, 0, 64)), "one cache row"),
+        (dict(parents=z(2, 4, dtype=torch.int32)), "parents must be"),
+        (dict(parents=z(2, 5, dtype=torch.int64)), "parents must be"),
+        (dict(query=z(2, 65, 4, 64), parents=z(65, dtype=torch.int32)), "at most 64 nodes"),
+        (dict(key_cache=z(2, 2, 16, 68)[..., :64]), "16-byte boundaries"),
+        (dict(cache_len=z(2, 1, dtype=torch.int32)), "cache_len must be"),
+    ],
+)
+def test_tree_attention_refusals(over, match):
+    with pytest.raises(ValueError, match=match):
+        ops.tree_attention(**tree_args(**over))
+
+
+def delta_args(**over):
+    a = dict(
+        state=z(2, 4, 16, 24, dtype=F32), query=z(2, 5, 2, 16), key=z(2, 5, 2, 16), value=z(2, 5, 4, 24), g=z(2, 5, 4, dtype=F32), beta=z(2, 5, 4, dtype=F32),
+        lengths=None, qk_l2norm=True,
+    )  # fmt: skip
+    return {**a, **over}
+
+
+@pytest.mark.parametrize(
+    "over,match",
+    [
+        (dict(state=z(2, 4, 16, 24)), "state must be fp32"),
+        (dict(state=z(4, 16, 24, dtype=F32)), "state must be fp32"),
+        (dict(key=z(2, 4, 2, 16)), "query and key must be"),
+        (dict(query=z(2, 5, 3, 16), key=z(2, 5, 3, 16)), "do not divide"),
+        (dict(query=z(2, 5, 0, 16), key=z(2, 5, 0, 16)), "do not divide"),
+        (dict(value=z(2, 5, 4, 16)), "value has shape"),
+        (dict(value=z(2, 5, 4, 24, dtype=F16)), "value must be bfloat16"),
+        (dict(g=z(2, 5, 2, dtype=F32)), "g must be"),
+        (dict(beta=z(2, 5, 4, dtype=torch.int32)), "beta must be"),
+        (dict(lengths=z(3, dtype=torch.int32)), "lengths must be"),
+        (dict(lengths=z(2, dtype=torch.int64)), "lengths must be"),
+        (dict(state=z(2, 4, 12, 24, dtype=F32), query=z(2, 5, 2, 12), key=z(2, 5, 2, 12)), "key dim 12"),
+        (dict(state=z(2, 4, 136, 24, dtype=F32), query=z(2, 5, 2, 136), key=z(2, 5, 2, 136)), "key dim 136"),
+        (dict(state=z(2, 4, 16, 20, dtype=F32), value=z(2, 5, 4, 20)), "value dim 20"),
+    ],
+)
+def test_delta_rule_refusals(over, match):
+    with pytest.raises(ValueError, match=match):
+        ops.delta_rule_chunk(**delta_args(**over))
+
+
+def test_delta_tree_refusals():
+    a = delta_args()
+    del a["lengths"]
+    with pytest.raises(ValueError, match="parents must be"):
+        ops.delta_rule_tree(**a, parents=z(2, 4, dtype=torch.int32))
+    a.update(query=z(2, 65, 2, 16), key=z(2, 65, 2, 16), value=z(2, 65, 4, 24), g=z(2, 65, 4, dtype=F32), beta=z(2, 65, 4, dtype=F32))
+    with pytest.raises(ValueError, match="at most 64 nodes"):
+        ops.delta_rule_tree(**a, parents=z(2, 65, dtype=torch.int32))
+
+
+def test_cpu_tensors_are_refused():
+    d = delta_args()
+    del d["lengths"]
+    for call in (
+        lambda: ops.rotary_qk(**rotary_args()),
+        lambda: ops.rotary_append(**append_args()),
+        lambda: ops.tree_attention(**tree_args()),
+        lambda: ops.delta_rule_chunk(**delta_args()),
+        lambda: ops.delta_rule_tree(**d, parents=z(2, 5, dtype=torch.int32)),
+    ):
+        with pytest.raises(RuntimeError, match="no PyTorch fallback"):
+            call()
+
+
+def test_c_entries_refuse_before_any_launch():
+    lib = _lib.load()
+    assert lib.dfb_rotary(None, None) == 2 and lib.dfb_tree_attention(None, None) == 2 and lib.dfb_delta_chunk(None, None) == 2
+    r = _lib.RotaryDesc()
+    r.batch = r.tokens = r.hq = r.hkv = 1
+    r.d, r.rotary_dim = 8, 3
+    assert lib.dfb_rotary(r, None) == 2 and b"even" in lib.dfb_last_error()
+    r.rotary_dim = 4
+    assert lib.dfb_rotary(r, None) == 2 and b"null" in lib.dfb_last_error()
+    t = _lib.TreeAttnDesc()
+    t.batch = t.nodes = t.hq = t.hkv = 1
+    t.d, t.max_seq = 48, 8
+    assert lib.dfb_tree_attention(t, None) == 2 and b"head dim" in lib.dfb_last_error()
+    t.d, t.nodes = 64, 65
+    assert lib.dfb_tree_attention(t, None) == 2 and b"at most 64" in lib.dfb_last_error()
+    t.nodes, t.max_seq = 1, 4096
+    t.q = t.kcache = t.vcache = t.cache_len = t.parents = t.out = 16  # never dereferenced: the scratch check comes first
+    need = lib.dfb_tree_attn_scratch_bytes(1, 1, 1, 1, 64, 4096)
+    assert need > 0
+    assert lib.dfb_tree_attention(t, None) == 2 and b"scratch" in lib.dfb_last_error()
+    d = _lib.DeltaChunkDesc()
+    d.batch = d.tokens = d.hk = d.hv = 1
+    d.dk, d.dv = 12, 16
+    assert lib.dfb_delta_chunk(d, None) == 2 and b"unsupported" in lib.dfb_last_error()
+    d.dk = 16
+    d.state = d.state_out = d.q = d.k = d.v = d.g = d.beta = d.out = 16
+    assert lib.dfb_delta_chunk(d, None) == 2 and b"scratch" in lib.dfb_last_error()
+    d.parents, d.lengths = 16, 16
+    assert lib.dfb_delta_chunk(d, None) == 2 and b"no lengths" in lib.dfb_last_error()
+
+
+def test_scratch_sizes():
+    lib = _lib.load()
+    assert lib.dfb_delta_chunk_scratch_bytes(1, 64, 16, 32, 128) == 16 * 32768 + 32 * 25600
+    # a long prompt is walked in segments: the scratch stays bounded
+    assert lib.dfb_delta_chunk_scratch_bytes(1, 1 << 20, 16, 32, 128) <= 64 << 20
+    assert lib.dfb_delta_chunk_scratch_bytes(0, 5, 1, 1, 8) == 0
+    assert lib.dfb_tree_attn_scratch_bytes(64, 64, 16, 4, 256, 32) == 0  # one split
+
+
+def test_rope_frequencies():
+    f, factor = ops.rope_frequencies(64, 1e7, device="cpu")
+    want = [1e7 ** (-2 * i / 64) for i in range(32)]
+    assert factor == 1.0 and f.dtype == torch.float64 and torch.allclose(f, torch.tensor(want, dtype=torch.float64), rtol=1e-15)
+    lin, _ = ops.rope_frequencies(64, 1e7, stretch=4.0, method="linear", device="cpu")
+    assert torch.equal(lin, f / 4)
+    base, _ = ops.rope_frequencies(64, 1e7, stretch=4.0, method="base", device="cpu")
+    assert base[0] == 1.0 and math.isclose(base[-1], f[-1] / 4, rel_tol=1e-12)
+    parts, factor = ops.rope_frequencies(64, 1e7, stretch=4.0, trained_len=32768, device="cpu")
+    turns = 32768 * f / (2 * math.pi)
+    assert torch.equal(parts[turns >= 32], f[turns >= 32]) and torch.allclose(parts[turns <= 1], f[turns <= 1] / 4, rtol=1e-15)
+    between = (turns > 1) & (turns < 32)
+    assert between.any() and bool(((parts < f) & (parts > f / 4))[between].all()) and math.isclose(factor, 0.1 * math.log(4) + 1)
+    for bad in (dict(rotary_dim=3), dict(stretch=0.5), dict(method="other"), dict(fast_turns=1.0)):
+        with pytest.raises(ValueError):
+            ops.rope_frequencies(**{"rotary_dim": 64, "theta": 1e4, "device": "cpu", **bad})
+
+
+def test_fake_kernels_give_shapes():
+    with torch._subclasses.fake_tensor.FakeTensorMode():
+        r = rotary_args()
+        q, k = torch.ops.dfb200.rotary_qk(**{n: torch.empty(t.shape, dtype=t.dtype) if isinstance(t, torch.Tensor) else t for n, t in r.items()})
+        assert q.shape == (2, 3, 4, 32) and k.shape == (2, 3, 2, 32)
+        t = {n: torch.empty(x.shape, dtype=x.dtype) if isinstance(x, torch.Tensor) else x for n, x in tree_args().items()}
+        assert torch.ops.dfb200.tree_attention(**t).shape == (2, 5, 4, 64)
+        d = {n: torch.empty(x.shape, dtype=x.dtype) if isinstance(x, torch.Tensor) else x for n, x in delta_args().items()}
+        out, state = torch.ops.dfb200.delta_rule_chunk(**d)
+        assert out.shape == (2, 5, 4, 24) and out.dtype == BF16 and state.shape == (2, 4, 16, 24) and state.dtype == F32
