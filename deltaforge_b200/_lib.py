@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 
 from . import build as _build
@@ -125,6 +126,16 @@ class ModelDesc(C.Structure):
         ("workspace", c_vp), ("workspace_bytes", c_sz), ("attn_splits", c_i32), ("math", c_i32),
         ("tp_size", c_i32), ("tp_rank", c_i32), ("tp_peer_slots", C.POINTER(c_vp)),
     ]  # fmt: skip
+
+
+def packer(cls: type[C.Structure]) -> struct.Struct:
+    """The C layout of a descriptor as a ``struct`` format: ``packer(cls).pack_into(cls(), 0, *values)`` fills every field in
+    one call (null pointers as 0), which costs a tenth of assigning them one by one."""
+    codes = {c_i32: "i", c_i64: "q", c_f32: "f", c_vp: "P", c_sz: "N"}
+    fmt = "@" + "".join(f"{t._length_}{codes[t._type_]}" if issubclass(t, C.Array) else codes[t] for _, t in cls._fields_)
+    packed = struct.Struct(fmt)
+    assert packed.size <= C.sizeof(cls)  # equal but for padding behind the last field
+    return packed
 
 
 # name -> (restype, argtypes); every exported symbol of include/dfb200.h

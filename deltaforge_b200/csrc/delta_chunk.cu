@@ -85,6 +85,8 @@ __device__ __forceinline__ int scale_exp(float m) {
   const int e = (int)((__float_as_uint(m) >> 23) & 255) - 127 - 12;
   return e < -110 ? -110 : e > 110 ? 110 : e;
 }
+// Largest of the lanes' non-negative values, whose bit patterns order like the values
+__device__ __forceinline__ float warp_max_abs(float m) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))); }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 
 // Images are rows of W fp16 with 16-byte chunks permuted within 128 bytes, so that 8x8 matrix loads are free of conflicts.
@@ -414,7 +416,7 @@ template <int VROW> __device__ __forceinline__ uint32_t v_off(int row, int chunk
   return (uint32_t)(row * VROW + (x << 4));
 }
 
-template <int DKP, int NW, bool TREE>
+template <int DKP, int NW, int NB, bool TREE>
 __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const DeltaChunkParams p) {
   using S_ = Scan<DKP, NW>;
   constexpr int NT = DKP / 8;
@@ -487,17 +489,17 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
     const unsigned char* st = smem + (n % S_::STAGES) * S_::STAGE;
     const uint32_t ks_s = smem_u32(st), qs_s = ks_s + S_::Q_OFF, ti_s = ks_s + S_::H_OFF, vs_s = ks_s + S_::V_OFF;
     const float* sc = (const float*)(st + S_::H_OFF + 3 * SQ);
-    const int tok0 = (p.chunk0 + n) * C, live = min(len - tok0, C), nb = (live + 15) / 16;  // blocks of 16 tokens
+    const int tok0 = (p.chunk0 + n) * C;
 
     // 1. S^T K^T (hi and lo) and S^T Q^T (hi)
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < NT; ++i) m = fmaxf(m, fmaxf(fmaxf(fabsf(S[i][0]), fabsf(S[i][1])), fmaxf(fabsf(S[i][2]), fabsf(S[i][3]))));
-    const int es = scale_exp(warp_max(m));
+    const int es = scale_exp(warp_max_abs(m));
     const float sdown = pow2(-es), sup = pow2(es);
-    float x[8][4], oq[8][4];
+    float x[2 * NB][4], oq[2 * NB][4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 2 * NB; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[i][e] = oq[i][e] = 0.f;
 #pragma unroll
@@ -508,8 +510,7 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
       split2(S[2 * ks + 1][0] * sdown, S[2 * ks + 1][1] * sdown, hi[2], lo[2]);
       split2(S[2 * ks + 1][2] * sdown, S[2 * ks + 1][3] * sdown, hi[3], lo[3]);
 #pragma unroll
-      for (int n2 = 0; n2 < 4; ++n2) {
-        if (n2 >= nb) continue;
+      for (int n2 = 0; n2 < NB; ++n2) {
         uint32_t kb[4], qb[4];
         const uint32_t off = img_off<DKP>(16 * n2 + (lane & 7) + 8 * (lane >> 4), 2 * ks + ((lane >> 3) & 1));
         ldsm4(ks_s + off, kb);
@@ -525,8 +526,7 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
     // 2. R = V - diag(e^G) K S, then its halves
     m = 0.f;
 #pragma unroll
-    for (int n2 = 0; n2 < 4; ++n2) {
-      if (n2 >= nb) continue;
+    for (int n2 = 0; n2 < NB; ++n2) {
       uint32_t vr[4];
       ldsm4_t(vs_s + v_off<S_::VROW>(16 * n2 + (lane & 15), warp * 2 + (lane >> 4)), vr);
 #pragma unroll
@@ -541,11 +541,11 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
         m = fmaxf(m, fmaxf(fmaxf(fabsf(x[nt][0]), fabsf(x[nt][1])), fmaxf(fabsf(x[nt][2]), fabsf(x[nt][3]))));
       }
     }
-    const int er = scale_exp(warp_max(m));
+    const int er = scale_exp(warp_max_abs(m));
     const float rdown = pow2(-er);
-    uint32_t rh[4][4], rl[4][4];
+    uint32_t rh[NB][4], rl[NB][4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < NB; ++k) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         split2(x[2 * k + h][0] * rdown, x[2 * k + h][1] * rdown, rh[k][2 * h], rl[k][2 * h]);
@@ -554,12 +554,11 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
     }
     // 3. V'^T = R^T T^T; block (i, j) of T is zero for j > i
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
+    for (int i = 0; i < 2 * NB; ++i) x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < NB; ++k) {
 #pragma unroll
-      for (int n2 = k; n2 < 4; ++n2) {
-        if (n2 >= nb) continue;
+      for (int n2 = k; n2 < NB; ++n2) {
         uint32_t th[4], tl[4];
         const uint32_t off = img_off<C>(16 * n2 + (lane & 7) + 8 * (lane >> 4), 2 * k + ((lane >> 3) & 1));
         ldsm4(ti_s + off, th);
@@ -576,24 +575,23 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
     {
       const float up = pow2(er) * sc[3 * C + 1];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 2 * NB; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[i][e] *= up, m = fmaxf(m, fabsf(x[i][e]));
     }
     // 4. O^T = (S^T Q^T) diag(e^G) + V'^T P^T
-    const int ev = scale_exp(warp_max(m));
+    const int ev = scale_exp(warp_max_abs(m));
     {
       const float vdown = pow2(-ev);
-      float o[8][4];
+      float o[2 * NB][4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+      for (int i = 0; i < 2 * NB; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < NB; ++k) {
         const uint32_t a[4] = {h2(x[2 * k][0] * vdown, x[2 * k][1] * vdown), h2(x[2 * k][2] * vdown, x[2 * k][3] * vdown),
                                h2(x[2 * k + 1][0] * vdown, x[2 * k + 1][1] * vdown), h2(x[2 * k + 1][2] * vdown, x[2 * k + 1][3] * vdown)};
 #pragma unroll
-        for (int n2 = k; n2 < 4; ++n2) {
-          if (n2 >= nb) continue;
+        for (int n2 = k; n2 < NB; ++n2) {
           uint32_t pb[4];
           ldsm4(ti_s + 2 * SQ + img_off<C>(16 * n2 + (lane & 7) + 8 * (lane >> 4), 2 * k + ((lane >> 3) & 1)), pb);
           mma_f16(o[2 * n2], a, pb[0], pb[1]);
@@ -603,8 +601,7 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
       const float up = pow2(ev) * sc[3 * C + 2];
       __syncwarp();  // the previous chunk's outputs have left the buffer
 #pragma unroll
-      for (int n2 = 0; n2 < 4; ++n2) {
-        if (n2 >= nb) continue;
+      for (int n2 = 0; n2 < NB; ++n2) {
         uint32_t w[4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -620,9 +617,9 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
       }
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < NB; ++i) {
         const int row = 16 * i + (lane >> 1), half = lane & 1, tok = tok0 + row;
-        if (row < 16 * nb && tok < p.tokens && col0 + half * 8 < p.dv)
+        if (tok < p.tokens && col0 + half * 8 < p.dv)
           *(uint4*)(out + tok * orow + half * 8) = *(const uint4*)(obuf + row * 32 + ((half ^ ((row >> 2) & 1)) << 4));
       }
     }
@@ -630,15 +627,15 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
     // 5. S^T = e^G_C S^T + (V' diag(e^(G_C - G)))^T K, accumulated apart
     m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 2 * NB; ++i) {
       const float2 w = *(const float2*)&sc[C + 8 * i + 2 * c];
       x[i][0] *= w.x, x[i][1] *= w.y, x[i][2] *= w.x, x[i][3] *= w.y;
       m = fmaxf(m, fmaxf(fmaxf(fabsf(x[i][0]), fabsf(x[i][1])), fmaxf(fabsf(x[i][2]), fabsf(x[i][3]))));
     }
-    const int eu = scale_exp(warp_max(m));
+    const int eu = scale_exp(warp_max_abs(m));
     const float udown = pow2(-eu), uup = pow2(eu), decay = sc[3 * C];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < NB; ++k) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         split2(x[2 * k + h][0] * udown, x[2 * k + h][1] * udown, rh[k][2 * h], rl[k][2 * h]);
@@ -649,8 +646,7 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
     for (int j2 = 0; j2 < NT / 2; ++j2) {
       float a0[4] = {0.f, 0.f, 0.f, 0.f}, a1[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (k >= nb) continue;
+      for (int k = 0; k < NB; ++k) {
         uint32_t kb[4];
         ldsm4_t(ks_s + img_off<DKP>(16 * k + (lane & 15), 2 * j2 + (lane >> 4)), kb);
         mma_f16(a0, rh[k], kb[0], kb[1]);
@@ -668,8 +664,7 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
 
   // rows of tokens that no chunk covered: zeros
   {
-    const int last = (p.chunk0 + nlive - 1) * C;  // first token of the last chunk with tokens; its written blocks end behind it
-    const int from = nlive ? last + (min(len - last, C) + 15) / 16 * 16 : p.chunk0 * C, to = min(p.tokens, (p.chunk0 + p.chunks) * C);
+    const int from = (p.chunk0 + nlive) * C, to = min(p.tokens, (p.chunk0 + p.chunks) * C);
     for (int i = lane; i < (to - from) * 2; i += 32) {
       const int tok = from + (i >> 1), half = i & 1;
       if (col0 + half * 8 < p.dv) *(uint4*)(out + tok * orow + half * 8) = make_uint4(0u, 0u, 0u, 0u);
@@ -703,41 +698,55 @@ int segment_chunks(int batch, int tokens, int hk, int hv, int dk) {
 
 template <int DKP> constexpr int prep_smem() { return 2 * C * DKP * 2 + 2 * C * TS * 4 + 32 * 36 * 4; }
 
-template <int DKP, int NW, bool TREE>
-int configure_scan() {
-  return cudaFuncSetAttribute(delta_scan_kernel<DKP, NW, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Scan<DKP, NW>::SMEM) == cudaSuccess
-             ? 0
-             : check_launch("delta rule scan: shared-memory opt-in");
+// Blocks of 16 tokens that a chunk computes: all four, or fewer where the whole call has no more tokens (a draft).
+int token_blocks(int tokens) { return tokens <= 16 ? 1 : tokens <= 32 ? 2 : 4; }
+
+// Calls f.template operator()<DKP, NW, NB, TREE>() for the instance that serves (dkp, nw, nb).
+template <bool TREE, int DKP, int NW, typename F>
+int with_nb(int nb, F f) {
+  return nb == 1 ? f.template operator()<DKP, NW, 1, TREE>() : nb == 2 ? f.template operator()<DKP, NW, 2, TREE>() : f.template operator()<DKP, NW, 4, TREE>();
 }
-template <int DKP, bool TREE>
-int configure_dkp() {
-  int rc = cudaFuncSetAttribute(delta_prep_kernel<DKP, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, prep_smem<DKP>()) == cudaSuccess
-               ? 0
-               : check_launch("delta rule preparation: shared-memory opt-in");
-  if (!rc) rc = configure_scan<DKP, 2, TREE>();
-  if (!rc) rc = configure_scan<DKP, 4, TREE>();
-  if (!rc) rc = configure_scan<DKP, 8, TREE>();
-  return rc;
+template <bool TREE, int DKP, typename F>
+int with_nw(int nw, int nb, F f) {
+  return nw == 2 ? with_nb<TREE, DKP, 2>(nb, f) : nw == 4 ? with_nb<TREE, DKP, 4>(nb, f) : with_nb<TREE, DKP, 8>(nb, f);
 }
-int configure_all() {
-  int rc = configure_dkp<64, false>();
-  if (!rc) rc = configure_dkp<64, true>();
-  if (!rc) rc = configure_dkp<128, false>();
-  if (!rc) rc = configure_dkp<128, true>();
-  return rc;
+template <typename F>
+int with_instance(bool tree, int dkp, int nw, int nb, F f) {
+  if (tree) return dkp == 64 ? with_nw<true, 64>(nw, nb, f) : with_nw<true, 128>(nw, nb, f);
+  return dkp == 64 ? with_nw<false, 64>(nw, nb, f) : with_nw<false, 128>(nw, nb, f);
 }
 
-template <int DKP, bool TREE>
-int launch_segment(const DeltaChunkParams& p, int nw, cudaStream_t stream) {
-  delta_prep_kernel<DKP, TREE><<<dim3(p.chunks, p.hk, p.batch), PREP_THREADS, prep_smem<DKP>(), stream>>>(p);
-  const int rc = check_launch("delta rule preparation");
-  if (rc) return rc;
-  const dim3 grid((p.dv + 16 * nw - 1) / (16 * nw), p.hv, p.batch);
-  if (nw == 2) delta_scan_kernel<DKP, 2, TREE><<<grid, Scan<DKP, 2>::THREADS, Scan<DKP, 2>::SMEM, stream>>>(p);
-  else if (nw == 4) delta_scan_kernel<DKP, 4, TREE><<<grid, Scan<DKP, 4>::THREADS, Scan<DKP, 4>::SMEM, stream>>>(p);
-  else delta_scan_kernel<DKP, 8, TREE><<<grid, Scan<DKP, 8>::THREADS, Scan<DKP, 8>::SMEM, stream>>>(p);
-  return check_launch("delta rule scan");
+struct Configure {
+  template <int DKP, int NW, int NB, bool TREE>
+  int operator()() const {
+    cudaError_t e = cudaFuncSetAttribute(delta_prep_kernel<DKP, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, prep_smem<DKP>());
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(delta_scan_kernel<DKP, NW, NB, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Scan<DKP, NW>::SMEM);
+    return e == cudaSuccess ? 0 : check_launch("delta rule: shared-memory opt-in");
+  }
+};
+int configure_all() {
+  for (int tree = 0; tree < 2; ++tree)
+    for (int dkp = 64; dkp <= 128; dkp *= 2)
+      for (int nw = 2; nw <= 8; nw *= 2)
+        for (int nb = 1; nb <= 4; nb *= 2)
+          if (const int rc = with_instance(tree, dkp, nw, nb, Configure())) return rc;
+  return 0;
 }
+
+struct LaunchSegment {
+  const DeltaChunkParams& p;
+  cudaStream_t stream;
+  template <int DKP, int NW, int NB, bool TREE>
+  int operator()() const {
+    delta_prep_kernel<DKP, TREE><<<dim3(p.chunks, p.hk, p.batch), PREP_THREADS, prep_smem<DKP>(), stream>>>(p);
+    const int rc = check_launch("delta rule preparation");
+    if (rc) return rc;
+    delta_scan_kernel<DKP, NW, NB, TREE>
+        <<<dim3((p.dv + 16 * NW - 1) / (16 * NW), p.hv, p.batch), Scan<DKP, NW>::THREADS, Scan<DKP, NW>::SMEM, stream>>>(p);
+    return check_launch("delta rule scan");
+  }
+};
 
 }  // namespace
 
@@ -761,9 +770,7 @@ int launch_delta_chunk(const DeltaChunkParams& args, cudaStream_t stream) {
     p.chunks = chunks - at < p.seg_chunks ? chunks - at : p.seg_chunks;
     p.first = at == 0;
     p.last = at + p.chunks == chunks;
-    const bool wide = pad_dk(p.dk) == 128;
-    if (tree) rc = wide ? launch_segment<128, true>(p, nw, stream) : launch_segment<64, true>(p, nw, stream);
-    else rc = wide ? launch_segment<128, false>(p, nw, stream) : launch_segment<64, false>(p, nw, stream);
+    rc = with_instance(tree, pad_dk(p.dk), nw, token_blocks(p.tokens), LaunchSegment{p, stream});
     if (rc) return rc;
   }
   return 0;

@@ -30,6 +30,8 @@ are coerced with ``.contiguous()``, shapes are not.
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import inspect
 import math
 
 import torch
@@ -805,45 +807,74 @@ def _(proj, q_norm_weight, k_norm_weight, eps, inv_freq, pos, key_cache, value_c
 
 MAX_TREE_NODES = 64
 _DTYPES = {BF16: 0, torch.float16: 1, torch.float32: 2}
+_ROTARY, _TREE, _DELTA = (_lib.packer(d) for d in (_lib.RotaryDesc, _lib.TreeAttnDesc, _lib.DeltaChunkDesc))
 
 
-def _three(t: Tensor):
-    return (C.c_int64 * 3)(t.stride(0), t.stride(1), t.stride(2))
+def _eager(op):
+    """The function of a custom op, called directly where the dispatcher has nothing to add: plain tensors, no tracing or
+    dispatch mode, no gradient asked for. The dispatcher's 20 us are more than the smallest of these calls takes. Everything
+    else goes through the op (and meets its errors there)."""
+    run, mutated = op._init_fn, [i for i, name in enumerate(inspect.signature(op._init_fn).parameters) if name in ("key_cache", "value_cache")]
+    if not op._opoverload._schema.is_mutable:
+        mutated = []
+
+    @functools.wraps(run)
+    def call(*args, **kwargs):
+        if kwargs or torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() or torch._C._functorch.peek_interpreter_stack() is not None:
+            return op(*args, **kwargs)
+        grad = torch.is_grad_enabled()
+        for x in args:
+            if isinstance(x, Tensor) and ((grad and x.requires_grad) or type(x) not in (Tensor, torch.nn.Parameter)):
+                return op(*args)
+        out = run(*args)
+        for i in mutated:
+            if not args[i].is_inference():  # (inference tensors have no version)
+                torch.autograd.graph.increment_version(args[i])
+        return out
+
+    call.op = op
+    return call
 
 
-def _launch(fn, desc, t: Tensor, op: str) -> None:
-    """Call a C entry point on the current stream of the tensors' device, whichever device is current."""
-    if t.device.index == torch.cuda.current_device():
-        _lib.check(fn(C.byref(desc), _stream(t)), f"dfb200::{op}")
+def _launch(fn, desc, index: int, op: str) -> None:
+    """Call a C entry point on the current stream of device `index`, whichever device is current."""
+    if index == torch._C._cuda_getDevice():
+        rc = fn(desc, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(t.device):
-            _lib.check(fn(C.byref(desc), _stream(t)), f"dfb200::{op}")
+        with torch.cuda.device(index):
+            rc = fn(desc, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, f"dfb200::{op}")
 
 
-def _same_device(op: str, first: Tensor, *rest: Tensor | None) -> None:
+def _same_device(op: str, first: Tensor, *rest: Tensor | None) -> torch.device:
     require_cuda(first, op)
+    device = first.device
     for t in rest:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{op}: all tensors must be on {first.device}, got one on {t.device}")
+        if t is not None and t.device != device:
+            raise ValueError(f"{op}: all tensors must be on {device}, got one on {t.device}")
+    return device
 
 
-def _last_contiguous(op: str, **tensors: Tensor) -> None:
-    for name, t in tensors.items():
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
-            raise ValueError(f"{op}: {name} must have its last dimension contiguous")
+def _rows(op: str, name: str, t: Tensor) -> tuple[int, int, int]:
+    """Strides of the three leading dimensions; the last one must be contiguous."""
+    s = t.stride()
+    if s[3] != 1 and t.shape[3] > 1:
+        raise ValueError(f"{op}: {name} must have its last dimension contiguous")
+    return s[:3]
 
 
 def _check_cache(op: str, batch: int, heads: int, dim: int, dtype: torch.dtype, key_cache: Tensor, value_cache: Tensor, cache_len: Tensor) -> int:
-    if key_cache.dim() != 4 or key_cache.shape != value_cache.shape:
-        raise ValueError(f"{op}: caches must both be (batch, kv_heads, max_seq, head_dim), got {tuple(key_cache.shape)} and {tuple(value_cache.shape)}")
-    if key_cache.shape[0] != batch or key_cache.shape[1] != heads or key_cache.shape[3] != dim:
-        raise ValueError(f"{op}: caches {tuple(key_cache.shape)} do not match batch {batch}, {heads} KV heads, head dim {dim}")
+    shape = key_cache.shape
+    if len(shape) != 4 or shape != value_cache.shape:
+        raise ValueError(f"{op}: caches must both be (batch, kv_heads, max_seq, head_dim), got {tuple(shape)} and {tuple(value_cache.shape)}")
+    if shape[0] != batch or shape[1] != heads or shape[3] != dim:
+        raise ValueError(f"{op}: caches {tuple(shape)} do not match batch {batch}, {heads} KV heads, head dim {dim}")
     if key_cache.dtype != dtype or value_cache.dtype != dtype:
         raise ValueError(f"{op}: caches must be {dtype}, got {key_cache.dtype} and {value_cache.dtype}")
-    if tuple(cache_len.shape) != (batch,) or cache_len.dtype != torch.int32 or not cache_len.is_contiguous():
+    if cache_len.shape != (batch,) or cache_len.dtype != torch.int32 or not cache_len.is_contiguous():
         raise ValueError(f"{op}: cache_len must be a contiguous int32 tensor of {batch} entries, got {tuple(cache_len.shape)} {cache_len.dtype}")
-    _last_contiguous(op, key_cache=key_cache, value_cache=value_cache)
-    return key_cache.shape[2]
+    return shape[2]
 
 
 def rope_frequencies(
@@ -878,55 +909,61 @@ def rope_frequencies(
     return f.to(device), factor
 
 
-def _rotary_desc(op: str, query: Tensor, key: Tensor, positions: Tensor, inv_freq: Tensor, factor: float, interleaved: bool) -> _lib.RotaryDesc:
-    if query.dim() != 4 or key.dim() != 4:
-        raise ValueError(f"{op}: expected query and key (batch, tokens, heads, head_dim), got {tuple(query.shape)} and {tuple(key.shape)}")
-    batch, tokens, hq, d = query.shape
-    if key.shape[0] != batch or key.shape[1] != tokens or key.shape[3] != d:
-        raise ValueError(f"{op}: key {tuple(key.shape)} does not match query {tuple(query.shape)}")
-    if hq < 1 or key.shape[2] < 1:
+def _check_rotary(op: str, query: Tensor, key: Tensor, positions: Tensor, inv_freq: Tensor) -> int:
+    """Checks what both rotary ops share; the number of dims that turn."""
+    qs, ks = query.shape, key.shape
+    if len(qs) != 4 or len(ks) != 4:
+        raise ValueError(f"{op}: expected query and key (batch, tokens, heads, head_dim), got {tuple(qs)} and {tuple(ks)}")
+    if ks[0] != qs[0] or ks[1] != qs[1] or ks[3] != qs[3]:
+        raise ValueError(f"{op}: key {tuple(ks)} does not match query {tuple(qs)}")
+    if qs[2] < 1 or ks[2] < 1:
         raise ValueError(f"{op}: query and key need at least one head")
     if query.dtype not in _DTYPES or key.dtype != query.dtype:
         raise ValueError(f"{op}: query and key must both be bfloat16, float16 or float32, got {query.dtype} and {key.dtype}")
-    if tuple(positions.shape) != (batch, tokens) or positions.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{op}: positions must be int32 or int64 {(batch, tokens)}, got {tuple(positions.shape)} {positions.dtype}")
+    if positions.shape != qs[:2] or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{op}: positions must be int32 or int64 {tuple(qs[:2])}, got {tuple(positions.shape)} {positions.dtype}")
     if inv_freq.dim() != 1 or inv_freq.dtype not in (torch.float64, torch.float32) or not inv_freq.is_contiguous():
         raise ValueError(f"{op}: inv_freq must be a contiguous 1-D float64 or float32 tensor, got {tuple(inv_freq.shape)} {inv_freq.dtype}")
-    rd = 2 * inv_freq.numel()
-    if rd < 2 or rd > d or rd > 512:
-        raise ValueError(f"{op}: rotary_dim {rd} must be at least 2 and at most the head dim {d} and 512")
-    if tokens > 1 and positions.stride(1) != 1:
+    rd = 2 * inv_freq.shape[0]
+    if rd < 2 or rd > qs[3] or rd > 512:
+        raise ValueError(f"{op}: rotary_dim {rd} must be at least 2 and at most the head dim {qs[3]} and 512")
+    if qs[1] > 1 and positions.stride(1) != 1:
         raise ValueError(f"{op}: positions of a sequence must be contiguous")
-    _last_contiguous(op, query=query, key=key)
-    p = _lib.RotaryDesc()
-    p.batch, p.tokens, p.hq, p.hkv, p.d, p.rotary_dim = batch, tokens, hq, key.shape[2], d, rd
-    p.interleaved, p.dtype, p.factor = interleaved, _DTYPES[query.dtype], factor
-    p.q, p.k, p.q_stride, p.k_stride = query.data_ptr(), key.data_ptr(), _three(query), _three(key)
-    p.pos, p.pos_stride, p.pos_is_i64 = positions.data_ptr(), positions.stride(0), positions.dtype == torch.int64
-    p.inv_freq, p.freq_is_f64 = inv_freq.data_ptr(), inv_freq.dtype == torch.float64
-    return p
+    return rd
 
 
+_NO_ROWS = (0, 0, 0)
+
+
+@_eager
 @torch.library.custom_op("dfb200::rotary_qk", mutates_args=())
 def rotary_qk(query: Tensor, key: Tensor, positions: Tensor, inv_freq: Tensor, factor: float, interleaved: bool) -> tuple[Tensor, Tensor]:
     """Rotate the leading ``2 * len(inv_freq)`` dims of ``query (batch, tokens, heads, head_dim)`` and ``key`` by
     ``positions (batch, tokens)``: pairs ``(i, i + r/2)``, or ``(2i, 2i + 1)`` when ``interleaved``. Angles are formed in 64
     bits; cos and sin, times ``factor``, in fp32; the result is rounded once. bf16, fp16 or fp32."""
-    p = _rotary_desc("rotary_qk", query, key, positions, inv_freq, factor, interleaved)
-    _same_device("rotary_qk", query, key, positions, inv_freq)
-    q_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    k_out = torch.empty(key.shape, dtype=key.dtype, device=key.device)
-    if positions.numel():
-        p.q_out, p.k_out = q_out.data_ptr(), k_out.data_ptr()
-        _launch(_lib.load().dfb_rotary, p, query, "rotary_qk")
+    op = "rotary_qk"
+    rd = _check_rotary(op, query, key, positions, inv_freq)
+    q_rows, k_rows = _rows(op, "query", query), _rows(op, "key", key)
+    device = _same_device(op, query, key, positions, inv_freq)
+    dtype, (batch, tokens, hq, d) = query.dtype, query.shape
+    q_out, k_out = torch.empty(query.shape, dtype=dtype, device=device), torch.empty(key.shape, dtype=dtype, device=device)
+    if batch and tokens:
+        p = _lib.RotaryDesc()
+        _ROTARY.pack_into(
+            p, 0, batch, tokens, hq, key.shape[2], d, rd, interleaved, _DTYPES[dtype], query.data_ptr(), key.data_ptr(), 0, *q_rows, *k_rows, *_NO_ROWS,
+            positions.data_ptr(), positions.stride(0), positions.dtype == torch.int64, inv_freq.data_ptr(), inv_freq.dtype == torch.float64, factor,
+            q_out.data_ptr(), k_out.data_ptr(), 0, 0, *_NO_ROWS, *_NO_ROWS, 0, 0,
+        )  # fmt: skip
+        _launch(_lib.load().dfb_rotary, p, device.index, op)
     return q_out, k_out
 
 
-@rotary_qk.register_fake
+@rotary_qk.op.register_fake
 def _(query, key, positions, inv_freq, factor, interleaved):
     return query.new_empty(query.shape), key.new_empty(key.shape)
 
 
+@_eager
 @torch.library.custom_op("dfb200::rotary_append", mutates_args=("key_cache", "value_cache"))
 def rotary_append(
     query: Tensor, key: Tensor, value: Tensor, positions: Tensor, inv_freq: Tensor, factor: float, interleaved: bool,
@@ -936,39 +973,50 @@ def rotary_append(
     instead of returned: token ``t`` of sequence ``b`` becomes row ``cache_len[b] + t`` (int32, on the device). Rows below 0 or
     from ``max_seq`` on are not written. Returns the rotated query."""
     op = "rotary_append"
-    p = _rotary_desc(op, query, key, positions, inv_freq, factor, interleaved)
-    if value.shape != key.shape or value.dtype != key.dtype:
+    rd = _check_rotary(op, query, key, positions, inv_freq)
+    dtype, (batch, tokens, hq, d) = query.dtype, query.shape
+    if value.shape != key.shape or value.dtype != dtype:
         raise ValueError(f"{op}: value {tuple(value.shape)} {value.dtype} must match key {tuple(key.shape)} {key.dtype}")
-    p.max_seq = _check_cache(op, key.shape[0], key.shape[2], key.shape[3], key.dtype, key_cache, value_cache, cache_len)
-    _last_contiguous(op, value=value)
-    for t in (key_cache, value_cache):
-        if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
-            raise ValueError(f"{op}: the caches are written in place and must not be expanded views")
-    _same_device(op, query, key, value, positions, inv_freq, key_cache, value_cache, cache_len)
-    q_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    if positions.numel():
-        p.v, p.v_stride, p.q_out = value.data_ptr(), _three(value), q_out.data_ptr()
-        p.kcache, p.vcache, p.kc_stride, p.vc_stride = key_cache.data_ptr(), value_cache.data_ptr(), _three(key_cache), _three(value_cache)
-        p.cache_len = cache_len.data_ptr()
-        if p.max_seq:
-            _launch(_lib.load().dfb_rotary, p, query, op)
+    max_seq = _check_cache(op, batch, key.shape[2], d, dtype, key_cache, value_cache, cache_len)
+    q_rows, k_rows, v_rows = _rows(op, "query", query), _rows(op, "key", key), _rows(op, "value", value)
+    kc_rows, vc_rows = _rows(op, "key_cache", key_cache), _rows(op, "value_cache", value_cache)
+    if 0 in kc_rows or 0 in vc_rows:
+        for t in (key_cache, value_cache):
+            if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+                raise ValueError(f"{op}: the caches are written in place and must not be expanded views")
+    device = _same_device(op, query, key, value, positions, inv_freq, key_cache, value_cache, cache_len)
+    if not max_seq:  # a cache without rows
+        return rotary_qk.op._init_fn(query, key, positions, inv_freq, factor, interleaved)[0]
+    q_out = torch.empty(query.shape, dtype=dtype, device=device)
+    if batch and tokens:
+        p = _lib.RotaryDesc()
+        _ROTARY.pack_into(
+            p, 0, batch, tokens, hq, key.shape[2], d, rd, interleaved, _DTYPES[dtype], query.data_ptr(), key.data_ptr(), value.data_ptr(),
+            *q_rows, *k_rows, *v_rows, positions.data_ptr(), positions.stride(0), positions.dtype == torch.int64,
+            inv_freq.data_ptr(), inv_freq.dtype == torch.float64, factor, q_out.data_ptr(), 0,
+            key_cache.data_ptr(), value_cache.data_ptr(), *kc_rows, *vc_rows, cache_len.data_ptr(), max_seq,
+        )  # fmt: skip
+        _launch(_lib.load().dfb_rotary, p, device.index, op)
     return q_out
 
 
-@rotary_append.register_fake
+@rotary_append.op.register_fake
 def _(query, key, value, positions, inv_freq, factor, interleaved, key_cache, value_cache, cache_len):
     return query.new_empty(query.shape)
 
 
-def _check_parents(op: str, parents: Tensor, batch: int, nodes: int) -> None:
+def _check_parents(op: str, parents: Tensor, batch: int, nodes: int) -> int:
+    """Elements between two sequences' parents, 0 for one tree for all."""
     if nodes > MAX_TREE_NODES:
         raise ValueError(f"{op}: a tree has at most {MAX_TREE_NODES} nodes, got {nodes}")
-    if tuple(parents.shape) not in ((batch, nodes), (nodes,)) or parents.dtype != torch.int32:
+    if parents.shape not in ((batch, nodes), (nodes,)) or parents.dtype != torch.int32:
         raise ValueError(f"{op}: parents must be int32 {(batch, nodes)} or {(nodes,)}, got {tuple(parents.shape)} {parents.dtype}")
     if nodes > 1 and parents.stride(-1) != 1:
         raise ValueError(f"{op}: parents of a sequence must be contiguous")
+    return parents.stride(0) if parents.dim() == 2 else 0
 
 
+@_eager
 @torch.library.custom_op("dfb200::tree_attention", mutates_args=())
 def tree_attention(query: Tensor, key_cache: Tensor, value_cache: Tensor, cache_len: Tensor, parents: Tensor, scale: float) -> Tensor:
     """Attention of a tree of up to 64 drafted tokens over an unexpanded KV cache ``(batch, kv_heads, max_seq, head_dim)``.
@@ -981,44 +1029,54 @@ def tree_attention(query: Tensor, key_cache: Tensor, value_cache: Tensor, cache_
     op = "tree_attention"
     if query.dim() != 4:
         raise ValueError(f"{op}: expected query (batch, nodes, heads, head_dim), got {tuple(query.shape)}")
-    batch, nodes, hq, d = query.shape
-    if query.dtype not in (BF16, torch.float16):
-        raise ValueError(f"{op}: query must be bfloat16 or float16, got {query.dtype}")
+    dtype, (batch, nodes, hq, d) = query.dtype, query.shape
+    if dtype is not BF16 and dtype is not torch.float16:
+        raise ValueError(f"{op}: query must be bfloat16 or float16, got {dtype}")
     hkv = key_cache.shape[1] if key_cache.dim() == 4 else 0
     if hkv and hq % hkv:
         raise ValueError(f"{op}: {hq} query heads do not divide into {hkv} KV heads")
     if d not in (32, 64, 128, 256):
         raise ValueError(f"{op}: head dim {d} is not 32, 64, 128 or 256")
-    max_seq = _check_cache(op, batch, hkv, d, query.dtype, key_cache, value_cache, cache_len)
+    max_seq = _check_cache(op, batch, hkv, d, dtype, key_cache, value_cache, cache_len)
     if hkv < 1 or hq < 1 or max_seq < 1:
         raise ValueError(f"{op}: need at least one head and one cache row, got {hq} / {hkv} heads, {max_seq} rows")
-    _check_parents(op, parents, batch, nodes)
-    _last_contiguous(op, query=query)
-    if any(s % 8 for t in (key_cache, value_cache) for s in t.stride()[:3]) or (key_cache.data_ptr() | value_cache.data_ptr()) % 16:
+    tree_stride = _check_parents(op, parents, batch, nodes)
+    q_rows, k_rows, v_rows = _rows(op, "query", query), _rows(op, "key_cache", key_cache), _rows(op, "value_cache", value_cache)
+    kp, vp = key_cache.data_ptr(), value_cache.data_ptr()
+    if (k_rows[0] | k_rows[1] | k_rows[2] | v_rows[0] | v_rows[1] | v_rows[2]) % 8 or (kp | vp) % 16:
         raise ValueError(f"{op}: cache rows must start on 16-byte boundaries")
-    if any(s % 2 for s in query.stride()[:3]) or query.data_ptr() % 4:
+    device = _same_device(op, query, key_cache, value_cache, cache_len, parents)
+    if (q_rows[0] | q_rows[1] | q_rows[2]) % 8 or query.data_ptr() % 16:
         query = query.contiguous()
-    _same_device(op, query, key_cache, value_cache, cache_len, parents)
-    out = torch.empty((batch, nodes, hq, d), dtype=query.dtype, device=query.device)
+        q_rows = query.stride()[:3]
+    out = torch.empty((batch, nodes, hq, d), dtype=dtype, device=device)
     if batch == 0 or nodes == 0:
         return out
     lib = _lib.load()
     nbytes = lib.dfb_tree_attn_scratch_bytes(batch, nodes, hq, hkv, d, max_seq)
     # from the allocator, not kept: calls on two streams, or two captured graphs, never share it
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     a = _lib.TreeAttnDesc()
-    a.batch, a.nodes, a.hq, a.hkv, a.d, a.max_seq, a.is_fp16 = batch, nodes, hq, hkv, d, max_seq, query.dtype == torch.float16
-    a.q, a.kcache, a.vcache = query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr()
-    a.q_stride, a.k_stride, a.v_stride = _three(query), _three(key_cache), _three(value_cache)
-    a.cache_len, a.parents, a.parents_stride = cache_len.data_ptr(), parents.data_ptr(), parents.stride(0) if parents.dim() == 2 else 0
-    a.scale, a.out, a.scratch, a.scratch_bytes = scale, out.data_ptr(), _ptr(scratch), nbytes
-    _launch(lib.dfb_tree_attention, a, query, op)
+    _TREE.pack_into(
+        a, 0, batch, nodes, hq, hkv, d, max_seq, dtype is torch.float16, query.data_ptr(), kp, vp, *q_rows, *k_rows, *v_rows,
+        cache_len.data_ptr(), parents.data_ptr(), tree_stride, scale, out.data_ptr(), scratch.data_ptr() if nbytes else 0, nbytes,
+    )  # fmt: skip
+    _launch(lib.dfb_tree_attention, a, device.index, op)
     return out
 
 
-@tree_attention.register_fake
+@tree_attention.op.register_fake
 def _(query, key_cache, value_cache, cache_len, parents, scale):
     return query.new_empty(query.shape)
+
+
+def _aligned_rows(t: Tensor) -> tuple[Tensor, tuple[int, int, int]]:
+    """`t` with rows on 16-byte boundaries (copied once if need be), and its strides."""
+    s = t.stride()
+    if (s[0] | s[1] | s[2]) % 8 or t.data_ptr() % 16:
+        t = t.contiguous()
+        s = t.stride()
+    return t, s[:3]
 
 
 def _delta_tokens(
@@ -1027,48 +1085,47 @@ def _delta_tokens(
     if state.dim() != 4 or state.dtype != torch.float32:
         raise ValueError(f"{op}: state must be fp32 (batch, heads, key_dim, value_dim), got {tuple(state.shape)} {state.dtype}")
     batch, hv, dk, dv = state.shape
-    if query.dim() != 4 or query.shape != key.shape or query.shape[0] != batch or query.shape[3] != dk:
-        raise ValueError(f"{op}: query and key must be (batch, tokens, key_heads, {dk}), got {tuple(query.shape)} and {tuple(key.shape)}")
-    tokens, hk = query.shape[1], query.shape[2]
+    shape = query.shape
+    if len(shape) != 4 or shape != key.shape or shape[0] != batch or shape[3] != dk:
+        raise ValueError(f"{op}: query and key must be (batch, tokens, key_heads, {dk}), got {tuple(shape)} and {tuple(key.shape)}")
+    tokens, hk = shape[1], shape[2]
     if hk == 0 or hv == 0 or hv % hk:
         raise ValueError(f"{op}: {hv} value heads do not divide into {hk} key heads")
-    if tuple(value.shape) != (batch, tokens, hv, dv):
+    if value.shape != (batch, tokens, hv, dv):
         raise ValueError(f"{op}: value has shape {tuple(value.shape)}, expected {(batch, tokens, hv, dv)}")
     for name, t in (("g", g), ("beta", beta)):
-        if tuple(t.shape) != (batch, tokens, hv) or not t.is_floating_point():
+        if t.shape != (batch, tokens, hv) or not t.is_floating_point():
             raise ValueError(f"{op}: {name} must be a floating tensor {(batch, tokens, hv)}, got {tuple(t.shape)} {t.dtype}")
     for name, t in (("query", query), ("key", key), ("value", value)):
         if t.dtype != BF16:
             raise ValueError(f"{op}: {name} must be bfloat16, got {t.dtype}")
+        _rows(op, name, t)
     if dk % 8 or dv % 8 or dk < 8 or dk > 128 or dv < 8:
         raise ValueError(f"{op}: key dim {dk} (a multiple of 8, at most 128) or value dim {dv} (a multiple of 8) unsupported")
-    if lengths is not None and (tuple(lengths.shape) != (batch,) or lengths.dtype != torch.int32 or not lengths.is_contiguous()):
+    if lengths is not None and (lengths.shape != (batch,) or lengths.dtype != torch.int32 or not lengths.is_contiguous()):
         raise ValueError(f"{op}: lengths must be a contiguous int32 tensor of {batch} entries, got {tuple(lengths.shape)} {lengths.dtype}")
-    if parents is not None:
-        _check_parents(op, parents, batch, tokens)
-    _last_contiguous(op, query=query, key=key, value=value)
-    _same_device(op, state, query, key, value, g, beta, lengths, parents)
-    # rows that do not start on 16-byte boundaries are copied once
-    query, key, value = (t.contiguous() if t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:3]) else t for t in (query, key, value))
+    tree_stride = 0 if parents is None else _check_parents(op, parents, batch, tokens)
+    device = _same_device(op, state, query, key, value, g, beta, lengths, parents)
+    (query, q_rows), (key, k_rows), (value, v_rows) = _aligned_rows(query), _aligned_rows(key), _aligned_rows(value)
     state, g, beta = state.contiguous(), g.float().contiguous(), beta.float().contiguous()
-    out = torch.empty((batch, tokens, hv, dv), dtype=BF16, device=state.device)
+    out = torch.empty((batch, tokens, hv, dv), dtype=BF16, device=device)
     if batch == 0 or tokens == 0:
         return out, None if parents is not None else state.clone()
     new_state = torch.empty_like(state) if parents is None else None
     lib = _lib.load()
     nbytes = lib.dfb_delta_chunk_scratch_bytes(batch, tokens, hk, hv, dk)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=state.device)  # not kept, as in tree_attention
-    d = _lib.DeltaChunkDesc()
-    d.batch, d.tokens, d.hk, d.hv, d.dk, d.dv = batch, tokens, hk, hv, dk, dv
-    d.q, d.k, d.v, d.q_stride, d.k_stride, d.v_stride = query.data_ptr(), key.data_ptr(), value.data_ptr(), _three(query), _three(key), _three(value)
-    d.g, d.beta, d.lengths, d.l2norm = g.data_ptr(), beta.data_ptr(), _ptr(lengths), l2norm
-    if parents is not None:
-        d.parents, d.parents_stride = parents.data_ptr(), parents.stride(0) if parents.dim() == 2 else 0
-    d.state, d.state_out, d.out, d.scratch, d.scratch_bytes = state.data_ptr(), _ptr(new_state), out.data_ptr(), scratch.data_ptr(), nbytes
-    _launch(lib.dfb_delta_chunk, d, state, op)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)  # not kept, as in tree_attention
+    p = _lib.DeltaChunkDesc()
+    _DELTA.pack_into(
+        p, 0, batch, tokens, hk, hv, dk, dv, query.data_ptr(), key.data_ptr(), value.data_ptr(), *q_rows, *k_rows, *v_rows,
+        g.data_ptr(), beta.data_ptr(), 0 if lengths is None else lengths.data_ptr(), 0 if parents is None else parents.data_ptr(), tree_stride, l2norm,
+        state.data_ptr(), 0 if new_state is None else new_state.data_ptr(), out.data_ptr(), scratch.data_ptr(), nbytes,
+    )  # fmt: skip
+    _launch(lib.dfb_delta_chunk, p, device.index, op)
     return out, new_state
 
 
+@_eager
 @torch.library.custom_op("dfb200::delta_rule_chunk", mutates_args=())
 def delta_rule_chunk(
     state: Tensor, query: Tensor, key: Tensor, value: Tensor, g: Tensor, beta: Tensor, lengths: Tensor | None, qk_l2norm: bool
@@ -1084,11 +1141,12 @@ def delta_rule_chunk(
     return _delta_tokens("delta_rule_chunk", state, query, key, value, g, beta, lengths, None, qk_l2norm)
 
 
-@delta_rule_chunk.register_fake
+@delta_rule_chunk.op.register_fake
 def _(state, query, key, value, g, beta, lengths, qk_l2norm):
     return value.new_empty(value.shape), state.new_empty(state.shape)
 
 
+@_eager
 @torch.library.custom_op("dfb200::delta_rule_tree", mutates_args=())
 def delta_rule_tree(state: Tensor, query: Tensor, key: Tensor, value: Tensor, g: Tensor, beta: Tensor, parents: Tensor, qk_l2norm: bool) -> Tensor:
     """The delta rule over a tree of up to 64 drafted tokens: node ``i`` continues from the state that the path from the root
@@ -1098,6 +1156,6 @@ def delta_rule_tree(state: Tensor, query: Tensor, key: Tensor, value: Tensor, g:
     return _delta_tokens("delta_rule_tree", state, query, key, value, g, beta, None, parents, qk_l2norm)[0]
 
 
-@delta_rule_tree.register_fake
+@delta_rule_tree.op.register_fake
 def _(state, query, key, value, g, beta, parents, qk_l2norm):
     return value.new_empty(value.shape)
