@@ -24,6 +24,8 @@
 // warps fill by cp.async one to two chunks ahead. No wait spins.
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -33,7 +35,7 @@ namespace {
 
 constexpr int C = 64;                // tokens per chunk
 constexpr int SQ = C * C * 2;        // bytes of one 64 x 64 fp16 image
-constexpr int SCAL = 4 * C * 4;      // scalars of a (chunk, value head): three per token, then a few
+constexpr int SCAL = 4 * C * 4;      // scalars of a (chunk, value head): three per token, the state's decay, four scales each of T and P
 constexpr int HEAD_BYTES = 3 * SQ + SCAL;
 constexpr float MIN_LOG_DECAY = -150.f;  // e^-150 is 0 in fp32: keeps sums finite when a log decay is -inf
 
@@ -94,27 +96,38 @@ template <int W> __device__ __forceinline__ uint32_t img_off(int row, int chunk)
   return (uint32_t)(row * W * 2 + ((chunk ^ (row & 7)) << 4));
 }
 
-constexpr int PREP_THREADS = 256;
+constexpr int PREP_THREADS = 128;
 constexpr int TS = 68;  // row stride (floats) of the 64 x 64 fp32 matrices: 16-byte rows, neighbouring rows in other banks
 
-// One CTA per (chunk, key head, sequence). Warps 0-3 form K K^T, warps 4-7 Q K^T, 16 rows each, once for all value heads of
-// the key head; then per value head the decays, A, T = (I + A)^-1 diag(beta) by blocks (16 x 16 by substitution, then two
-// doublings: the lower left block of a pair is -T22 A21 T11) and the images.
+// 2^x: one instruction, 2 ulp
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// One CTA per (chunk, value head, sequence); warp w owns rows 16 w .. 16 w + 15 of all 64 x 64 matrices.
+//   1. keys and queries to shared memory (bf16), their norms and fp16 images; log decays summed (in units of log 2)
+//   2. K K^T and Q K^T rows by mma; decays; A to shared memory, P to its image
+//   3. the 16 x 16 diagonal blocks of (I + A)^-1 by substitution, a column per lane
+//   4. the blocks below by block forward substitution, T_ij = -T_ii sum_k A_ik T_kj. Columns of T are independent: warp 1
+//      takes block column 1, warp 2 block column 2, warps 0 and 3 half of block column 0 each (5, 2, 4.5, 4.5 products)
+//   5. T diag(beta) in halves to its images
+// Bound by latency: three to four CTAs share an SM. Scales are per warp (16 rows), so no CTA-wide maximum is needed.
 template <int DKP, bool TREE>
-__global__ void __launch_bounds__(PREP_THREADS) delta_prep_kernel(const DeltaChunkParams p) {
+__global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const DeltaChunkParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
   unsigned char* kt = smem;                                  // bf16 [64][DKP]
   unsigned char* qt = smem + C * DKP * 2;
-  float* A = (float*)(smem + 2 * C * DKP * 2);               // [64][TS]
-  float* T = A + C * TS;
-  float* X = T + C * TS;                                     // [32][TS / 2 ..]: product of two blocks
-  __shared__ float rk[C], rq[C], ghi[C], glo[C], bet[C], sk[C], sq[C];
-  __shared__ float wmax[8];
+  float* A = (float*)(smem + (2 * C * DKP * 2 > C * TS * 4 ? 2 * C * DKP * 2 : C * TS * 4));  // [64][TS]
+  float* T = (float*)smem;                                   // [64][TS], over the tiles once they have been read
+  __shared__ float4 col[C];                                  // per token: log2 decay sum (hi, lo), 1/|k|, beta
+  __shared__ float rq[C], sk[C], sq[C];
   __shared__ unsigned long long anc[C];
   __shared__ int up[C];
   __shared__ double gsum[C];
 
-  const int cl = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+  const int cl = blockIdx.x, hv = blockIdx.y, b = blockIdx.z, group = p.hv / p.hk, hk = hv / group;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, g = lane >> 2, c = lane & 3;
   const int tok0 = (p.chunk0 + cl) * C;
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.tokens) : p.tokens;
@@ -129,7 +142,7 @@ __global__ void __launch_bounds__(PREP_THREADS) delta_prep_kernel(const DeltaChu
       up[t] = node ? pa : -1;
     }
     __syncthreads();
-    for (int step = 1; step < C; step *= 2) {
+    for (int step = 1; step < live; step *= 2) {
       unsigned long long bits = 0;
       int u = -1;
       if (t < C) {
@@ -142,95 +155,41 @@ __global__ void __launch_bounds__(PREP_THREADS) delta_prep_kernel(const DeltaChu
     }
   }
 
-  // ---- the chunk's keys and queries: bf16 tiles for the products, norms, fp16 images for the scan ----
   const long sbase = ((long)b * p.seg_chunks + cl) * (p.hk * (2L * C * DKP * 2) + p.hv * (long)HEAD_BYTES);
   unsigned char* kimg = p.scratch + sbase + (long)hk * (2 * C * DKP * 2);
+  unsigned char* himg = p.scratch + sbase + p.hk * (2L * C * DKP * 2) + (long)hv * HEAD_BYTES;
+  const bool first = hv % group == 0;  // the first value head of a key head writes the key head's images
+
+  // ---- 1 ----
   {
-    // four threads per row: key rows 0 .. 63 by threads 0 .. 255, then query rows
+    constexpr int N = DKP / 64;  // 16-byte chunks per thread and row: eight threads per row, 16 rows per pass
+    const int part = t & 7;
+    uint4 raw[2][4][N];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const int row = t >> 2, part = t & 3;
-      const bf16* src = which ? p.q + b * p.q_stride[0] + (long)(tok0 + row) * p.q_stride[1] + hk * p.q_stride[2]
-                              : p.k + b * p.k_stride[0] + (long)(tok0 + row) * p.k_stride[1] + hk * p.k_stride[2];
-      const bool ok = row < live && (!TREE || anc[row] != 0);
-      constexpr int N = DKP / 8 / 4;  // 16-byte chunks per thread
-      uint4 raw[N];
-      float ss = 0.f, mx = 0.f;
+    for (int which = 0; which < 2; ++which)
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int ch = part + 4 * i;
-        raw[i] = ok && ch * 8 < p.dk ? *(const uint4*)(src + ch * 8) : make_uint4(0, 0, 0, 0);
-        const bf16* e = (const bf16*)&raw[i];
+      for (int pass = 0; pass < 4; ++pass) {
+        const int row = pass * 16 + (t >> 3);
+        const bf16* src = which ? p.q + b * p.q_stride[0] + (long)(tok0 + row) * p.q_stride[1] + hk * p.q_stride[2]
+                                : p.k + b * p.k_stride[0] + (long)(tok0 + row) * p.k_stride[1] + hk * p.k_stride[2];
+        const bool ok = row < live && (!TREE || anc[row] != 0);
 #pragma unroll
-        for (int y = 0; y < 8; ++y) {
-          const float x = bf2f(e[y]);
-          ss = fmaf(x, x, ss);
-          mx = fmaxf(mx, fabsf(x));
+        for (int i = 0; i < N; ++i) {
+          const int ch = part + 8 * i;
+          raw[which][pass][i] = ok && ch * 8 < p.dk ? *(const uint4*)(src + ch * 8) : make_uint4(0, 0, 0, 0);
         }
       }
-      ss += __shfl_xor_sync(0xffffffffu, ss, 1);
-      ss += __shfl_xor_sync(0xffffffffu, ss, 2);
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const int e2 = scale_exp(mx);
-      const float down = pow2(-e2);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int ch = part + 4 * i;
-        const bf16* e = (const bf16*)&raw[i];
-        *(uint4*)((which ? qt : kt) + img_off<DKP>(row, ch)) = raw[i];
-        uint4 im;
-        im.x = h2(bf2f(e[0]) * down, bf2f(e[1]) * down), im.y = h2(bf2f(e[2]) * down, bf2f(e[3]) * down);
-        im.z = h2(bf2f(e[4]) * down, bf2f(e[5]) * down), im.w = h2(bf2f(e[6]) * down, bf2f(e[7]) * down);
-        *(uint4*)(kimg + which * (C * DKP * 2) + img_off<DKP>(row, ch)) = im;
-      }
-      if (part == 0) {
-        float r = p.l2norm ? rsqrt_2step(__fadd_rn(ss, 1e-6f)) : 1.f;
-        if (which && p.l2norm) r = __fdiv_rn(r, sqrtf((float)p.dk));
-        (which ? rq : rk)[row] = r;
-        (which ? sq : sk)[row] = r * pow2(e2);
-      }
-    }
-  }
-  __syncthreads();
-
-  // ---- rows 16 (warp % 4) .. + 15 of K K^T (warps 0-3) or Q K^T (warps 4-7) ----
-  const int r0 = (warp & 3) * 16;
-  float dot[8][4];
-#pragma unroll
-  for (int nt = 0; nt < 8; ++nt) dot[nt][0] = dot[nt][1] = dot[nt][2] = dot[nt][3] = 0.f;
-  {
-    const uint32_t as = smem_u32(warp < 4 ? kt : qt), bs = smem_u32(kt);
-#pragma unroll
-    for (int ks = 0; ks < DKP / 16; ++ks) {
-      uint32_t a[4];
-      ldsm4(as + img_off<DKP>(r0 + (lane & 15), 2 * ks + (lane >> 4)), a);
-#pragma unroll
-      for (int n2 = 0; n2 < 4; ++n2) {
-        if (16 * n2 > r0) continue;  // above the diagonal
-        uint32_t kb[4];
-        ldsm4(bs + img_off<DKP>(16 * n2 + (lane & 7) + 8 * (lane >> 4), 2 * ks + ((lane >> 3) & 1)), kb);
-        mma_bf16(dot[2 * n2], a, kb[0], kb[1]);
-        mma_bf16(dot[2 * n2 + 1], a, kb[2], kb[3]);
-      }
-    }
-  }
-
-  const int group = p.hv / p.hk;
-  for (int r = 0; r < group; ++r) {
-    const int hv = hk * group + r;
-    unsigned char* himg = p.scratch + sbase + p.hk * (2L * C * DKP * 2) + (long)hv * HEAD_BYTES;
-    __syncthreads();  // the previous head's matrices have been read
+    // decays and beta: warps 0 and 1 one token per lane; the sum by warp 0 while the tiles arrive
+    float bv = 0.f;
     if (t < C) {
-      const bool ok = t < live && (!TREE || anc[t] != 0);
-      float gv = 0.f, bv = 0.f;
-      if (ok) {
+      float gv = 0.f;
+      if (t < live && (!TREE || anc[t] != 0)) {
         gv = p.g[((long)b * p.tokens + tok0 + t) * p.hv + hv];
         bv = p.beta[((long)b * p.tokens + tok0 + t) * p.hv + hv];
         gv = gv < MIN_LOG_DECAY ? MIN_LOG_DECAY : gv;
       }
-      bet[t] = bv;
-      gsum[t] = gv;
+      gsum[t] = (double)gv * 1.4426950408889634074;  // log2(e)
+      col[t].w = bv;
     }
     __syncthreads();
     if (!TREE) {
@@ -242,14 +201,9 @@ __global__ void __launch_bounds__(PREP_THREADS) delta_prep_kernel(const DeltaChu
           const double y = __shfl_up_sync(0xffffffffu, s, o);
           if (lane >= o) s += y;
         }
-        gsum[2 * lane] = s - a1;
-        gsum[2 * lane + 1] = s;
-      }
-      __syncthreads();
-      if (t < C) {
-        const double s = gsum[t];
-        ghi[t] = (float)s;
-        glo[t] = (float)(s - (double)(float)s);
+        const double s0 = s - a1;
+        col[2 * lane].x = (float)s0, col[2 * lane].y = (float)(s0 - (double)(float)s0);
+        col[2 * lane + 1].x = (float)s, col[2 * lane + 1].y = (float)(s - (double)(float)s);
       }
     } else if (t < C) {  // along the path
       double s = 0.;
@@ -258,142 +212,235 @@ __global__ void __launch_bounds__(PREP_THREADS) delta_prep_kernel(const DeltaChu
         s += gsum[__ffsll(bits) - 1];
         bits &= bits - 1;
       }
-      ghi[t] = (float)s;
-      glo[t] = (float)(s - (double)(float)s);
+      col[t].x = (float)s, col[t].y = (float)(s - (double)(float)s);
     }
-    __syncthreads();
-    // decayed entries of this warp's rows; A to shared memory, P kept for its scale
-    float pm = 0.f;
-    float pr[8][4];
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+      for (int pass = 0; pass < 4; ++pass) {
+        const int row = pass * 16 + (t >> 3);
+        float ss = 0.f, mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const bf16* e = (const bf16*)&raw[which][pass][i];
+#pragma unroll
+          for (int y = 0; y < 8; ++y) {
+            const float x = bf2f(e[y]);
+            ss = fmaf(x, x, ss);
+            mx = fmaxf(mx, fabsf(x));
+          }
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o *= 2) {
+          ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        }
+        const int e2 = scale_exp(mx);
+        const float down = pow2(-e2);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int ch = part + 8 * i;
+          const bf16* e = (const bf16*)&raw[which][pass][i];
+          *(uint4*)((which ? qt : kt) + img_off<DKP>(row, ch)) = raw[which][pass][i];
+          if (first) {
+            uint4 im;
+            im.x = h2(bf2f(e[0]) * down, bf2f(e[1]) * down), im.y = h2(bf2f(e[2]) * down, bf2f(e[3]) * down);
+            im.z = h2(bf2f(e[4]) * down, bf2f(e[5]) * down), im.w = h2(bf2f(e[6]) * down, bf2f(e[7]) * down);
+            *(uint4*)(kimg + which * (C * DKP * 2) + img_off<DKP>(row, ch)) = im;
+          }
+        }
+        if (part == 0) {
+          float r = p.l2norm ? rsqrt_2step(__fadd_rn(ss, 1e-6f)) : 1.f;
+          if (which && p.l2norm) r = __fdiv_rn(r, sqrtf((float)p.dk));
+          if (which) rq[row] = r;
+          else col[row].z = r;
+          (which ? sq : sk)[row] = r * pow2(e2);
+        }
+      }
+  }
+  __syncthreads();
+
+  // ---- 2 ----
+  const int r0 = warp * 16;
+  {
+    float kk[8][4], qk[8][4];
 #pragma unroll
     for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = r0 + g + 8 * (e >> 1), j = nt * 8 + 2 * c + (e & 1);
-        const bool seen = TREE ? (anc[i] >> j) & 1 : j <= i;
-        float x = 0.f;
-        if (seen && i < live) {
-          const float d = expf((ghi[i] - ghi[j]) + (glo[i] - glo[j]));
-          x = dot[nt][e] * rk[j] * d * (warp < 4 ? rk[i] * bet[i] : rq[i]);
+      for (int e = 0; e < 4; ++e) kk[nt][e] = qk[nt][e] = 0.f;
+    const uint32_t ks_s = smem_u32(kt), qs_s = smem_u32(qt);
+#pragma unroll
+    for (int ks = 0; ks < DKP / 16; ++ks) {
+      uint32_t ka[4], qa[4];
+      ldsm4(ks_s + img_off<DKP>(r0 + (lane & 15), 2 * ks + (lane >> 4)), ka);
+      ldsm4(qs_s + img_off<DKP>(r0 + (lane & 15), 2 * ks + (lane >> 4)), qa);
+#pragma unroll
+      for (int n2 = 0; n2 < 4; ++n2) {
+        if (n2 > warp) continue;  // above the diagonal
+        uint32_t kb[4];
+        ldsm4(ks_s + img_off<DKP>(16 * n2 + (lane & 7) + 8 * (lane >> 4), 2 * ks + ((lane >> 3) & 1)), kb);
+        mma_bf16(kk[2 * n2], ka, kb[0], kb[1]);
+        mma_bf16(kk[2 * n2 + 1], ka, kb[2], kb[3]);
+        mma_bf16(qk[2 * n2], qa, kb[0], kb[1]);
+        mma_bf16(qk[2 * n2 + 1], qa, kb[2], kb[3]);
+      }
+    }
+    float pm = 0.f;
+    float ri[2], qi[2], hi[2], lo[2];
+    unsigned long long bits[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int i = r0 + g + 8 * r;
+      const float4 v = col[i];
+      hi[r] = v.x, lo[r] = v.y, ri[r] = v.z * v.w, qi[r] = rq[i];
+      bits[r] = TREE ? anc[i] : i < live ? (2ull << i) - 1 : 0ull;  // row i sees columns 0 .. i (2 << 63 wraps to 0: all of them)
+    }
+#pragma unroll
+    for (int nt = 0; nt < 8; ++nt) {
+      if (nt > 2 * warp + 1) {  // above the diagonal: kk and qk are zero there
+        continue;
+      }
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int j = nt * 8 + 2 * c + y;
+        const float4 v = col[j];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float d = (bits[r] >> j) & 1 ? v.z * exp2_fast((hi[r] - v.x) + (lo[r] - v.y)) : 0.f;
+          const int e = 2 * r + y;
+          kk[nt][e] = d == 0.f ? 0.f : kk[nt][e] * (ri[r] * d);
+          qk[nt][e] = d == 0.f ? 0.f : qk[nt][e] * (qi[r] * d);
+          pm = fmaxf(pm, fabsf(qk[nt][e]));
         }
-        if (warp < 4)
-          A[i * TS + j] = i == j ? 0.f : x;
-        else
-          pr[nt][e] = x, pm = fmaxf(pm, fabsf(x));
       }
-    pm = warp_max(pm);
-    if (lane == 0) wmax[warp] = pm;
-    __syncthreads();
-    const int ep = scale_exp(fmaxf(fmaxf(wmax[4], wmax[5]), fmaxf(wmax[6], wmax[7])));
-    if (warp >= 4) {
-      const float down = pow2(-ep);
 #pragma unroll
-      for (int nt = 0; nt < 8; ++nt) {
-        *(uint32_t*)(himg + 2 * SQ + img_off<C>(r0 + g, nt) + 4 * c) = h2(pr[nt][0] * down, pr[nt][1] * down);
-        *(uint32_t*)(himg + 2 * SQ + img_off<C>(r0 + g + 8, nt) + 4 * c) = h2(pr[nt][2] * down, pr[nt][3] * down);
-      }
+      for (int r = 0; r < 2; ++r) *(float2*)&A[(r0 + g + 8 * r) * TS + nt * 8 + 2 * c] = make_float2(kk[nt][2 * r], kk[nt][2 * r + 1]);
     }
-    // (I + A)^-1: the four diagonal blocks, a column per lane
-    if (warp < 4) {
-      const int j = lane & 15, base = warp * 16;
-      float x[16];
+    const int ep = scale_exp(warp_max_abs(pm));
+    const float down = pow2(-ep);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float s = 0.f;
-#pragma unroll
-        for (int m = 0; m < i; ++m) s = fmaf(A[(base + i) * TS + base + m], x[m], s);
-        x[i] = (i == j ? 1.f : 0.f) - s;
-      }
-      if (lane < 16) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) T[(base + i) * TS + base + j] = x[i];
-      }
-    } else {  // zeros above the diagonal blocks
-      for (int i = t - 128; i < C * C; i += 128)
-        if ((i & 63) / 16 > (i >> 6) / 16) T[(i >> 6) * TS + (i & 63)] = 0.f;
+    for (int nt = 0; nt < 8; ++nt) {
+      *(uint32_t*)(himg + 2 * SQ + img_off<C>(r0 + g, nt) + 4 * c) = h2(qk[nt][0] * down, qk[nt][1] * down);
+      *(uint32_t*)(himg + 2 * SQ + img_off<C>(r0 + g + 8, nt) + 4 * c) = h2(qk[nt][2] * down, qk[nt][3] * down);
     }
-    __syncthreads();
-    // pairs of 16: X = A21 T11 (two products of 16 x 16), T21 = -T22 X
-    {
-      const int pair = t >> 7, i = (t >> 3) & 15, j = (t & 7) * 2, o = 32 * pair;
-      float x0 = 0.f, x1 = 0.f;
+    if (lane == 0) ((float*)(himg + 3 * SQ))[3 * C + 8 + warp] = pow2(ep);
+  }
+  __syncwarp();
+
+  // ---- 3: column (lane & 15) of this warp's diagonal block, rows in registers ----
+  float x[16];
+  {
+    const int j = lane & 15;
 #pragma unroll
-      for (int m = 0; m < 16; ++m) {
-        const float a = A[(o + 16 + i) * TS + o + m];
-        const float2 y = *(const float2*)&T[(o + m) * TS + o + j];
-        x0 = fmaf(a, y.x, x0), x1 = fmaf(a, y.y, x1);
-      }
-      *(float2*)&X[(pair * 16 + i) * 36 + j] = make_float2(x0, x1);
-      __syncthreads();
-      x0 = x1 = 0.f;
+    for (int i = 0; i < 16; ++i) x[i] = i == j ? 1.f : 0.f;
 #pragma unroll
-      for (int m = 0; m < 16; ++m) {
-        const float a = T[(o + 16 + i) * TS + o + 16 + m];
-        const float2 y = *(const float2*)&X[(pair * 16 + m) * 36 + j];
-        x0 = fmaf(a, y.x, x0), x1 = fmaf(a, y.y, x1);
-      }
-      *(float2*)&T[(o + 16 + i) * TS + o + j] = make_float2(-x0, -x1);
+    for (int i = 1; i < 16; ++i) {
+      float a[16];
+#pragma unroll
+      for (int m = 0; m < i; m += 4) *(float4*)&a[m] = *(const float4*)&A[(r0 + i) * TS + r0 + m];
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int m = 0; m < i; ++m) (m & 1 ? s1 : s0) = fmaf(a[m], x[m], m & 1 ? s1 : s0);
+      x[i] -= s0 + s1;
     }
-    __syncthreads();
-    // the pair of 32
-    {
-      const int i = t >> 3, j = (t & 7) * 4;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int m = 0; m < 32; ++m) {
-        const float a = A[(32 + i) * TS + m];
-        const float4 y = *(const float4*)&T[m * TS + j];
-        x.x = fmaf(a, y.x, x.x), x.y = fmaf(a, y.y, x.y), x.z = fmaf(a, y.z, x.z), x.w = fmaf(a, y.w, x.w);
-      }
-      *(float4*)&X[i * 36 + j] = x;
-      __syncthreads();
-      x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int m = 0; m < 32; ++m) {
-        const float a = T[(32 + i) * TS + 32 + m];
-        const float4 y = *(const float4*)&X[m * 36 + j];
-        x.x = fmaf(a, y.x, x.x), x.y = fmaf(a, y.y, x.y), x.z = fmaf(a, y.z, x.z), x.w = fmaf(a, y.w, x.w);
-      }
-      *(float4*)&T[(32 + i) * TS + j] = make_float4(-x.x, -x.y, -x.z, -x.w);
-    }
-    __syncthreads();
-    // T diag(beta) as hi and lo images
-    float tv[2][8], tm = 0.f;
+  }
+  __syncthreads();  // A is complete, the tiles have been read
+  if (lane < 16) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int i = (t + k * PREP_THREADS) >> 3, j0 = (t & 7) * 8;
+    for (int i = 0; i < 16; ++i) T[(r0 + i) * TS + r0 + lane] = x[i];
+  }
+  // zeros right of the diagonal block
+  for (int i = lane; i < 16 * 4 * (3 - warp); i += 32) {
+    const int r = i & 15, q4 = i >> 4;
+    *(float4*)&T[(r0 + r) * TS + r0 + 16 + 4 * q4] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  __syncthreads();
+
+  // ---- 4 ----
+  // lane -> (column, rows): all 16 columns with two row halves (warps 1, 2), or eight columns with four row quarters
+  auto substitute = [&](auto rows_c, int jb, int column, int part) {
+    constexpr int R = decltype(rows_c)::value;  // rows per lane
+    const int j = 16 * jb + column;
+#pragma unroll 1
+    for (int ib = jb + 1; ib < 4; ++ib) {
+      float s[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) s[r] = 0.f;
+#pragma unroll 1
+      for (int kb = jb; kb < ib; ++kb) {
+        float y[16];
+#pragma unroll
+        for (int m = 0; m < 16; ++m) y[m] = T[(16 * kb + m) * TS + j];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+          for (int m = 0; m < 16; m += 4) {
+            const float4 a = *(const float4*)&A[(16 * ib + part * R + r) * TS + 16 * kb + m];
+            s[r] = fmaf(a.x, y[m], fmaf(a.y, y[m + 1], fmaf(a.z, y[m + 2], fmaf(a.w, y[m + 3], s[r]))));
+          }
+        }
+      }
+      // the block's place in T holds the sum until it is multiplied by -T_ii
+#pragma unroll
+      for (int r = 0; r < R; ++r) T[(16 * ib + part * R + r) * TS + j] = s[r];
+      __syncwarp();
+      float y[16];
+#pragma unroll
+      for (int m = 0; m < 16; ++m) y[m] = T[(16 * ib + m) * TS + j];
+      __syncwarp();
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float z = 0.f;
+#pragma unroll
+        for (int m = 0; m < 16; m += 4) {
+          const float4 a = *(const float4*)&T[(16 * ib + part * R + r) * TS + 16 * ib + m];
+          z = fmaf(a.x, y[m], fmaf(a.y, y[m + 1], fmaf(a.z, y[m + 2], fmaf(a.w, y[m + 3], z))));
+        }
+        T[(16 * ib + part * R + r) * TS + j] = -z;
+      }
+      __syncwarp();
+    }
+  };
+  if (warp == 1 || warp == 2) substitute(std::integral_constant<int, 8>(), warp, lane & 15, lane >> 4);
+  else substitute(std::integral_constant<int, 4>(), 0, (warp ? 8 : 0) + (lane & 7), lane >> 3);
+  __syncthreads();
+
+  // ---- 5: this warp's 16 rows, eight columns per lane and pass ----
+  {
+    float tv[4][8], tm = 0.f;
+    const int j0 = (lane & 7) * 8;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float* src = &T[(r0 + 4 * k + (lane >> 3)) * TS + j0];
+      *(float4*)&tv[k][0] = *(const float4*)src;
+      *(float4*)&tv[k][4] = *(const float4*)(src + 4);
 #pragma unroll
       for (int y = 0; y < 8; ++y) {
-        tv[k][y] = T[i * TS + j0 + y] * bet[j0 + y];
+        tv[k][y] *= col[j0 + y].w;
         tm = fmaxf(tm, fabsf(tv[k][y]));
       }
     }
-    tm = warp_max(tm);
-    if (lane == 0) wmax[warp] = tm;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; ++w) tm = fmaxf(tm, wmax[w]);
-    const int et = scale_exp(tm);
+    const int et = scale_exp(warp_max_abs(tm));
     const float down = pow2(-et);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int i = (t + k * PREP_THREADS) >> 3;
+    for (int k = 0; k < 4; ++k) {
       uint4 hi, lo;
       split2(tv[k][0] * down, tv[k][1] * down, hi.x, lo.x);
       split2(tv[k][2] * down, tv[k][3] * down, hi.y, lo.y);
       split2(tv[k][4] * down, tv[k][5] * down, hi.z, lo.z);
       split2(tv[k][6] * down, tv[k][7] * down, hi.w, lo.w);
-      *(uint4*)(himg + img_off<C>(i, t & 7)) = hi;
-      *(uint4*)(himg + SQ + img_off<C>(i, t & 7)) = lo;
+      *(uint4*)(himg + img_off<C>(r0 + 4 * k + (lane >> 3), lane & 7)) = hi;
+      *(uint4*)(himg + SQ + img_off<C>(r0 + 4 * k + (lane >> 3), lane & 7)) = lo;
     }
     float* sc = (float*)(himg + 3 * SQ);
+    if (lane == 0) sc[3 * C + 4 + warp] = pow2(et);
     if (t < C) {
-      const float eg = expf(ghi[t] + glo[t]);
-      sc[t] = eg * sk[t];                                                                  // on K S
-      sc[C + t] = expf((ghi[C - 1] - ghi[t]) + (glo[C - 1] - glo[t])) * sk[t];             // on V' into the state
-      sc[2 * C + t] = eg * sq[t];                                                          // on Q S
-      if (t == C - 1) sc[3 * C] = eg;                                                      // decay of the state
-      if (t == 0) sc[3 * C + 1] = pow2(et), sc[3 * C + 2] = pow2(ep);
+      const float4 v = col[t], e = col[C - 1];
+      const float eg = exp2_fast(v.x + v.y);
+      sc[t] = eg * sk[t];                                             // on K S
+      sc[C + t] = exp2_fast((e.x - v.x) + (e.y - v.y)) * sk[t];       // on V' into the state
+      sc[2 * C + t] = eg * sq[t];                                     // on Q S
+      if (t == C - 1) sc[3 * C] = eg;                                 // decay of the state
     }
   }
 }
@@ -573,11 +620,13 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
     }
     m = 0.f;
     {
-      const float up = pow2(er) * sc[3 * C + 1];
+      const float up = pow2(er);
 #pragma unroll
-      for (int i = 0; i < 2 * NB; ++i)
+      for (int i = 0; i < 2 * NB; ++i) {
+        const float u = up * sc[3 * C + 4 + i / 2];  // T is scaled per 16 rows
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[i][e] *= up, m = fmaxf(m, fabsf(x[i][e]));
+        for (int e = 0; e < 4; ++e) x[i][e] *= u, m = fmaxf(m, fabsf(x[i][e]));
+      }
     }
     // 4. O^T = (S^T Q^T) diag(e^G) + V'^T P^T
     const int ev = scale_exp(warp_max_abs(m));
@@ -598,11 +647,12 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
           mma_f16(o[2 * n2 + 1], a, pb[2], pb[3]);
         }
       }
-      const float up = pow2(ev) * sc[3 * C + 2];
+      const float vup = pow2(ev);
       __syncwarp();  // the previous chunk's outputs have left the buffer
 #pragma unroll
       for (int n2 = 0; n2 < NB; ++n2) {
         uint32_t w[4];
+        const float up = vup * sc[3 * C + 8 + n2];  // as is P
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int nt = 2 * n2 + h;
@@ -696,7 +746,7 @@ int segment_chunks(int batch, int tokens, int hk, int hv, int dk) {
   return (chunks + parts - 1) / parts;
 }
 
-template <int DKP> constexpr int prep_smem() { return 2 * C * DKP * 2 + 2 * C * TS * 4 + 32 * 36 * 4; }
+template <int DKP> constexpr int prep_smem() { return (2 * C * DKP * 2 > C * TS * 4 ? 2 * C * DKP * 2 : C * TS * 4) + C * TS * 4; }
 
 // Blocks of 16 tokens that a chunk computes: all four, or fewer where the whole call has no more tokens (a draft).
 int token_blocks(int tokens) { return tokens <= 16 ? 1 : tokens <= 32 ? 2 : 4; }
@@ -739,7 +789,7 @@ struct LaunchSegment {
   cudaStream_t stream;
   template <int DKP, int NW, int NB, bool TREE>
   int operator()() const {
-    delta_prep_kernel<DKP, TREE><<<dim3(p.chunks, p.hk, p.batch), PREP_THREADS, prep_smem<DKP>(), stream>>>(p);
+    delta_prep_kernel<DKP, TREE><<<dim3(p.chunks, p.hv, p.batch), PREP_THREADS, prep_smem<DKP>(), stream>>>(p);
     const int rc = check_launch("delta rule preparation");
     if (rc) return rc;
     delta_scan_kernel<DKP, NW, NB, TREE>
