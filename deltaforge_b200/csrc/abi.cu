@@ -407,12 +407,15 @@ int dfb_rotary(const dfb_rotary_desc* d, void* stream) {
   return launch_rotary(p, (cudaStream_t)stream);
 }
 
-size_t dfb_tree_attn_scratch_bytes(int batch, int nodes, int hq, int hkv, int d, int max_seq) {
-  if (batch < 1 || nodes < 1 || hkv < 1 || hq < hkv || max_seq < 1) return 0;
-  const TreePlan plan = tree_plan(batch, nodes, hq, hkv, max_seq);
+static size_t tree_scratch(const TreePlan& plan, int batch, int nodes, int hq, int d) {
   if (plan.splits <= 1) return 0;
   const size_t rows = (size_t)batch * hq * nodes * plan.splits;
   return align_up(rows * d * 4, 256) + align_up(rows * 2 * 4, 256);
+}
+
+size_t dfb_tree_attn_scratch_bytes(int batch, int nodes, int hq, int hkv, int d, int max_seq) {
+  if (batch < 1 || nodes < 1 || hkv < 1 || hq < hkv || max_seq < 1) return 0;
+  return tree_scratch(tree_plan(batch, nodes, hq, hkv, max_seq), batch, nodes, hq, d);
 }
 
 int dfb_tree_attention(const dfb_tree_attn_desc* d, void* stream) {
@@ -427,9 +430,9 @@ int dfb_tree_attention(const dfb_tree_attn_desc* d, void* stream) {
   if (!aligned16(d->kcache) || !aligned16(d->vcache) || !multiples(d->k_stride, 8) || !multiples(d->v_stride, 8))
     return bad("dfb_tree_attention: cache rows must start on 16-byte boundaries");
   if (((uintptr_t)d->q & 3) || !multiples(d->q_stride, 2)) return bad("dfb_tree_attention: query rows must start on 4-byte boundaries");
-  const size_t need = dfb_tree_attn_scratch_bytes(d->batch, d->nodes, d->hq, d->hkv, d->d, d->max_seq);
-  if (need && (!d->scratch || d->scratch_bytes < need || !aligned16(d->scratch))) return bad("dfb_tree_attention: aligned scratch of %zu bytes required", need);
   const TreePlan plan = tree_plan(d->batch, d->nodes, d->hq, d->hkv, d->max_seq);
+  const size_t need = tree_scratch(plan, d->batch, d->nodes, d->hq, d->d);
+  if (need && (!d->scratch || d->scratch_bytes < need || !aligned16(d->scratch))) return bad("dfb_tree_attention: aligned scratch of %zu bytes required", need);
   TreeAttnParams p = {};
   p.batch = d->batch;
   p.nodes = d->nodes;

@@ -731,6 +731,96 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
     }
 }
 
+// ---- a few tokens, one by one ---------------------------------------------------------------------------------------
+
+// One or a few tokens per sequence: the recurrence itself in fp32, bound by reading and writing the state once. A CTA owns 32
+// value columns of a head: lane = column, each of the eight warps holds 16 key rows of them in registers from the first
+// token to the last; the two sums over the key rows go through shared memory.
+constexpr int FEW = 4;  // most tokens (what the chunked form needs for one chunk is reached at about that many)
+constexpr int FEW_THREADS = 256, FEW_ROWS = 16;
+
+__global__ void __launch_bounds__(FEW_THREADS) delta_few_kernel(const DeltaChunkParams p) {
+  __shared__ float qn[FEW][128], kn[FEW][128], gate[FEW][2];
+  __shared__ float red[2][8][32];
+  const int vb = blockIdx.x, hv = blockIdx.y, b = blockIdx.z, hk = hv / (p.hv / p.hk);
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, col = vb * 32 + lane;
+  const bool cok = col < p.dv;
+  const long sb = ((long)b * p.hv + hv) * p.dk * p.dv;
+  float s[FEW_ROWS];
+#pragma unroll
+  for (int i = 0; i < FEW_ROWS; ++i) {
+    const int k = warp * FEW_ROWS + i;
+    s[i] = cok && k < p.dk ? p.state[sb + (long)k * p.dv + col] : 0.f;
+  }
+  const int len = p.lengths ? min(max(p.lengths[b], 0), p.tokens) : p.tokens;
+  // queries by warps 0 .. 3, keys by warps 4 .. 7, a token each
+  const int tok = warp & 3, is_k = warp >> 2;
+  if (tok < len) {
+    const bf16* src = is_k ? p.k + b * p.k_stride[0] + tok * p.k_stride[1] + hk * p.k_stride[2] : p.q + b * p.q_stride[0] + tok * p.q_stride[1] + hk * p.q_stride[2];
+    float x[4], ss = 0.f;
+    uint2 raw = make_uint2(0u, 0u);
+    if (4 * lane < p.dk) raw = *(const uint2*)(src + 4 * lane);
+    const bf16* e = (const bf16*)&raw;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = bf2f(e[i]), ss = fmaf(x[i], x[i], ss);
+    float r = 1.f;
+    if (p.l2norm) {
+      r = rsqrt_2step(__fadd_rn(warp_sum(ss), 1e-6f));
+      if (!is_k) r = __fdiv_rn(r, sqrtf((float)p.dk));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) (is_k ? kn : qn)[tok][4 * lane + i] = x[i] * r;
+    if (is_k && lane == 0) {
+      gate[tok][0] = expf(p.g[((long)b * p.tokens + tok) * p.hv + hv]);
+      gate[tok][1] = p.beta[((long)b * p.tokens + tok) * p.hv + hv];
+    }
+  }
+  float v[FEW];
+#pragma unroll
+  for (int n = 0; n < FEW; ++n) v[n] = cok && n < len ? bf2f(p.v[b * p.v_stride[0] + n * p.v_stride[1] + hv * p.v_stride[2] + col]) : 0.f;
+  __syncthreads();
+#pragma unroll 1
+  for (int n = 0; n < len; ++n) {
+    const float decay = gate[n][0];
+    float r = 0.f;
+#pragma unroll
+    for (int i = 0; i < FEW_ROWS; ++i) {
+      s[i] *= decay;
+      r = fmaf(s[i], kn[n][warp * FEW_ROWS + i], r);
+    }
+    red[0][warp][lane] = r;
+    __syncthreads();
+    r = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) r += red[0][w][lane];
+    float vn = v[0];
+#pragma unroll
+    for (int i = 1; i < FEW; ++i) vn = n == i ? v[i] : vn;
+    const float d = (vn - r) * gate[n][1];
+    float o = 0.f;
+#pragma unroll
+    for (int i = 0; i < FEW_ROWS; ++i) {
+      s[i] = fmaf(kn[n][warp * FEW_ROWS + i], d, s[i]);
+      o = fmaf(s[i], qn[n][warp * FEW_ROWS + i], o);
+    }
+    red[1][warp][lane] = o;
+    __syncthreads();
+    if (warp == 0 && cok) {
+      o = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) o += red[1][w][lane];
+      p.out[(((long)b * p.tokens + n) * p.hv + hv) * p.dv + col] = f2bf(o);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < FEW_ROWS; ++i) {
+    const int k = warp * FEW_ROWS + i;
+    if (cok && k < p.dk) p.state_out[sb + (long)k * p.dv + col] = s[i];
+  }
+  for (int n = len + warp; n < p.tokens; n += 8)
+    if (cok) p.out[(((long)b * p.tokens + n) * p.hv + hv) * p.dv + col] = f2bf(0.f);
+}
+
 int pad_dk(int dk) { return dk <= 64 ? 64 : 128; }
 size_t chunk_bytes(int hk, int hv, int dk) { return (size_t)hk * 2 * C * pad_dk(dk) * 2 + (size_t)hv * HEAD_BYTES; }
 
@@ -800,7 +890,7 @@ struct LaunchSegment {
 
 }  // namespace
 
-size_t delta_chunk_scratch_bytes(int batch, int tokens, int hk, int hv, int dk) {
+size_t delta_chunk_scratch_bytes(int batch, int tokens, int hk, int hv, int dk) {  // (what a tree of `tokens` nodes needs too)
   return chunk_bytes(hk, hv, dk) * batch * segment_chunks(batch, tokens, hk, hv, dk);
 }
 
@@ -810,6 +900,10 @@ int launch_delta_chunk(const DeltaChunkParams& args, cudaStream_t stream) {
   if (rc) return rc;
   DeltaChunkParams p = args;
   const bool tree = p.parents != nullptr;
+  if (!tree && p.tokens <= FEW) {
+    delta_few_kernel<<<dim3((p.dv + 31) / 32, p.hv, p.batch), FEW_THREADS, 0, stream>>>(p);
+    return check_launch("delta rule, few tokens");
+  }
   const int chunks = (p.tokens + C - 1) / C;
   p.seg_chunks = segment_chunks(p.batch, p.tokens, p.hk, p.hv, p.dk);
   // Columns per CTA: few (32) while that is what it takes to put every SM to work, else as many as share the loads.

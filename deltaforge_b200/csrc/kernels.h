@@ -321,7 +321,9 @@ struct RotaryParams {
   long kc_stride[3], vc_stride[3];
   const int* cache_len;  // [batch]: token t of sequence b goes to row cache_len[b] + t
   int max_seq;
-  int lanes_per_head;  // set by the launcher
+  // set by the launcher: vectors per head that turn and that pass through, and multipliers that divide by them
+  int turn_units, pass_units;
+  unsigned long long turn_mul, pass_mul, value_mul;
 };
 int launch_rotary(const RotaryParams& p, cudaStream_t stream);
 

@@ -9,8 +9,8 @@
 // turns in fp64 (position * inv_freq / 2 pi), its whole turns are dropped there, and only the fraction is rounded to fp32 for
 // sincospif. That is r/2 fp64 products per token, shared by all its heads.
 //
-// Bound: HBM. Each input element is read once and each output element written once, in 16-byte vectors; one CTA owns a
-// token, a group of lanes a head, and every lane issues the loads of UNROLL heads before the first use.
+// Bound: HBM. Each input element is read once and each output element written once, in 16-byte vectors; a CTA owns a
+// token, and its threads have up to five vectors each under way while the angles are computed.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -31,89 +31,118 @@ template <> __device__ __forceinline__ float from_f(float v) { return v; }
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Vec { T e[V]; };
 
-// V elements per access: 16 bytes where every address allows it, else single elements. A "unit" of a head is what one
-// lane moves at a time: a rotated vector (half layout: the vector and its partner r/2 further on), or a vector beyond r.
+__device__ __forceinline__ int fast_div(int x, unsigned long long mul) { return (int)(((unsigned long long)(unsigned)x * mul) >> 32); }
+
+// V elements per access: 16 bytes where every address allows it, else single elements. One CTA per token. Its work is two
+// lists: vectors that turn (half layout: a vector and its partner r/2 further on) of the query and key heads, and vectors that
+// pass through (dims from r on of those heads, and the value heads of the appending form as a whole).
 template <typename T, int V, bool INTERLEAVED>
 __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const RotaryParams p) {
   __shared__ float2 cs[MAX_ROTARY_DIM / 2];
   using Pack = Vec<T, V>;
+  constexpr int COPIES = 3, TURNS = INTERLEAVED ? 2 : 1;  // under way per thread before the first use
+  constexpr bool PAIRS = !INTERLEAVED || V == 1;          // a unit is two vectors
   const int tok = blockIdx.x % p.tokens, b = blockIdx.x / p.tokens, t = threadIdx.x;
   const int half = p.rotary_dim / 2;
-  const long pi = (long)b * p.pos_stride + tok;
-  const double position = p.pos_is_i64 ? (double)((const int64_t*)p.pos)[pi] : (double)((const int*)p.pos)[pi];
-  for (int i = t; i < half; i += ROT_THREADS) {
-    const double f = p.freq_is_f64 ? ((const double*)p.inv_freq)[i] : (double)((const float*)p.inv_freq)[i];
-    const double turns = position * (f * 0.15915494309189533577);  // 1 / (2 pi)
-    float s, c;
-    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-    cs[i] = make_float2(c * p.factor, s * p.factor);
-  }
-  __syncthreads();
-
-  const int rot_units = INTERLEAVED ? p.rotary_dim / (V == 1 ? 2 : V) : half / V;
-  const int units = rot_units + (p.d - p.rotary_dim) / V;
-  const int lph = p.lanes_per_head, u0 = t % lph, slots = ROT_THREADS / lph;
   const bool append = p.kcache != nullptr;
-  long row = 0;
   bool row_ok = true;
+  long row = 0;
   if (append) {
     row = (long)p.cache_len[b] + tok;
-    row_ok = row >= 0 && row < p.max_seq;
+    row_ok = row >= 0 && row < p.max_seq;  // a row the cache does not have is not written
   }
-  const int heads = p.hq + p.hkv;
-#pragma unroll 2
-  for (int h = t / lph; h < heads; h += slots) {
-    const bool is_q = h < p.hq;
-    const int hk = h - p.hq;
-    const T* in = is_q ? (const T*)p.q + b * p.q_stride[0] + tok * p.q_stride[1] + h * p.q_stride[2]
-                       : (const T*)p.k + b * p.k_stride[0] + tok * p.k_stride[1] + hk * p.k_stride[2];
-    T* out;
-    if (is_q)
-      out = (T*)p.q_out + (((long)b * p.tokens + tok) * p.hq + h) * p.d;
-    else if (append)
-      out = (T*)p.kcache + b * p.kc_stride[0] + hk * p.kc_stride[1] + row * p.kc_stride[2];
-    else
-      out = (T*)p.k_out + (((long)b * p.tokens + tok) * p.hkv + hk) * p.d;
-    if (!is_q && !row_ok) continue;  // a row the cache does not have is not written
-    for (int u = u0; u < units; u += lph) {
-      if (u >= rot_units) {
-        const int at = p.rotary_dim + (u - rot_units) * V;
-        *(Pack*)(out + at) = *(const Pack*)(in + at);
-      } else if (INTERLEAVED && V == 1) {  // one pair, element by element
-        const float x = to_f<T>(in[2 * u]), y = to_f<T>(in[2 * u + 1]);
-        const float2 w = cs[u];
-        out[2 * u] = from_f<T>(x * w.x - y * w.y);
-        out[2 * u + 1] = from_f<T>(y * w.x + x * w.y);
-      } else if (INTERLEAVED) {
-        Pack v = *(const Pack*)(in + u * V);
-#pragma unroll
-        for (int e = 0; e + 1 < V; e += 2) {
-          const float x = to_f<T>(v.e[e]), y = to_f<T>(v.e[e + 1]);
-          const float2 w = cs[(u * V + e) / 2];
-          v.e[e] = from_f<T>(x * w.x - y * w.y);
-          v.e[e + 1] = from_f<T>(y * w.x + x * w.y);
-        }
-        *(Pack*)(out + u * V) = v;
-      } else {
-        Pack v = *(const Pack*)(in + u * V), z = *(const Pack*)(in + half + u * V);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float x = to_f<T>(v.e[e]), y = to_f<T>(z.e[e]);
-          const float2 w = cs[u * V + e];
-          v.e[e] = from_f<T>(x * w.x - y * w.y);
-          z.e[e] = from_f<T>(y * w.x + x * w.y);
-        }
-        *(Pack*)(out + u * V) = v;
-        *(Pack*)(out + half + u * V) = z;
-      }
+  const T *q = (const T*)p.q + b * p.q_stride[0] + tok * p.q_stride[1], *k = (const T*)p.k + b * p.k_stride[0] + tok * p.k_stride[1];
+  const long bt = (long)b * p.tokens + tok;
+  T *qo = (T*)p.q_out + bt * p.hq * p.d, *ko = append ? (T*)p.kcache + b * p.kc_stride[0] + row * p.kc_stride[2] : (T*)p.k_out + bt * p.hkv * p.d;
+  const long ko_stride = append ? p.kc_stride[1] : p.d;
+  const T* v = append ? (const T*)p.v + b * p.v_stride[0] + tok * p.v_stride[1] : nullptr;
+  T* vo = append ? (T*)p.vcache + b * p.vc_stride[0] + row * p.vc_stride[2] : nullptr;
+  const int heads = row_ok ? p.hq + p.hkv : p.hq;
+  const int n_turn = heads * p.turn_units, n_pass = heads * p.pass_units, n_copy = n_pass + (append && row_ok ? p.hkv * (p.d / V) : 0);
+
+  // places of copy i and of turn i
+  auto copy_at = [&](int i, const T*& from, T*& to) {
+    if (i < n_pass) {
+      const int h = fast_div(i, p.pass_mul), at = p.rotary_dim + (i - h * p.pass_units) * V;
+      if (h < p.hq) from = q + h * p.q_stride[2] + at, to = qo + h * p.d + at;
+      else from = k + (h - p.hq) * p.k_stride[2] + at, to = ko + (h - p.hq) * ko_stride + at;
+    } else {
+      const int h = fast_div(i - n_pass, p.value_mul), at = (i - n_pass - h * (p.d / V)) * V;
+      from = v + h * p.v_stride[2] + at, to = vo + h * p.vc_stride[1] + at;
     }
-  }
-  if (!append || !row_ok) return;
-  const int vvec = p.d / V;
-  for (int i = t; i < p.hkv * vvec; i += ROT_THREADS) {
-    const int h = i / vvec, at = (i - h * vvec) * V;
-    *(Pack*)((T*)p.vcache + b * p.vc_stride[0] + h * p.vc_stride[1] + row * p.vc_stride[2] + at) =
-        *(const Pack*)((const T*)p.v + b * p.v_stride[0] + tok * p.v_stride[1] + h * p.v_stride[2] + at);
+  };
+  auto turn_at = [&](int i, const T*& from, T*& to, int& u) {
+    const int h = fast_div(i, p.turn_mul);
+    u = i - h * p.turn_units;
+    const int at = INTERLEAVED && V == 1 ? 2 * u : u * V;
+    if (h < p.hq) from = q + h * p.q_stride[2] + at, to = qo + h * p.d + at;
+    else from = k + (h - p.hq) * p.k_stride[2] + at, to = ko + (h - p.hq) * ko_stride + at;
+  };
+  const int second = INTERLEAVED ? 1 : half;  // from the first vector of a pair to the second
+
+  bool angles = false;
+  for (int c0 = t, r0 = t; c0 < n_copy || r0 < n_turn || !angles; c0 += COPIES * ROT_THREADS, r0 += TURNS * ROT_THREADS) {
+    Pack cv[COPIES], x[TURNS], y[TURNS];
+    const T* from;
+    T* to;
+    int u;
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i)
+      if (c0 + i * ROT_THREADS < n_copy) {
+        copy_at(c0 + i * ROT_THREADS, from, to);
+        cv[i] = *(const Pack*)from;
+      }
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i)
+      if (r0 + i * ROT_THREADS < n_turn) {
+        turn_at(r0 + i * ROT_THREADS, from, to, u);
+        x[i] = *(const Pack*)from;
+        if (PAIRS) y[i] = *(const Pack*)(from + second);
+      }
+    if (!angles) {  // while the first loads are on their way
+      const long pi = (long)b * p.pos_stride + tok;
+      const double position = p.pos_is_i64 ? (double)((const int64_t*)p.pos)[pi] : (double)((const int*)p.pos)[pi];
+      for (int i = t; i < half; i += ROT_THREADS) {
+        const double f = p.freq_is_f64 ? ((const double*)p.inv_freq)[i] : (double)((const float*)p.inv_freq)[i];
+        const double turns = position * (f * 0.15915494309189533577);  // 1 / (2 pi)
+        float sn, cn;
+        sincospif(2.f * (float)(turns - rint(turns)), &sn, &cn);
+        cs[i] = make_float2(cn * p.factor, sn * p.factor);
+      }
+      __syncthreads();
+      angles = true;
+    }
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i)
+      if (c0 + i * ROT_THREADS < n_copy) {
+        copy_at(c0 + i * ROT_THREADS, from, to);
+        *(Pack*)to = cv[i];
+      }
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i)
+      if (r0 + i * ROT_THREADS < n_turn) {
+        turn_at(r0 + i * ROT_THREADS, from, to, u);
+        if (PAIRS) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float a = to_f<T>(x[i].e[e]), z = to_f<T>(y[i].e[e]);
+            const float2 w = cs[u * V + e];
+            x[i].e[e] = from_f<T>(a * w.x - z * w.y);
+            y[i].e[e] = from_f<T>(z * w.x + a * w.y);
+          }
+          *(Pack*)to = x[i];
+          *(Pack*)(to + second) = y[i];
+        } else {
+#pragma unroll
+          for (int e = 0; e + 1 < V; e += 2) {
+            const float a = to_f<T>(x[i].e[e]), z = to_f<T>(x[i].e[e + 1]);
+            const float2 w = cs[(u * V + e) / 2];
+            x[i].e[e] = from_f<T>(a * w.x - z * w.y);
+            x[i].e[e + 1] = from_f<T>(z * w.x + a * w.y);
+          }
+          *(Pack*)to = x[i];
+        }
+      }
   }
 }
 
@@ -128,9 +157,12 @@ int launch_rotary_t(RotaryParams p, cudaStream_t stream) {
                    whole(p.k, p.k_stride) && whole(p.v, p.v_stride) && whole(p.kcache, p.kc_stride) && whole(p.vcache, p.vc_stride) &&
                    whole(p.q_out, none) && whole(p.k_out, none);
   const int v = vec ? V : 1;
-  const int units = (p.interleaved ? p.rotary_dim / (v == 1 ? 2 : v) : p.rotary_dim / 2 / v) + (p.d - p.rotary_dim) / v;
-  p.lanes_per_head = 1;
-  while (p.lanes_per_head < units && p.lanes_per_head < 32) p.lanes_per_head *= 2;
+  p.turn_units = p.interleaved ? p.rotary_dim / (v == 1 ? 2 : v) : p.rotary_dim / 2 / v;
+  p.pass_units = (p.d - p.rotary_dim) / v;
+  auto mul = [](int n) { return n > 0 ? ((1ull << 32) + n - 1) / n : 0ull; };  // x / n = x * mul >> 32 for x below 2^32 / n
+  p.turn_mul = mul(p.turn_units);
+  p.pass_mul = mul(p.pass_units);
+  p.value_mul = mul(p.d / v);
   const dim3 grid((unsigned)((long)p.batch * p.tokens)), block(ROT_THREADS);
   if (vec && p.interleaved) rotary_kernel<T, V, true><<<grid, block, 0, stream>>>(p);
   else if (vec) rotary_kernel<T, V, false><<<grid, block, 0, stream>>>(p);

@@ -78,9 +78,6 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
 template <typename T> __device__ __forceinline__ float elem_f(T v);
 template <> __device__ __forceinline__ float elem_f(bf16 v) { return __bfloat162float(v); }
 template <> __device__ __forceinline__ float elem_f(__half v) { return __half2float(v); }
-template <typename T> __device__ __forceinline__ T elem_t(float v);
-template <> __device__ __forceinline__ bf16 elem_t(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half elem_t(float v) { return __float2half_rn(v); }
 template <typename T> __device__ __forceinline__ uint16_t exp_mask() { return 0x7f80; }  // all ones: infinity or NaN
 template <> __device__ __forceinline__ uint16_t exp_mask<__half>() { return 0x7c00; }
 
@@ -124,6 +121,8 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_attention_kernel(const Tre
   const int hk = blockIdx.y / row_tiles, rt = blockIdx.y % row_tiles;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, g = lane >> 2, c = lane & 3;
   const int group = warp / MT, gt = t - group * MT * 32;  // group of warps, thread within it
+
+  pdl_launch_dependents();  // the merge may set itself up; it waits for this grid's end before it reads
 
   // ---- which rows of the cache this CTA scans ----
   const int cached = min(max(p.cache_len[b], 0), p.max_seq);
@@ -426,62 +425,57 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_attention_kernel(const Tre
       if (d2 == 0) *(float2*)(p.part_ml + (pbase + gr) * 2) = make_float2(m, l);
     }
   }
-  if (p.splits > 1) pdl_launch_dependents();
 }
 
-// One warp per output row: the splits' partial results in split order.
+// One CTA per output row: D / 4 lanes of four dims each, times as many groups as 256 threads hold; group i adds splits i, i +
+// GROUPS, .. in order, then the groups' sums are added in order. All loads of a thread are independent of one another.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) tree_merge_kernel(const TreeAttnParams p) {
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const long r = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (r >= (long)p.batch * p.hkv * p.rows) return;
+__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttnParams p) {
+  constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+  __shared__ float4 part[GROUPS][LANES];
+  __shared__ float part_l[GROUPS], top[8];
+  const int t = threadIdx.x, li = t % LANES, gi = t / LANES;
+  const long r = blockIdx.x;
   const int row = (int)(r % p.rows);
   const long bh = r / p.rows;
   const int hk = (int)(bh % p.hkv), b = (int)(bh / p.hkv), node = row / p.group;
   const int pa = p.parents[(long)b * p.parents_stride + node];
   const bool ok = pa >= -1 && pa < node;
-  const float* ml = p.part_ml + (bh * p.splits * p.rows + row) * 2;
-  const float* acc = p.part_acc + (bh * p.splits * p.rows + row) * D;
-  float m = -INFINITY;
-  for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, __ldcg(ml + (long)s * p.rows * 2));
+  pdl_wait();
+  const float2* ml = (const float2*)p.part_ml + bh * p.splits * p.rows + row;
+  const float* acc = p.part_acc + (bh * p.splits * p.rows + row) * D + 4 * li;
+  float m = t < p.splits ? __ldcg(ml + (long)t * p.rows).x : -INFINITY;  // at most 128 splits
   m = warp_max(m);
-  const float ref = m == -INFINITY ? 0.f : m;
-  constexpr int E = D / 32;
-  float a[E], l = 0.f;
+  if ((t & 31) == 0) top[t >> 5] = m;
+  __syncthreads();
 #pragma unroll
-  for (int e = 0; e < E; ++e) a[e] = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 v = __ldcg((const float2*)(ml + (long)s * p.rows * 2));
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, top[w]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 8
+  for (int s = gi; s < p.splits; s += GROUPS) {
+    const float2 v = __ldcg(ml + (long)s * p.rows);
+    const float4 y = __ldcg((const float4*)(acc + (long)s * p.rows * D));
     const float w = exp2_fast(v.x - ref);
     l = fmaf(v.y, w, l);
-    const float* x = acc + (long)s * p.rows * D;
-    if constexpr (E >= 4) {
+    a.x = fmaf(y.x, w, a.x), a.y = fmaf(y.y, w, a.y), a.z = fmaf(y.z, w, a.z), a.w = fmaf(y.w, w, a.w);
+  }
+  part[gi][li] = a;
+  if (li == 0) part_l[gi] = l;
+  __syncthreads();
+  if (gi) return;
 #pragma unroll
-      for (int e = 0; e < E; e += 4) {
-        const float4 y = __ldcg((const float4*)(x + e * 32 + lane * 4));
-        a[e] = fmaf(y.x, w, a[e]), a[e + 1] = fmaf(y.y, w, a[e + 1]);
-        a[e + 2] = fmaf(y.z, w, a[e + 2]), a[e + 3] = fmaf(y.w, w, a[e + 3]);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) a[e] = fmaf(__ldcg(x + e * 32 + lane), w, a[e]);
-    }
+  for (int i = 1; i < GROUPS; ++i) {
+    const float4 y = part[i][li];
+    a.x += y.x, a.y += y.y, a.z += y.z, a.w += y.w;
+    l += part_l[i];
   }
   const float inv = 1.f / l;
-  T* out = (T*)p.out + (((long)b * p.nodes + node) * p.hq + hk * p.group + row % p.group) * D;
-  if constexpr (E >= 4) {
-#pragma unroll
-    for (int e = 0; e < E; e += 4) {
-      uint2 v = make_uint2(pack2<T>(a[e] * inv, a[e + 1] * inv), pack2<T>(a[e + 2] * inv, a[e + 3] * inv));
-      if (!ok) v = make_uint2(0u, 0u);
-      *(uint2*)(out + e * 32 + lane * 4) = v;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) out[e * 32 + lane] = ok ? elem_t<T>(a[e] * inv) : elem_t<T>(0.f);
-  }
+  T* out = (T*)p.out + (((long)b * p.nodes + node) * p.hq + hk * p.group + row % p.group) * D + 4 * li;
+  uint2 v = make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
+  if (!ok) v = make_uint2(0u, 0u);
+  *(uint2*)out = v;
 }
 
 template <typename T, int D, int MT>
@@ -520,7 +514,7 @@ int launch_d(const TreeAttnParams& p, cudaStream_t stream) {
   int rc = check_launch("tree attention");
   if (rc || p.splits == 1) return rc;
   const long rows = (long)p.batch * p.hkv * p.rows;
-  if (launch_pdl(tree_merge_kernel<T, D>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, p) != cudaSuccess)
+  if (launch_pdl(tree_merge_kernel<T, D>, dim3((unsigned)rows), dim3(256), 0, stream, p) != cudaSuccess)
     return check_launch("tree attention: merge");
   return check_launch("tree attention: merge");
 }

@@ -810,6 +810,16 @@ _DTYPES = {BF16: 0, torch.float16: 1, torch.float32: 2}
 _ROTARY, _TREE, _DELTA = (_lib.packer(d) for d in (_lib.RotaryDesc, _lib.TreeAttnDesc, _lib.DeltaChunkDesc))
 
 
+_dispatch_modes, _transforms = torch._C._len_torch_dispatch_stack, torch._C._functorch.peek_interpreter_stack
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+@functools.cache
+def _scratch_bytes(query: str, *sizes: int) -> int:
+    """What a scratch-size query of the library says; it depends on the sizes alone."""
+    return getattr(_lib.load(), query)(*sizes)
+
+
 def _eager(op):
     """The function of a custom op, called directly where the dispatcher has nothing to add: plain tensors, no tracing or
     dispatch mode, no gradient asked for. The dispatcher's 20 us are more than the smallest of these calls takes. Everything
@@ -820,11 +830,14 @@ def _eager(op):
 
     @functools.wraps(run)
     def call(*args, **kwargs):
-        if kwargs or torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() or torch._C._functorch.peek_interpreter_stack() is not None:
+        if kwargs or _dispatch_modes() or _transforms() is not None or torch.compiler.is_compiling():
             return op(*args, **kwargs)
-        grad = torch.is_grad_enabled()
         for x in args:
-            if isinstance(x, Tensor) and ((grad and x.requires_grad) or type(x) not in (Tensor, torch.nn.Parameter)):
+            kind = type(x)
+            if kind is Tensor or kind is torch.nn.Parameter:
+                if x.requires_grad and torch.is_grad_enabled():
+                    return op(*args)
+            elif isinstance(x, Tensor):
                 return op(*args)
         out = run(*args)
         for i in mutated:
@@ -838,22 +851,22 @@ def _eager(op):
 
 def _launch(fn, desc, index: int, op: str) -> None:
     """Call a C entry point on the current stream of device `index`, whichever device is current."""
-    if index == torch._C._cuda_getDevice():
-        rc = fn(desc, torch._C._cuda_getCurrentRawStream(index))
+    if index == _current_device():
+        rc = fn(desc, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(desc, torch._C._cuda_getCurrentRawStream(index))
+            rc = fn(desc, _raw_stream(index))
     if rc:
         _lib.check(rc, f"dfb200::{op}")
 
 
 def _same_device(op: str, first: Tensor, *rest: Tensor | None) -> torch.device:
     require_cuda(first, op)
-    device = first.device
+    index = first.get_device()
     for t in rest:
-        if t is not None and t.device != device:
-            raise ValueError(f"{op}: all tensors must be on {device}, got one on {t.device}")
-    return device
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{op}: all tensors must be on {first.device}, got one on {t.device}")
+    return first.device
 
 
 def _rows(op: str, name: str, t: Tensor) -> tuple[int, int, int]:
@@ -1053,7 +1066,7 @@ def tree_attention(query: Tensor, key_cache: Tensor, value_cache: Tensor, cache_
     if batch == 0 or nodes == 0:
         return out
     lib = _lib.load()
-    nbytes = lib.dfb_tree_attn_scratch_bytes(batch, nodes, hq, hkv, d, max_seq)
+    nbytes = _scratch_bytes("dfb_tree_attn_scratch_bytes", batch, nodes, hq, hkv, d, max_seq)
     # from the allocator, not kept: calls on two streams, or two captured graphs, never share it
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     a = _lib.TreeAttnDesc()
@@ -1113,7 +1126,7 @@ def _delta_tokens(
         return out, None if parents is not None else state.clone()
     new_state = torch.empty_like(state) if parents is None else None
     lib = _lib.load()
-    nbytes = lib.dfb_delta_chunk_scratch_bytes(batch, tokens, hk, hv, dk)
+    nbytes = _scratch_bytes("dfb_delta_chunk_scratch_bytes", batch, tokens, hk, hv, dk)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)  # not kept, as in tree_attention
     p = _lib.DeltaChunkDesc()
     _DELTA.pack_into(
