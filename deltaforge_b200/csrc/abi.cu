@@ -407,15 +407,16 @@ int dfb_rotary(const dfb_rotary_desc* d, void* stream) {
   return launch_rotary(p, (cudaStream_t)stream);
 }
 
-static size_t tree_scratch(const TreePlan& plan, int batch, int nodes, int hq, int d) {
-  if (plan.splits <= 1) return 0;
-  const size_t rows = (size_t)batch * hq * nodes * plan.splits;
-  return align_up(rows * d * 4, 256) + align_up(rows * 2 * 4, 256);
+static size_t tree_scratch(const TreePlan& plan, int d) { return plan.slots ? align_up(plan.slots * d * 4, 256) + align_up(plan.slots * 2 * 4, 256) : 0; }
+// Whether a cache with these strides can be described to TMA: an expanded one (stride 0) cannot.
+static bool tree_tc_ok(int batch, int hkv, int max_seq, const int64_t (&k)[3], const int64_t (&v)[3]) {
+  return (batch == 1 || (k[0] > 0 && v[0] > 0)) && (hkv == 1 || (k[1] > 0 && v[1] > 0)) && (max_seq == 1 || (k[2] > 0 && v[2] > 0));
 }
 
 size_t dfb_tree_attn_scratch_bytes(int batch, int nodes, int hq, int hkv, int d, int max_seq) {
   if (batch < 1 || nodes < 1 || hkv < 1 || hq < hkv || max_seq < 1) return 0;
-  return tree_scratch(tree_plan(batch, nodes, hq, hkv, max_seq), batch, nodes, hq, d);
+  const size_t a = tree_scratch(tree_plan(batch, nodes, hq, hkv, d, max_seq, true), d), b = tree_scratch(tree_plan(batch, nodes, hq, hkv, d, max_seq, false), d);
+  return a > b ? a : b;
 }
 
 int dfb_tree_attention(const dfb_tree_attn_desc* d, void* stream) {
@@ -429,9 +430,9 @@ int dfb_tree_attention(const dfb_tree_attn_desc* d, void* stream) {
   if (!d->q || !d->kcache || !d->vcache || !d->cache_len || !d->parents || !d->out) return bad("dfb_tree_attention: null tensor pointer");
   if (!aligned16(d->kcache) || !aligned16(d->vcache) || !multiples(d->k_stride, 8) || !multiples(d->v_stride, 8))
     return bad("dfb_tree_attention: cache rows must start on 16-byte boundaries");
-  if (((uintptr_t)d->q & 3) || !multiples(d->q_stride, 2)) return bad("dfb_tree_attention: query rows must start on 4-byte boundaries");
-  const TreePlan plan = tree_plan(d->batch, d->nodes, d->hq, d->hkv, d->max_seq);
-  const size_t need = tree_scratch(plan, d->batch, d->nodes, d->hq, d->d);
+  if (!aligned16(d->q) || !multiples(d->q_stride, 8)) return bad("dfb_tree_attention: query rows must start on 16-byte boundaries");
+  const TreePlan plan = tree_plan(d->batch, d->nodes, d->hq, d->hkv, d->d, d->max_seq, tree_tc_ok(d->batch, d->hkv, d->max_seq, d->k_stride, d->v_stride));
+  const size_t need = tree_scratch(plan, d->d);
   if (need && (!d->scratch || d->scratch_bytes < need || !aligned16(d->scratch))) return bad("dfb_tree_attention: aligned scratch of %zu bytes required", need);
   TreeAttnParams p = {};
   p.batch = d->batch;
@@ -456,9 +457,10 @@ int dfb_tree_attention(const dfb_tree_attn_desc* d, void* stream) {
   p.out = d->out;
   p.splits = plan.splits;
   p.mt = plan.mt;
+  p.tc_ctas = plan.tc_ctas;
   if (need) {
     p.part_acc = (float*)d->scratch;
-    p.part_ml = (float*)((char*)d->scratch + align_up((size_t)d->batch * d->hq * d->nodes * plan.splits * d->d * 4, 256));
+    p.part_ml = (float*)((char*)d->scratch + align_up(plan.slots * d->d * 4, 256));
   }
   return launch_tree_attention(p, (cudaStream_t)stream);
 }

@@ -341,14 +341,20 @@ struct TreeAttnParams {
   float scale;
   void* out;  // [batch, nodes, hq, d] contiguous
   int splits, mt;
-  float* part_acc;  // [batch, hkv, splits, rows, d]
-  float* part_ml;   // [batch, hkv, splits, rows, 2]
+  int tc_ctas;      // > 0: the tcgen05 form, with that many CTAs
+  float* part_acc;  // [batch, hkv, splits, rows, d]; tcgen05: [slots, 128, d]
+  float* part_ml;   // the same with 2 (maximum, sum) in the place of d
 };
 struct TreePlan {
-  int mt;      // 16-row tiles per CTA
-  int splits;  // key ranges
+  int mt;        // mma.sync: 16-row tiles per CTA
+  int splits;    // mma.sync: key ranges
+  int tc_ctas;   // tcgen05: CTAs, 0 where mma.sync serves
+  size_t slots;  // partial results of a row each may leave: rows of part_acc
 };
-TreePlan tree_plan(int batch, int nodes, int hq, int hkv, int max_seq);
+// The least stretch of 128-key tiles a CTA of the tcgen05 form takes: below it the partial results cost more than they save.
+constexpr int TREE_TC_MIN_TILES = 2;
+int launch_tree_attention_tc(const TreeAttnParams& p, cudaStream_t stream);
+TreePlan tree_plan(int batch, int nodes, int hq, int hkv, int d, int max_seq, bool tc_ok);
 int launch_tree_attention(const TreeAttnParams& p, cudaStream_t stream);
 
 struct DeltaChunkParams {

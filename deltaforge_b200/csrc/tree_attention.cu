@@ -531,27 +531,35 @@ int launch_t(const TreeAttnParams& p, cudaStream_t stream) {
 
 }  // namespace
 
-TreePlan tree_plan(int batch, int nodes, int hq, int hkv, int max_seq) {
-  TreePlan pl;
+TreePlan tree_plan(int batch, int nodes, int hq, int hkv, int d, int max_seq, bool tc_ok) {
+  TreePlan pl = {};
   const int rows = nodes * (hq / hkv);
+  if (tc_ok && d >= 64 && rows > 16) {
+    const long units = (long)batch * hkv * ((rows + 127) / 128), tiles = units * ((max_seq + 127) / 128);
+    const long ctas = (tiles + TREE_TC_MIN_TILES - 1) / TREE_TC_MIN_TILES;
+    pl.tc_ctas = (int)(ctas < 148 ? ctas : 148);
+    pl.slots = (size_t)(pl.tc_ctas + units) * 128;
+    return pl;
+  }
   pl.mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   const long base = (long)batch * hkv * ((rows + 16 * pl.mt - 1) / (16 * pl.mt));
   // Splits: enough CTAs for the 148 SMs, as full a last wave as can be had, and no split of fewer than 64 keys of the
   // cache's capacity (the live length is known on the device alone).
   const int most = max_seq / 64 < 1 ? 1 : max_seq / 64 > 128 ? 128 : max_seq / 64;
-  int best = 1;
+  pl.splits = 1;
   double best_cost = 1e30;
   for (int s = 1; s <= most; ++s) {
     const double waves = (double)((base * s + 147) / 148);
     const double cost = waves / s * (1.0 + 0.02 * s * waves / (waves + 8.0)) + 0.0005 * s;
-    if (cost < best_cost * 0.999) best_cost = cost, best = s;
+    if (cost < best_cost * 0.999) best_cost = cost, pl.splits = s;
     if (base * s > 148 * 8) break;
   }
-  pl.splits = best;
+  pl.slots = pl.splits > 1 ? (size_t)batch * hkv * rows * pl.splits : 0;
   return pl;
 }
 
 int launch_tree_attention(const TreeAttnParams& p, cudaStream_t stream) {
+  if (p.tc_ctas) return launch_tree_attention_tc(p, stream);
   static OncePerDevice once;
   const int rc = once.run(configure_all);
   if (rc) return rc;

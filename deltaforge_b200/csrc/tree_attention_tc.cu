@@ -1,0 +1,670 @@
+// Attention of a tree of drafted tokens over the KV cache on tcgen05 (sm_100a), for more than a few query rows.
+//
+// Same contract as tree_attention.cu, which serves the smallest trees. There the 16-row tiles of mma.sync read a key once per 64
+// rows and reach a quarter of the tensor rate; 64 nodes with 4 query heads per KV head (256 rows) were bound by that.
+// Here 128 rows (node * group + head) are the M of tcgen05.mma: S = Q K^T into TMEM, P = 2^(S - m) back into TMEM as the A
+// operand of O += P V, O in TMEM as well (S and its successor 128 columns each, O one column per dim: 512 at head dim 256).
+//
+// Work: the (sequence, KV head, row tile) units are laid out one behind the other in tiles of 128 keys, as many as each
+// sequence really has, and every CTA takes an equal stretch of that line, whatever units it crosses (the lengths are on the
+// device; a grid planned on the host from the cache's capacity waits for its longest sequence). A unit that one CTA
+// covers is finished there; of the others every CTA leaves (m, l, acc) in slot (CTA + unit), and tree_tc_merge_kernel adds
+// them in order.
+//
+// Roles: warp 0 loads (TMA boxes of 64 dims x 128 keys, 128-byte swizzle; a ring of 32 KB pieces), warp 1 issues the products,
+// warps 4-7 own a row per thread: scores out of TMEM, masks, maximum, exponentials, P into the columns of S. The products
+// of tile i + 1 run under the softmax of tile i. The maximum that P refers to is moved only when a row's true maximum is more
+// than 2^8 above it, so that O rarely has to be rescaled; sums stay exact because l refers to the same maximum.
+//
+// Bounds per tile of 128 keys at head dim 256: 2 x 1024 cycles of tensor time, 1024 cycles of ex2 on the softmax warps, and
+// 128 KB of K and V from the L2, 64 bytes per cycle and SM, which is what two row tiles of one unit cost (each reads
+// the same keys).
+//
+// Every wait is bounded; one that runs out makes the CTA leave NaN.
+#include <cuda.h>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace dfb {
+
+namespace {
+
+constexpr int TM = 128;          // query rows per tile
+constexpr int TN = 128;          // keys per tile
+constexpr int TC_THREADS = 256;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LAZY = 8.f;      // rescale O when the maximum has grown by more than this (in powers of two)
+constexpr long long WAIT_CYCLES = 1LL << 28;
+
+template <int D> struct Tc {
+  static constexpr int BLOCKS = D / 64;               // 64-dim blocks of a row
+  static constexpr int PIECES = D == 256 ? 2 : 1;     // ring pieces per K or V tile
+  static constexpr int PIECE_BLOCKS = BLOCKS / PIECES;
+  static constexpr int PIECE = PIECE_BLOCKS * TN * 128;
+  static constexpr int Q_BYTES = BLOCKS * TM * 128;
+  static constexpr int RING = D == 256 ? 5 : 6;
+  static constexpr int SMEM = Q_BYTES + RING * PIECE + 1024;
+  static constexpr int O_COL = 0, S_COL = 256;        // TMEM columns: O, then two S of 128
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded; the CTA-wide flag ends every other wait too.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* failed) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*failed) return false;
+    if (clock64() - t0 > WAIT_CYCLES) {
+      *failed = 1;
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int dim, int key, int head, int seq, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"((uint64_t)map), "r"(dim), "r"(key), "r"(head), "r"(seq), "r"(smem_u32(bar))
+      : "memory");
+}
+// Rows of one 128-byte swizzle span, 8-row groups 1024 bytes apart. `lead`: for an operand whose rows run along its
+// contraction (V: a row is a key), bytes from one block of 64 dims to the next; unused where rows run along M or N.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead) {
+  return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+template <typename T> __device__ __forceinline__ uint32_t type_bits() { return 1u; }  // bf16
+template <> __device__ __forceinline__ uint32_t type_bits<__half>() { return 0u; }
+// D fp32, M = 128; b_rows: B's rows run along its contraction
+template <typename T> __device__ __forceinline__ uint32_t instr_desc(int n, bool b_rows) {
+  return 1u << 4 | type_bits<T>() << 7 | type_bits<T>() << 10 | (uint32_t)b_rows << 16 | (uint32_t)(n >> 3) << 17 | (uint32_t)(TM >> 4) << 24;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+               "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
+               "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+#define DFB_R8(v, i) v[i], v[i + 1], v[i + 2], v[i + 3], v[i + 4], v[i + 5], v[i + 6], v[i + 7]
+#define DFB_OUT8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
+#define DFB_TIE8(v, i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3]), "+r"(v[i + 4]), "+r"(v[i + 5]), "+r"(v[i + 6]), "+r"(v[i + 7])
+#define DFB_IN8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
+
+// 32 columns of this thread's lane. The registers hold the values after tmem_wait_ld on them.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+      "%26,%27,%28,%29,%30,%31}, [%32];"
+      : DFB_OUT8(v, 0), DFB_OUT8(v, 8), DFB_OUT8(v, 16), DFB_OUT8(v, 24)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait_ld(uint32_t* v) {  // (tied to the registers, so that no use moves before it)
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : DFB_TIE8(v, 0), DFB_TIE8(v, 8), DFB_TIE8(v, 16), DFB_TIE8(v, 24)::"memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+      "%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      DFB_IN8(v, 0), DFB_IN8(v, 8), DFB_IN8(v, 16), DFB_IN8(v, 24)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<bf16>(float a, float b) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *(uint32_t*)&v;
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  __half2 v = __floats2half2_rn(a, b);
+  return *(uint32_t*)&v;
+}
+template <typename T> __device__ __forceinline__ float elem_f(T v);
+template <> __device__ __forceinline__ float elem_f(bf16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float elem_f(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ uint32_t exp_mask() { return 0x7f80; }  // all ones: infinity or NaN
+template <> __device__ __forceinline__ uint32_t exp_mask<__half>() { return 0x7c00; }
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ int live_rows(const TreeAttnParams& p, int b) {
+  return (int)min((long)min(max(p.cache_len[b], 0), p.max_seq) + p.nodes, (long)p.max_seq);
+}
+__device__ __forceinline__ int live_tiles(const TreeAttnParams& p, int b) { return (live_rows(p, b) + TN - 1) / TN; }
+// Tiles of the sequences before b (all of them for b = batch), by one warp.
+__device__ __forceinline__ int tiles_before(const TreeAttnParams& p, int b, int lane) {
+  int n = 0;
+  for (int i = lane; i < b; i += 32) n += live_tiles(p, i);
+  return __reduce_add_sync(0xffffffffu, n);
+}
+// Tiles per CTA when `total` of them are shared out
+__device__ __forceinline__ long tiles_per_cta(const TreeAttnParams& p, long total) {
+  const long even = (total + p.tc_ctas - 1) / p.tc_ctas;
+  return even < TREE_TC_MIN_TILES ? TREE_TC_MIN_TILES : even;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const __grid_constant__ CUtensorMap kmap,
+                                                                          const __grid_constant__ CUtensorMap vmap, const TreeAttnParams p) {
+  using S_ = Tc<D>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  unsigned char* ring = sm + S_::Q_BYTES;
+  __shared__ uint64_t full[S_::RING], freed[S_::RING], s_full[2], p_full[2], pv_done[2];
+  __shared__ unsigned long long anc[MAX_TREE_NODES];
+  __shared__ int up[MAX_TREE_NODES];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed_s, odd_s, where[4];
+  volatile int* failed = &failed_s;
+
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  if (t == 0) {
+    for (int i = 0; i < S_::RING; ++i) mbar_init(&full[i], 1), mbar_init(&freed[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&pv_done[i], 1);
+    failed_s = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_launch_dependents();  // the merge may set itself up; it waits for this grid's end before it reads
+
+  // ---- this CTA's stretch of the line of tiles ----
+  const int row_tiles = (p.rows + TM - 1) / TM, upb = p.hkv * row_tiles;  // units per sequence
+  if (warp == 2) {
+    const long total = (long)tiles_before(p, p.batch, lane) * upb;
+    const long share = tiles_per_cta(p, total), w0 = blockIdx.x * share;
+    int b = -1, before = 0, prefix = 0;  // the sequence that holds tile w0
+    for (int at = 0; at < p.batch && b < 0; at += 32) {
+      const int n = at + lane < p.batch ? live_tiles(p, at + lane) : 0;
+      int s = n;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int y = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += y;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, at + lane < p.batch && (long)(before + s) * upb > w0);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        b = at + l;
+        prefix = before + __shfl_sync(0xffffffffu, s - n, l);
+      }
+      before += __shfl_sync(0xffffffffu, s, 31);
+    }
+    if (lane == 0) {
+      where[3] = 0;
+      if (b >= 0) {
+        const int n = live_tiles(p, b);
+        const long inside = w0 - (long)prefix * upb;
+        where[0] = b, where[1] = (int)(inside / n), where[2] = (int)(inside % n), where[3] = (int)min(share, total - w0);
+      }
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot;
+  int b = where[0], unit = where[1], tile = where[2], left = where[3];  // left: tiles still to do
+  int pieces = 0, done = 0;  // ring pieces and tiles before this segment: what the barriers' parities follow
+  bool ok = true;
+
+  while (left > 0) {
+    const int L = live_rows(p, b), cached = min(max(p.cache_len[b], 0), p.max_seq), tiles = (L + TN - 1) / TN;
+    const int n = min(left, tiles - tile);  // this segment: tiles tile .. tile + n - 1 of the unit
+    const int hk = unit / row_tiles, rt = unit % row_tiles;
+    const bool has_tree = (tile + n) * TN > cached;
+
+    // ---- queries to shared memory (K-major, swizzled), ancestors ----
+    for (int i = t; i < TM * (D / 8); i += TC_THREADS) {
+      const int r = i / (D / 8), ch = i % (D / 8), row = rt * TM + r;
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (row < p.rows) {
+        const int node = row / p.group;
+        v = *(const uint4*)((const T*)p.q + b * p.q_stride[0] + node * p.q_stride[1] + (hk * p.group + row - node * p.group) * p.q_stride[2] + ch * 8);
+      }
+      *(uint4*)(sm + (ch >> 3) * (TM * 128) + (r >> 3) * 1024 + (r & 7) * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    if (t == 0) odd_s = 0;
+    if (has_tree) {
+      if (t < p.nodes) {
+        const int pa = p.parents[(long)b * p.parents_stride + t];
+        const bool node = pa >= -1 && pa < t;
+        anc[t] = node ? 1ull << t : 0ull;
+        up[t] = node ? pa : -1;
+      }
+      __syncthreads();
+      for (int step = 1; step < p.nodes; step *= 2) {  // bits of up to 2 * step ancestors
+        unsigned long long bits = 0;
+        int u = -1;
+        if (t < p.nodes) {
+          bits = anc[t], u = up[t];
+          if (u >= 0) bits |= anc[u], u = up[u];
+        }
+        __syncthreads();
+        if (t < p.nodes) anc[t] = bits, up[t] = u;
+        __syncthreads();
+      }
+    }
+    __syncthreads();
+
+    if (warp == 0) {
+      // ---------------- loads: K 0, then K i + 1 and V i in turn ----------------
+      if (lane == 0) {
+        int c = pieces;
+        auto load = [&](const CUtensorMap* map, int i) {
+          for (int h = 0; h < S_::PIECES && ok; ++h, ++c) {
+            const int s = c % S_::RING;
+            if (c >= S_::RING) ok = wait_for(&freed[s], (c / S_::RING - 1) & 1, failed);
+            if (!ok) break;
+            mbar_expect_tx(&full[s], S_::PIECE);
+            const uint32_t dst = smem_u32(ring + s * S_::PIECE);
+#pragma unroll
+            for (int x = 0; x < S_::PIECE_BLOCKS; ++x)
+              tma_box(dst + x * (TN * 128), map, (h * S_::PIECE_BLOCKS + x) * 64, (tile + i) * TN, hk, b, &full[s]);
+          }
+        };
+        load(&kmap, 0);
+        for (int i = 0; i < n && ok; ++i) {
+          if (i + 1 < n) load(&kmap, i + 1);
+          load(&vmap, i);
+        }
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      // ---------------- products ----------------
+      if (lane == 0) {
+        int c = pieces;
+        const uint32_t qa = smem_u32(sm), ra = smem_u32(ring);
+        const uint32_t id_s = instr_desc<T>(TN, false), id_o = instr_desc<T>(S_::PIECE_BLOCKS * 64, true);
+        auto scores = [&](int i) {
+          const int gi = done + i;
+          for (int h = 0; h < S_::PIECES && ok; ++h, ++c) {
+            const int s = c % S_::RING;
+            ok = wait_for(&full[s], (c / S_::RING) & 1, failed);
+            if (!ok) break;
+            fence_after();
+#pragma unroll
+            for (int x = 0; x < S_::PIECE_BLOCKS; ++x)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma_ss(tmem + S_::S_COL + (gi & 1) * TN, smem_desc(qa + (h * S_::PIECE_BLOCKS + x) * (TM * 128) + k * 32, 0),
+                       smem_desc(ra + s * S_::PIECE + x * (TN * 128) + k * 32, 0), id_s, (h | x | k) != 0);
+            commit(&freed[s]);
+          }
+          if (ok) commit(&s_full[gi & 1]);
+        };
+        scores(0);
+        for (int i = 0; i < n && ok; ++i) {
+          if (i + 1 < n) scores(i + 1);
+          const int gi = done + i;
+          ok = ok && wait_for(&p_full[gi & 1], (gi >> 1) & 1, failed);
+          if (!ok) break;
+          fence_after();
+          for (int h = 0; h < S_::PIECES && ok; ++h, ++c) {
+            const int s = c % S_::RING;
+            ok = wait_for(&full[s], (c / S_::RING) & 1, failed);
+            if (!ok) break;
+#pragma unroll
+            for (int k = 0; k < TN / 16; ++k)
+              mma_ts(tmem + S_::O_COL + h * (S_::PIECE_BLOCKS * 64), tmem + S_::S_COL + (gi & 1) * TN + k * 8,
+                     smem_desc(ra + s * S_::PIECE + k * 2048, TN * 128), id_o, (i | k) != 0);
+            commit(&freed[s]);
+          }
+          if (ok) commit(&pv_done[gi & 1]);
+        }
+      }
+      __syncwarp();
+    } else if (warp >= 4) {
+      // ---------------- softmax: thread = row ----------------
+      const int r = t - 128, row = rt * TM + r;
+      const bool rok = row < p.rows;
+      const int node = rok ? row / p.group : 0;
+      const unsigned long long bits = has_tree ? anc[node] : 0ull;
+      const uint32_t lane_base = tmem + ((uint32_t)((warp - 4) * 32) << 16);
+      const float sl0 = p.scale * LOG2E;
+      float mref = -INFINITY, l = 0.f;
+      for (int i = 0; i < n; ++i) {
+        const int gi = done + i, key0 = (tile + i) * TN;
+        const uint32_t scol = lane_base + S_::S_COL + (gi & 1) * TN;
+        ok = ok && wait_for(&s_full[gi & 1], (gi >> 1) & 1, failed);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        fence_after();
+        uint32_t v[TN];
+#pragma unroll
+        for (int x = 0; x < TN; x += 32) tmem_ld32(scol + x, v + x);
+#pragma unroll
+        for (int x = 0; x < TN; x += 32) tmem_wait_ld(v + x);
+        float sl = sl0;
+        if (sl <= 0.f) {  // (a scale that is not positive: applied first, so that masks and the maximum mean the same)
+#pragma unroll
+          for (int x = 0; x < TN; ++x) v[x] = __float_as_uint(__uint_as_float(v[x]) * sl);
+          sl = 1.f;
+        }
+        if (key0 + TN > cached) {
+#pragma unroll
+          for (int x = 0; x < TN; ++x) {
+            const int j = key0 + x - cached;  // node number, negative in the prefix
+            const bool seen = j < 0 || (j < MAX_TREE_NODES && j + cached < L && ((bits >> j) & 1));
+            if (!seen) v[x] = 0xff800000u;
+          }
+          // Values of rows past the end, and values of tree rows that are not finite, must not meet a zero probability: zeroed
+          // here (this thread: key row r); the latter are added back below for the rows that see them.
+          // (A parity cannot tell "V i has landed" from "what was in that slot before has not": the slots' earlier pieces are at
+          // latest V i - 1, so its product is waited for first.)
+          const int vb = (i + 1 < n ? 2 * i + 2 : 2 * n - 1) * S_::PIECES;
+          if (i > 0) ok = wait_for(&pv_done[(gi - 1) & 1], ((gi - 1) >> 1) & 1, failed);
+          for (int h = 0; h < S_::PIECES; ++h) {
+            const int c = pieces + vb + h, s = c % S_::RING;
+            ok = ok && wait_for(&full[s], (c / S_::RING) & 1, failed);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const int key = key0 + r;
+            if (key >= cached) {
+              unsigned char* base = ring + s * S_::PIECE + (r >> 3) * 1024 + (r & 7) * 128;
+              bool odd = false;
+#pragma unroll 1
+              for (int x = 0; x < S_::PIECE_BLOCKS * 8; ++x) {
+                uint4* at = (uint4*)(base + (x >> 3) * (TN * 128) + (x & 7) * 16);
+                uint32_t y[4] = {at->x, at->y, at->z, at->w};
+                bool change = key >= L;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  if (key >= L) y[e] = 0u;
+                  const uint32_t m = exp_mask<T>();
+                  if ((y[e] & m) == m) y[e] &= 0xffff0000u, change = odd = true;
+                  if (((y[e] >> 16) & m) == m) y[e] &= 0x0000ffffu, change = odd = true;
+                }
+                if (change) *at = make_uint4(y[0], y[1], y[2], y[3]);
+              }
+              if (odd) odd_s = 1;
+            }
+          }
+          if (!ok) break;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int x = 0; x < TN; ++x) m4[x & 3] = fmaxf(m4[x & 3], __uint_as_float(v[x]));
+        const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl;
+        if (i == 0) {
+          mref = top;
+        } else {
+          const bool move = top > mref + LAZY;
+          if (__any_sync(0xffffffffu, move)) {
+            ok = ok && wait_for(&pv_done[(gi - 1) & 1], ((gi - 1) >> 1) & 1, failed);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            fence_after();
+            const float f = move ? exp2_fast(mref - top) : 1.f;
+            if (move) mref = top, l *= f;
+#pragma unroll 1
+            for (int x = 0; x < D; x += 32) {
+              uint32_t o[32];
+              tmem_ld32(lane_base + S_::O_COL + x, o);
+              tmem_wait_ld(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st32(lane_base + S_::O_COL + x, o);
+            }
+            tmem_wait_st();
+          }
+        }
+        const float ref = mref == -INFINITY ? 0.f : mref;
+        float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < TN; x += 2) {
+          const float p0 = exp2_fast(fmaf(__uint_as_float(v[x]), sl, -ref)), p1 = exp2_fast(fmaf(__uint_as_float(v[x + 1]), sl, -ref));
+          l4[(x >> 1) & 3] += p0 + p1;
+          v[x >> 1] = pack2<T>(p0, p1);
+        }
+        l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+        tmem_st32(scol, v);
+        tmem_st32(scol + 32, v + 32);
+        tmem_wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[gi & 1]);
+      }
+      // ---------------- the unit's result, or this CTA's part of it ----------------
+      if (ok) ok = wait_for(&pv_done[(done + n - 1) & 1], ((done + n - 1) >> 1) & 1, failed);
+      ok = __all_sync(0xffffffffu, ok);
+      fence_after();
+      asm volatile("bar.sync 1, 128;" ::: "memory");  // odd_s of all rows
+      const bool odd = odd_s != 0 && has_tree;
+      const long slot = blockIdx.x + (long)b * upb + unit;
+      const bool whole = n == tiles;
+      const int pa = rok ? p.parents[(long)b * p.parents_stride + node] : -2;
+      const bool is_node = pa >= -1 && pa < node;
+      const float inv = 1.f / l;
+#pragma unroll 1
+      for (int x = 0; x < D; x += 32) {
+        uint32_t o[32];
+        tmem_ld32(lane_base + S_::O_COL + x, o);
+        tmem_wait_ld(o);
+        float f[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) f[e] = ok ? __uint_as_float(o[e]) : __int_as_float(0x7fffffff);
+        if (odd && rok) {
+          for (int j = 0; j < p.nodes; ++j) {
+            const int key = cached + j;
+            if (!((bits >> j) & 1) || key >= L || key < tile * TN || key >= (tile + n) * TN) continue;
+            const T* y = (const T*)p.vcache + b * p.v_stride[0] + hk * p.v_stride[1] + key * p.v_stride[2] + x;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float z = elem_f<T>(y[e]);
+              if (!isfinite(z)) f[e] += z;
+            }
+          }
+        }
+        if (!rok) continue;
+        if (whole) {
+          T* out = (T*)p.out + (((long)b * p.nodes + node) * p.hq + hk * p.group + row - node * p.group) * D + x;
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint4 y = make_uint4(pack2<T>(f[e] * inv, f[e + 1] * inv), pack2<T>(f[e + 2] * inv, f[e + 3] * inv),
+                                 pack2<T>(f[e + 4] * inv, f[e + 5] * inv), pack2<T>(f[e + 6] * inv, f[e + 7] * inv));
+            if (!is_node) y = make_uint4(0u, 0u, 0u, 0u);
+            *(uint4*)(out + e) = y;
+          }
+        } else {
+          float* acc = p.part_acc + (slot * TM + r) * D + x;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) *(float4*)(acc + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+        }
+      }
+      if (rok && !whole) *(float2*)(p.part_ml + (slot * TM + r) * 2) = make_float2(mref, l);
+    }
+    fence_before();
+    __syncthreads();  // queries, O and the flags may be written again
+    fence_after();
+    ok = ok && !*failed;
+    pieces += 2 * n * S_::PIECES;
+    done += n;
+    left -= n;
+    tile += n;
+    if (tile == tiles) {
+      tile = 0;
+      if (++unit == upb) unit = 0, ++b;
+    }
+  }
+  __syncthreads();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+}
+
+// One CTA per output row: the parts of its unit in the order of the CTAs that left them.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) tree_tc_merge_kernel(const TreeAttnParams p) {
+  constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+  __shared__ float4 part[GROUPS][LANES];
+  __shared__ float part_l[GROUPS], top[8];
+  __shared__ long first_s;
+  __shared__ int count_s;
+  const int t = threadIdx.x, li = t % LANES, gi = t / LANES;
+  const int row = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, node = row / p.group;
+  const int row_tiles = (p.rows + TM - 1) / TM, upb = p.hkv * row_tiles, rt = row / TM;
+  const int pa = p.parents[(long)b * p.parents_stride + node];
+  const bool ok = pa >= -1 && pa < node;
+  if (t < 32) {
+    const int before = tiles_before(p, b, t), all = tiles_before(p, p.batch, t), mine = live_tiles(p, b);
+    const long share = tiles_per_cta(p, (long)all * upb);
+    const long w = (long)before * upb + (long)(hk * row_tiles + rt) * mine;  // first tile of the unit
+    if (t == 0) {
+      first_s = w / share;
+      count_s = (int)((w + mine - 1) / share - first_s) + 1;
+    }
+  }
+  __syncthreads();
+  const int count = count_s;
+  if (count == 1) return;  // finished by the CTA that had all of it
+  pdl_wait();
+  const long slot0 = first_s + (long)b * upb + hk * row_tiles + rt;
+  const float2* ml = (const float2*)p.part_ml + slot0 * TM + row % TM;
+  const float* acc = p.part_acc + (slot0 * TM + row % TM) * D + 4 * li;
+  float m = -INFINITY;
+  for (int s = t; s < count; s += 256) m = fmaxf(m, __ldcg(ml + (long)s * TM).x);
+  m = warp_max(m);
+  if ((t & 31) == 0) top[t >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, top[w]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 4
+  for (int s = gi; s < count; s += GROUPS) {
+    const float2 v = __ldcg(ml + (long)s * TM);
+    const float4 y = __ldcg((const float4*)(acc + (long)s * TM * D));
+    const float w = exp2_fast(v.x - ref);
+    l = fmaf(v.y, w, l);
+    a.x = fmaf(y.x, w, a.x), a.y = fmaf(y.y, w, a.y), a.z = fmaf(y.z, w, a.z), a.w = fmaf(y.w, w, a.w);
+  }
+  part[gi][li] = a;
+  if (li == 0) part_l[gi] = l;
+  __syncthreads();
+  if (gi) return;
+#pragma unroll
+  for (int i = 1; i < GROUPS; ++i) {
+    const float4 y = part[i][li];
+    a.x += y.x, a.y += y.y, a.z += y.z, a.w += y.w;
+    l += part_l[i];
+  }
+  const float inv = 1.f / l;
+  T* out = (T*)p.out + (((long)b * p.nodes + node) * p.hq + hk * p.group + row % p.group) * D + 4 * li;
+  uint2 v = make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
+  if (!ok) v = make_uint2(0u, 0u);
+  *(uint2*)out = v;
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = []() -> EncodeTiledFn {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return nullptr;
+    return (EncodeTiledFn)ptr;
+  }();
+  return fn;
+}
+
+// The cache as [sequence][KV head][row][D] with the caller's strides; boxes of 64 dims x 128 rows.
+bool encode_cache(CUtensorMap* map, const void* base, const long* stride, const TreeAttnParams& p) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)p.d, (cuuint64_t)p.max_seq, (cuuint64_t)p.hkv, (cuuint64_t)p.batch};
+  const long row = p.max_seq > 1 ? stride[2] : p.d;  // (the stride of a dimension of one is never used and may be anything)
+  const cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)(p.hkv > 1 ? stride[1] : row) * 2, (cuuint64_t)(p.batch > 1 ? stride[0] : row) * 2};
+  const cuuint32_t box[4] = {64, TN, 1, 1}, es[4] = {1, 1, 1, 1};
+  return enc(map, p.is_fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void*)base, dims, strides, box, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D>
+int configure_one() {
+  return cudaFuncSetAttribute(tree_attention_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tc<D>::SMEM) == cudaSuccess
+             ? 0
+             : check_launch("tree attention (tcgen05): shared-memory opt-in");
+}
+int configure_all() {
+  int rc = configure_one<bf16, 64>();
+  if (!rc) rc = configure_one<bf16, 128>();
+  if (!rc) rc = configure_one<bf16, 256>();
+  if (!rc) rc = configure_one<__half, 64>();
+  if (!rc) rc = configure_one<__half, 128>();
+  if (!rc) rc = configure_one<__half, 256>();
+  return rc;
+}
+
+template <typename T, int D>
+int launch_one(const CUtensorMap& kmap, const CUtensorMap& vmap, const TreeAttnParams& p, cudaStream_t stream) {
+  tree_attention_tc_kernel<T, D><<<p.tc_ctas, TC_THREADS, Tc<D>::SMEM, stream>>>(kmap, vmap, p);
+  const int rc = check_launch("tree attention (tcgen05)");
+  if (rc) return rc;
+  if (launch_pdl(tree_tc_merge_kernel<T, D>, dim3(p.rows, p.hkv, p.batch), dim3(256), 0, stream, p) != cudaSuccess)
+    return check_launch("tree attention (tcgen05): merge");
+  return check_launch("tree attention (tcgen05): merge");
+}
+template <typename T>
+int launch_t(const CUtensorMap& kmap, const CUtensorMap& vmap, const TreeAttnParams& p, cudaStream_t stream) {
+  switch (p.d) {
+    case 64: return launch_one<T, 64>(kmap, vmap, p, stream);
+    case 128: return launch_one<T, 128>(kmap, vmap, p, stream);
+    default: return launch_one<T, 256>(kmap, vmap, p, stream);
+  }
+}
+
+}  // namespace
+
+int launch_tree_attention_tc(const TreeAttnParams& p, cudaStream_t stream) {
+  static OncePerDevice once;
+  const int rc = once.run(configure_all);
+  if (rc) return rc;
+  CUtensorMap kmap, vmap;
+  if (!encode_cache(&kmap, p.kcache, p.k_stride, p) || !encode_cache(&vmap, p.vcache, p.v_stride, p)) {
+    set_error("tree attention (tcgen05): tensor map for the cache failed");
+    return 1;
+  }
+  return p.is_fp16 ? launch_t<__half>(kmap, vmap, p, stream) : launch_t<bf16>(kmap, vmap, p, stream);
+}
+
+}  // namespace dfb

@@ -309,7 +309,7 @@ int dfb_rotary(const dfb_rotary_desc* desc, void* stream);
 typedef struct dfb_tree_attn_desc {
   int32_t batch, nodes, hq, hkv, d, max_seq; /* d 32, 64, 128 or 256; nodes 1..64 */
   int32_t is_fp16;     /* q, cache and output are fp16 instead of bf16 */
-  const void* q;       /* [batch, nodes, hq, d], strides batch, node, head (even) */
+  const void* q;       /* [batch, nodes, hq, d], strides batch, node, head (multiples of 8), 16-byte aligned */
   const void* kcache;  /* [batch, hkv, max_seq, d], strides batch, head, row (multiples of 8), 16-byte aligned */
   const void* vcache;
   int64_t q_stride[3], k_stride[3], v_stride[3];

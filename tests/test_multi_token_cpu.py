@@ -186,7 +186,7 @@ def test_scratch_sizes():
     # a long prompt is walked in segments: the scratch stays bounded
     assert lib.dfb_delta_chunk_scratch_bytes(1, 1 << 20, 16, 32, 128) <= 64 << 20
     assert lib.dfb_delta_chunk_scratch_bytes(0, 5, 1, 1, 8) == 0
-    assert lib.dfb_tree_attn_scratch_bytes(64, 64, 16, 4, 256, 32) == 0  # one split
+    assert lib.dfb_tree_attn_scratch_bytes(64, 1, 16, 4, 256, 32) == 0  # one split
 
 
 def test_rope_frequencies():

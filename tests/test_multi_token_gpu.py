@@ -244,7 +244,7 @@ def test_tree_attention_layouts_streams_and_graphs():
     wide[..., :d], wide[..., d:] = kc, vc
     assert torch.equal(ops.tree_attention(q, wide[..., :d], wide[..., d:], lt, pt.expand(b, n).contiguous(), 0.09), base)
     shared = ops.tree_attention(q, kc[:1].expand(b, -1, -1, -1), vc[:1].expand(b, -1, -1, -1), lt, pt, 0.09)
-    assert torch.equal(shared[0], base[0])
+    within(shared[:1], want[:1], tree_bound(want, size, q, kc, 0.09, rows)[:1])  # (an expanded cache takes the other kernel)
     odd = rnd(31, b, n, hq, d + 1, dtype=BF16)[..., :d]  # rows on odd elements: copied
     assert torch.equal(ops.tree_attention(odd, kc, vc, lt, pt, 0.09), ops.tree_attention(odd.contiguous(), kc, vc, lt, pt, 0.09))
     # two streams at once, and a captured graph whose lengths change between replays
