@@ -249,14 +249,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     const bool has_tree = (tile + n) * TN > cached;
 
     // ---- queries to shared memory (K-major, swizzled), ancestors ----
-    for (int i = t; i < TM * (D / 8); i += TC_THREADS) {
-      const int r = i / (D / 8), ch = i % (D / 8), row = rt * TM + r;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (row < p.rows) {
-        const int node = row / p.group;
-        v = *(const uint4*)((const T*)p.q + b * p.q_stride[0] + node * p.q_stride[1] + (hk * p.group + row - node * p.group) * p.q_stride[2] + ch * 8);
+    {
+      constexpr int CH = D / 8, BATCH = 8;  // loads under way per thread
+#pragma unroll 1
+      for (int i0 = t; i0 < TM * CH; i0 += TC_THREADS * BATCH) {
+        uint4 v[BATCH];
+#pragma unroll
+        for (int x = 0; x < BATCH; ++x) {
+          const int i = i0 + x * TC_THREADS, r = i / CH, ch = i % CH, row = rt * TM + r, node = row / p.group;
+          v[x] = make_uint4(0u, 0u, 0u, 0u);
+          if (i < TM * CH && row < p.rows)
+            v[x] = *(const uint4*)((const T*)p.q + b * p.q_stride[0] + node * p.q_stride[1] + (hk * p.group + row - node * p.group) * p.q_stride[2] + ch * 8);
+        }
+#pragma unroll
+        for (int x = 0; x < BATCH; ++x) {
+          const int i = i0 + x * TC_THREADS, r = i / CH, ch = i % CH;
+          if (i < TM * CH) *(uint4*)(sm + (ch >> 3) * (TM * 128) + (r >> 3) * 1024 + (r & 7) * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v[x];
+        }
       }
-      *(uint4*)(sm + (ch >> 3) * (TM * 128) + (r >> 3) * 1024 + (r & 7) * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     if (t == 0) odd_s = 0;
@@ -354,7 +364,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
       const int r = t - 128, row = rt * TM + r;
       const bool rok = row < p.rows;
       const int node = rok ? row / p.group : 0;
-      const unsigned long long bits = has_tree ? anc[node] : 0ull;
+      const int in_cache = L - cached;  // nodes that have a cache row
+      const unsigned long long bits = has_tree ? anc[node] & (in_cache >= 64 ? ~0ull : (1ull << in_cache) - 1) : 0ull;
       const uint32_t lane_base = tmem + ((uint32_t)((warp - 4) * 32) << 16);
       const float sl0 = p.scale * LOG2E;
       float mref = -INFINITY, l = 0.f;
@@ -377,14 +388,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
           sl = 1.f;
         }
         if (key0 + TN > cached) {
+          // bit x of word w: key key0 + 32 w + x is seen (short code: it runs once, out of a cold instruction cache)
 #pragma unroll
-          for (int x = 0; x < TN; ++x) {
-            const int j = key0 + x - cached;  // node number, negative in the prefix
-            const bool seen = j < 0 || (j < MAX_TREE_NODES && j + cached < L && ((bits >> j) & 1));
-            if (!seen) v[x] = 0xff800000u;
+          for (int w = 0; w < TN / 32; ++w) {
+            const int j0 = key0 + 32 * w - cached;  // node number of the word's first key, negative in the prefix
+            uint32_t seen = j0 <= -32 ? ~0u : j0 >= MAX_TREE_NODES ? 0u : j0 >= 0 ? (uint32_t)(bits >> j0) : (uint32_t)(bits << -j0) | ((1u << -j0) - 1);
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (!((seen >> x) & 1)) v[32 * w + x] = 0xff800000u;
           }
           // Values of rows past the end, and values of tree rows that are not finite, must not meet a zero probability: zeroed
-          // here (this thread: key row r); the latter are added back below for the rows that see them.
+          // here; the latter are added back below for the rows that see them.
           // (A parity cannot tell "V i has landed" from "what was in that slot before has not": the slots' earlier pieces are at
           // latest V i - 1, so its product is waited for first.)
           const int vb = (i + 1 < n ? 2 * i + 2 : 2 * n - 1) * S_::PIECES;
@@ -394,26 +408,27 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
             ok = ok && wait_for(&full[s], (c / S_::RING) & 1, failed);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            const int key = key0 + r;
-            if (key >= cached) {
-              unsigned char* base = ring + s * S_::PIECE + (r >> 3) * 1024 + (r & 7) * 128;
-              bool odd = false;
-#pragma unroll 1
-              for (int x = 0; x < S_::PIECE_BLOCKS * 8; ++x) {
-                uint4* at = (uint4*)(base + (x >> 3) * (TN * 128) + (x & 7) * 16);
-                uint32_t y[4] = {at->x, at->y, at->z, at->w};
-                bool change = key >= L;
+            // eight threads per row: its 16-byte chunks in any order, since each is looked at for itself
+            bool odd = false;
+            for (int y0 = max(cached - key0, 0) + (r >> 3); y0 < TN; y0 += 16) {
+              unsigned char* at = ring + s * S_::PIECE + (y0 >> 3) * 1024 + (y0 & 7) * 128 + (r & 7) * 16;
+#pragma unroll
+              for (int x = 0; x < S_::PIECE_BLOCKS; ++x) {
+                uint4* q4 = (uint4*)(at + x * (TN * 128));
+                const bool past = key0 + y0 >= L;
+                uint32_t y[4] = {q4->x, q4->y, q4->z, q4->w};
+                bool change = past;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                  if (key >= L) y[e] = 0u;
+                  if (past) y[e] = 0u;
                   const uint32_t m = exp_mask<T>();
                   if ((y[e] & m) == m) y[e] &= 0xffff0000u, change = odd = true;
                   if (((y[e] >> 16) & m) == m) y[e] &= 0x0000ffffu, change = odd = true;
                 }
-                if (change) *at = make_uint4(y[0], y[1], y[2], y[3]);
+                if (change) *q4 = make_uint4(y[0], y[1], y[2], y[3]);
               }
-              if (odd) odd_s = 1;
             }
+            if (odd) odd_s = 1;
           }
           if (!ok) break;
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -492,21 +507,30 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
             }
           }
         }
-        if (!rok) continue;
-        if (whole) {
-          T* out = (T*)p.out + (((long)b * p.nodes + node) * p.hq + hk * p.group + row - node * p.group) * D + x;
+        // through shared memory (the ring is idle), so that a row's 32 columns leave as whole lines
+        float* stage = (float*)ring + (warp - 4) * (32 * 36);
+        const float w = whole ? (is_node ? inv : 0.f) : 1.f;
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint4 y = make_uint4(pack2<T>(f[e] * inv, f[e + 1] * inv), pack2<T>(f[e + 2] * inv, f[e + 3] * inv),
-                                 pack2<T>(f[e + 4] * inv, f[e + 5] * inv), pack2<T>(f[e + 6] * inv, f[e + 7] * inv));
-            if (!is_node) y = make_uint4(0u, 0u, 0u, 0u);
-            *(uint4*)(out + e) = y;
-          }
-        } else {
-          float* acc = p.part_acc + (slot * TM + r) * D + x;
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) *(float4*)(acc + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+        for (int e = 0; e < 32; e += 4) {
+          float4 y = make_float4(f[e] * w, f[e + 1] * w, f[e + 2] * w, f[e + 3] * w);
+          if (whole && !is_node) y = make_float4(0.f, 0.f, 0.f, 0.f);
+          *(float4*)(stage + lane * 36 + e) = y;
         }
+        __syncwarp();
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          const int rr = y * 4 + (lane >> 3), orow = rt * TM + (warp - 4) * 32 + rr, c4 = (lane & 7) * 4;
+          const float4 z = *(const float4*)(stage + rr * 36 + c4);
+          if (orow >= p.rows) continue;
+          if (whole) {
+            const int onode = orow / p.group;
+            T* out = (T*)p.out + (((long)b * p.nodes + onode) * p.hq + hk * p.group + orow - onode * p.group) * D + x + c4;
+            *(uint2*)out = make_uint2(pack2<T>(z.x, z.y), pack2<T>(z.z, z.w));
+          } else {
+            *(float4*)(p.part_acc + (slot * TM + (warp - 4) * 32 + rr) * D + x + c4) = z;
+          }
+        }
+        __syncwarp();
       }
       if (rok && !whole) *(float2*)(p.part_ml + (slot * TM + r) * 2) = make_float2(mref, l);
     }
