@@ -7,9 +7,9 @@
 //
 // Work: the (sequence, KV head, row tile) units are laid out one behind the other in tiles of 128 keys, as many as each
 // sequence really has, and every CTA takes an equal stretch of that line, whatever units it crosses (the lengths are on the
-// device; a grid planned on the host from the cache's capacity waits for its longest sequence). A unit that one CTA
-// covers is finished there; of the others every CTA leaves (m, l, acc) in slot (CTA + unit), and tree_tc_merge_kernel adds
-// them in order.
+// device; a grid planned on the host from the cache's capacity waits for its longest sequence); cut_line has the
+// exception. A unit that one CTA covers is finished there; of the others every CTA leaves (m, l, acc) in a slot of its own, and
+// tree_tc_merge_kernel adds them in order.
 //
 // Roles: warp 0 loads (TMA boxes of 64 dims x 128 keys, 128-byte swizzle; a ring of 32 KB pieces), warp 1 issues the products,
 // warps 4-7 own a row per thread: scores out of TMEM, masks, maximum, exponentials, P into the columns of S. The products
@@ -164,17 +164,35 @@ __device__ __forceinline__ int live_rows(const TreeAttnParams& p, int b) {
   return (int)min((long)min(max(p.cache_len[b], 0), p.max_seq) + p.nodes, (long)p.max_seq);
 }
 __device__ __forceinline__ int live_tiles(const TreeAttnParams& p, int b) { return (live_rows(p, b) + TN - 1) / TN; }
-// Tiles of the sequences before b (all of them for b = batch), by one warp.
-__device__ __forceinline__ int tiles_before(const TreeAttnParams& p, int b, int lane) {
-  int n = 0;
-  for (int i = lane; i < b; i += 32) n += live_tiles(p, i);
-  return __reduce_add_sync(0xffffffffu, n);
+// How the line of tiles is cut, found by one warp (the same in the kernel and in the merge).
+struct Cut {
+  int before;  // tiles per unit of the sequences before b
+  int per_unit;  // > 0: that many CTAs for every unit, whose cuts then start with the unit; 0: equal stretches of the line
+  long share;    // tiles per CTA (equal stretches)
+};
+// Equal stretches keep every CTA busy whatever the lengths; a CTA that crosses into another unit, though, pays for its start
+// and its result twice (about EXTRA tiles' time), so units that are about equally long are cut each by itself.
+constexpr int EXTRA = 5;
+__device__ __forceinline__ Cut cut_line(const TreeAttnParams& p, int upb, int b, int lane) {
+  int before = 0, all = 0, longest = 0;
+  for (int i = lane; i < p.batch; i += 32) {
+    const int n = live_tiles(p, i);
+    all += n;
+    if (i < b) before += n;
+    longest = max(longest, n);
+  }
+  before = __reduce_add_sync(0xffffffffu, before);
+  all = __reduce_add_sync(0xffffffffu, all);
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  Cut c;
+  c.before = before;
+  const long even = ((long)all * upb + p.tc_ctas - 1) / p.tc_ctas;
+  c.share = even < TREE_TC_MIN_TILES ? TREE_TC_MIN_TILES : even;
+  const long per = p.tc_ctas / ((long)p.batch * upb);
+  c.per_unit = per > 0 && (longest + per - 1) / per <= c.share + EXTRA ? (int)per : 0;
+  return c;
 }
-// Tiles per CTA when `total` of them are shared out
-__device__ __forceinline__ long tiles_per_cta(const TreeAttnParams& p, long total) {
-  const long even = (total + p.tc_ctas - 1) / p.tc_ctas;
-  return even < TREE_TC_MIN_TILES ? TREE_TC_MIN_TILES : even;
-}
+__device__ __forceinline__ int unit_share(const Cut& c, int tiles) { return (tiles + c.per_unit - 1) / c.per_unit; }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const __grid_constant__ CUtensorMap kmap,
@@ -187,7 +205,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
   __shared__ unsigned long long anc[MAX_TREE_NODES];
   __shared__ int up[MAX_TREE_NODES];
   __shared__ uint32_t tmem_slot;
-  __shared__ int failed_s, odd_s, where[4];
+  __shared__ int failed_s, odd_s, where[5];
   volatile int* failed = &failed_s;
 
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
@@ -206,33 +224,38 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
   // ---- this CTA's stretch of the line of tiles ----
   const int row_tiles = (p.rows + TM - 1) / TM, upb = p.hkv * row_tiles;  // units per sequence
   if (warp == 2) {
-    const long total = (long)tiles_before(p, p.batch, lane) * upb;
-    const long share = tiles_per_cta(p, total), w0 = blockIdx.x * share;
-    int b = -1, before = 0, prefix = 0;  // the sequence that holds tile w0
-    for (int at = 0; at < p.batch && b < 0; at += 32) {
-      const int n = at + lane < p.batch ? live_tiles(p, at + lane) : 0;
-      int s = n;
+    const Cut cut = cut_line(p, upb, 0, lane);
+    int w_b = 0, w_unit = 0, w_tile = 0, w_left = 0;
+    if (cut.per_unit) {
+      const int u = blockIdx.x / cut.per_unit, part = blockIdx.x % cut.per_unit;
+      if (u < p.batch * upb) {
+        const int n = live_tiles(p, u / upb), share = unit_share(cut, n);
+        w_b = u / upb, w_unit = u % upb, w_tile = part * share, w_left = max(min(share, n - w_tile), 0);
+      }
+    } else {
+      const long w0 = blockIdx.x * cut.share;
+      int before = 0;
+      bool found = false;
+      for (int at = 0; at < p.batch && !found; at += 32) {  // the sequence that holds tile w0
+        const int n = at + lane < p.batch ? live_tiles(p, at + lane) : 0;
+        int s = n;
 #pragma unroll
-      for (int o = 1; o < 32; o *= 2) {
-        const int y = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += y;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, at + lane < p.batch && (long)(before + s) * upb > w0);
-      if (hit) {
-        const int l = __ffs(hit) - 1;
-        b = at + l;
-        prefix = before + __shfl_sync(0xffffffffu, s - n, l);
-      }
-      before += __shfl_sync(0xffffffffu, s, 31);
-    }
-    if (lane == 0) {
-      where[3] = 0;
-      if (b >= 0) {
-        const int n = live_tiles(p, b);
-        const long inside = w0 - (long)prefix * upb;
-        where[0] = b, where[1] = (int)(inside / n), where[2] = (int)(inside % n), where[3] = (int)min(share, total - w0);
+        for (int o = 1; o < 32; o *= 2) {
+          const int y = __shfl_up_sync(0xffffffffu, s, o);
+          if (lane >= o) s += y;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, at + lane < p.batch && (long)(before + s) * upb > w0);
+        if (hit) {
+          const int l = __ffs(hit) - 1, tiles = __shfl_sync(0xffffffffu, n, l);
+          const long inside = w0 - (long)(before + __shfl_sync(0xffffffffu, s - n, l)) * upb;
+          w_b = at + l, w_unit = (int)(inside / tiles), w_tile = (int)(inside % tiles);
+          w_left = (int)cut.share;  // (the last CTA's stretch ends with the last sequence)
+          found = true;
+        }
+        before += __shfl_sync(0xffffffffu, s, 31);
       }
     }
+    if (lane == 0) where[0] = w_b, where[1] = w_unit, where[2] = w_tile, where[3] = w_left, where[4] = cut.per_unit;
   }
   fence_before();
   __syncthreads();
@@ -242,55 +265,59 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
   int pieces = 0, done = 0;  // ring pieces and tiles before this segment: what the barriers' parities follow
   bool ok = true;
 
-  while (left > 0) {
+  const int per_unit = where[4];
+
+  while (left > 0 && b < p.batch) {
     const int L = live_rows(p, b), cached = min(max(p.cache_len[b], 0), p.max_seq), tiles = (L + TN - 1) / TN;
     const int n = min(left, tiles - tile);  // this segment: tiles tile .. tile + n - 1 of the unit
     const int hk = unit / row_tiles, rt = unit % row_tiles;
     const bool has_tree = (tile + n) * TN > cached;
 
-    // ---- queries to shared memory (K-major, swizzled), ancestors ----
-    {
-      constexpr int CH = D / 8, BATCH = 8;  // loads under way per thread
+    // ---- queries to shared memory (K-major, swizzled), ancestors: by warps 1 to 7, while warp 0 starts loading ----
+    auto sync_others = []() { asm volatile("bar.sync 2, %0;" ::"n"(TC_THREADS - 32) : "memory"); };
+    if (warp > 0) {
+      constexpr int CH = D / 8, BATCH = 10, N = TC_THREADS - 32;  // BATCH loads under way per thread
+      const int count = min(TM, p.rows - rt * TM) * CH;           // (rows past the last compute on what they find: nobody reads them)
 #pragma unroll 1
-      for (int i0 = t; i0 < TM * CH; i0 += TC_THREADS * BATCH) {
+      for (int i0 = t - 32; i0 < count; i0 += N * BATCH) {
         uint4 v[BATCH];
 #pragma unroll
         for (int x = 0; x < BATCH; ++x) {
-          const int i = i0 + x * TC_THREADS, r = i / CH, ch = i % CH, row = rt * TM + r, node = row / p.group;
-          v[x] = make_uint4(0u, 0u, 0u, 0u);
-          if (i < TM * CH && row < p.rows)
+          const int i = i0 + x * N, r = i / CH, ch = i % CH, row = rt * TM + r, node = row / p.group;
+          if (i < count)
             v[x] = *(const uint4*)((const T*)p.q + b * p.q_stride[0] + node * p.q_stride[1] + (hk * p.group + row - node * p.group) * p.q_stride[2] + ch * 8);
         }
 #pragma unroll
         for (int x = 0; x < BATCH; ++x) {
-          const int i = i0 + x * TC_THREADS, r = i / CH, ch = i % CH;
-          if (i < TM * CH) *(uint4*)(sm + (ch >> 3) * (TM * 128) + (r >> 3) * 1024 + (r & 7) * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v[x];
+          const int i = i0 + x * N, r = i / CH, ch = i % CH;
+          if (i < count) *(uint4*)(sm + (ch >> 3) * (TM * 128) + (r >> 3) * 1024 + (r & 7) * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v[x];
         }
       }
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    if (t == 0) odd_s = 0;
-    if (has_tree) {
-      if (t < p.nodes) {
-        const int pa = p.parents[(long)b * p.parents_stride + t];
-        const bool node = pa >= -1 && pa < t;
-        anc[t] = node ? 1ull << t : 0ull;
-        up[t] = node ? pa : -1;
-      }
-      __syncthreads();
-      for (int step = 1; step < p.nodes; step *= 2) {  // bits of up to 2 * step ancestors
-        unsigned long long bits = 0;
-        int u = -1;
-        if (t < p.nodes) {
-          bits = anc[t], u = up[t];
-          if (u >= 0) bits |= anc[u], u = up[u];
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (t == 32) odd_s = 0;
+      if (has_tree) {
+        const int i = t - 32;
+        if (i < p.nodes) {
+          const int pa = p.parents[(long)b * p.parents_stride + i];
+          const bool node = pa >= -1 && pa < i;
+          anc[i] = node ? 1ull << i : 0ull;
+          up[i] = node ? pa : -1;
         }
-        __syncthreads();
-        if (t < p.nodes) anc[t] = bits, up[t] = u;
-        __syncthreads();
+        sync_others();
+        for (int step = 1; step < p.nodes; step *= 2) {  // bits of up to 2 * step ancestors
+          unsigned long long bits = 0;
+          int u = -1;
+          if (i < p.nodes) {
+            bits = anc[i], u = up[i];
+            if (u >= 0) bits |= anc[u], u = up[u];
+          }
+          sync_others();
+          if (i < p.nodes) anc[i] = bits, up[i] = u;
+          sync_others();
+        }
       }
+      sync_others();
     }
-    __syncthreads();
 
     if (warp == 0) {
       // ---------------- loads: K 0, then K i + 1 and V i in turn ----------------
@@ -482,7 +509,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
       fence_after();
       asm volatile("bar.sync 1, 128;" ::: "memory");  // odd_s of all rows
       const bool odd = odd_s != 0 && has_tree;
-      const long slot = blockIdx.x + (long)b * upb + unit;
+      const long slot = per_unit ? blockIdx.x : blockIdx.x + (long)b * upb + unit;
       const bool whole = n == tiles;
       const int pa = rok ? p.parents[(long)b * p.parents_stride + node] : -2;
       const bool is_node = pa >= -1 && pa < node;
@@ -517,17 +544,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
           *(float4*)(stage + lane * 36 + e) = y;
         }
         __syncwarp();
+        float4 z[8];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) z[y] = *(const float4*)(stage + (y * 4 + (lane >> 3)) * 36 + (lane & 7) * 4);
 #pragma unroll
         for (int y = 0; y < 8; ++y) {
-          const int rr = y * 4 + (lane >> 3), orow = rt * TM + (warp - 4) * 32 + rr, c4 = (lane & 7) * 4;
-          const float4 z = *(const float4*)(stage + rr * 36 + c4);
+          const int rr = (warp - 4) * 32 + y * 4 + (lane >> 3), orow = rt * TM + rr, c4 = (lane & 7) * 4;
           if (orow >= p.rows) continue;
           if (whole) {
             const int onode = orow / p.group;
             T* out = (T*)p.out + (((long)b * p.nodes + onode) * p.hq + hk * p.group + orow - onode * p.group) * D + x + c4;
-            *(uint2*)out = make_uint2(pack2<T>(z.x, z.y), pack2<T>(z.z, z.w));
+            *(uint2*)out = make_uint2(pack2<T>(z[y].x, z[y].y), pack2<T>(z[y].z, z[y].w));
           } else {
-            *(float4*)(p.part_acc + (slot * TM + (warp - 4) * 32 + rr) * D + x + c4) = z;
+            *(float4*)(p.part_acc + (slot * TM + rr) * D + x + c4) = z[y];
           }
         }
         __syncwarp();
@@ -565,19 +594,26 @@ __global__ void __launch_bounds__(256) tree_tc_merge_kernel(const TreeAttnParams
   const int pa = p.parents[(long)b * p.parents_stride + node];
   const bool ok = pa >= -1 && pa < node;
   if (t < 32) {
-    const int before = tiles_before(p, b, t), all = tiles_before(p, p.batch, t), mine = live_tiles(p, b);
-    const long share = tiles_per_cta(p, (long)all * upb);
-    const long w = (long)before * upb + (long)(hk * row_tiles + rt) * mine;  // first tile of the unit
+    const Cut cut = cut_line(p, upb, b, t);
+    const int mine = live_tiles(p, b), u = b * upb + hk * row_tiles + rt;
     if (t == 0) {
-      first_s = w / share;
-      count_s = (int)((w + mine - 1) / share - first_s) + 1;
+      if (cut.per_unit) {
+        const int share = unit_share(cut, mine);
+        first_s = (long)u * cut.per_unit;
+        count_s = (mine + share - 1) / share;
+      } else {
+        const long w = (long)cut.before * upb + (long)(hk * row_tiles + rt) * mine;  // first tile of the unit
+        const long c0 = w / cut.share;
+        first_s = c0 + u;
+        count_s = (int)((w + mine - 1) / cut.share - c0) + 1;
+      }
     }
   }
   __syncthreads();
   const int count = count_s;
   if (count == 1) return;  // finished by the CTA that had all of it
   pdl_wait();
-  const long slot0 = first_s + (long)b * upb + hk * row_tiles + rt;
+  const long slot0 = first_s;
   const float2* ml = (const float2*)p.part_ml + slot0 * TM + row % TM;
   const float* acc = p.part_acc + (slot0 * TM + row % TM) * D + 4 * li;
   float m = -INFINITY;
