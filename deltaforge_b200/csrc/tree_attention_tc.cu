@@ -201,7 +201,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   unsigned char* ring = sm + S_::Q_BYTES;
-  __shared__ uint64_t full[S_::RING], freed[S_::RING], s_full[2], p_full[2], pv_done[2];
+  __shared__ uint64_t full[S_::RING], freed[S_::RING], s_full[2], p_full[2], pv_done[2], at_tree, v_fixed;
+  __shared__ float2 ml_s[TM];
   __shared__ unsigned long long anc[MAX_TREE_NODES];
   __shared__ int up[MAX_TREE_NODES];
   __shared__ uint32_t tmem_slot;
@@ -212,6 +213,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
   if (t == 0) {
     for (int i = 0; i < S_::RING; ++i) mbar_init(&full[i], 1), mbar_init(&freed[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&pv_done[i], 1);
+    mbar_init(&at_tree, 4);
+    mbar_init(&v_fixed, 2);
     failed_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -262,7 +265,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
   fence_after();
   const uint32_t tmem = tmem_slot;
   int b = where[0], unit = where[1], tile = where[2], left = where[3];  // left: tiles still to do
-  int pieces = 0, done = 0;  // ring pieces and tiles before this segment: what the barriers' parities follow
+  int pieces = 0, done = 0, fixes = 0;  // ring pieces, tiles and (warps 1 to 3) tiles with tree rows so far: what the barriers' parities follow
   bool ok = true;
 
   const int per_unit = where[4];
@@ -370,6 +373,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
           if (i + 1 < n) scores(i + 1);
           const int gi = done + i;
           ok = ok && wait_for(&p_full[gi & 1], (gi >> 1) & 1, failed);
+          if ((tile + i + 1) * TN > cached) {
+            ok = ok && wait_for(&v_fixed, fixes & 1, failed);
+            ++fixes;
+          }
           if (!ok) break;
           fence_after();
           for (int h = 0; h < S_::PIECES && ok; ++h, ++c) {
@@ -389,8 +396,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     } else if (warp >= 4) {
       // ---------------- softmax: thread = row ----------------
       const int r = t - 128, row = rt * TM + r;
-      const bool rok = row < p.rows;
-      const int node = rok ? row / p.group : 0;
+      const int node = row < p.rows ? row / p.group : 0;
       const int in_cache = L - cached;  // nodes that have a cache row
       const unsigned long long bits = has_tree ? anc[node] & (in_cache >= 64 ? ~0ull : (1ull << in_cache) - 1) : 0ull;
       const uint32_t lane_base = tmem + ((uint32_t)((warp - 4) * 32) << 16);
@@ -415,6 +421,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
           sl = 1.f;
         }
         if (key0 + TN > cached) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&at_tree);
           // bit x of word w: key key0 + 32 w + x is seen (short code: it runs once, out of a cold instruction cache)
 #pragma unroll
           for (int w = 0; w < TN / 32; ++w) {
@@ -424,41 +432,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
             for (int x = 0; x < 32; ++x)
               if (!((seen >> x) & 1)) v[32 * w + x] = 0xff800000u;
           }
-          // Values of rows past the end, and values of tree rows that are not finite, must not meet a zero probability: zeroed
-          // here; the latter are added back below for the rows that see them.
-          // (A parity cannot tell "V i has landed" from "what was in that slot before has not": the slots' earlier pieces are at
-          // latest V i - 1, so its product is waited for first.)
-          const int vb = (i + 1 < n ? 2 * i + 2 : 2 * n - 1) * S_::PIECES;
-          if (i > 0) ok = wait_for(&pv_done[(gi - 1) & 1], ((gi - 1) >> 1) & 1, failed);
-          for (int h = 0; h < S_::PIECES; ++h) {
-            const int c = pieces + vb + h, s = c % S_::RING;
-            ok = ok && wait_for(&full[s], (c / S_::RING) & 1, failed);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            // eight threads per row: its 16-byte chunks in any order, since each is looked at for itself
-            bool odd = false;
-            for (int y0 = max(cached - key0, 0) + (r >> 3); y0 < TN; y0 += 16) {
-              unsigned char* at = ring + s * S_::PIECE + (y0 >> 3) * 1024 + (y0 & 7) * 128 + (r & 7) * 16;
-#pragma unroll
-              for (int x = 0; x < S_::PIECE_BLOCKS; ++x) {
-                uint4* q4 = (uint4*)(at + x * (TN * 128));
-                const bool past = key0 + y0 >= L;
-                uint32_t y[4] = {q4->x, q4->y, q4->z, q4->w};
-                bool change = past;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  if (past) y[e] = 0u;
-                  const uint32_t m = exp_mask<T>();
-                  if ((y[e] & m) == m) y[e] &= 0xffff0000u, change = odd = true;
-                  if (((y[e] >> 16) & m) == m) y[e] &= 0x0000ffffu, change = odd = true;
-                }
-                if (change) *q4 = make_uint4(y[0], y[1], y[2], y[3]);
-              }
-            }
-            if (odd) odd_s = 1;
-          }
-          if (!ok) break;
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -503,65 +476,111 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[gi & 1]);
       }
-      // ---------------- the unit's result, or this CTA's part of it ----------------
       if (ok) ok = wait_for(&pv_done[(done + n - 1) & 1], ((done + n - 1) >> 1) & 1, failed);
-      ok = __all_sync(0xffffffffu, ok);
-      fence_after();
-      asm volatile("bar.sync 1, 128;" ::: "memory");  // odd_s of all rows
-      const bool odd = odd_s != 0 && has_tree;
-      const long slot = per_unit ? blockIdx.x : blockIdx.x + (long)b * upb + unit;
-      const bool whole = n == tiles;
-      const int pa = rok ? p.parents[(long)b * p.parents_stride + node] : -2;
-      const bool is_node = pa >= -1 && pa < node;
-      const float inv = 1.f / l;
-#pragma unroll 1
-      for (int x = 0; x < D; x += 32) {
-        uint32_t o[32];
-        tmem_ld32(lane_base + S_::O_COL + x, o);
-        tmem_wait_ld(o);
-        float f[32];
+      ml_s[r] = make_float2(mref, ok ? l : __int_as_float(0x7fffffff));  // (a wait that ran out: NaN)
+    } else {
+      // ---------------- warps 2 and 3: values that must not meet a zero probability ----------------
+      // Those of rows past the end are zeroed, and so are values of tree rows that are not finite; the latter are added back
+      // below for the rows that see them.
+      const int first = max(cached / TN - tile, 0);
+      for (int i = first; i < n; ++i) {
+        const int gi = done + i, key0 = (tile + i) * TN, r = t - 64;
+        // A parity cannot tell "this round has come" from "the round before the last has": the softmax warps say that they are at
+        // tile i (S i is there, hence PV i - 2 has been done), then PV i - 1 is waited for, at latest V of which was in V i's slots.
+        ok = ok && wait_for(&at_tree, fixes & 1, failed);
+        ++fixes;
+        if (i > 0) ok = ok && wait_for(&pv_done[(gi - 1) & 1], ((gi - 1) >> 1) & 1, failed);
+        const int vb = (i + 1 < n ? 2 * i + 2 : 2 * n - 1) * S_::PIECES;
+        bool odd = false;
+        for (int h = 0; h < S_::PIECES; ++h) {
+          const int c = pieces + vb + h, s = c % S_::RING;
+          ok = ok && wait_for(&full[s], (c / S_::RING) & 1, failed);
+          if (!ok) break;
+          // eight threads per row: its 16-byte chunks in any order, since each is looked at for itself
+          for (int y = max(cached - key0, 0) + (r >> 3); y < TN; y += 8) {
+            uint4* at = (uint4*)(ring + s * S_::PIECE + (y >> 3) * 1024 + (y & 7) * 128 + (r & 7) * 16);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) f[e] = ok ? __uint_as_float(o[e]) : __int_as_float(0x7fffffff);
-        if (odd && rok) {
+            for (int x = 0; x < S_::PIECE_BLOCKS; ++x, at += TN * 128 / 16) {
+              if (key0 + y >= L) {
+                *at = make_uint4(0u, 0u, 0u, 0u);
+                continue;
+              }
+              uint32_t v[4] = {at->x, at->y, at->z, at->w};
+              bool change = false;
+              const uint32_t m = exp_mask<T>();
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if ((v[e] & m) == m) v[e] &= 0xffff0000u, change = true;
+                if (((v[e] >> 16) & m) == m) v[e] &= 0x0000ffffu, change = true;
+              }
+              if (change) *at = make_uint4(v[0], v[1], v[2], v[3]), odd = true;
+            }
+          }
+        }
+        if (odd) odd_s = 1;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_fixed);
+      }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+
+    // ---------------- the unit's result, or this CTA's part of it: all warps, half of the columns each four ----------------
+    {
+      const int quarter = warp & 3, r = quarter * 32 + lane, row = rt * TM + r;
+      const bool odd = odd_s != 0 && has_tree, whole = n == tiles;
+      const uint32_t o_base = tmem + ((uint32_t)(quarter * 32) << 16) + S_::O_COL;
+      const long slot = per_unit ? blockIdx.x : blockIdx.x + (long)b * upb + unit;
+      const float2 ml = ml_s[r];
+      const float w = whole ? 1.f / ml.y : 1.f;
+      float* stage = (float*)ring + warp * (32 * 36);  // the ring is idle: a row's 32 columns leave as whole lines
+#pragma unroll 1
+      for (int x = (warp >> 2) * (D / 2); x < (warp >> 2) * (D / 2) + D / 2; x += 32) {
+        uint32_t o[32];
+        tmem_ld32(o_base + x, o);
+        tmem_wait_ld(o);
+        if (odd && row < p.rows) {
           for (int j = 0; j < p.nodes; ++j) {
             const int key = cached + j;
-            if (!((bits >> j) & 1) || key >= L || key < tile * TN || key >= (tile + n) * TN) continue;
+            if (!((anc[row / p.group] >> j) & 1) || key >= L || key < tile * TN || key >= (tile + n) * TN) continue;
             const T* y = (const T*)p.vcache + b * p.v_stride[0] + hk * p.v_stride[1] + key * p.v_stride[2] + x;
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
               const float z = elem_f<T>(y[e]);
-              if (!isfinite(z)) f[e] += z;
+              if (!isfinite(z)) o[e] = __float_as_uint(__uint_as_float(o[e]) + z);
             }
           }
         }
-        // through shared memory (the ring is idle), so that a row's 32 columns leave as whole lines
-        float* stage = (float*)ring + (warp - 4) * (32 * 36);
-        const float w = whole ? (is_node ? inv : 0.f) : 1.f;
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          float4 y = make_float4(f[e] * w, f[e + 1] * w, f[e + 2] * w, f[e + 3] * w);
-          if (whole && !is_node) y = make_float4(0.f, 0.f, 0.f, 0.f);
-          *(float4*)(stage + lane * 36 + e) = y;
-        }
+        for (int e = 0; e < 32; e += 4)
+          *(float4*)(stage + lane * 36 + e) = make_float4(__uint_as_float(o[e]) * w, __uint_as_float(o[e + 1]) * w, __uint_as_float(o[e + 2]) * w,
+                                                          __uint_as_float(o[e + 3]) * w);
         __syncwarp();
         float4 z[8];
 #pragma unroll
         for (int y = 0; y < 8; ++y) z[y] = *(const float4*)(stage + (y * 4 + (lane >> 3)) * 36 + (lane & 7) * 4);
+        const int rr0 = quarter * 32 + (lane >> 3), c4 = (lane & 7) * 4;
+        if (whole) {
 #pragma unroll
-        for (int y = 0; y < 8; ++y) {
-          const int rr = (warp - 4) * 32 + y * 4 + (lane >> 3), orow = rt * TM + rr, c4 = (lane & 7) * 4;
-          if (orow >= p.rows) continue;
-          if (whole) {
-            const int onode = orow / p.group;
-            T* out = (T*)p.out + (((long)b * p.nodes + onode) * p.hq + hk * p.group + orow - onode * p.group) * D + x + c4;
-            *(uint2*)out = make_uint2(pack2<T>(z[y].x, z[y].y), pack2<T>(z[y].z, z[y].w));
-          } else {
-            *(float4*)(p.part_acc + (slot * TM + rr) * D + x + c4) = z[y];
+          for (int y = 0; y < 8; ++y) {
+            const int orow = rt * TM + rr0 + 4 * y;
+            if (orow >= p.rows) break;
+            const int node = orow / p.group, pa = p.parents[(long)b * p.parents_stride + node];
+            T* out = (T*)p.out + (((long)b * p.nodes + node) * p.hq + hk * p.group + orow - node * p.group) * D + x + c4;
+            const bool is_node = pa >= -1 && pa < node;
+            *(uint2*)out = is_node ? make_uint2(pack2<T>(z[y].x, z[y].y), pack2<T>(z[y].z, z[y].w)) : make_uint2(0u, 0u);
           }
+        } else {
+          float* acc = p.part_acc + (slot * TM + rr0) * D + x + c4;
+#pragma unroll
+          for (int y = 0; y < 8; ++y)
+            if (rt * TM + rr0 + 4 * y < p.rows) *(float4*)(acc + 4 * y * D) = z[y];
         }
         __syncwarp();
       }
-      if (rok && !whole) *(float2*)(p.part_ml + (slot * TM + r) * 2) = make_float2(mref, l);
+      if (warp < 4 && row < p.rows && !whole) *(float2*)(p.part_ml + (slot * TM + r) * 2) = ml;
     }
     fence_before();
     __syncthreads();  // queries, O and the flags may be written again
