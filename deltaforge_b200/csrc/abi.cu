@@ -457,7 +457,7 @@ int dfb_tree_attention(const dfb_tree_attn_desc* d, void* stream) {
   p.out = d->out;
   p.splits = plan.splits;
   p.mt = plan.mt;
-  p.tc_ctas = plan.tc_ctas;
+  p.tc_groups = plan.tc_groups;
   if (need) {
     p.part_acc = (float*)d->scratch;
     p.part_ml = (float*)((char*)d->scratch + align_up(plan.slots * d->d * 4, 256));

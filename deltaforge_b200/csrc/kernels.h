@@ -341,14 +341,14 @@ struct TreeAttnParams {
   float scale;
   void* out;  // [batch, nodes, hq, d] contiguous
   int splits, mt;
-  int tc_ctas;      // > 0: the tcgen05 form, with that many CTAs
+  int tc_groups;    // > 0: the tcgen05 form, with that many groups of one CTA per 128 rows
   float* part_acc;  // [batch, hkv, splits, rows, d]; tcgen05: [slots, 128, d]
   float* part_ml;   // the same with 2 (maximum, sum) in the place of d
 };
 struct TreePlan {
   int mt;        // mma.sync: 16-row tiles per CTA
   int splits;    // mma.sync: key ranges
-  int tc_ctas;   // tcgen05: CTAs, 0 where mma.sync serves
+  int tc_groups; // tcgen05: groups of CTAs, 0 where mma.sync serves
   size_t slots;  // partial results of a row each may leave: rows of part_acc
 };
 // The least stretch of 128-key tiles a CTA of the tcgen05 form takes: below it the partial results cost more than they save.

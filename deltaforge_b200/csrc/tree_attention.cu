@@ -535,10 +535,10 @@ TreePlan tree_plan(int batch, int nodes, int hq, int hkv, int d, int max_seq, bo
   TreePlan pl = {};
   const int rows = nodes * (hq / hkv);
   if (tc_ok && d >= 64 && rows > 16) {
-    const long units = (long)batch * hkv * ((rows + 127) / 128), tiles = units * ((max_seq + 127) / 128);
-    const long ctas = (tiles + TREE_TC_MIN_TILES - 1) / TREE_TC_MIN_TILES;
-    pl.tc_ctas = (int)(ctas < 148 ? ctas : 148);
-    pl.slots = (size_t)(pl.tc_ctas + units) * 128;
+    const long row_tiles = (rows + 127) / 128, units = (long)batch * hkv, tiles = units * ((max_seq + 127) / 128);
+    const long most = row_tiles < 148 ? 148 / row_tiles : 1, groups = (tiles + TREE_TC_MIN_TILES - 1) / TREE_TC_MIN_TILES;
+    pl.tc_groups = (int)(groups < most ? groups : most);
+    pl.slots = (size_t)(pl.tc_groups + units) * row_tiles * 128;
     return pl;
   }
   pl.mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
@@ -559,7 +559,7 @@ TreePlan tree_plan(int batch, int nodes, int hq, int hkv, int d, int max_seq, bo
 }
 
 int launch_tree_attention(const TreeAttnParams& p, cudaStream_t stream) {
-  if (p.tc_ctas) return launch_tree_attention_tc(p, stream);
+  if (p.tc_groups) return launch_tree_attention_tc(p, stream);
   static OncePerDevice once;
   const int rc = once.run(configure_all);
   if (rc) return rc;
