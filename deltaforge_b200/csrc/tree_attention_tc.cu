@@ -602,29 +602,26 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
 }
 
-// One CTA per output row: the parts of its unit in the order of the CTAs that left them.
+// D / 4 lanes per output row, as many rows per CTA as 256 threads hold: the parts of the row's unit in the order of the groups
+// that left them, with a running maximum; the loads of eight parts are under way at once.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tree_tc_merge_kernel(const TreeAttnParams p) {
-  constexpr int LANES = D / 4, GROUPS = 256 / LANES;
-  __shared__ float4 part[GROUPS][LANES];
-  __shared__ float part_l[GROUPS], top[8];
+  constexpr int LANES = D / 4, ROWS = 256 / LANES, AHEAD = 8;
   __shared__ long first_s;
   __shared__ int count_s;
-  const int t = threadIdx.x, li = t % LANES, gi = t / LANES;
-  const int row = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, node = row / p.group;
-  const int row_tiles = (p.rows + TM - 1) / TM, upb = p.hkv, rt = row / TM;
-  const int pa = p.parents[(long)b * p.parents_stride + node];
-  const bool ok = pa >= -1 && pa < node;
+  const int t = threadIdx.x, li = t % LANES;
+  const int row = blockIdx.x * ROWS + t / LANES, hk = blockIdx.y, b = blockIdx.z;
+  const int row_tiles = (p.rows + TM - 1) / TM;
   if (t < 32) {
     const Cut cut = cut_line(p, b, t);
-    const int mine = live_tiles(p, b), u = b * upb + hk;
+    const int mine = live_tiles(p, b), u = b * p.hkv + hk;
     if (t == 0) {
       if (cut.per_unit) {
         const int share = unit_share(cut, mine);
         first_s = (long)u * cut.per_unit;
         count_s = (mine + share - 1) / share;
       } else {
-        const long w = (long)cut.before * upb + (long)hk * mine;  // first tile of the unit
+        const long w = (long)cut.before * p.hkv + (long)hk * mine;  // first tile of the unit
         const long c0 = w / cut.share;
         first_s = c0 + u;
         count_s = (int)((w + mine - 1) / cut.share - c0) + 1;
@@ -633,45 +630,36 @@ __global__ void __launch_bounds__(256) tree_tc_merge_kernel(const TreeAttnParams
   }
   __syncthreads();
   const int count = count_s;
-  if (count == 1) return;  // finished by the CTA that had all of it
+  if (count == 1 || row >= p.rows) return;  // one part: finished by the CTA that had all of it
+  const int node = row / p.group, pa = p.parents[(long)b * p.parents_stride + node];
+  const bool ok = pa >= -1 && pa < node;
+  const long step = (long)row_tiles * TM, at = (first_s * row_tiles + row / TM) * TM + row % TM;  // rows from one part to the next
+  const float2* ml = (const float2*)p.part_ml + at;
+  const float* acc = p.part_acc + at * D + 4 * li;
   pdl_wait();
-  const long slot0 = first_s;
-  const long step = (long)row_tiles * TM;  // rows from one slot of the unit to the next
-  const float2* ml = (const float2*)p.part_ml + (slot0 * row_tiles + rt) * TM + row % TM;
-  const float* acc = p.part_acc + ((slot0 * row_tiles + rt) * TM + row % TM) * D + 4 * li;
-  float m = -INFINITY;
-  for (int s = t; s < count; s += 256) m = fmaxf(m, __ldcg(ml + s * step).x);
-  m = warp_max(m);
-  if ((t & 31) == 0) top[t >> 5] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 8; ++w) m = fmaxf(m, top[w]);
-  const float ref = m == -INFINITY ? 0.f : m;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-#pragma unroll 4
-  for (int s = gi; s < count; s += GROUPS) {
-    const float2 v = __ldcg(ml + s * step);
-    const float4 y = __ldcg((const float4*)(acc + s * step * D));
-    const float w = exp2_fast(v.x - ref);
-    l = fmaf(v.y, w, l);
-    a.x = fmaf(y.x, w, a.x), a.y = fmaf(y.y, w, a.y), a.z = fmaf(y.z, w, a.z), a.w = fmaf(y.w, w, a.w);
-  }
-  part[gi][li] = a;
-  if (li == 0) part_l[gi] = l;
-  __syncthreads();
-  if (gi) return;
+  float m = -INFINITY, l = 0.f;
+  for (int s0 = 0; s0 < count; s0 += AHEAD) {
+    float2 v[AHEAD];
+    float4 y[AHEAD];
 #pragma unroll
-  for (int i = 1; i < GROUPS; ++i) {
-    const float4 y = part[i][li];
-    a.x += y.x, a.y += y.y, a.z += y.z, a.w += y.w;
-    l += part_l[i];
+    for (int i = 0; i < AHEAD; ++i) {
+      const int s = min(s0 + i, count - 1);
+      v[i] = __ldcg(ml + s * step);
+      y[i] = __ldcg((const float4*)(acc + s * step * D));
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (s0 + i >= count) break;
+      const float mn = fmaxf(m, v[i].x), ref = mn == -INFINITY ? 0.f : mn, f = exp2_fast(m - ref), w = exp2_fast(v[i].x - ref);
+      m = mn;
+      l = l * f + v[i].y * w;
+      a.x = a.x * f + y[i].x * w, a.y = a.y * f + y[i].y * w, a.z = a.z * f + y[i].z * w, a.w = a.w * f + y[i].w * w;
+    }
   }
   const float inv = 1.f / l;
-  T* out = (T*)p.out + (((long)b * p.nodes + node) * p.hq + hk * p.group + row % p.group) * D + 4 * li;
-  uint2 v = make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
-  if (!ok) v = make_uint2(0u, 0u);
-  *(uint2*)out = v;
+  T* out = (T*)p.out + (((long)b * p.nodes + node) * p.hq + hk * p.group + row - node * p.group) * D + 4 * li;
+  *(uint2*)out = ok ? make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv)) : make_uint2(0u, 0u);
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -723,7 +711,7 @@ int launch_one(const CUtensorMap& kmap, const CUtensorMap& vmap, const TreeAttnP
   tree_attention_tc_kernel<T, D><<<p.tc_groups * ((p.rows + TM - 1) / TM), TC_THREADS, Tc<D>::SMEM, stream>>>(kmap, vmap, p);
   const int rc = check_launch("tree attention (tcgen05)");
   if (rc) return rc;
-  if (launch_pdl(tree_tc_merge_kernel<T, D>, dim3(p.rows, p.hkv, p.batch), dim3(256), 0, stream, p) != cudaSuccess)
+  if (launch_pdl(tree_tc_merge_kernel<T, D>, dim3((p.rows + 1024 / D - 1) / (1024 / D), p.hkv, p.batch), dim3(256), 0, stream, p) != cudaSuccess)
     return check_launch("tree attention (tcgen05): merge");
   return check_launch("tree attention (tcgen05): merge");
 }
