@@ -5,7 +5,7 @@
 // Here 128 rows (node * group + head) are the M of tcgen05.mma: S = Q K^T into TMEM, P = 2^(S - m) back into TMEM as the A
 // operand of O += P V, O in TMEM as well (S and its successor 128 columns each, O one column per dim: 512 at head dim 256).
 //
-// Work: the (sequence, KV head) units are laid out one behind the other in tiles of 128 keys, as many as each sequence
+// Work: the (sequence, KV head) units are laid out one behind the other in tiles of 64 keys, as many as each sequence
 // really has, and every group of CTAs takes an equal stretch of that line, whatever units it crosses (the lengths are on the
 // device; a grid planned on the host from the cache's capacity waits for its longest sequence); cut_line has the
 // exception. The CTAs of a group are the row tiles: they walk through the same keys side by side, so that the second
@@ -13,14 +13,16 @@
 // one group covers is finished there; of the others every CTA leaves (m, l, acc) in a slot of its own, and
 // tree_tc_merge_kernel adds them in order.
 //
-// Roles: warp 0 loads (TMA boxes of 64 dims x 128 keys, 128-byte swizzle; a ring of 32 KB pieces), warp 1 issues the products,
-// warps 4-7 own a row per thread: scores out of TMEM, masks, maximum, exponentials, P into the columns of S. The products
-// of tile i + 1 run under the softmax of tile i. The maximum that P refers to is moved only when a row's true maximum is more
-// than 2^8 above it, so that O rarely has to be rescaled; sums stay exact because l refers to the same maximum.
+// Roles: warp 0 loads (TMA boxes of 64 dims x 64 keys, 128-byte swizzle; a ring of K and V tiles), warp 1 issues the products,
+// warps 2 and 3 look after values that must not meet a zero probability, warps 4-11 have two threads per row, half of a
+// tile's keys each: scores out of TMEM, masks, maximum, exponentials, P into the columns of S. The product of tile i + 1 runs
+// under the softmax of tile i. The maximum that P refers to is moved only when a row's true maximum is more than 2^8
+// above it, so that O rarely has to be rescaled; sums stay exact because l refers to the same maximum.
+// Q is in TMEM too (as A of the first product): shared memory is all ring, 224 KB of K and V on their way. With Q in 64 KB
+// of shared memory and tiles of 128 keys the ring held 2.5 tiles and the loop ran at 30 bytes per cycle and SM, limited by the
+// latency of the loads: 238 us at 8 sequences x 64 nodes x 32K rows.
 //
-// Bounds per tile of 128 keys at head dim 256: 2 x 1024 cycles of tensor time, 1024 cycles of ex2 on the softmax warps, and
-// 128 KB of K and V from the L2, 64 bytes per cycle and SM, which is what two row tiles of one unit cost (each reads
-// the same keys).
+// Bounds per tile of 64 keys at head dim 256: 1024 cycles of tensor time, 512 of ex2, 64 KB of K and V from the L2.
 //
 // Every wait is bounded; one that runs out makes the CTA leave NaN.
 #include <cuda.h>
@@ -33,21 +35,20 @@ namespace dfb {
 namespace {
 
 constexpr int TM = 128;          // query rows per tile
-constexpr int TN = 128;          // keys per tile
-constexpr int TC_THREADS = 256;
+constexpr int TN = 64;           // keys per tile
+constexpr int TC_WARPS = 12, TC_THREADS = TC_WARPS * 32;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LAZY = 8.f;      // rescale O when the maximum has grown by more than this (in powers of two)
 constexpr long long WAIT_CYCLES = 1LL << 28;
 
 template <int D> struct Tc {
-  static constexpr int BLOCKS = D / 64;               // 64-dim blocks of a row
-  static constexpr int PIECES = D == 256 ? 2 : 1;     // ring pieces per K or V tile
-  static constexpr int PIECE_BLOCKS = BLOCKS / PIECES;
-  static constexpr int PIECE = PIECE_BLOCKS * TN * 128;
-  static constexpr int Q_BYTES = BLOCKS * TM * 128;
-  static constexpr int RING = D == 256 ? 5 : 6;
-  static constexpr int SMEM = Q_BYTES + RING * PIECE + 1024;
-  static constexpr int O_COL = 0, S_COL = 256;        // TMEM columns: O, then two S of 128
+  static constexpr int BLOCKS = D / 64;                // 64-dim blocks of a row
+  static constexpr int PIECE = BLOCKS * TN * 128;      // bytes of a K or V tile, one slot of the ring
+  static constexpr int FIT = 224 * 1024 / PIECE, RING = FIT > 12 ? 12 : FIT;
+  static_assert(RING * PIECE >= 40960 + 3 * TM * 4, "the ring serves as the result's staging buffer");
+  static constexpr int SMEM = RING * PIECE + 1024;
+  // TMEM columns: O, one per dim; two S of 64, each with its P (two values per column) over its first half; Q, two values per column
+  static constexpr int O_COL = 0, S_COL = 256, Q_COL = 384;
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -101,11 +102,7 @@ template <> __device__ __forceinline__ uint32_t type_bits<__half>() { return 0u;
 template <typename T> __device__ __forceinline__ uint32_t instr_desc(int n, bool b_rows) {
   return 1u << 4 | type_bits<T>() << 7 | type_bits<T>() << 10 | (uint32_t)b_rows << 16 | (uint32_t)(n >> 3) << 17 | (uint32_t)(TM >> 4) << 24;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
-               "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-               : "memory");
-}
+// D (+)= A B, A in TMEM (a lane per row, two values per column), B in shared memory
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
                "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
@@ -139,6 +136,11 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
       "%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
       DFB_IN8(v, 0), DFB_IN8(v, 8), DFB_IN8(v, 16), DFB_IN8(v, 24)
       : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), DFB_IN8(v, 0),
+               DFB_IN8(v, 8)
+               : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -174,7 +176,7 @@ struct Cut {
 };
 // Equal stretches keep every CTA busy whatever the lengths; a CTA that crosses into another unit, though, pays for its start
 // and its result twice (about EXTRA tiles' time), so units that are about equally long are cut each by itself.
-constexpr int EXTRA = 5;
+constexpr int EXTRA = 10;
 __device__ __forceinline__ Cut cut_line(const TreeAttnParams& p, int b, int lane) {
   int before = 0, all = 0, longest = 0;
   for (int i = lane; i < p.batch; i += 32) {
@@ -201,12 +203,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
                                                                           const __grid_constant__ CUtensorMap vmap, const TreeAttnParams p) {
   using S_ = Tc<D>;
   extern __shared__ unsigned char smem_raw[];
-  unsigned char* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  unsigned char* ring = sm + S_::Q_BYTES;
+  unsigned char* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ uint64_t full[S_::RING], freed[S_::RING], s_full[2], p_full[2], pv_done[2], at_tree, v_fixed;
-  __shared__ float2 ml_s[TM];
+  __shared__ bf16 part_m[2][2][TM];  // by turns: the largest score of each half of a row, rounded (any reference will do, if both use the same)
+  float *row_l = (float*)(ring + 40960), *row_m = row_l + 2 * TM;  // at a unit's end, when the ring is idle: [2][TM] sums, [TM] maxima
   __shared__ unsigned long long anc[MAX_TREE_NODES];
-  __shared__ int up[MAX_TREE_NODES];
+  __shared__ unsigned char up[MAX_TREE_NODES];
   __shared__ uint32_t tmem_slot;
   __shared__ int failed_s, odd_s, where[5];
   volatile int* failed = &failed_s;
@@ -214,8 +216,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   if (t == 0) {
     for (int i = 0; i < S_::RING; ++i) mbar_init(&full[i], 1), mbar_init(&freed[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&pv_done[i], 1);
-    mbar_init(&at_tree, 4);
+    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 8), mbar_init(&pv_done[i], 1);
+    mbar_init(&at_tree, 8);
     mbar_init(&v_fixed, 2);
     failed_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -279,67 +281,63 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     const int hk = unit;
     const bool has_tree = (tile + n) * TN > cached;
 
-    // ---- queries to shared memory (K-major, swizzled), ancestors: by warps 1 to 7, while warp 0 starts loading ----
+    // ---- queries to TMEM (warps 4 to 11: a thread has half a row), ancestors (warps 2 and 3), while warp 0 starts loading ----
     auto sync_others = []() { asm volatile("bar.sync 2, %0;" ::"n"(TC_THREADS - 32) : "memory"); };
-    if (warp > 0) {
-      constexpr int CH = D / 8, BATCH = 10, N = TC_THREADS - 32;  // BATCH loads under way per thread
-      const int count = min(TM, p.rows - rt * TM) * CH;           // (rows past the last compute on what they find: nobody reads them)
-#pragma unroll 1
-      for (int i0 = t - 32; i0 < count; i0 += N * BATCH) {
-        uint4 v[BATCH];
+    const int half = (warp - 4) >> 2, r = (warp & 3) * 32 + lane, row = rt * TM + r;  // (warps 4 to 11)
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    if (warp >= 4) {
+      const int node = row / p.group;
+      const uint4* src = (const uint4*)((const T*)p.q + b * p.q_stride[0] + node * p.q_stride[1] + (hk * p.group + row - node * p.group) * p.q_stride[2] + half * (D / 2));
+      uint32_t v[D / 4];
 #pragma unroll
-        for (int x = 0; x < BATCH; ++x) {
-          const int i = i0 + x * N, r = i / CH, ch = i % CH, row = rt * TM + r, node = row / p.group;
-          if (i < count)
-            v[x] = *(const uint4*)((const T*)p.q + b * p.q_stride[0] + node * p.q_stride[1] + (hk * p.group + row - node * p.group) * p.q_stride[2] + ch * 8);
-        }
-#pragma unroll
-        for (int x = 0; x < BATCH; ++x) {
-          const int i = i0 + x * N, r = i / CH, ch = i % CH;
-          if (i < count) *(uint4*)(sm + (ch >> 3) * (TM * 128) + (r >> 3) * 1024 + (r & 7) * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v[x];
-        }
+      for (int x = 0; x < D / 16; ++x) {
+        const uint4 y = row < p.rows ? src[x] : make_uint4(0u, 0u, 0u, 0u);
+        v[4 * x] = y.x, v[4 * x + 1] = y.y, v[4 * x + 2] = y.z, v[4 * x + 3] = y.w;
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      if (t == 32) odd_s = 0;
+#pragma unroll
+      for (int x = 0; x < D / 4; x += 16) tmem_st16(lane_base + S_::Q_COL + half * (D / 4) + x, v + x);
+      tmem_wait_st();
+      fence_before();
+    } else if (warp >= 2) {
+      const int i = t - 64;
+      if (i == 0) odd_s = 0;
       if (has_tree) {
-        const int i = t - 32;
+        auto sync_two = []() { asm volatile("bar.sync 3, 64;" ::: "memory"); };
         if (i < p.nodes) {
           const int pa = p.parents[(long)b * p.parents_stride + i];
           const bool node = pa >= -1 && pa < i;
           anc[i] = node ? 1ull << i : 0ull;
-          up[i] = node ? pa : -1;
+          up[i] = node && pa >= 0 ? pa : 255;
         }
-        sync_others();
+        sync_two();
         for (int step = 1; step < p.nodes; step *= 2) {  // bits of up to 2 * step ancestors
           unsigned long long bits = 0;
-          int u = -1;
+          int u = 255;
           if (i < p.nodes) {
             bits = anc[i], u = up[i];
-            if (u >= 0) bits |= anc[u], u = up[u];
+            if (u < 255) bits |= anc[u], u = up[u];
           }
-          sync_others();
+          sync_two();
           if (i < p.nodes) anc[i] = bits, up[i] = u;
-          sync_others();
+          sync_two();
         }
       }
-      sync_others();
     }
+    if (warp > 0) sync_others();
 
     if (warp == 0) {
       // ---------------- loads: K 0, then K i + 1 and V i in turn ----------------
       if (lane == 0) {
         int c = pieces;
         auto load = [&](const CUtensorMap* map, int i) {
-          for (int h = 0; h < S_::PIECES && ok; ++h, ++c) {
-            const int s = c % S_::RING;
-            if (c >= S_::RING) ok = wait_for(&freed[s], (c / S_::RING - 1) & 1, failed);
-            if (!ok) break;
-            mbar_expect_tx(&full[s], S_::PIECE);
-            const uint32_t dst = smem_u32(ring + s * S_::PIECE);
+          const int s = c % S_::RING;
+          if (c >= S_::RING) ok = ok && wait_for(&freed[s], (c / S_::RING - 1) & 1, failed);
+          if (!ok) return;
+          mbar_expect_tx(&full[s], S_::PIECE);
+          const uint32_t dst = smem_u32(ring + s * S_::PIECE);
 #pragma unroll
-            for (int x = 0; x < S_::PIECE_BLOCKS; ++x)
-              tma_box(dst + x * (TN * 128), map, (h * S_::PIECE_BLOCKS + x) * 64, (tile + i) * TN, hk, b, &full[s]);
-          }
+          for (int x = 0; x < S_::BLOCKS; ++x) tma_box(dst + x * (TN * 128), map, x * 64, (tile + i) * TN, hk, b, &full[s]);
+          ++c;
         };
         load(&kmap, 0);
         for (int i = 0; i < n && ok; ++i) {
@@ -351,108 +349,99 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     } else if (warp == 1) {
       // ---------------- products ----------------
       if (lane == 0) {
+        fence_after();
         int c = pieces;
-        const uint32_t qa = smem_u32(sm), ra = smem_u32(ring);
-        const uint32_t id_s = instr_desc<T>(TN, false), id_o = instr_desc<T>(S_::PIECE_BLOCKS * 64, true);
+        const uint32_t ra = smem_u32(ring);
+        const uint32_t id_s = instr_desc<T>(TN, false), id_o = instr_desc<T>(D, true);
         auto scores = [&](int i) {
-          const int gi = done + i;
-          for (int h = 0; h < S_::PIECES && ok; ++h, ++c) {
-            const int s = c % S_::RING;
-            ok = wait_for(&full[s], (c / S_::RING) & 1, failed);
-            if (!ok) break;
-            fence_after();
+          const int gi = done + i, s = c % S_::RING;
+          ok = ok && wait_for(&full[s], (c / S_::RING) & 1, failed);
+          if (!ok) return;
 #pragma unroll
-            for (int x = 0; x < S_::PIECE_BLOCKS; ++x)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                mma_ss(tmem + S_::S_COL + (gi & 1) * TN, smem_desc(qa + (h * S_::PIECE_BLOCKS + x) * (TM * 128) + k * 32, 0),
-                       smem_desc(ra + s * S_::PIECE + x * (TN * 128) + k * 32, 0), id_s, (h | x | k) != 0);
-            commit(&freed[s]);
-          }
-          if (ok) commit(&s_full[gi & 1]);
+          for (int k = 0; k < D / 16; ++k)
+            mma_ts(tmem + S_::S_COL + (gi & 1) * TN, tmem + S_::Q_COL + k * 8, smem_desc(ra + s * S_::PIECE + (k >> 2) * (TN * 128) + (k & 3) * 32, 0), id_s,
+                   k != 0);
+          commit(&freed[s]);
+          commit(&s_full[gi & 1]);
+          ++c;
         };
         scores(0);
         for (int i = 0; i < n && ok; ++i) {
           if (i + 1 < n) scores(i + 1);
-          const int gi = done + i;
+          const int gi = done + i, s = c % S_::RING;
           ok = ok && wait_for(&p_full[gi & 1], (gi >> 1) & 1, failed);
           if ((tile + i + 1) * TN > cached) {
             ok = ok && wait_for(&v_fixed, fixes & 1, failed);
             ++fixes;
           }
+          ok = ok && wait_for(&full[s], (c / S_::RING) & 1, failed);
           if (!ok) break;
           fence_after();
-          for (int h = 0; h < S_::PIECES && ok; ++h, ++c) {
-            const int s = c % S_::RING;
-            ok = wait_for(&full[s], (c / S_::RING) & 1, failed);
-            if (!ok) break;
 #pragma unroll
-            for (int k = 0; k < TN / 16; ++k)
-              mma_ts(tmem + S_::O_COL + h * (S_::PIECE_BLOCKS * 64), tmem + S_::S_COL + (gi & 1) * TN + k * 8,
-                     smem_desc(ra + s * S_::PIECE + k * 2048, TN * 128), id_o, (i | k) != 0);
-            commit(&freed[s]);
-          }
-          if (ok) commit(&pv_done[gi & 1]);
+          for (int k = 0; k < TN / 16; ++k)
+            mma_ts(tmem + S_::O_COL, tmem + S_::S_COL + (gi & 1) * TN + k * 8, smem_desc(ra + s * S_::PIECE + k * 2048, TN * 128), id_o, (i | k) != 0);
+          commit(&freed[s]);
+          commit(&pv_done[gi & 1]);
+          ++c;
         }
       }
       __syncwarp();
     } else if (warp >= 4) {
-      // ---------------- softmax: thread = row ----------------
-      const int r = t - 128, row = rt * TM + r;
-      const int node = row < p.rows ? row / p.group : 0;
+      // ---------------- softmax: two threads per row, half of the tile's keys each ----------------
       const int in_cache = L - cached;  // nodes that have a cache row
-      const unsigned long long bits = has_tree ? anc[node] & (in_cache >= 64 ? ~0ull : (1ull << in_cache) - 1) : 0ull;
-      const uint32_t lane_base = tmem + ((uint32_t)((warp - 4) * 32) << 16);
+      const unsigned long long bits = !has_tree || row >= p.rows ? 0ull : anc[row / p.group] & (in_cache >= 64 ? ~0ull : (1ull << in_cache) - 1);
       const float sl0 = p.scale * LOG2E;
       float mref = -INFINITY, l = 0.f;
       for (int i = 0; i < n; ++i) {
-        const int gi = done + i, key0 = (tile + i) * TN;
+        const int gi = done + i, key0 = (tile + i) * TN + half * 32;
         const uint32_t scol = lane_base + S_::S_COL + (gi & 1) * TN;
         ok = ok && wait_for(&s_full[gi & 1], (gi >> 1) & 1, failed);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
         fence_after();
-        uint32_t v[TN];
-#pragma unroll
-        for (int x = 0; x < TN; x += 32) tmem_ld32(scol + x, v + x);
-#pragma unroll
-        for (int x = 0; x < TN; x += 32) tmem_wait_ld(v + x);
+        uint32_t v[32];
+        tmem_ld32(scol + half * 32, v);
+        tmem_wait_ld(v);
         float sl = sl0;
         if (sl <= 0.f) {  // (a scale that is not positive: applied first, so that masks and the maximum mean the same)
 #pragma unroll
-          for (int x = 0; x < TN; ++x) v[x] = __float_as_uint(__uint_as_float(v[x]) * sl);
+          for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(__uint_as_float(v[x]) * sl);
           sl = 1.f;
         }
-        if (key0 + TN > cached) {
+        if ((tile + i + 1) * TN > cached) {
           __syncwarp();
           if (lane == 0) mbar_arrive(&at_tree);
-          // bit x of word w: key key0 + 32 w + x is seen (short code: it runs once, out of a cold instruction cache)
+          const int j0 = key0 - cached;  // node number of the first key, negative in the prefix
+          const uint32_t seen = j0 <= -32 ? ~0u : j0 >= MAX_TREE_NODES ? 0u : j0 >= 0 ? (uint32_t)(bits >> j0) : (uint32_t)(bits << -j0) | ((1u << -j0) - 1);
 #pragma unroll
-          for (int w = 0; w < TN / 32; ++w) {
-            const int j0 = key0 + 32 * w - cached;  // node number of the word's first key, negative in the prefix
-            uint32_t seen = j0 <= -32 ? ~0u : j0 >= MAX_TREE_NODES ? 0u : j0 >= 0 ? (uint32_t)(bits >> j0) : (uint32_t)(bits << -j0) | ((1u << -j0) - 1);
-#pragma unroll
-            for (int x = 0; x < 32; ++x)
-              if (!((seen >> x) & 1)) v[32 * w + x] = 0xff800000u;
-          }
+          for (int x = 0; x < 32; ++x)
+            if (!((seen >> x) & 1)) v[x] = 0xff800000u;
         }
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int x = 0; x < TN; ++x) m4[x & 3] = fmaxf(m4[x & 3], __uint_as_float(v[x]));
-        const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl;
+        for (int x = 0; x < 32; ++x) m4[x & 3] = fmaxf(m4[x & 3], __uint_as_float(v[x]));
+        float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl;
+        const bf16 mine = f2bf(top);
+        part_m[gi & 1][half][r] = mine;
+        {  // the two warps of these rows meet: both have read S, and both go on or both give up
+          uint32_t go;
+          asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                       : "=r"(go)
+                       : "r"((uint32_t)ok), "r"(4 + (warp & 3))
+                       : "memory");
+          ok = go != 0;
+        }
+        if (!ok) break;
+        top = fmaxf(bf2f(mine), bf2f(part_m[gi & 1][half ^ 1][r]));
         if (i == 0) {
           mref = top;
         } else {
           const bool move = top > mref + LAZY;
-          if (__any_sync(0xffffffffu, move)) {
-            ok = ok && wait_for(&pv_done[(gi - 1) & 1], ((gi - 1) >> 1) & 1, failed);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+          if (__any_sync(0xffffffffu, move)) {  // (the same in both warps)
+            ok = wait_for(&pv_done[(gi - 1) & 1], ((gi - 1) >> 1) & 1, failed);
             fence_after();
             const float f = move ? exp2_fast(mref - top) : 1.f;
             if (move) mref = top, l *= f;
 #pragma unroll 1
-            for (int x = 0; x < D; x += 32) {
+            for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
               uint32_t o[32];
               tmem_ld32(lane_base + S_::O_COL + x, o);
               tmem_wait_ld(o);
@@ -460,64 +449,58 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
               for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
               tmem_st32(lane_base + S_::O_COL + x, o);
             }
-            tmem_wait_st();
           }
         }
         const float ref = mref == -INFINITY ? 0.f : mref;
         float l4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int x = 0; x < TN; x += 2) {
+        for (int x = 0; x < 32; x += 2) {
           const float p0 = exp2_fast(fmaf(__uint_as_float(v[x]), sl, -ref)), p1 = exp2_fast(fmaf(__uint_as_float(v[x + 1]), sl, -ref));
           l4[(x >> 1) & 3] += p0 + p1;
           v[x >> 1] = pack2<T>(p0, p1);
         }
         l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-        tmem_st32(scol, v);
-        tmem_st32(scol + 32, v + 32);
+        tmem_st16(scol + half * 16, v);
         tmem_wait_st();
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[gi & 1]);
       }
       if (ok) ok = wait_for(&pv_done[(done + n - 1) & 1], ((done + n - 1) >> 1) & 1, failed);
-      ml_s[r] = make_float2(mref, ok ? l : __int_as_float(0x7fffffff));  // (a wait that ran out: NaN)
+      row_l[half * TM + r] = ok ? l : __int_as_float(0x7fffffff);  // (a wait that ran out: NaN)
+      if (half == 0) row_m[r] = mref;
     } else {
       // ---------------- warps 2 and 3: values that must not meet a zero probability ----------------
       // Those of rows past the end are zeroed, and so are values of tree rows that are not finite; the latter are added back
       // below for the rows that see them.
       const int first = max(cached / TN - tile, 0);
       for (int i = first; i < n; ++i) {
-        const int gi = done + i, key0 = (tile + i) * TN, r = t - 64;
+        const int key0 = (tile + i) * TN, fr = t - 64;
         // A parity cannot tell "this round has come" from "the round before the last has": the softmax warps say that they are at
-        // tile i (S i is there, hence PV i - 2 has been done), then PV i - 1 is waited for, at latest V of which was in V i's slots.
+        // tile i. Then S i is there, PV i - 2 has been done, and what was in V i's slot before is older than that.
         ok = ok && wait_for(&at_tree, fixes & 1, failed);
         ++fixes;
-        if (i > 0) ok = ok && wait_for(&pv_done[(gi - 1) & 1], ((gi - 1) >> 1) & 1, failed);
-        const int vb = (i + 1 < n ? 2 * i + 2 : 2 * n - 1) * S_::PIECES;
+        const int c = pieces + (i + 1 < n ? 2 * i + 2 : 2 * n - 1), s = c % S_::RING;
+        ok = ok && wait_for(&full[s], (c / S_::RING) & 1, failed);
         bool odd = false;
-        for (int h = 0; h < S_::PIECES; ++h) {
-          const int c = pieces + vb + h, s = c % S_::RING;
-          ok = ok && wait_for(&full[s], (c / S_::RING) & 1, failed);
-          if (!ok) break;
-          // eight threads per row: its 16-byte chunks in any order, since each is looked at for itself
-          for (int y = max(cached - key0, 0) + (r >> 3); y < TN; y += 8) {
-            uint4* at = (uint4*)(ring + s * S_::PIECE + (y >> 3) * 1024 + (y & 7) * 128 + (r & 7) * 16);
+        // eight threads per row: its 16-byte chunks in any order, since each is looked at for itself
+        for (int y = max(cached - key0, 0) + (fr >> 3); ok && y < TN; y += 8) {
+          uint4* at = (uint4*)(ring + s * S_::PIECE + (y >> 3) * 1024 + (y & 7) * 128 + (fr & 7) * 16);
 #pragma unroll
-            for (int x = 0; x < S_::PIECE_BLOCKS; ++x, at += TN * 128 / 16) {
-              if (key0 + y >= L) {
-                *at = make_uint4(0u, 0u, 0u, 0u);
-                continue;
-              }
-              uint32_t v[4] = {at->x, at->y, at->z, at->w};
-              bool change = false;
-              const uint32_t m = exp_mask<T>();
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if ((v[e] & m) == m) v[e] &= 0xffff0000u, change = true;
-                if (((v[e] >> 16) & m) == m) v[e] &= 0x0000ffffu, change = true;
-              }
-              if (change) *at = make_uint4(v[0], v[1], v[2], v[3]), odd = true;
+          for (int x = 0; x < S_::BLOCKS; ++x, at += TN * 128 / 16) {
+            if (key0 + y >= L) {
+              *at = make_uint4(0u, 0u, 0u, 0u);
+              continue;
             }
+            uint32_t v[4] = {at->x, at->y, at->z, at->w};
+            bool change = false;
+            const uint32_t m = exp_mask<T>();
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if ((v[e] & m) == m) v[e] &= 0xffff0000u, change = true;
+              if (((v[e] >> 16) & m) == m) v[e] &= 0x0000ffffu, change = true;
+            }
+            if (change) *at = make_uint4(v[0], v[1], v[2], v[3]), odd = true;
           }
         }
         if (odd) odd_s = 1;
@@ -530,13 +513,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     __syncthreads();
     fence_after();
 
-    // ---------------- the unit's result, or this CTA's part of it: all warps, half of the columns each four ----------------
-    {
-      const int quarter = warp & 3, r = quarter * 32 + lane, row = rt * TM + r;
+    // ---------------- the unit's result, or this CTA's part of it: warps 0 to 7, half of the columns each four ----------------
+    if (warp < 8) {
+      const int quarter = warp & 3;
       const bool odd = odd_s != 0 && has_tree, whole = n == tiles;
-      const uint32_t o_base = tmem + ((uint32_t)(quarter * 32) << 16) + S_::O_COL;
+      const uint32_t o_base = lane_base + S_::O_COL;
       const long slot = (per_unit ? grp : grp + (long)b * upb + unit) * row_tiles + rt;
-      const float2 ml = ml_s[r];
+      const float2 ml = make_float2(row_m[r], row_l[r] + row_l[TM + r]);
       const float w = whole ? 1.f / ml.y : 1.f;
       float* stage = (float*)ring + warp * (32 * 36);  // the ring is idle: a row's 32 columns leave as whole lines
 #pragma unroll 1
@@ -589,7 +572,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     __syncthreads();  // queries, O and the flags may be written again
     fence_after();
     ok = ok && !*failed;
-    pieces += 2 * n * S_::PIECES;
+    pieces += 2 * n;
     done += n;
     left -= n;
     tile += n;
