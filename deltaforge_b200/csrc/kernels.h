@@ -351,8 +351,8 @@ struct TreePlan {
   int tc_groups; // tcgen05: groups of CTAs, 0 where mma.sync serves
   size_t slots;  // partial results of a row each may leave: rows of part_acc
 };
-// The least stretch of 64-key tiles a CTA of the tcgen05 form takes: below it the partial results cost more than they save.
-constexpr int TREE_TC_MIN_TILES = 4;
+// The least stretch of 128-key tiles a CTA of the tcgen05 form takes: below it the partial results cost more than they save.
+constexpr int TREE_TC_MIN_TILES = 2;
 int launch_tree_attention_tc(const TreeAttnParams& p, cudaStream_t stream);
 TreePlan tree_plan(int batch, int nodes, int hq, int hkv, int d, int max_seq, bool tc_ok);
 int launch_tree_attention(const TreeAttnParams& p, cudaStream_t stream);

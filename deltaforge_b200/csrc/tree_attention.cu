@@ -535,7 +535,7 @@ TreePlan tree_plan(int batch, int nodes, int hq, int hkv, int d, int max_seq, bo
   TreePlan pl = {};
   const int rows = nodes * (hq / hkv);
   if (tc_ok && d >= 64 && rows > 16) {
-    const long row_tiles = (rows + 127) / 128, units = (long)batch * hkv, tiles = units * ((max_seq + 63) / 64);
+    const long row_tiles = (rows + 127) / 128, units = (long)batch * hkv, tiles = units * ((max_seq + 127) / 128);
     const long most = row_tiles < 148 ? 148 / row_tiles : 1, groups = (tiles + TREE_TC_MIN_TILES - 1) / TREE_TC_MIN_TILES;
     pl.tc_groups = (int)(groups < most ? groups : most);
     pl.slots = (size_t)(pl.tc_groups + units) * row_tiles * 128;

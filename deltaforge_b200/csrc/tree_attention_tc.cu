@@ -5,7 +5,7 @@
 // Here 128 rows (node * group + head) are the M of tcgen05.mma: S = Q K^T into TMEM, P = 2^(S - m) back into TMEM as the A
 // operand of O += P V, O in TMEM as well (S and its successor 128 columns each, O one column per dim: 512 at head dim 256).
 //
-// Work: the (sequence, KV head) units are laid out one behind the other in tiles of 64 keys, as many as each sequence
+// Work: the (sequence, KV head) units are laid out one behind the other in tiles of 128 keys, as many as each sequence
 // really has, and every group of CTAs takes an equal stretch of that line, whatever units it crosses (the lengths are on the
 // device; a grid planned on the host from the cache's capacity waits for its longest sequence); cut_line has the
 // exception. The CTAs of a group are the row tiles: they walk through the same keys side by side, so that the second
@@ -13,16 +13,15 @@
 // one group covers is finished there; of the others every CTA leaves (m, l, acc) in a slot of its own, and
 // tree_tc_merge_kernel adds them in order.
 //
-// Roles: warp 0 loads (TMA boxes of 64 dims x 64 keys, 128-byte swizzle; a ring of K and V tiles), warp 1 issues the products,
-// warps 2 and 3 look after values that must not meet a zero probability, warps 4-11 have two threads per row, half of a
-// tile's keys each: scores out of TMEM, masks, maximum, exponentials, P into the columns of S. The product of tile i + 1 runs
-// under the softmax of tile i. The maximum that P refers to is moved only when a row's true maximum is more than 2^8
-// above it, so that O rarely has to be rescaled; sums stay exact because l refers to the same maximum.
-// Q is in TMEM too (as A of the first product): shared memory is all ring, 224 KB of K and V on their way. With Q in 64 KB
-// of shared memory and tiles of 128 keys the ring held 2.5 tiles and the loop ran at 30 bytes per cycle and SM, limited by the
-// latency of the loads: 238 us at 8 sequences x 64 nodes x 32K rows.
+// Roles: warp 0 loads (TMA boxes 64 dims wide, 128-byte swizzle; a ring of K and V pieces), warp 1 issues the products, warps
+// 2 and 3 look after values that must not meet a zero probability, warps 4-11 have two threads per row, half of a tile's
+// keys each: scores out of TMEM, masks, maximum, exponentials, P into the columns of S. The product of tile i + 1 runs under
+// the softmax of tile i. The maximum that P refers to is moved only when a row's true maximum is more than 2^8 above it,
+// so that O rarely has to be rescaled; sums stay exact because l refers to the same maximum.
 //
-// Bounds per tile of 64 keys at head dim 256: 1024 cycles of tensor time, 512 of ex2, 64 KB of K and V from the L2.
+// Bounds per tile of 128 keys at head dim 256: 2 x 1024 cycles of tensor time, 1024 of ex2, 128 KB of K and V from the L2. The
+// tensor time asks for wide products: with Q in TMEM (all of shared memory a ring) and tiles of 64 keys, an M 128 x N 64 x K 16
+// product took 75 cycles instead of 32, and 8 sequences x 64 nodes x 32K rows 247 us.
 //
 // Every wait is bounded; one that runs out makes the CTA leave NaN.
 #include <cuda.h>
@@ -35,20 +34,25 @@ namespace dfb {
 namespace {
 
 constexpr int TM = 128;          // query rows per tile
-constexpr int TN = 64;           // keys per tile
+constexpr int TN = 128;          // keys per tile
 constexpr int TC_WARPS = 12, TC_THREADS = TC_WARPS * 32;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LAZY = 8.f;      // rescale O when the maximum has grown by more than this (in powers of two)
 constexpr long long WAIT_CYCLES = 1LL << 28;
 
 template <int D> struct Tc {
-  static constexpr int BLOCKS = D / 64;                // 64-dim blocks of a row
-  static constexpr int PIECE = BLOCKS * TN * 128;      // bytes of a K or V tile, one slot of the ring
-  static constexpr int FIT = 224 * 1024 / PIECE, RING = FIT > 12 ? 12 : FIT;
+  static constexpr int BLOCKS = D / 64;                          // 64-dim blocks of a row
+  static constexpr int Q_BYTES = BLOCKS * TM * 128;
+  // A K or V tile comes in one or two pieces of at most 32 KB, one slot of the ring each: K cut along the dims (the first
+  // product contracts over them), V along the keys, so that every product has the widest N there is.
+  static constexpr int PIECES = D == 256 ? 2 : 1;
+  static constexpr int K_BLOCKS = BLOCKS / PIECES, V_KEYS = TN / PIECES;
+  static constexpr int PIECE = K_BLOCKS * TN * 128;
+  static constexpr int RING = D == 256 ? 5 : 6;
+  static constexpr int SMEM = Q_BYTES + RING * PIECE + 1024;
   static_assert(RING * PIECE >= 40960 + 3 * TM * 4, "the ring serves as the result's staging buffer");
-  static constexpr int SMEM = RING * PIECE + 1024;
-  // TMEM columns: O, one per dim; two S of 64, each with its P (two values per column) over its first half; Q, two values per column
-  static constexpr int O_COL = 0, S_COL = 256, Q_COL = 384;
+  // TMEM columns: O, one per dim; two S of 128, each with its P (two values per column) over its first half
+  static constexpr int O_COL = 0, S_COL = 256;
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -102,7 +106,12 @@ template <> __device__ __forceinline__ uint32_t type_bits<__half>() { return 0u;
 template <typename T> __device__ __forceinline__ uint32_t instr_desc(int n, bool b_rows) {
   return 1u << 4 | type_bits<T>() << 7 | type_bits<T>() << 10 | (uint32_t)b_rows << 16 | (uint32_t)(n >> 3) << 17 | (uint32_t)(TM >> 4) << 24;
 }
-// D (+)= A B, A in TMEM (a lane per row, two values per column), B in shared memory
+// D (+)= A B, B in shared memory, A there too (ss) or in TMEM (ts: a lane per row, two values per column)
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+               "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+               : "memory");
+}
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
                "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
@@ -136,11 +145,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
       "%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
       DFB_IN8(v, 0), DFB_IN8(v, 8), DFB_IN8(v, 16), DFB_IN8(v, 24)
       : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), DFB_IN8(v, 0),
-               DFB_IN8(v, 8)
-               : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -176,7 +180,7 @@ struct Cut {
 };
 // Equal stretches keep every CTA busy whatever the lengths; a CTA that crosses into another unit, though, pays for its start
 // and its result twice (about EXTRA tiles' time), so units that are about equally long are cut each by itself.
-constexpr int EXTRA = 10;
+constexpr int EXTRA = 5;
 __device__ __forceinline__ Cut cut_line(const TreeAttnParams& p, int b, int lane) {
   int before = 0, all = 0, longest = 0;
   for (int i = lane; i < p.batch; i += 32) {
@@ -203,7 +207,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
                                                                           const __grid_constant__ CUtensorMap vmap, const TreeAttnParams p) {
   using S_ = Tc<D>;
   extern __shared__ unsigned char smem_raw[];
-  unsigned char* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  unsigned char* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  unsigned char* ring = sm + S_::Q_BYTES;
   __shared__ uint64_t full[S_::RING], freed[S_::RING], s_full[2], p_full[2], pv_done[2], at_tree, v_fixed;
   __shared__ bf16 part_m[2][2][TM];  // by turns: the largest score of each half of a row, rounded (any reference will do, if both use the same)
   float *row_l = (float*)(ring + 40960), *row_m = row_l + 2 * TM;  // at a unit's end, when the ring is idle: [2][TM] sums, [TM] maxima
@@ -281,23 +286,29 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     const int hk = unit;
     const bool has_tree = (tile + n) * TN > cached;
 
-    // ---- queries to TMEM (warps 4 to 11: a thread has half a row), ancestors (warps 2 and 3), while warp 0 starts loading ----
+    // ---- queries to shared memory (warps 4 to 11; K-major, swizzled), ancestors (warps 2 and 3), while warp 0 starts loading ----
     auto sync_others = []() { asm volatile("bar.sync 2, %0;" ::"n"(TC_THREADS - 32) : "memory"); };
     const int half = (warp - 4) >> 2, r = (warp & 3) * 32 + lane, row = rt * TM + r;  // (warps 4 to 11)
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     if (warp >= 4) {
-      const int node = row / p.group;
-      const uint4* src = (const uint4*)((const T*)p.q + b * p.q_stride[0] + node * p.q_stride[1] + (hk * p.group + row - node * p.group) * p.q_stride[2] + half * (D / 2));
-      uint32_t v[D / 4];
+      constexpr int CH = D / 8, BATCH = CH / 4, N = 256;  // BATCH loads under way per thread, TM * CH in four rounds or fewer
+      const int count = min(TM, p.rows - rt * TM) * CH;    // (rows past the last compute on what they find: nobody reads them)
+#pragma unroll 1
+      for (int i0 = t - 128; i0 < count; i0 += N * BATCH) {
+        uint4 v[BATCH];
 #pragma unroll
-      for (int x = 0; x < D / 16; ++x) {
-        const uint4 y = row < p.rows ? src[x] : make_uint4(0u, 0u, 0u, 0u);
-        v[4 * x] = y.x, v[4 * x + 1] = y.y, v[4 * x + 2] = y.z, v[4 * x + 3] = y.w;
+        for (int x = 0; x < BATCH; ++x) {
+          const int i = i0 + x * N, qr = i / CH, ch = i % CH, qrow = rt * TM + qr, node = qrow / p.group;
+          if (i < count)
+            v[x] = *(const uint4*)((const T*)p.q + b * p.q_stride[0] + node * p.q_stride[1] + (hk * p.group + qrow - node * p.group) * p.q_stride[2] + ch * 8);
+        }
+#pragma unroll
+        for (int x = 0; x < BATCH; ++x) {
+          const int i = i0 + x * N, qr = i / CH, ch = i % CH;
+          if (i < count) *(uint4*)(sm + (ch >> 3) * (TM * 128) + (qr >> 3) * 1024 + (qr & 7) * 128 + (((ch & 7) ^ (qr & 7)) << 4)) = v[x];
+        }
       }
-#pragma unroll
-      for (int x = 0; x < D / 4; x += 16) tmem_st16(lane_base + S_::Q_COL + half * (D / 4) + x, v + x);
-      tmem_wait_st();
-      fence_before();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     } else if (warp >= 2) {
       const int i = t - 64;
       if (i == 0) odd_s = 0;
@@ -329,60 +340,82 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
       // ---------------- loads: K 0, then K i + 1 and V i in turn ----------------
       if (lane == 0) {
         int c = pieces;
-        auto load = [&](const CUtensorMap* map, int i) {
+        auto slot = [&]() {  // the next slot, once it is free
           const int s = c % S_::RING;
           if (c >= S_::RING) ok = ok && wait_for(&freed[s], (c / S_::RING - 1) & 1, failed);
-          if (!ok) return;
-          mbar_expect_tx(&full[s], S_::PIECE);
-          const uint32_t dst = smem_u32(ring + s * S_::PIECE);
-#pragma unroll
-          for (int x = 0; x < S_::BLOCKS; ++x) tma_box(dst + x * (TN * 128), map, x * 64, (tile + i) * TN, hk, b, &full[s]);
+          if (ok) mbar_expect_tx(&full[s], S_::PIECE);
           ++c;
+          return s;
         };
-        load(&kmap, 0);
+        auto load_k = [&](int i) {
+          for (int h = 0; h < S_::PIECES; ++h) {
+            const int s = slot();
+            if (!ok) return;
+#pragma unroll
+            for (int x = 0; x < S_::K_BLOCKS; ++x)
+              tma_box(smem_u32(ring + s * S_::PIECE) + x * (TN * 128), &kmap, (h * S_::K_BLOCKS + x) * 64, (tile + i) * TN, hk, b, &full[s]);
+          }
+        };
+        auto load_v = [&](int i) {
+          for (int h = 0; h < S_::PIECES; ++h) {
+            const int s = slot();
+            if (!ok) return;
+#pragma unroll
+            for (int x = 0; x < S_::BLOCKS; ++x)
+              tma_box(smem_u32(ring + s * S_::PIECE) + x * (S_::V_KEYS * 128), &vmap, x * 64, (tile + i) * TN + h * S_::V_KEYS, hk, b, &full[s]);
+          }
+        };
+        load_k(0);
         for (int i = 0; i < n && ok; ++i) {
-          if (i + 1 < n) load(&kmap, i + 1);
-          load(&vmap, i);
+          if (i + 1 < n) load_k(i + 1);
+          load_v(i);
         }
       }
       __syncwarp();
     } else if (warp == 1) {
       // ---------------- products ----------------
       if (lane == 0) {
-        fence_after();
         int c = pieces;
-        const uint32_t ra = smem_u32(ring);
+        const uint32_t qa = smem_u32(sm), ra = smem_u32(ring);
         const uint32_t id_s = instr_desc<T>(TN, false), id_o = instr_desc<T>(D, true);
         auto scores = [&](int i) {
-          const int gi = done + i, s = c % S_::RING;
-          ok = ok && wait_for(&full[s], (c / S_::RING) & 1, failed);
-          if (!ok) return;
+          const int gi = done + i;
+          for (int h = 0; h < S_::PIECES && ok; ++h, ++c) {
+            const int s = c % S_::RING;
+            ok = wait_for(&full[s], (c / S_::RING) & 1, failed);
+            if (!ok) return;
+            const uint64_t qd = smem_desc(qa + h * S_::K_BLOCKS * (TM * 128), 0), kd = smem_desc(ra + s * S_::PIECE, 0);
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            mma_ts(tmem + S_::S_COL + (gi & 1) * TN, tmem + S_::Q_COL + k * 8, smem_desc(ra + s * S_::PIECE + (k >> 2) * (TN * 128) + (k & 3) * 32, 0), id_s,
-                   k != 0);
-          commit(&freed[s]);
-          commit(&s_full[gi & 1]);
-          ++c;
+            for (int k = 0; k < S_::K_BLOCKS * 4; ++k) {  // (a descriptor's low bits are the address in units of 16 bytes)
+              const uint64_t at = (k >> 2) * (TM * 128 / 16) + (k & 3) * 2;
+              mma_ss(tmem + S_::S_COL + (gi & 1) * TN, qd + at, kd + at, id_s, (h | k) != 0);
+            }
+            commit(&freed[s]);
+          }
+          if (ok) commit(&s_full[gi & 1]);
         };
         scores(0);
         for (int i = 0; i < n && ok; ++i) {
           if (i + 1 < n) scores(i + 1);
-          const int gi = done + i, s = c % S_::RING;
+          const int gi = done + i;
           ok = ok && wait_for(&p_full[gi & 1], (gi >> 1) & 1, failed);
           if ((tile + i + 1) * TN > cached) {
             ok = ok && wait_for(&v_fixed, fixes & 1, failed);
             ++fixes;
           }
-          ok = ok && wait_for(&full[s], (c / S_::RING) & 1, failed);
           if (!ok) break;
           fence_after();
+          for (int h = 0; h < S_::PIECES && ok; ++h, ++c) {
+            const int s = c % S_::RING;
+            ok = wait_for(&full[s], (c / S_::RING) & 1, failed);
+            if (!ok) break;
+            const uint64_t vd = smem_desc(ra + s * S_::PIECE, S_::V_KEYS * 128);
+            const uint32_t pa = tmem + S_::S_COL + (gi & 1) * TN + h * (S_::V_KEYS / 2);
 #pragma unroll
-          for (int k = 0; k < TN / 16; ++k)
-            mma_ts(tmem + S_::O_COL, tmem + S_::S_COL + (gi & 1) * TN + k * 8, smem_desc(ra + s * S_::PIECE + k * 2048, TN * 128), id_o, (i | k) != 0);
-          commit(&freed[s]);
-          commit(&pv_done[gi & 1]);
-          ++c;
+            for (int k = 0; k < S_::V_KEYS / 16; ++k) mma_ts(tmem + S_::O_COL, pa + k * 8, vd + k * (2048 / 16), id_o, (i | h | k) != 0);
+            commit(&freed[s]);
+          }
+          if (ok) commit(&pv_done[gi & 1]);
         }
       }
       __syncwarp();
@@ -393,31 +426,36 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
       const float sl0 = p.scale * LOG2E;
       float mref = -INFINITY, l = 0.f;
       for (int i = 0; i < n; ++i) {
-        const int gi = done + i, key0 = (tile + i) * TN + half * 32;
+        const int gi = done + i, key0 = (tile + i) * TN + half * 64;
         const uint32_t scol = lane_base + S_::S_COL + (gi & 1) * TN;
         ok = ok && wait_for(&s_full[gi & 1], (gi >> 1) & 1, failed);
         fence_after();
-        uint32_t v[32];
-        tmem_ld32(scol + half * 32, v);
+        uint32_t v[64];
+        tmem_ld32(scol + half * 64, v);
+        tmem_ld32(scol + half * 64 + 32, v + 32);
         tmem_wait_ld(v);
+        tmem_wait_ld(v + 32);
         float sl = sl0;
         if (sl <= 0.f) {  // (a scale that is not positive: applied first, so that masks and the maximum mean the same)
 #pragma unroll
-          for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(__uint_as_float(v[x]) * sl);
+          for (int x = 0; x < 64; ++x) v[x] = __float_as_uint(__uint_as_float(v[x]) * sl);
           sl = 1.f;
         }
         if ((tile + i + 1) * TN > cached) {
           __syncwarp();
           if (lane == 0) mbar_arrive(&at_tree);
-          const int j0 = key0 - cached;  // node number of the first key, negative in the prefix
-          const uint32_t seen = j0 <= -32 ? ~0u : j0 >= MAX_TREE_NODES ? 0u : j0 >= 0 ? (uint32_t)(bits >> j0) : (uint32_t)(bits << -j0) | ((1u << -j0) - 1);
 #pragma unroll
-          for (int x = 0; x < 32; ++x)
-            if (!((seen >> x) & 1)) v[x] = 0xff800000u;
+          for (int w = 0; w < 2; ++w) {
+            const int j0 = key0 + 32 * w - cached;  // node number of the first key, negative in the prefix
+            const uint32_t seen = j0 <= -32 ? ~0u : j0 >= MAX_TREE_NODES ? 0u : j0 >= 0 ? (uint32_t)(bits >> j0) : (uint32_t)(bits << -j0) | ((1u << -j0) - 1);
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (!((seen >> x) & 1)) v[32 * w + x] = 0xff800000u;
+          }
         }
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int x = 0; x < 32; ++x) m4[x & 3] = fmaxf(m4[x & 3], __uint_as_float(v[x]));
+        for (int x = 0; x < 64; ++x) m4[x & 3] = fmaxf(m4[x & 3], __uint_as_float(v[x]));
         float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl;
         const bf16 mine = f2bf(top);
         part_m[gi & 1][half][r] = mine;
@@ -454,13 +492,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
         const float ref = mref == -INFINITY ? 0.f : mref;
         float l4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int x = 0; x < 32; x += 2) {
+        for (int x = 0; x < 64; x += 2) {
           const float p0 = exp2_fast(fmaf(__uint_as_float(v[x]), sl, -ref)), p1 = exp2_fast(fmaf(__uint_as_float(v[x + 1]), sl, -ref));
           l4[(x >> 1) & 3] += p0 + p1;
           v[x >> 1] = pack2<T>(p0, p1);
         }
         l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-        tmem_st16(scol + half * 16, v);
+        tmem_st32(scol + half * 32, v);
         tmem_wait_st();
         fence_before();
         __syncwarp();
@@ -475,32 +513,36 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
       // below for the rows that see them.
       const int first = max(cached / TN - tile, 0);
       for (int i = first; i < n; ++i) {
-        const int key0 = (tile + i) * TN, fr = t - 64;
+        const int gi = done + i, key0 = (tile + i) * TN, fr = t - 64;
         // A parity cannot tell "this round has come" from "the round before the last has": the softmax warps say that they are at
-        // tile i. Then S i is there, PV i - 2 has been done, and what was in V i's slot before is older than that.
+        // tile i (S i is there, hence PV i - 2 has been done), then PV i - 1 is waited for: nothing younger was in V i's slots.
         ok = ok && wait_for(&at_tree, fixes & 1, failed);
         ++fixes;
-        const int c = pieces + (i + 1 < n ? 2 * i + 2 : 2 * n - 1), s = c % S_::RING;
-        ok = ok && wait_for(&full[s], (c / S_::RING) & 1, failed);
+        if (i > 0) ok = ok && wait_for(&pv_done[(gi - 1) & 1], ((gi - 1) >> 1) & 1, failed);
         bool odd = false;
-        // eight threads per row: its 16-byte chunks in any order, since each is looked at for itself
-        for (int y = max(cached - key0, 0) + (fr >> 3); ok && y < TN; y += 8) {
-          uint4* at = (uint4*)(ring + s * S_::PIECE + (y >> 3) * 1024 + (y & 7) * 128 + (fr & 7) * 16);
+        for (int h = 0; h < S_::PIECES; ++h) {
+          const int c = pieces + (i + 1 < n ? 2 * i + 2 : 2 * n - 1) * S_::PIECES + h, s = c % S_::RING;
+          ok = ok && wait_for(&full[s], (c / S_::RING) & 1, failed);
+          // eight threads per row: its 16-byte chunks in any order, since each is looked at for itself
+          const int k0 = key0 + h * S_::V_KEYS;
+          for (int y = max(cached - k0, 0) + (fr >> 3); ok && y < S_::V_KEYS; y += 8) {
+            uint4* at = (uint4*)(ring + s * S_::PIECE + (y >> 3) * 1024 + (y & 7) * 128 + (fr & 7) * 16);
 #pragma unroll
-          for (int x = 0; x < S_::BLOCKS; ++x, at += TN * 128 / 16) {
-            if (key0 + y >= L) {
-              *at = make_uint4(0u, 0u, 0u, 0u);
-              continue;
-            }
-            uint32_t v[4] = {at->x, at->y, at->z, at->w};
-            bool change = false;
-            const uint32_t m = exp_mask<T>();
+            for (int x = 0; x < S_::BLOCKS; ++x, at += S_::V_KEYS * 128 / 16) {
+              if (k0 + y >= L) {
+                *at = make_uint4(0u, 0u, 0u, 0u);
+                continue;
+              }
+              uint32_t v[4] = {at->x, at->y, at->z, at->w};
+              bool change = false;
+              const uint32_t m = exp_mask<T>();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if ((v[e] & m) == m) v[e] &= 0xffff0000u, change = true;
-              if (((v[e] >> 16) & m) == m) v[e] &= 0x0000ffffu, change = true;
+              for (int e = 0; e < 4; ++e) {
+                if ((v[e] & m) == m) v[e] &= 0xffff0000u, change = true;
+                if (((v[e] >> 16) & m) == m) v[e] &= 0x0000ffffu, change = true;
+              }
+              if (change) *at = make_uint4(v[0], v[1], v[2], v[3]), odd = true;
             }
-            if (change) *at = make_uint4(v[0], v[1], v[2], v[3]), odd = true;
           }
         }
         if (odd) odd_s = 1;
@@ -572,7 +614,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     __syncthreads();  // queries, O and the flags may be written again
     fence_after();
     ok = ok && !*failed;
-    pieces += 2 * n;
+    pieces += 2 * n * S_::PIECES;
     done += n;
     left -= n;
     tile += n;
@@ -660,14 +702,14 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// The cache as [sequence][KV head][row][D] with the caller's strides; boxes of 64 dims x 128 rows.
-bool encode_cache(CUtensorMap* map, const void* base, const long* stride, const TreeAttnParams& p) {
+// The cache as [sequence][KV head][row][D] with the caller's strides; boxes of 64 dims x `rows` rows.
+bool encode_cache(CUtensorMap* map, const void* base, const long* stride, int rows, const TreeAttnParams& p) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return false;
   const cuuint64_t dims[4] = {(cuuint64_t)p.d, (cuuint64_t)p.max_seq, (cuuint64_t)p.hkv, (cuuint64_t)p.batch};
   const long row = p.max_seq > 1 ? stride[2] : p.d;  // (the stride of a dimension of one is never used and may be anything)
   const cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)(p.hkv > 1 ? stride[1] : row) * 2, (cuuint64_t)(p.batch > 1 ? stride[0] : row) * 2};
-  const cuuint32_t box[4] = {64, TN, 1, 1}, es[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, es[4] = {1, 1, 1, 1};
   return enc(map, p.is_fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void*)base, dims, strides, box, es,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -714,7 +756,7 @@ int launch_tree_attention_tc(const TreeAttnParams& p, cudaStream_t stream) {
   const int rc = once.run(configure_all);
   if (rc) return rc;
   CUtensorMap kmap, vmap;
-  if (!encode_cache(&kmap, p.kcache, p.k_stride, p) || !encode_cache(&vmap, p.vcache, p.v_stride, p)) {
+  if (!encode_cache(&kmap, p.kcache, p.k_stride, TN, p) || !encode_cache(&vmap, p.vcache, p.v_stride, p.d == 256 ? TN / 2 : TN, p)) {
     set_error("tree attention (tcgen05): tensor map for the cache failed");
     return 1;
   }
