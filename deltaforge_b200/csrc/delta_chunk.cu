@@ -18,10 +18,11 @@
 // added in fp32 (the tensor core truncates what it adds to a large accumulator). Log decays are summed in fp64 and kept as
 // two floats, so that differences of large sums stay exact.
 //
-// Scan: one warp owns 16 value columns and all key rows of its head's state, in registers, as the accumulators of
-// S^T (16 x dk). Their layout is that of the A operand of the next product, so R^T, V'^T, O^T and S^T follow from one
-// another inside the warp without an exchange or a barrier; k, q, T, P of the chunk come from shared memory, which two loader
-// warps fill by cp.async one to two chunks ahead. No wait spins.
+// Scan: two warps own 16 value columns of a head's state, half of the key rows each, in registers, as the accumulators of
+// S^T (16 x dk/2). Their layout is that of the A operand of the next product, so R^T, V'^T, O^T and S^T follow from one
+// another inside the warp; the two exchange their partial sums of K S and Q S once per chunk and share the tokens of the
+// output. k, q, T, P of the chunk come from shared memory, which two loader warps fill by cp.async one to two chunks
+// ahead. No wait spins.
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -447,15 +448,18 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
 
 // ---- the scan -------------------------------------------------------------------------------------------------------
 
+// NW: column tiles (of 16) per CTA; two warps each, and two loader warps.
 template <int DKP, int NW> struct Scan {
-  static constexpr int THREADS = (NW + 2) * 32;
+  static constexpr int THREADS = (2 * NW + 2) * 32;
   static constexpr int VROW = NW * 32;  // bytes of a token's values in a stage
   static constexpr int Q_OFF = C * DKP * 2, H_OFF = 2 * C * DKP * 2, V_OFF = H_OFF + HEAD_BYTES;
   static constexpr int STAGE = V_OFF + C * VROW;
-  static constexpr int OUT = NW * C * 32;  // per warp: 64 tokens x 16 columns
-  static constexpr int FIT = (224 * 1024 - OUT) / STAGE;
+  static constexpr int OUT = C / 2 * 32;                     // per warp: 32 tokens x 16 columns
+  static constexpr int SWAP = 2 * (32 + 16) * 32 * 4;       // per column tile: partial sums of both warps
+  static constexpr int REST = NW * (2 * OUT + SWAP);
+  static constexpr int FIT = (224 * 1024 - REST) / STAGE;
   static constexpr int STAGES = FIT > 3 ? 3 : FIT;
-  static constexpr int SMEM = STAGES * STAGE + OUT;
+  static constexpr int SMEM = STAGES * STAGE + REST;
 };
 
 template <int VROW> __device__ __forceinline__ uint32_t v_off(int row, int chunk) {
@@ -464,9 +468,9 @@ template <int VROW> __device__ __forceinline__ uint32_t v_off(int row, int chunk
 }
 
 template <int DKP, int NW, int NB, bool TREE>
-__global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const DeltaChunkParams p) {
+__global__ void __launch_bounds__((2 * NW + 2) * 32, 1) delta_scan_kernel(const DeltaChunkParams p) {
   using S_ = Scan<DKP, NW>;
-  constexpr int NT = DKP / 8;
+  constexpr int NT = DKP / 16;  // 8-wide tiles of key rows per warp: half of them
   extern __shared__ __align__(128) unsigned char smem[];
   const int vb = blockIdx.x, hv = blockIdx.y, b = blockIdx.z, hk = hv / (p.hv / p.hk);
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, g = lane >> 2, c = lane & 3;
@@ -474,8 +478,8 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
   const int nlive = min(max((len + C - 1) / C - p.chunk0, 0), p.chunks);  // chunks of this segment with tokens
   const int col_cta = vb * NW * 16;
 
-  if (warp >= NW) {  // ---- loader warps ----
-    const int lt = t - NW * 32;
+  if (warp >= 2 * NW) {  // ---- loader warps ----
+    const int lt = t - 2 * NW * 32;
     const long per = p.hk * (2L * C * DKP * 2) + p.hv * (long)HEAD_BYTES;
     auto load = [&](int n) {
       if (n < nlive) {
@@ -513,8 +517,9 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
     return;
   }
 
-  // ---- compute warps: 16 value columns each ----
-  const int col0 = col_cta + warp * 16;
+  // ---- compute warps: 16 value columns and half of the key rows each ----
+  const int ct = warp >> 1, hd = warp & 1;
+  const int col0 = col_cta + ct * 16;
   const bool cok0 = col0 + g < p.dv, cok1 = col0 + g + 8 < p.dv;
   const long sb = ((long)b * p.hv + hv) * p.dk * p.dv;
   const float* Sin = p.first ? p.state + sb : p.state_out + sb;
@@ -523,11 +528,13 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int d = 8 * n + 2 * c + (e & 1);
+      const int d = 8 * (hd * NT + n) + 2 * c + (e & 1);
       const bool ok = d < p.dk && (e < 2 ? cok0 : cok1);
       S[n][e] = ok ? Sin[(long)d * p.dv + col0 + g + 8 * (e >> 1)] : 0.f;
     }
-  unsigned char* obuf = smem + S_::STAGES * S_::STAGE + warp * (C * 32);
+  unsigned char* obuf = smem + S_::STAGES * S_::STAGE + warp * S_::OUT;
+  float4* swap = (float4*)(smem + S_::STAGES * S_::STAGE + 2 * NW * S_::OUT + ct * S_::SWAP);
+  float4 *mine = swap + hd * (12 * 32) + lane, *other = swap + (hd ^ 1) * (12 * 32) + lane;
   bf16* out = p.out + ((long)b * p.tokens * p.hv + hv) * p.dv + col0;
   const long orow = (long)p.hv * p.dv;
 
@@ -538,7 +545,7 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
     const float* sc = (const float*)(st + S_::H_OFF + 3 * SQ);
     const int tok0 = (p.chunk0 + n) * C;
 
-    // 1. S^T K^T (hi and lo) and S^T Q^T (hi)
+    // 1. S^T K^T (hi and lo) and S^T Q^T (hi) over this warp's key rows
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < NT; ++i) m = fmaxf(m, fmaxf(fmaxf(fabsf(S[i][0]), fabsf(S[i][1])), fmaxf(fabsf(S[i][2]), fabsf(S[i][3]))));
@@ -559,7 +566,7 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
 #pragma unroll
       for (int n2 = 0; n2 < NB; ++n2) {
         uint32_t kb[4], qb[4];
-        const uint32_t off = img_off<DKP>(16 * n2 + (lane & 7) + 8 * (lane >> 4), 2 * ks + ((lane >> 3) & 1));
+        const uint32_t off = img_off<DKP>(16 * n2 + (lane & 7) + 8 * (lane >> 4), hd * NT + 2 * ks + ((lane >> 3) & 1));
         ldsm4(ks_s + off, kb);
         ldsm4(qs_s + off, qb);
         mma_f16(x[2 * n2], hi, kb[0], kb[1]);
@@ -570,21 +577,48 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
         mma_f16(x[2 * n2 + 1], lo, kb[2], kb[3]);
       }
     }
+    // The other warp of these columns has the other key rows: K S is needed by both, Q S by the one that finishes a token's
+    // output (blocks of 16 tokens 0 and 3 here for the first warp, 1 and 2 for the second).
+    float o[2][2][4];  // own blocks, eight tokens each
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[i][e] *= sup, oq[i][e] *= sup;
+      mine[i * 32] = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        constexpr int LAST = 2 * NB - 1;
+        const int f0 = 6 * j + h, f1 = 2 + 2 * j + h;  // tile of block 0 or 3, of block 1 or 2
+        float4 give;
+        float* gv = &give.x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float a = f0 <= LAST ? oq[f0 <= LAST ? f0 : 0][e] : 0.f, z = f1 <= LAST ? oq[f1 <= LAST ? f1 : 0][e] : 0.f;
+          o[j][h][e] = hd ? z : a;
+          gv[e] = hd ? a : z;
+        }
+        mine[(8 + 2 * j + h) * 32] = give;
+      }
+    asm volatile("bar.sync %0, 64;" ::"r"(1 + ct) : "memory");
     // 2. R = V - diag(e^G) K S, then its halves
     m = 0.f;
 #pragma unroll
     for (int n2 = 0; n2 < NB; ++n2) {
       uint32_t vr[4];
-      ldsm4_t(vs_s + v_off<S_::VROW>(16 * n2 + (lane & 15), warp * 2 + (lane >> 4)), vr);
+      ldsm4_t(vs_s + v_off<S_::VROW>(16 * n2 + (lane & 15), ct * 2 + (lane >> 4)), vr);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int nt = 2 * n2 + h;
         const float2 w = *(const float2*)&sc[8 * nt + 2 * c];
+        const float4 y = other[nt * 32];
         const float2 v0 = __bfloat1622float2(*(const __nv_bfloat162*)&vr[h]), v1 = __bfloat1622float2(*(const __nv_bfloat162*)&vr[2 + h]);
-        x[nt][0] = v0.x - x[nt][0] * (w.x * sup);
-        x[nt][1] = v0.y - x[nt][1] * (w.y * sup);
-        x[nt][2] = v1.x - x[nt][2] * (w.x * sup);
-        x[nt][3] = v1.y - x[nt][3] * (w.y * sup);
+        x[nt][0] = v0.x - (x[nt][0] + y.x) * w.x;
+        x[nt][1] = v0.y - (x[nt][1] + y.y) * w.y;
+        x[nt][2] = v1.x - (x[nt][2] + y.z) * w.x;
+        x[nt][3] = v1.y - (x[nt][3] + y.w) * w.y;
         m = fmaxf(m, fmaxf(fmaxf(fabsf(x[nt][0]), fabsf(x[nt][1])), fmaxf(fabsf(x[nt][2]), fabsf(x[nt][3]))));
       }
     }
@@ -599,7 +633,7 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
         split2(x[2 * k + h][2] * rdown, x[2 * k + h][3] * rdown, rh[k][2 * h + 1], rl[k][2 * h + 1]);
       }
     }
-    // 3. V'^T = R^T T^T; block (i, j) of T is zero for j > i
+    // 3. V'^T = R^T T^T (both warps); block (i, j) of T is zero for j > i
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i) x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
 #pragma unroll
@@ -628,53 +662,55 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
         for (int e = 0; e < 4; ++e) x[i][e] *= u, m = fmaxf(m, fabsf(x[i][e]));
       }
     }
-    // 4. O^T = (S^T Q^T) diag(e^G) + V'^T P^T
-    const int ev = scale_exp(warp_max_abs(m));
+    // 4. O^T = (S^T Q^T) diag(e^G) + V'^T P^T for this warp's blocks of tokens (P is stored with its zeros)
     {
-      const float vdown = pow2(-ev);
-      float o[2 * NB][4];
+      const int ev = scale_exp(warp_max_abs(m));
+      const float vdown = pow2(-ev), vup = pow2(ev);
+      float pv[2][2][4];
 #pragma unroll
-      for (int i = 0; i < 2 * NB; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) pv[j][h][0] = pv[j][h][1] = pv[j][h][2] = pv[j][h][3] = 0.f;
+      const int block[2] = {hd ? 1 : 0, hd ? 2 : 3};
 #pragma unroll
       for (int k = 0; k < NB; ++k) {
         const uint32_t a[4] = {h2(x[2 * k][0] * vdown, x[2 * k][1] * vdown), h2(x[2 * k][2] * vdown, x[2 * k][3] * vdown),
                                h2(x[2 * k + 1][0] * vdown, x[2 * k + 1][1] * vdown), h2(x[2 * k + 1][2] * vdown, x[2 * k + 1][3] * vdown)};
 #pragma unroll
-        for (int n2 = k; n2 < NB; ++n2) {
+        for (int j = 0; j < (NB > 2 ? 2 : 1); ++j) {
+          if (j == 0 && k > 1) continue;
           uint32_t pb[4];
-          ldsm4(ti_s + 2 * SQ + img_off<C>(16 * n2 + (lane & 7) + 8 * (lane >> 4), 2 * k + ((lane >> 3) & 1)), pb);
-          mma_f16(o[2 * n2], a, pb[0], pb[1]);
-          mma_f16(o[2 * n2 + 1], a, pb[2], pb[3]);
+          ldsm4(ti_s + 2 * SQ + img_off<C>(16 * block[j] + (lane & 7) + 8 * (lane >> 4), 2 * k + ((lane >> 3) & 1)), pb);
+          mma_f16(pv[j][0], a, pb[0], pb[1]);
+          mma_f16(pv[j][1], a, pb[2], pb[3]);
         }
       }
-      const float vup = pow2(ev);
       __syncwarp();  // the previous chunk's outputs have left the buffer
 #pragma unroll
-      for (int n2 = 0; n2 < NB; ++n2) {
+      for (int j = 0; j < (NB > 2 ? 2 : 1); ++j) {
         uint32_t w[4];
-        const float up = vup * sc[3 * C + 8 + n2];  // as is P
+        const float up = vup * sc[3 * C + 8 + block[j]];  // P too is scaled per 16 rows
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int nt = 2 * n2 + h;
-          const float2 f = *(const float2*)&sc[2 * C + 8 * nt + 2 * c];
-          const float f0 = f.x * sup, f1 = f.y * sup;
-          const __nv_bfloat162 a = __floats2bfloat162_rn(oq[nt][0] * f0 + o[nt][0] * up, oq[nt][1] * f1 + o[nt][1] * up);
-          const __nv_bfloat162 z = __floats2bfloat162_rn(oq[nt][2] * f0 + o[nt][2] * up, oq[nt][3] * f1 + o[nt][3] * up);
+          const float2 f = *(const float2*)&sc[2 * C + 16 * block[j] + 8 * h + 2 * c];
+          const float4 y = other[(8 + 2 * j + h) * 32];
+          const __nv_bfloat162 a = __floats2bfloat162_rn((o[j][h][0] + y.x) * f.x + pv[j][h][0] * up, (o[j][h][1] + y.y) * f.y + pv[j][h][1] * up);
+          const __nv_bfloat162 z = __floats2bfloat162_rn((o[j][h][2] + y.z) * f.x + pv[j][h][2] * up, (o[j][h][3] + y.w) * f.y + pv[j][h][3] * up);
           w[2 * h] = *(const uint32_t*)&a, w[2 * h + 1] = *(const uint32_t*)&z;
         }
-        const int row = 16 * n2 + 8 * (lane >> 4) + (lane & 7), half = (lane >> 3) & 1;
+        const int row = 16 * j + 8 * (lane >> 4) + (lane & 7), half = (lane >> 3) & 1;
         stsm4_t(smem_u32(obuf) + row * 32 + ((half ^ ((row >> 2) & 1)) << 4), w[0], w[1], w[2], w[3]);
       }
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const int row = 16 * i + (lane >> 1), half = lane & 1, tok = tok0 + row;
-        if (tok < p.tokens && col0 + half * 8 < p.dv)
+      for (int j = 0; j < (NB > 2 ? 2 : 1); ++j) {
+        const int row = 16 * j + (lane >> 1), half = lane & 1, tok = tok0 + 16 * block[j] + (lane >> 1);
+        if (block[j] < NB && tok < p.tokens && col0 + half * 8 < p.dv)
           *(uint4*)(out + tok * orow + half * 8) = *(const uint4*)(obuf + row * 32 + ((half ^ ((row >> 2) & 1)) << 4));
       }
     }
     if (TREE) break;
-    // 5. S^T = e^G_C S^T + (V' diag(e^(G_C - G)))^T K, accumulated apart
+    // 5. S^T = e^G_C S^T + (V' diag(e^(G_C - G)))^T K over this warp's key rows, accumulated apart
     m = 0.f;
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i) {
@@ -692,30 +728,37 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
         split2(x[2 * k + h][2] * udown, x[2 * k + h][3] * udown, rh[k][2 * h + 1], rl[k][2 * h + 1]);
       }
     }
+    // two pairs of tiles at a time: four chains of products
 #pragma unroll
-    for (int j2 = 0; j2 < NT / 2; ++j2) {
-      float a0[4] = {0.f, 0.f, 0.f, 0.f}, a1[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int j4 = 0; j4 < NT / 4; ++j4) {
+      float a[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i][0] = a[i][1] = a[i][2] = a[i][3] = 0.f;
 #pragma unroll
       for (int k = 0; k < NB; ++k) {
-        uint32_t kb[4];
-        ldsm4_t(ks_s + img_off<DKP>(16 * k + (lane & 15), 2 * j2 + (lane >> 4)), kb);
-        mma_f16(a0, rh[k], kb[0], kb[1]);
-        mma_f16(a1, rh[k], kb[2], kb[3]);
-        mma_f16(a0, rl[k], kb[0], kb[1]);
-        mma_f16(a1, rl[k], kb[2], kb[3]);
+        uint32_t k0[4], k1[4];
+        ldsm4_t(ks_s + img_off<DKP>(16 * k + (lane & 15), hd * NT + 4 * j4 + (lane >> 4)), k0);
+        ldsm4_t(ks_s + img_off<DKP>(16 * k + (lane & 15), hd * NT + 4 * j4 + 2 + (lane >> 4)), k1);
+        mma_f16(a[0], rh[k], k0[0], k0[1]);
+        mma_f16(a[1], rh[k], k0[2], k0[3]);
+        mma_f16(a[2], rh[k], k1[0], k1[1]);
+        mma_f16(a[3], rh[k], k1[2], k1[3]);
+        mma_f16(a[0], rl[k], k0[0], k0[1]);
+        mma_f16(a[1], rl[k], k0[2], k0[3]);
+        mma_f16(a[2], rl[k], k1[0], k1[1]);
+        mma_f16(a[3], rl[k], k1[2], k1[3]);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        S[2 * j2][e] = fmaf(a0[e], uup, S[2 * j2][e] * decay);
-        S[2 * j2 + 1][e] = fmaf(a1[e], uup, S[2 * j2 + 1][e] * decay);
-      }
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) S[4 * j4 + i][e] = fmaf(a[i][e], uup, S[4 * j4 + i][e] * decay);
     }
   }
 
   // rows of tokens that no chunk covered: zeros
   {
     const int from = (p.chunk0 + nlive) * C, to = min(p.tokens, (p.chunk0 + p.chunks) * C);
-    for (int i = lane; i < (to - from) * 2; i += 32) {
+    for (int i = lane + 32 * hd; i < (to - from) * 2; i += 64) {
       const int tok = from + (i >> 1), half = i & 1;
       if (col0 + half * 8 < p.dv) *(uint4*)(out + tok * orow + half * 8) = make_uint4(0u, 0u, 0u, 0u);
     }
@@ -726,7 +769,7 @@ __global__ void __launch_bounds__((NW + 2) * 32, 1) delta_scan_kernel(const Delt
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int d = 8 * n + 2 * c + (e & 1);
+      const int d = 8 * (hd * NT + n) + 2 * c + (e & 1);
       if (d < p.dk && (e < 2 ? cok0 : cok1)) So[(long)d * p.dv + col0 + g + 8 * (e >> 1)] = S[n][e];
     }
 }
@@ -848,7 +891,7 @@ int with_nb(int nb, F f) {
 }
 template <bool TREE, int DKP, typename F>
 int with_nw(int nw, int nb, F f) {
-  return nw == 2 ? with_nb<TREE, DKP, 2>(nb, f) : nw == 4 ? with_nb<TREE, DKP, 4>(nb, f) : with_nb<TREE, DKP, 8>(nb, f);
+  return nw == 2 ? with_nb<TREE, DKP, 2>(nb, f) : with_nb<TREE, DKP, 4>(nb, f);
 }
 template <typename F>
 int with_instance(bool tree, int dkp, int nw, int nb, F f) {
@@ -868,7 +911,7 @@ struct Configure {
 int configure_all() {
   for (int tree = 0; tree < 2; ++tree)
     for (int dkp = 64; dkp <= 128; dkp *= 2)
-      for (int nw = 2; nw <= 8; nw *= 2)
+      for (int nw = 2; nw <= 4; nw *= 2)
         for (int nb = 1; nb <= 4; nb *= 2)
           if (const int rc = with_instance(tree, dkp, nw, nb, Configure())) return rc;
   return 0;
@@ -907,8 +950,8 @@ int launch_delta_chunk(const DeltaChunkParams& args, cudaStream_t stream) {
   const int chunks = (p.tokens + C - 1) / C;
   p.seg_chunks = segment_chunks(p.batch, p.tokens, p.hk, p.hv, p.dk);
   // Columns per CTA: few (32) while that is what it takes to put every SM to work, else as many as share the loads.
-  const long warps = (long)p.batch * p.hv * ((p.dv + 15) / 16);
-  const int nw = warps <= 2 * 148 ? 2 : warps <= 4 * 148 ? 4 : 8;
+  const long col_tiles = (long)p.batch * p.hv * ((p.dv + 15) / 16);  // column tiles
+  const int nw = col_tiles <= 2 * 148 ? 2 : 4;
   for (int at = 0; at < chunks; at += p.seg_chunks) {
     p.chunk0 = at;
     p.chunks = chunks - at < p.seg_chunks ? chunks - at : p.seg_chunks;
