@@ -25,8 +25,6 @@
 // ahead. No wait spins.
 #include <cuda_fp16.h>
 
-#include <type_traits>
-
 #include "common.cuh"
 #include "kernels.h"
 
@@ -88,6 +86,8 @@ __device__ __forceinline__ int scale_exp(float m) {
   const int e = (int)((__float_as_uint(m) >> 23) & 255) - 127 - 12;
   return e < -110 ? -110 : e > 110 ? 110 : e;
 }
+// The same for a row whose sum of squares is ss: no element exceeds its root.
+__device__ __forceinline__ int norm_exp(float ss) { return (((int)((__float_as_uint(ss) >> 23) & 255) - 127 + 2) >> 1) - 13; }
 // Largest of the lanes' non-negative values, whose bit patterns order like the values
 __device__ __forceinline__ float warp_max_abs(float m) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))); }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
@@ -107,12 +107,28 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// z[r] = sum over m < M of a[4 r][m] y[m]: every fourth row of a (stride TS) against one column of y (stride TS). The four groups
+// of lanes take neighbouring rows, which lie in different banks.
+template <int R, int M>
+__device__ __forceinline__ void block_product(float (&z)[R], const float* a, const float* y) {
+#pragma unroll
+  for (int r = 0; r < R; ++r) z[r] = 0.f;
+#pragma unroll
+  for (int m = 0; m < M; m += 4) {
+    const float y0 = y[m * TS], y1 = y[(m + 1) * TS], y2 = y[(m + 2) * TS], y3 = y[(m + 3) * TS];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float4 x = *(const float4*)(a + 4 * r * TS + m);
+      z[r] = fmaf(x.x, y0, fmaf(x.y, y1, fmaf(x.z, y2, fmaf(x.w, y3, z[r]))));
+    }
+  }
+}
+
 // One CTA per (chunk, value head, sequence); warp w owns rows 16 w .. 16 w + 15 of all 64 x 64 matrices.
 //   1. keys and queries to shared memory (bf16), their norms and fp16 images; log decays summed (in units of log 2)
 //   2. K K^T and Q K^T rows by mma; decays; A to shared memory, P to its image
 //   3. the 16 x 16 diagonal blocks of (I + A)^-1 by substitution, a column per lane
-//   4. the blocks below by block forward substitution, T_ij = -T_ii sum_k A_ik T_kj. Columns of T are independent: warp 1
-//      takes block column 1, warp 2 block column 2, warps 0 and 3 half of block column 0 each (5, 2, 4.5, 4.5 products)
+//   4. two doublings, 16 -> 32 -> 64
 //   5. T diag(beta) in halves to its images
 // Bound by latency: three to four CTAs share an SM. Scales are per warp (16 rows), so no CTA-wide maximum is needed.
 template <int DKP, bool TREE>
@@ -220,24 +236,16 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
 #pragma unroll
       for (int pass = 0; pass < 4; ++pass) {
         const int row = pass * 16 + (t >> 3);
-        float ss = 0.f, mx = 0.f;
+        float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const bf16* e = (const bf16*)&raw[which][pass][i];
 #pragma unroll
-          for (int y = 0; y < 8; ++y) {
-            const float x = bf2f(e[y]);
-            ss = fmaf(x, x, ss);
-            mx = fmaxf(mx, fabsf(x));
-          }
+          for (int y = 0; y < 8; ++y) ss = fmaf(bf2f(e[y]), bf2f(e[y]), ss);
         }
 #pragma unroll
-        for (int o = 1; o < 8; o *= 2) {
-          ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        }
-        const int e2 = scale_exp(mx);
-        const float down = pow2(-e2);
+        for (int o = 1; o < 8; o *= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float down = pow2(-norm_exp(ss));
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const int ch = part + 8 * i;
@@ -250,16 +258,20 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
             *(uint4*)(kimg + which * (C * DKP * 2) + img_off<DKP>(row, ch)) = im;
           }
         }
-        if (part == 0) {
-          float r = p.l2norm ? rsqrt_2step(__fadd_rn(ss, 1e-6f)) : 1.f;
-          if (which && p.l2norm) r = __fdiv_rn(r, sqrtf((float)p.dk));
-          if (which) rq[row] = r;
-          else col[row].z = r;
-          (which ? sq : sk)[row] = r * pow2(e2);
-        }
+        if (part == 0) (which ? sq : sk)[row] = ss;
       }
   }
   __syncthreads();
+  {  // norms and image scales, a row per thread (used behind the next barrier)
+    const int row = t & 63;
+    const bool is_q = t >= 64;
+    const float ss = (is_q ? sq : sk)[row];
+    float r = p.l2norm ? rsqrt_2step(__fadd_rn(ss, 1e-6f)) : 1.f;
+    if (is_q && p.l2norm) r = __fdiv_rn(r, sqrtf((float)p.dk));
+    if (is_q) rq[row] = r;
+    else col[row].z = r;
+    (is_q ? sq : sk)[row] = r * pow2(norm_exp(ss));
+  }
 
   // ---- 2 ----
   const int r0 = warp * 16;
@@ -286,6 +298,7 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
         mma_bf16(qk[2 * n2 + 1], qa, kb[2], kb[3]);
       }
     }
+    __syncthreads();
     float pm = 0.f;
     float ri[2], qi[2], hi[2], lo[2];
     unsigned long long bits[2];
@@ -358,52 +371,33 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
   __syncthreads();
 
   // ---- 4 ----
-  // lane -> (column, rows): all 16 columns with two row halves (warps 1, 2), or eight columns with four row quarters
-  auto substitute = [&](auto rows_c, int jb, int column, int part) {
-    constexpr int R = decltype(rows_c)::value;  // rows per lane
-    const int j = 16 * jb + column;
-#pragma unroll 1
-    for (int ib = jb + 1; ib < 4; ++ib) {
-      float s[R];
+  // The lower left block of a pair of diagonal blocks is -T22 (A21 T11); A21 T11 waits in its place in T. All rows of a column
+  // belong to one warp: lanes are eight columns by four groups of rows.
+  {
+    const int pair = 32 * (warp >> 1), j = pair + 8 * (warp & 1) + (lane & 7), i0 = pair + 16 + (lane >> 3);
+    float z[4];
+    block_product<4, 16>(z, A + i0 * TS + pair, T + pair * TS + j);
 #pragma unroll
-      for (int r = 0; r < R; ++r) s[r] = 0.f;
-#pragma unroll 1
-      for (int kb = jb; kb < ib; ++kb) {
-        float y[16];
+    for (int r = 0; r < 4; ++r) T[(i0 + 4 * r) * TS + j] = z[r];
+    __syncwarp();
+    block_product<4, 16>(z, T + i0 * TS + pair + 16, T + (pair + 16) * TS + j);
+    __syncwarp();
 #pragma unroll
-        for (int m = 0; m < 16; ++m) y[m] = T[(16 * kb + m) * TS + j];
+    for (int r = 0; r < 4; ++r) T[(i0 + 4 * r) * TS + j] = -z[r];
+  }
+  __syncthreads();
+  {
+    const int j = 8 * warp + (lane & 7), i0 = 32 + (lane >> 3);
+    float z[8];
+    block_product<8, 32>(z, A + i0 * TS, T + j);
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
+    for (int r = 0; r < 8; ++r) T[(i0 + 4 * r) * TS + j] = z[r];
+    __syncwarp();
+    block_product<8, 32>(z, T + i0 * TS + 32, T + 32 * TS + j);
+    __syncwarp();
 #pragma unroll
-          for (int m = 0; m < 16; m += 4) {
-            const float4 a = *(const float4*)&A[(16 * ib + part * R + r) * TS + 16 * kb + m];
-            s[r] = fmaf(a.x, y[m], fmaf(a.y, y[m + 1], fmaf(a.z, y[m + 2], fmaf(a.w, y[m + 3], s[r]))));
-          }
-        }
-      }
-      // the block's place in T holds the sum until it is multiplied by -T_ii
-#pragma unroll
-      for (int r = 0; r < R; ++r) T[(16 * ib + part * R + r) * TS + j] = s[r];
-      __syncwarp();
-      float y[16];
-#pragma unroll
-      for (int m = 0; m < 16; ++m) y[m] = T[(16 * ib + m) * TS + j];
-      __syncwarp();
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float z = 0.f;
-#pragma unroll
-        for (int m = 0; m < 16; m += 4) {
-          const float4 a = *(const float4*)&T[(16 * ib + part * R + r) * TS + 16 * ib + m];
-          z = fmaf(a.x, y[m], fmaf(a.y, y[m + 1], fmaf(a.z, y[m + 2], fmaf(a.w, y[m + 3], z))));
-        }
-        T[(16 * ib + part * R + r) * TS + j] = -z;
-      }
-      __syncwarp();
-    }
-  };
-  if (warp == 1 || warp == 2) substitute(std::integral_constant<int, 8>(), warp, lane & 15, lane >> 4);
-  else substitute(std::integral_constant<int, 4>(), 0, (warp ? 8 : 0) + (lane & 7), lane >> 3);
+    for (int r = 0; r < 8; ++r) T[(i0 + 4 * r) * TS + j] = -z[r];
+  }
   __syncthreads();
 
   // ---- 5: this warp's 16 rows, eight columns per lane and pass ----
