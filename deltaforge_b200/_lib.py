@@ -167,7 +167,7 @@ SIGNATURES = {
     "dfb_rotary": (C.c_int, [C.POINTER(RotaryDesc), c_vp]),
     "dfb_tree_attn_scratch_bytes": (c_sz, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
     "dfb_tree_attention": (C.c_int, [C.POINTER(TreeAttnDesc), c_vp]),
-    "dfb_delta_chunk_scratch_bytes": (c_sz, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "dfb_delta_chunk_scratch_bytes": (c_sz, [C.c_int] * 7),
     "dfb_delta_chunk": (C.c_int, [C.POINTER(DeltaChunkDesc), c_vp]),
     "dfb_engine_workspace_bytes": (c_sz, [C.POINTER(ModelDesc)]),
     "dfb_engine_num_segments": (C.c_int, [c_vp]),

@@ -465,9 +465,9 @@ int dfb_tree_attention(const dfb_tree_attn_desc* d, void* stream) {
   return launch_tree_attention(p, (cudaStream_t)stream);
 }
 
-size_t dfb_delta_chunk_scratch_bytes(int batch, int tokens, int hk, int hv, int dk) {
-  if (batch < 1 || tokens < 1 || hk < 1 || hv < hk || dk < 1) return 0;
-  return delta_chunk_scratch_bytes(batch, tokens, hk, hv, dk);
+size_t dfb_delta_chunk_scratch_bytes(int batch, int tokens, int hk, int hv, int dk, int dv, int tree) {
+  if (batch < 1 || tokens < 1 || hk < 1 || hv < hk || dk < 1 || dv < 1) return 0;
+  return delta_chunk_scratch_bytes(batch, tokens, hk, hv, dk, dv, tree != 0);
 }
 
 int dfb_delta_chunk(const dfb_delta_chunk_desc* d, void* stream) {
@@ -486,8 +486,8 @@ int dfb_delta_chunk(const dfb_delta_chunk_desc* d, void* stream) {
   if (!aligned16(d->q) || !aligned16(d->k) || !aligned16(d->v) || !aligned16(d->out) || !multiples(d->q_stride, 8) || !multiples(d->k_stride, 8) ||
       !multiples(d->v_stride, 8))
     return bad("dfb_delta_chunk: rows of q, k and v must start on 16-byte boundaries");
-  const size_t need = dfb_delta_chunk_scratch_bytes(d->batch, d->tokens, d->hk, d->hv, d->dk);
-  if (!d->scratch || d->scratch_bytes < need || !aligned16(d->scratch)) return bad("dfb_delta_chunk: aligned scratch of %zu bytes required", need);
+  const size_t need = delta_chunk_scratch_bytes(d->batch, d->tokens, d->hk, d->hv, d->dk, d->dv, tree);
+  if (need && (!d->scratch || d->scratch_bytes < need || !aligned16(d->scratch))) return bad("dfb_delta_chunk: aligned scratch of %zu bytes required", need);
   DeltaChunkParams p = {};
   p.batch = d->batch;
   p.tokens = d->tokens;

@@ -375,9 +375,10 @@ struct DeltaChunkParams {
   unsigned char* scratch;
   // set by the launcher
   int chunk0, chunks, seg_chunks;  // this segment: chunks chunk0 .. chunk0 + chunks - 1; scratch holds seg_chunks
-  int first, last;                 // first / last segment of the prompt
+  int first;                       // first segment of the prompt: the state comes from `state`
+  int beside;                      // its preparation runs beside the scan of the segment before
 };
-size_t delta_chunk_scratch_bytes(int batch, int tokens, int hk, int hv, int dk);
+size_t delta_chunk_scratch_bytes(int batch, int tokens, int hk, int hv, int dk, int dv, bool tree);
 int launch_delta_chunk(const DeltaChunkParams& p, cudaStream_t stream);
 
 }  // namespace dfb

@@ -860,13 +860,17 @@ def _launch(fn, desc, index: int, op: str) -> None:
         _lib.check(rc, f"dfb200::{op}")
 
 
-def _same_device(op: str, first: Tensor, *rest: Tensor | None) -> torch.device:
+def _same_device(op: str, first: Tensor, *rest: Tensor | None) -> None:
     require_cuda(first, op)
     index = first.get_device()
     for t in rest:
         if t is not None and t.get_device() != index:
             raise ValueError(f"{op}: all tensors must be on {first.device}, got one on {t.device}")
-    return first.device
+
+
+def _new_like(t: Tensor) -> Tensor:
+    """A new contiguous tensor of `t`'s shape and type (a third of the host time of ``torch.empty(t.shape, ...)``)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _rows(op: str, name: str, t: Tensor) -> tuple[int, int, int]:
@@ -957,9 +961,9 @@ def rotary_qk(query: Tensor, key: Tensor, positions: Tensor, inv_freq: Tensor, f
     op = "rotary_qk"
     rd = _check_rotary(op, query, key, positions, inv_freq)
     q_rows, k_rows = _rows(op, "query", query), _rows(op, "key", key)
-    device = _same_device(op, query, key, positions, inv_freq)
+    _same_device(op, query, key, positions, inv_freq)
     dtype, (batch, tokens, hq, d) = query.dtype, query.shape
-    q_out, k_out = torch.empty(query.shape, dtype=dtype, device=device), torch.empty(key.shape, dtype=dtype, device=device)
+    q_out, k_out = _new_like(query), _new_like(key)
     if batch and tokens:
         p = _lib.RotaryDesc()
         _ROTARY.pack_into(
@@ -967,7 +971,7 @@ def rotary_qk(query: Tensor, key: Tensor, positions: Tensor, inv_freq: Tensor, f
             positions.data_ptr(), positions.stride(0), positions.dtype == torch.int64, inv_freq.data_ptr(), inv_freq.dtype == torch.float64, factor,
             q_out.data_ptr(), k_out.data_ptr(), 0, 0, *_NO_ROWS, *_NO_ROWS, 0, 0,
         )  # fmt: skip
-        _launch(_lib.load().dfb_rotary, p, device.index, op)
+        _launch(_lib.load().dfb_rotary, p, query.get_device(), op)
     return q_out, k_out
 
 
@@ -997,10 +1001,10 @@ def rotary_append(
         for t in (key_cache, value_cache):
             if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
                 raise ValueError(f"{op}: the caches are written in place and must not be expanded views")
-    device = _same_device(op, query, key, value, positions, inv_freq, key_cache, value_cache, cache_len)
+    _same_device(op, query, key, value, positions, inv_freq, key_cache, value_cache, cache_len)
     if not max_seq:  # a cache without rows
         return rotary_qk.op._init_fn(query, key, positions, inv_freq, factor, interleaved)[0]
-    q_out = torch.empty(query.shape, dtype=dtype, device=device)
+    q_out = _new_like(query)
     if batch and tokens:
         p = _lib.RotaryDesc()
         _ROTARY.pack_into(
@@ -1009,7 +1013,7 @@ def rotary_append(
             inv_freq.data_ptr(), inv_freq.dtype == torch.float64, factor, q_out.data_ptr(), 0,
             key_cache.data_ptr(), value_cache.data_ptr(), *kc_rows, *vc_rows, cache_len.data_ptr(), max_seq,
         )  # fmt: skip
-        _launch(_lib.load().dfb_rotary, p, device.index, op)
+        _launch(_lib.load().dfb_rotary, p, query.get_device(), op)
     return q_out
 
 
@@ -1058,23 +1062,22 @@ def tree_attention(query: Tensor, key_cache: Tensor, value_cache: Tensor, cache_
     kp, vp = key_cache.data_ptr(), value_cache.data_ptr()
     if (k_rows[0] | k_rows[1] | k_rows[2] | v_rows[0] | v_rows[1] | v_rows[2]) % 8 or (kp | vp) % 16:
         raise ValueError(f"{op}: cache rows must start on 16-byte boundaries")
-    device = _same_device(op, query, key_cache, value_cache, cache_len, parents)
+    _same_device(op, query, key_cache, value_cache, cache_len, parents)
     if (q_rows[0] | q_rows[1] | q_rows[2]) % 8 or query.data_ptr() % 16:
         query = query.contiguous()
         q_rows = query.stride()[:3]
-    out = torch.empty((batch, nodes, hq, d), dtype=dtype, device=device)
+    out = _new_like(query)
     if batch == 0 or nodes == 0:
         return out
-    lib = _lib.load()
     nbytes = _scratch_bytes("dfb_tree_attn_scratch_bytes", batch, nodes, hq, hkv, d, max_seq)
     # from the allocator, not kept: calls on two streams, or two captured graphs, never share it
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
     a = _lib.TreeAttnDesc()
     _TREE.pack_into(
         a, 0, batch, nodes, hq, hkv, d, max_seq, dtype is torch.float16, query.data_ptr(), kp, vp, *q_rows, *k_rows, *v_rows,
         cache_len.data_ptr(), parents.data_ptr(), tree_stride, scale, out.data_ptr(), scratch.data_ptr() if nbytes else 0, nbytes,
     )  # fmt: skip
-    _launch(lib.dfb_tree_attention, a, device.index, op)
+    _launch(_lib.load().dfb_tree_attention, a, query.get_device(), op)
     return out
 
 
@@ -1083,13 +1086,10 @@ def _(query, key_cache, value_cache, cache_len, parents, scale):
     return query.new_empty(query.shape)
 
 
-def _aligned_rows(t: Tensor) -> tuple[Tensor, tuple[int, int, int]]:
-    """`t` with rows on 16-byte boundaries (copied once if need be), and its strides."""
+def _aligned_rows(t: Tensor) -> Tensor:
+    """`t`, copied if its rows do not start on 16-byte boundaries."""
     s = t.stride()
-    if (s[0] | s[1] | s[2]) % 8 or t.data_ptr() % 16:
-        t = t.contiguous()
-        s = t.stride()
-    return t, s[:3]
+    return t.contiguous() if (s[0] | s[1] | s[2]) % 8 or t.data_ptr() % 16 else t
 
 
 def _delta_tokens(
@@ -1098,43 +1098,53 @@ def _delta_tokens(
     if state.dim() != 4 or state.dtype != torch.float32:
         raise ValueError(f"{op}: state must be fp32 (batch, heads, key_dim, value_dim), got {tuple(state.shape)} {state.dtype}")
     batch, hv, dk, dv = state.shape
-    shape = query.shape
+    shape, per_head = query.shape, (batch, query.shape[1] if query.dim() == 4 else -1, hv)
     if len(shape) != 4 or shape != key.shape or shape[0] != batch or shape[3] != dk:
         raise ValueError(f"{op}: query and key must be (batch, tokens, key_heads, {dk}), got {tuple(shape)} and {tuple(key.shape)}")
-    tokens, hk = shape[1], shape[2]
+    _, tokens, hk, _ = shape
     if hk == 0 or hv == 0 or hv % hk:
         raise ValueError(f"{op}: {hv} value heads do not divide into {hk} key heads")
-    if value.shape != (batch, tokens, hv, dv):
-        raise ValueError(f"{op}: value has shape {tuple(value.shape)}, expected {(batch, tokens, hv, dv)}")
-    for name, t in (("g", g), ("beta", beta)):
-        if t.shape != (batch, tokens, hv) or not t.is_floating_point():
-            raise ValueError(f"{op}: {name} must be a floating tensor {(batch, tokens, hv)}, got {tuple(t.shape)} {t.dtype}")
-    for name, t in (("query", query), ("key", key), ("value", value)):
-        if t.dtype != BF16:
-            raise ValueError(f"{op}: {name} must be bfloat16, got {t.dtype}")
-        _rows(op, name, t)
+    if value.shape != (*per_head, dv):
+        raise ValueError(f"{op}: value has shape {tuple(value.shape)}, expected {(*per_head, dv)}")
+    if g.shape != per_head or not g.is_floating_point():
+        raise ValueError(f"{op}: g must be a floating tensor {per_head}, got {tuple(g.shape)} {g.dtype}")
+    if beta.shape != per_head or not beta.is_floating_point():
+        raise ValueError(f"{op}: beta must be a floating tensor {per_head}, got {tuple(beta.shape)} {beta.dtype}")
+    if not query.dtype == key.dtype == value.dtype == BF16:
+        raise ValueError(f"{op}: query, key and value must be bfloat16, got {query.dtype}, {key.dtype} and {value.dtype}")
     if dk % 8 or dv % 8 or dk < 8 or dk > 128 or dv < 8:
         raise ValueError(f"{op}: key dim {dk} (a multiple of 8, at most 128) or value dim {dv} (a multiple of 8) unsupported")
     if lengths is not None and (lengths.shape != (batch,) or lengths.dtype != torch.int32 or not lengths.is_contiguous()):
         raise ValueError(f"{op}: lengths must be a contiguous int32 tensor of {batch} entries, got {tuple(lengths.shape)} {lengths.dtype}")
-    tree_stride = 0 if parents is None else _check_parents(op, parents, batch, tokens)
-    device = _same_device(op, state, query, key, value, g, beta, lengths, parents)
-    (query, q_rows), (key, k_rows), (value, v_rows) = _aligned_rows(query), _aligned_rows(key), _aligned_rows(value)
-    state, g, beta = state.contiguous(), g.float().contiguous(), beta.float().contiguous()
-    out = torch.empty((batch, tokens, hv, dv), dtype=BF16, device=device)
+    tree = parents is not None
+    tree_stride = _check_parents(op, parents, batch, tokens) if tree else 0
+    q_rows, k_rows, v_rows = _rows(op, "query", query), _rows(op, "key", key), _rows(op, "value", value)
+    _same_device(op, state, query, key, value, g, beta, lengths, parents)
+    qp, kp, vp = query.data_ptr(), key.data_ptr(), value.data_ptr()
+    if (q_rows[0] | q_rows[1] | q_rows[2] | k_rows[0] | k_rows[1] | k_rows[2] | v_rows[0] | v_rows[1] | v_rows[2]) % 8 or (qp | kp | vp) % 16:
+        query, key, value = _aligned_rows(query), _aligned_rows(key), _aligned_rows(value)
+        q_rows, k_rows, v_rows = query.stride()[:3], key.stride()[:3], value.stride()[:3]
+        qp, kp, vp = query.data_ptr(), key.data_ptr(), value.data_ptr()
+    if not state.is_contiguous():
+        state = state.contiguous()
+    if g.dtype != torch.float32 or not g.is_contiguous():
+        g = g.float().contiguous()
+    if beta.dtype != torch.float32 or not beta.is_contiguous():
+        beta = beta.float().contiguous()
+    out = _new_like(value)
     if batch == 0 or tokens == 0:
-        return out, None if parents is not None else state.clone()
-    new_state = torch.empty_like(state) if parents is None else None
-    lib = _lib.load()
-    nbytes = _scratch_bytes("dfb_delta_chunk_scratch_bytes", batch, tokens, hk, hv, dk)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)  # not kept, as in tree_attention
+        return out, None if tree else state.clone()
+    new_state = None if tree else torch.empty_like(state)
+    nbytes = _scratch_bytes("dfb_delta_chunk_scratch_bytes", batch, tokens, hk, hv, dk, dv, tree)
+    # from the allocator, not kept, as in tree_attention
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=state.device) if nbytes else None
     p = _lib.DeltaChunkDesc()
     _DELTA.pack_into(
-        p, 0, batch, tokens, hk, hv, dk, dv, query.data_ptr(), key.data_ptr(), value.data_ptr(), *q_rows, *k_rows, *v_rows,
-        g.data_ptr(), beta.data_ptr(), 0 if lengths is None else lengths.data_ptr(), 0 if parents is None else parents.data_ptr(), tree_stride, l2norm,
-        state.data_ptr(), 0 if new_state is None else new_state.data_ptr(), out.data_ptr(), scratch.data_ptr(), nbytes,
+        p, 0, batch, tokens, hk, hv, dk, dv, qp, kp, vp, *q_rows, *k_rows, *v_rows,
+        g.data_ptr(), beta.data_ptr(), 0 if lengths is None else lengths.data_ptr(), parents.data_ptr() if tree else 0, tree_stride, l2norm,
+        state.data_ptr(), 0 if tree else new_state.data_ptr(), out.data_ptr(), scratch.data_ptr() if nbytes else 0, nbytes,
     )  # fmt: skip
-    _launch(lib.dfb_delta_chunk, p, device.index, op)
+    _launch(_lib.load().dfb_delta_chunk, p, state.get_device(), op)
     return out, new_state
 
 

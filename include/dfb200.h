@@ -350,7 +350,8 @@ typedef struct dfb_delta_chunk_desc {
   size_t scratch_bytes;
 } dfb_delta_chunk_desc;
 
-size_t dfb_delta_chunk_scratch_bytes(int batch, int tokens, int hk, int hv, int dk);
+/* tree: 1 for the tree form. 0 where none is needed. */
+size_t dfb_delta_chunk_scratch_bytes(int batch, int tokens, int hk, int hv, int dk, int dv, int tree);
 
 /* The gated delta rule over several tokens of each sequence: delta_rule_step (src/deltaforge/kernels/
  * gated_delta_step.py:109-177) token after token, computed in chunks of 64; with `parents`, over a tree of drafted

@@ -110,7 +110,7 @@ def delta_args(**over):
         (dict(query=z(2, 5, 3, 16), key=z(2, 5, 3, 16)), "do not divide"),
         (dict(query=z(2, 5, 0, 16), key=z(2, 5, 0, 16)), "do not divide"),
         (dict(value=z(2, 5, 4, 16)), "value has shape"),
-        (dict(value=z(2, 5, 4, 24, dtype=F16)), "value must be bfloat16"),
+        (dict(value=z(2, 5, 4, 24, dtype=F16)), "must be bfloat16"),
         (dict(g=z(2, 5, 2, dtype=F32)), "g must be"),
         (dict(beta=z(2, 5, 4, dtype=torch.int32)), "beta must be"),
         (dict(lengths=z(3, dtype=torch.int32)), "lengths must be"),
@@ -173,7 +173,7 @@ def test_c_entries_refuse_before_any_launch():
     d.batch = d.tokens = d.hk = d.hv = 1
     d.dk, d.dv = 12, 16
     assert lib.dfb_delta_chunk(d, None) == 2 and b"unsupported" in lib.dfb_last_error()
-    d.dk = 16
+    d.dk, d.tokens = 16, 5
     d.state = d.state_out = d.q = d.k = d.v = d.g = d.beta = d.out = 16
     assert lib.dfb_delta_chunk(d, None) == 2 and b"scratch" in lib.dfb_last_error()
     d.parents, d.lengths = 16, 16
@@ -182,10 +182,12 @@ def test_c_entries_refuse_before_any_launch():
 
 def test_scratch_sizes():
     lib = _lib.load()
-    assert lib.dfb_delta_chunk_scratch_bytes(1, 64, 16, 32, 128) == 16 * 32768 + 32 * 25600
+    assert lib.dfb_delta_chunk_scratch_bytes(1, 64, 16, 32, 128, 128, 0) == 16 * 32768 + 32 * 25600
     # a long prompt is walked in segments: the scratch stays bounded
-    assert lib.dfb_delta_chunk_scratch_bytes(1, 1 << 20, 16, 32, 128) <= 64 << 20
-    assert lib.dfb_delta_chunk_scratch_bytes(0, 5, 1, 1, 8) == 0
+    assert lib.dfb_delta_chunk_scratch_bytes(1, 1 << 20, 16, 32, 128, 128, 0) <= 64 << 20
+    assert lib.dfb_delta_chunk_scratch_bytes(16, 1, 16, 32, 128, 128, 0) == 0  # token by token
+    assert lib.dfb_delta_chunk_scratch_bytes(16, 1, 16, 32, 128, 128, 1) > 0
+    assert lib.dfb_delta_chunk_scratch_bytes(0, 5, 1, 1, 8, 8, 0) == 0
     assert lib.dfb_tree_attn_scratch_bytes(64, 1, 16, 4, 256, 32) == 0  # one split
 
 

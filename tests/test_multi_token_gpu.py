@@ -320,7 +320,7 @@ def delta_state_bound(want, tokens):
 @pytest.mark.parametrize("l2norm", [False, True])
 @pytest.mark.parametrize(
     "b,t,hk,hv,dk,dv",
-    [(1, 1, 2, 4, 128, 128), (2, 3, 1, 1, 16, 16), (1, 64, 2, 4, 128, 128), (2, 65, 2, 2, 64, 128), (1, 200, 3, 9, 96, 80), (3, 129, 2, 4, 8, 8), (1, 17, 1, 2, 128, 264), (20, 70, 2, 8, 128, 64)],
+    [(1, 1, 2, 4, 128, 128), (2, 3, 1, 1, 16, 16), (1, 64, 2, 4, 128, 128), (2, 65, 2, 2, 64, 128), (1, 200, 3, 9, 96, 80), (3, 129, 2, 4, 8, 8), (1, 17, 1, 2, 128, 264), (20, 70, 2, 8, 128, 64), (1, 1337, 16, 32, 64, 32)],
 )
 def test_delta_rule_chunk(b, t, hk, hv, dk, dv, l2norm):
     a = delta_inputs(41, b, t, hk, hv, dk, dv, l2norm)
