@@ -19,10 +19,10 @@
 // two floats, so that differences of large sums stay exact.
 //
 // Scan: two warps own 16 value columns of a head's state, half of the key rows each, in registers, as the accumulators of
-// S^T (16 x dk/2). Their layout is that of the A operand of the next product, so R^T, V'^T, O^T and S^T follow from one
-// another inside the warp; the two exchange their partial sums of K S and Q S once per chunk and share the tokens of the
-// output. k, q, T, P of the chunk come from shared memory, which two loader warps fill by cp.async one to two chunks
-// ahead. No wait spins.
+// S^T (16 x dk/2). Their layout is that of the A operand of the next product, so R^T, V'^T and S^T follow from one another
+// inside the warp; the two exchange their partial sums of K S once per chunk. A third warp makes the output of the chunk
+// before from S and V', handed over as fp16 fragments, so that only what the next state needs is in the chain from chunk to
+// chunk. k, q, T, P come through shared memory, which two loader warps fill by cp.async. No wait spins.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -449,19 +449,20 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
 
 // ---- the scan -------------------------------------------------------------------------------------------------------
 
-// NW: column tiles (of 16) per CTA; two warps each, and two loader warps.
+// NW: column tiles (of 16) per CTA; two warps each for the recurrence, one for the output, and two loader warps.
 template <int DKP, int NW> struct Scan {
-  static constexpr int THREADS = (2 * NW + 2) * 32;
+  static constexpr int WARPS = 3 * NW + 2, THREADS = WARPS * 32;
   static constexpr int VROW = NW * 32;  // bytes of a token's values in a stage
-  static constexpr int Q_OFF = C * DKP * 2, H_OFF = 2 * C * DKP * 2, V_OFF = H_OFF + HEAD_BYTES;
-  static constexpr int STAGE = V_OFF + C * VROW;
-  static constexpr int OUT = C / 2 * 32;                     // per warp: 32 tokens x 16 columns
-  static constexpr int SWAP = 2 * (32 + 16) * 32 * 4;       // per column tile: partial sums of both warps
-  static constexpr int REST = NW * (2 * OUT + SWAP);
-  static constexpr int STAGES = 2;
-  static constexpr int SMEM = STAGES * STAGE + REST;
-  // NW == 2 leaves room for a CTA of the preparation on the same SM: 75 KB of shared memory, and a quarter of the registers
-  static constexpr int REGS = NW == 2 ? 192 : 168;
+  // two stages of what the recurrence reads of a chunk: k, T (hi, lo), scalars, values
+  static constexpr int T_OFF = C * DKP * 2, A_SC = T_OFF + 2 * SQ, V_OFF = A_SC + SCAL, A_STAGE = V_OFF + C * VROW;
+  // two stages of what the output reads, a chunk behind: q, P, scalars
+  static constexpr int P_OFF = C * DKP * 2, B_SC = P_OFF + SQ, B_STAGE = B_SC + SCAL;
+  // per column tile: partial sums K S of both warps; two handovers (S as fp16 fragments, V' likewise); output rows
+  static constexpr int SWAP = 2 * 8 * 32 * 16, HAND = (DKP / 16 + 4) * 32 * 16, OUT = C * 32;
+  static constexpr int B_AT = 2 * A_STAGE, SWAP_AT = B_AT + 2 * B_STAGE, HAND_AT = SWAP_AT + NW * SWAP, OUT_AT = HAND_AT + 2 * NW * HAND;
+  static constexpr int SMEM = OUT_AT + NW * OUT;
+  // NW == 2 leaves room for a CTA of the preparation on the same SM: 55 KB of shared memory, and a quarter of the registers
+  static constexpr int REGS = NW == 2 ? 192 : 128;
 };
 
 template <int VROW> __device__ __forceinline__ uint32_t v_off(int row, int chunk) {
@@ -470,10 +471,11 @@ template <int VROW> __device__ __forceinline__ uint32_t v_off(int row, int chunk
 }
 
 template <int DKP, int NW, int NB, bool TREE>
-__global__ void __launch_bounds__((2 * NW + 2) * 32) __maxnreg__((Scan<DKP, NW>::REGS)) delta_scan_kernel(const DeltaChunkParams p) {
+__global__ void __launch_bounds__((3 * NW + 2) * 32) __maxnreg__((Scan<DKP, NW>::REGS)) delta_scan_kernel(const DeltaChunkParams p) {
   using S_ = Scan<DKP, NW>;
-  constexpr int NT = DKP / 16;  // 8-wide tiles of key rows per warp: half of them
+  constexpr int NT = DKP / 16;  // 8-wide tiles of key rows per recurrence warp: half of them
   extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int hand_exp[2][NW][3];  // scales of a handover: S of the two warps, V'
   const int vb = blockIdx.x, hv = blockIdx.y, b = blockIdx.z, hk = hv / (p.hv / p.hk);
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, g = lane >> 2, c = lane & 3;
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.tokens) : p.tokens;
@@ -481,20 +483,26 @@ __global__ void __launch_bounds__((2 * NW + 2) * 32) __maxnreg__((Scan<DKP, NW>:
   const int col_cta = vb * NW * 16;
   pdl_launch_dependents();  // the preparation of the next segment may run beside this one
 
-  if (warp >= 2 * NW) {  // ---- loader warps ----
-    const int lt = t - 2 * NW * 32;
+  // One barrier per chunk for all warps: behind barrier n the recurrence works on chunk n, the output on chunk n - 1, the loads
+  // bring chunk n + 1 of the one and chunk n of the other.
+  if (warp >= 3 * NW) {  // ---- loader warps ----
+    const int lt = t - 3 * NW * 32;
     const long per = p.hk * (2L * C * DKP * 2) + p.hv * (long)HEAD_BYTES;
-    auto load = [&](int n) {
-      if (n < nlive) {
-        const unsigned char* base = p.scratch + ((long)b * p.seg_chunks + n) * per;
-        const unsigned char* kq = base + (long)hk * (2 * C * DKP * 2);
-        const unsigned char* hd = base + p.hk * (2L * C * DKP * 2) + (long)hv * HEAD_BYTES;
-        const uint32_t st = smem_u32(smem + (n % S_::STAGES) * S_::STAGE);
-#pragma unroll 8
-        for (int i = lt; i < 2 * C * DKP * 2 / 16; i += 64) cp_async16(st + i * 16, kq + i * 16, 16);
-#pragma unroll 5
-        for (int i = lt; i < HEAD_BYTES / 16; i += 64) cp_async16(st + S_::H_OFF + i * 16, hd + i * 16, 16);
-        const int tok0 = (p.chunk0 + n) * C;
+    auto copy = [&](uint32_t to, const unsigned char* from, int bytes) {
+#pragma unroll 4
+      for (int i = lt * 16; i < bytes; i += 64 * 16) cp_async16(to + i, from + i, 16);
+    };
+    for (int n = -1; n <= nlive; ++n) {
+      cp_async_wait<0>();
+      if (n >= 0) __syncthreads();
+      const unsigned char* base = p.scratch + (long)b * p.seg_chunks * per + (long)hk * (2 * C * DKP * 2);
+      const unsigned char* head = p.scratch + (long)b * p.seg_chunks * per + p.hk * (2L * C * DKP * 2) + (long)hv * HEAD_BYTES;
+      if (n + 1 < nlive) {
+        const uint32_t st = smem_u32(smem + ((n + 1) & 1) * S_::A_STAGE);
+        copy(st, base + (n + 1) * per, C * DKP * 2);
+        copy(st + S_::T_OFF, head + (n + 1) * per, 2 * SQ);
+        copy(st + S_::A_SC, head + (n + 1) * per + 3 * SQ, SCAL);
+        const int tok0 = (p.chunk0 + n + 1) * C;
 #pragma unroll 4
         for (int i = lt; i < C * NW * 2; i += 64) {
           const int row = i / (NW * 2), ch = i % (NW * 2), col = col_cta + ch * 8, tok = tok0 + row;
@@ -507,20 +515,107 @@ __global__ void __launch_bounds__((2 * NW + 2) * 32) __maxnreg__((Scan<DKP, NW>:
                      p.v + b * p.v_stride[0] + (ok ? tok : 0) * p.v_stride[1] + hv * p.v_stride[2] + (ok ? col : 0), ok ? 16 : 0);
         }
       }
+      if (n >= 0 && n < nlive) {
+        const uint32_t st = smem_u32(smem + S_::B_AT + (n & 1) * S_::B_STAGE);
+        copy(st, base + n * per + C * DKP * 2, C * DKP * 2);
+        copy(st + S_::P_OFF, head + n * per + 2 * SQ, SQ);
+        copy(st + S_::B_SC, head + n * per + 3 * SQ, SCAL);
+      }
       cp_async_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < S_::STAGES - 1; ++i) load(i);
-    for (int n = 0; n < nlive; ++n) {
-      cp_async_wait<S_::STAGES - 2>();
-      __syncthreads();  // chunk n is there, chunk n - 1 has been used up
-      load(n + S_::STAGES - 1);
     }
-    cp_async_wait<0>();
     return;
   }
 
-  // ---- compute warps: 16 value columns and half of the key rows each ----
+  if (warp >= 2 * NW) {  // ---- output warps: 16 value columns each ----
+    const int ct = warp - 2 * NW, col0 = col_cta + ct * 16;
+    unsigned char* obuf = smem + S_::OUT_AT + ct * S_::OUT;
+    bf16* out = p.out + ((long)b * p.tokens * p.hv + hv) * p.dv + col0;
+    const long orow = (long)p.hv * p.dv;
+    for (int n = 0; n <= nlive; ++n) {
+      __syncthreads();
+      if (n == 0) continue;
+      const int k_ = n - 1, buf = k_ & 1, tok0 = (p.chunk0 + k_) * C;
+      const unsigned char* st = smem + S_::B_AT + buf * S_::B_STAGE;
+      const uint32_t qs_s = smem_u32(st);
+      const float* sc = (const float*)(st + S_::B_SC);
+      const uint4* hand = (const uint4*)(smem + S_::HAND_AT + (buf * NW + ct) * S_::HAND) + lane;
+      // O^T = (S^T Q^T) diag(e^G) + V'^T P^T
+      float o[2 * NB][4];
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+#pragma unroll
+      for (int hd = 0; hd < 2; ++hd) {
+        float x[2 * NB][4];
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < NT / 2; ++ks) {
+          const uint4 av = hand[(hd * (NT / 2) + ks) * 32];
+          const uint32_t a[4] = {av.x, av.y, av.z, av.w};
+#pragma unroll
+          for (int n2 = 0; n2 < NB; ++n2) {
+            uint32_t qb[4];
+            ldsm4(qs_s + img_off<DKP>(16 * n2 + (lane & 7) + 8 * (lane >> 4), hd * NT + 2 * ks + ((lane >> 3) & 1)), qb);
+            mma_f16(x[2 * n2], a, qb[0], qb[1]);
+            mma_f16(x[2 * n2 + 1], a, qb[2], qb[3]);
+          }
+        }
+        const float up = pow2(hand_exp[buf][ct][hd]);
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][e] = fmaf(x[i][e], up, o[i][e]);
+      }
+      float x[2 * NB][4];
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        const uint4 av = hand[(DKP / 16 + k) * 32];
+        const uint32_t a[4] = {av.x, av.y, av.z, av.w};
+#pragma unroll
+        for (int n2 = k; n2 < NB; ++n2) {
+          uint32_t pb[4];
+          ldsm4(qs_s + S_::P_OFF + img_off<C>(16 * n2 + (lane & 7) + 8 * (lane >> 4), 2 * k + ((lane >> 3) & 1)), pb);
+          mma_f16(x[2 * n2], a, pb[0], pb[1]);
+          mma_f16(x[2 * n2 + 1], a, pb[2], pb[3]);
+        }
+      }
+      const float vup = pow2(hand_exp[buf][ct][2]);
+      __syncwarp();  // the previous chunk's outputs have left the buffer
+#pragma unroll
+      for (int n2 = 0; n2 < NB; ++n2) {
+        uint32_t w[4];
+        const float up = vup * sc[3 * C + 8 + n2];  // P is scaled per 16 rows
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int nt = 2 * n2 + h;
+          const float2 f = *(const float2*)&sc[2 * C + 8 * nt + 2 * c];
+          const __nv_bfloat162 y = __floats2bfloat162_rn(o[nt][0] * f.x + x[nt][0] * up, o[nt][1] * f.y + x[nt][1] * up);
+          const __nv_bfloat162 z = __floats2bfloat162_rn(o[nt][2] * f.x + x[nt][2] * up, o[nt][3] * f.y + x[nt][3] * up);
+          w[2 * h] = *(const uint32_t*)&y, w[2 * h + 1] = *(const uint32_t*)&z;
+        }
+        const int row = 16 * n2 + 8 * (lane >> 4) + (lane & 7), half = (lane >> 3) & 1;
+        stsm4_t(smem_u32(obuf) + row * 32 + ((half ^ ((row >> 2) & 1)) << 4), w[0], w[1], w[2], w[3]);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int row = 16 * i + (lane >> 1), half = lane & 1, tok = tok0 + row;
+        if (tok < p.tokens && col0 + half * 8 < p.dv)
+          *(uint4*)(out + tok * orow + half * 8) = *(const uint4*)(obuf + row * 32 + ((half ^ ((row >> 2) & 1)) << 4));
+      }
+    }
+    // rows of tokens that no chunk covered: zeros
+    const int from = (p.chunk0 + nlive) * C, to = min(p.tokens, (p.chunk0 + p.chunks) * C);
+    for (int i = lane; i < (to - from) * 2; i += 32) {
+      const int tok = from + (i >> 1), half = i & 1;
+      if (col0 + half * 8 < p.dv) *(uint4*)(out + tok * orow + half * 8) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    return;
+  }
+
+  // ---- recurrence warps: 16 value columns and half of the key rows each ----
   const int ct = warp >> 1, hd = warp & 1;
   const int col0 = col_cta + ct * 16;
   const bool cok0 = col0 + g < p.dv, cok1 = col0 + g + 8 < p.dv;
@@ -535,30 +630,29 @@ __global__ void __launch_bounds__((2 * NW + 2) * 32) __maxnreg__((Scan<DKP, NW>:
       const bool ok = d < p.dk && (e < 2 ? cok0 : cok1);
       S[n][e] = ok ? Sin[(long)d * p.dv + col0 + g + 8 * (e >> 1)] : 0.f;
     }
-  unsigned char* obuf = smem + S_::STAGES * S_::STAGE + warp * S_::OUT;
-  float4* swap = (float4*)(smem + S_::STAGES * S_::STAGE + 2 * NW * S_::OUT + ct * S_::SWAP);
-  float4 *mine = swap + hd * (12 * 32) + lane, *other = swap + (hd ^ 1) * (12 * 32) + lane;
-  bf16* out = p.out + ((long)b * p.tokens * p.hv + hv) * p.dv + col0;
-  const long orow = (long)p.hv * p.dv;
+  float4* swap = (float4*)(smem + S_::SWAP_AT + ct * S_::SWAP);
+  float4 *mine = swap + hd * (8 * 32) + lane, *other = swap + (hd ^ 1) * (8 * 32) + lane;
 
-  for (int n = 0; n < nlive; ++n) {
+  for (int n = 0; n <= nlive; ++n) {
     __syncthreads();
-    const unsigned char* st = smem + (n % S_::STAGES) * S_::STAGE;
-    const uint32_t ks_s = smem_u32(st), qs_s = ks_s + S_::Q_OFF, ti_s = ks_s + S_::H_OFF, vs_s = ks_s + S_::V_OFF;
-    const float* sc = (const float*)(st + S_::H_OFF + 3 * SQ);
-    const int tok0 = (p.chunk0 + n) * C;
+    if (n == nlive) break;
+    const unsigned char* st = smem + (n & 1) * S_::A_STAGE;
+    const uint32_t ks_s = smem_u32(st), ti_s = ks_s + S_::T_OFF, vs_s = ks_s + S_::V_OFF;
+    const float* sc = (const float*)(st + S_::A_SC);
+    uint4* hand = (uint4*)(smem + S_::HAND_AT + ((n & 1) * NW + ct) * S_::HAND) + lane;
 
-    // 1. S^T K^T (hi and lo) and S^T Q^T (hi) over this warp's key rows
+    // 1. S^T K^T over this warp's key rows; hi goes to the output warp too
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < NT; ++i) m = fmaxf(m, fmaxf(fmaxf(fabsf(S[i][0]), fabsf(S[i][1])), fmaxf(fabsf(S[i][2]), fabsf(S[i][3]))));
     const int es = scale_exp(warp_max_abs(m));
     const float sdown = pow2(-es), sup = pow2(es);
-    float x[2 * NB][4], oq[2 * NB][4];
+    if (lane == 0) hand_exp[n & 1][ct][hd] = es;
+    float x[2 * NB][4];
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[i][e] = oq[i][e] = 0.f;
+      for (int e = 0; e < 4; ++e) x[i][e] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < NT / 2; ++ks) {
       uint32_t hi[4], lo[4];
@@ -566,45 +660,27 @@ __global__ void __launch_bounds__((2 * NW + 2) * 32) __maxnreg__((Scan<DKP, NW>:
       split2(S[2 * ks][2] * sdown, S[2 * ks][3] * sdown, hi[1], lo[1]);
       split2(S[2 * ks + 1][0] * sdown, S[2 * ks + 1][1] * sdown, hi[2], lo[2]);
       split2(S[2 * ks + 1][2] * sdown, S[2 * ks + 1][3] * sdown, hi[3], lo[3]);
+      hand[(hd * (NT / 2) + ks) * 32] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      uint32_t kb[NB][4];
 #pragma unroll
       for (int n2 = 0; n2 < NB; ++n2) {
-        uint32_t kb[4], qb[4];
-        const uint32_t off = img_off<DKP>(16 * n2 + (lane & 7) + 8 * (lane >> 4), hd * NT + 2 * ks + ((lane >> 3) & 1));
-        ldsm4(ks_s + off, kb);
-        ldsm4(qs_s + off, qb);
-        mma_f16(x[2 * n2], hi, kb[0], kb[1]);
-        mma_f16(x[2 * n2 + 1], hi, kb[2], kb[3]);
-        mma_f16(oq[2 * n2], hi, qb[0], qb[1]);
-        mma_f16(oq[2 * n2 + 1], hi, qb[2], qb[3]);
-        mma_f16(x[2 * n2], lo, kb[0], kb[1]);
-        mma_f16(x[2 * n2 + 1], lo, kb[2], kb[3]);
+        ldsm4(ks_s + img_off<DKP>(16 * n2 + (lane & 7) + 8 * (lane >> 4), hd * NT + 2 * ks + ((lane >> 3) & 1)), kb[n2]);
+        mma_f16(x[2 * n2], hi, kb[n2][0], kb[n2][1]);
+        mma_f16(x[2 * n2 + 1], hi, kb[n2][2], kb[n2][3]);
+      }
+#pragma unroll
+      for (int n2 = 0; n2 < NB; ++n2) {
+        mma_f16(x[2 * n2], lo, kb[n2][0], kb[n2][1]);
+        mma_f16(x[2 * n2 + 1], lo, kb[n2][2], kb[n2][3]);
       }
     }
-    // The other warp of these columns has the other key rows: K S is needed by both, Q S by the one that finishes a token's
-    // output (blocks of 16 tokens 0 and 3 here for the first warp, 1 and 2 for the second).
-    float o[2][2][4];  // own blocks, eight tokens each
+    // the other warp of these columns has the other key rows
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[i][e] *= sup, oq[i][e] *= sup;
+      for (int e = 0; e < 4; ++e) x[i][e] *= sup;
       mine[i * 32] = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
     }
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        constexpr int LAST = 2 * NB - 1;
-        const int f0 = 6 * j + h, f1 = 2 + 2 * j + h;  // tile of block 0 or 3, of block 1 or 2
-        float4 give;
-        float* gv = &give.x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float a = f0 <= LAST ? oq[f0 <= LAST ? f0 : 0][e] : 0.f, z = f1 <= LAST ? oq[f1 <= LAST ? f1 : 0][e] : 0.f;
-          o[j][h][e] = hd ? z : a;
-          gv[e] = hd ? a : z;
-        }
-        mine[(8 + 2 * j + h) * 32] = give;
-      }
     asm volatile("bar.sync %0, 64;" ::"r"(1 + ct) : "memory");
     // 2. R = V - diag(e^G) K S, then its halves
     m = 0.f;
@@ -665,55 +741,18 @@ __global__ void __launch_bounds__((2 * NW + 2) * 32) __maxnreg__((Scan<DKP, NW>:
         for (int e = 0; e < 4; ++e) x[i][e] *= u, m = fmaxf(m, fabsf(x[i][e]));
       }
     }
-    // 4. O^T = (S^T Q^T) diag(e^G) + V'^T P^T for this warp's blocks of tokens (P is stored with its zeros)
-    {
+    {  // V' for the output warp, every second block of 16 tokens
       const int ev = scale_exp(warp_max_abs(m));
-      const float vdown = pow2(-ev), vup = pow2(ev);
-      float pv[2][2][4];
+      const float vdown = pow2(-ev);
+      if (lane == 0) hand_exp[n & 1][ct][2] = ev;  // (both warps have the same)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) pv[j][h][0] = pv[j][h][1] = pv[j][h][2] = pv[j][h][3] = 0.f;
-      const int block[2] = {hd ? 1 : 0, hd ? 2 : 3};
-#pragma unroll
-      for (int k = 0; k < NB; ++k) {
-        const uint32_t a[4] = {h2(x[2 * k][0] * vdown, x[2 * k][1] * vdown), h2(x[2 * k][2] * vdown, x[2 * k][3] * vdown),
-                               h2(x[2 * k + 1][0] * vdown, x[2 * k + 1][1] * vdown), h2(x[2 * k + 1][2] * vdown, x[2 * k + 1][3] * vdown)};
-#pragma unroll
-        for (int j = 0; j < (NB > 2 ? 2 : 1); ++j) {
-          if (j == 0 && k > 1) continue;
-          uint32_t pb[4];
-          ldsm4(ti_s + 2 * SQ + img_off<C>(16 * block[j] + (lane & 7) + 8 * (lane >> 4), 2 * k + ((lane >> 3) & 1)), pb);
-          mma_f16(pv[j][0], a, pb[0], pb[1]);
-          mma_f16(pv[j][1], a, pb[2], pb[3]);
-        }
-      }
-      __syncwarp();  // the previous chunk's outputs have left the buffer
-#pragma unroll
-      for (int j = 0; j < (NB > 2 ? 2 : 1); ++j) {
-        uint32_t w[4];
-        const float up = vup * sc[3 * C + 8 + block[j]];  // P too is scaled per 16 rows
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float2 f = *(const float2*)&sc[2 * C + 16 * block[j] + 8 * h + 2 * c];
-          const float4 y = other[(8 + 2 * j + h) * 32];
-          const __nv_bfloat162 a = __floats2bfloat162_rn((o[j][h][0] + y.x) * f.x + pv[j][h][0] * up, (o[j][h][1] + y.y) * f.y + pv[j][h][1] * up);
-          const __nv_bfloat162 z = __floats2bfloat162_rn((o[j][h][2] + y.z) * f.x + pv[j][h][2] * up, (o[j][h][3] + y.w) * f.y + pv[j][h][3] * up);
-          w[2 * h] = *(const uint32_t*)&a, w[2 * h + 1] = *(const uint32_t*)&z;
-        }
-        const int row = 16 * j + 8 * (lane >> 4) + (lane & 7), half = (lane >> 3) & 1;
-        stsm4_t(smem_u32(obuf) + row * 32 + ((half ^ ((row >> 2) & 1)) << 4), w[0], w[1], w[2], w[3]);
-      }
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < (NB > 2 ? 2 : 1); ++j) {
-        const int row = 16 * j + (lane >> 1), half = lane & 1, tok = tok0 + 16 * block[j] + (lane >> 1);
-        if (block[j] < NB && tok < p.tokens && col0 + half * 8 < p.dv)
-          *(uint4*)(out + tok * orow + half * 8) = *(const uint4*)(obuf + row * 32 + ((half ^ ((row >> 2) & 1)) << 4));
-      }
+      for (int k = 0; k < NB; ++k)
+        if ((k & 1) == hd)
+          hand[(DKP / 16 + k) * 32] = make_uint4(h2(x[2 * k][0] * vdown, x[2 * k][1] * vdown), h2(x[2 * k][2] * vdown, x[2 * k][3] * vdown),
+                                                 h2(x[2 * k + 1][0] * vdown, x[2 * k + 1][1] * vdown), h2(x[2 * k + 1][2] * vdown, x[2 * k + 1][3] * vdown));
     }
-    if (TREE) break;
-    // 5. S^T = e^G_C S^T + (V' diag(e^(G_C - G)))^T K over this warp's key rows, accumulated apart
+    if (TREE) continue;
+    // 4. S^T = e^G_C S^T + (V' diag(e^(G_C - G)))^T K over this warp's key rows, accumulated apart
     m = 0.f;
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i) {
@@ -755,15 +794,6 @@ __global__ void __launch_bounds__((2 * NW + 2) * 32) __maxnreg__((Scan<DKP, NW>:
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) S[4 * j4 + i][e] = fmaf(a[i][e], uup, S[4 * j4 + i][e] * decay);
-    }
-  }
-
-  // rows of tokens that no chunk covered: zeros
-  {
-    const int from = (p.chunk0 + nlive) * C, to = min(p.tokens, (p.chunk0 + p.chunks) * C);
-    for (int i = lane + 32 * hd; i < (to - from) * 2; i += 64) {
-      const int tok = from + (i >> 1), half = i & 1;
-      if (col0 + half * 8 < p.dv) *(uint4*)(out + tok * orow + half * 8) = make_uint4(0u, 0u, 0u, 0u);
     }
   }
   if (TREE) return;
