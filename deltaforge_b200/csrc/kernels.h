@@ -380,6 +380,7 @@ struct DeltaChunkParams {
 };
 size_t delta_chunk_scratch_bytes(int batch, int tokens, int hk, int hv, int dk, int dv, bool tree);
 int launch_delta_chunk(const DeltaChunkParams& p, cudaStream_t stream);
+int launch_delta_scan(const DeltaChunkParams& p, cudaStream_t stream);  // one segment, prepared
 
 }  // namespace dfb
 

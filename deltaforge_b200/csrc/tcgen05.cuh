@@ -1,0 +1,139 @@
+// What the kernels on the fifth-generation tensor cores share: mbarriers with bounded waits, TMA and bulk copies, descriptors,
+// tcgen05 instructions, TMEM loads and stores.
+#pragma once
+
+#include <cuda.h>
+
+#include "common.cuh"
+
+namespace dfb {
+namespace {
+
+constexpr long long WAIT_CYCLES = 1LL << 28;
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// One lane of a converged warp. The compiler knows what this predicate is: products issued under it take 20 cycles and up, under
+// `lane == 0` 93, because every operand is then moved to the uniform registers under a loop over the active lanes.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// Bounded; the CTA-wide flag ends every other wait too.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* failed) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*failed) return false;
+    if (clock64() - t0 > WAIT_CYCLES) {
+      *failed = 1;
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int dim, int key, int head, int seq, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"((uint64_t)map), "r"(dim), "r"(key), "r"(head), "r"(seq), "r"(smem_u32(bar))
+      : "memory");
+}
+// Rows of one 128-byte swizzle span, 8-row groups 1024 bytes apart. `lead`: for an operand whose rows run along its
+// contraction (V: a row is a key), bytes from one block of 64 dims to the next; unused where rows run along M or N.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead) {
+  return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+template <typename T> __device__ __forceinline__ uint32_t type_bits() { return 1u; }  // bf16
+template <> __device__ __forceinline__ uint32_t type_bits<__half>() { return 0u; }
+// D fp32, M = 128; b_rows: B's rows run along its contraction
+template <typename T> __device__ __forceinline__ uint32_t instr_desc(int n, bool b_rows) {
+  return 1u << 4 | type_bits<T>() << 7 | type_bits<T>() << 10 | (uint32_t)b_rows << 16 | (uint32_t)(n >> 3) << 17 | 8u << 24;
+}
+// D (+)= A B, B in shared memory, A there too (ss) or in TMEM (ts: a lane per row, two values per column)
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+               "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
+               "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+#define DFB_OUT8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
+#define DFB_TIE8(v, i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3]), "+r"(v[i + 4]), "+r"(v[i + 5]), "+r"(v[i + 6]), "+r"(v[i + 7])
+#define DFB_IN8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
+
+// 32 columns of this thread's lane. The registers hold the values after tmem_wait_ld on them.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+      "%26,%27,%28,%29,%30,%31}, [%32];"
+      : DFB_OUT8(v, 0), DFB_OUT8(v, 8), DFB_OUT8(v, 16), DFB_OUT8(v, 24)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait_ld(uint32_t* v) {  // (tied to the registers, so that no use moves before it)
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : DFB_TIE8(v, 0), DFB_TIE8(v, 8), DFB_TIE8(v, 16), DFB_TIE8(v, 24)::"memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+      "%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      DFB_IN8(v, 0), DFB_IN8(v, 8), DFB_IN8(v, 16), DFB_IN8(v, 24)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : DFB_OUT8(v, 0), DFB_OUT8(v, 8)
+               : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : DFB_TIE8(v, 0), DFB_TIE8(v, 8)::"memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), DFB_IN8(v, 0),
+               DFB_IN8(v, 8)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// bytes (a multiple of 16) from global to shared memory, both 16-byte aligned
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// 2^x: one instruction, 2 ulp
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+}  // namespace
+}  // namespace dfb
