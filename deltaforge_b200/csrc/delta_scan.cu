@@ -8,9 +8,9 @@
 // (mma.sync is no alternative on this GPU: its fp32 pipe does not run beside it. A product m16n8k16 and its eight
 // cycles add to the conversions instead of hiding them; that form took 4200 cycles per chunk on four times the SMs.)
 //
-// Warps 0-7: two threads per value column, half of the key rows (of S) and half of the tokens (of R, V') each; S stays there
-// in fp32 from the first chunk to the last. Warps 8-11: the output, a thread per column, from TMEM to memory, while the
-// others go on; one lane of them also refills the two stages of shared memory by bulk copies. Warp 12 issues the products.
+// Warps 0-15: four threads per value column, a quarter of the key rows (of S) and of the tokens (of R, V') each; S stays
+// there in fp32 from the first chunk to the last. Warps 16-19: the output, a thread per column, from TMEM to memory, while the
+// others go on. Warp 20 fills the two stages of shared memory by bulk copies, warp 21 issues the products.
 //
 // Bound by the chain from chunk to chunk: 664 cycles of tensor time for K S, 500 for T R, 330 for half of the update, and
 // between them the conversions of 128 x 128 + 2 x 128 x 64 values on the threads (about 700 instructions each) and six
@@ -23,11 +23,11 @@ namespace dfb {
 namespace {
 
 constexpr int COLS = 128;  // value columns per CTA
-constexpr int SCAN_WARPS = 13, SCAN_THREADS = SCAN_WARPS * 32;
+constexpr int SCAN_WARPS = 22, SCAN_THREADS = SCAN_WARPS * 32;
 
 template <int DKP> struct Stage {
   static constexpr int T = key_bytes(DKP), P = T + 2 * SQ, SC = P + SQ, V = SC + SCAL, BYTES = V + C * COLS * 2;
-  static constexpr int SMEM = 2 * BYTES + 1024;
+  static constexpr int SMEM = 2 * BYTES + C * COLS * 2 + 1024;
 };
 // TMEM columns. S, R and V' are A operands, two fp16 values per column; the others are accumulators. V' takes the place
 // of R, the product with P that of K S, the update that of T R.
@@ -36,11 +36,11 @@ constexpr int SH = 0, SL = 64, KS = 128, QS = 192, RH = 256, RL = 288, VH = 320,
 template <int DKP, bool TREE>
 __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const DeltaChunkParams p) {
   using G = Stage<DKP>;
-  constexpr int NS = DKP / 2;  // key rows per thread
+  constexpr int NS = DKP / 4;  // key rows per thread
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ uint64_t full[2], s_in[2], ks_out, r_in, vp_out, u_in, u_out[2], o_out, o_read;
-  __shared__ float s_max[2][COLS], v_max[2][COLS], vp_max[2][COLS];
+  __shared__ float s_max[4][COLS], v_max[4][COLS], vp_max[4][COLS];
   __shared__ int s_exp[2][COLS], v_exp[2][COLS];  // by chunk parity, for the output
   __shared__ uint32_t tmem_slot;
   __shared__ int failed_s;
@@ -51,13 +51,13 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.tokens) : p.tokens;
   const int nlive = min(max((len + C - 1) / C - p.chunk0, 0), p.chunks);  // chunks of this segment with tokens
   if (t == 0) {
-    for (int i = 0; i < 2; ++i) mbar_init(&full[i], 1), mbar_init(&s_in[i], 4), mbar_init(&u_out[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&full[i], 1), mbar_init(&s_in[i], 8), mbar_init(&u_out[i], 1);
     mbar_init(&ks_out, 1), mbar_init(&vp_out, 1), mbar_init(&o_out, 1);
-    mbar_init(&r_in, 8), mbar_init(&u_in, 8), mbar_init(&o_read, 4);
+    mbar_init(&r_in, 16), mbar_init(&u_in, 16), mbar_init(&o_read, 4);
     failed_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 12) {
+  if (warp == 21) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -71,11 +71,12 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
   const uint32_t base = tmem + ((uint32_t)(q * 32) << 16);
   bool ok = true;  // a wait that ran out lets everything run to its end on garbage; NaN is what is left then
 
-  if (warp < 8) {
+  if (warp < 16) {
     // ---------------- the recurrence ----------------
     const int h = warp >> 2;
     const long sb = ((long)b * p.hv + hv) * p.dk * p.dv + gcol;
-    auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory"); };  // the two warps of these columns
+    auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + q) : "memory"); };  // the four warps of these columns
+    auto most = [&](const float (&m)[4][COLS]) { return fmaxf(fmaxf(m[0][col], m[1][col]), fmaxf(m[2][col], m[3][col])); };
     float S[NS];
     const float* Sin = p.first ? p.state + sb : p.state_out + sb;
     float ms = 0.f;
@@ -87,66 +88,68 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
     }
     s_max[h][col] = ms;
     meet();
-    int es = scale_exp(fmaxf(ms, s_max[h ^ 1][col]));
+    int es = scale_exp(most(s_max));
     meet();
 
     for (int n = 0; n < nlive; ++n) {
       const unsigned char* st = sm + (n & 1) * G::BYTES;
       const float* sc = (const float*)(st + G::SC);
       // S in halves to TMEM; its largest on the side
-      const float sdown = pow2(-es);
-      ms = 0.f;
+      {
+        const float sdown = pow2(-es);
+        ms = 0.f;
 #pragma unroll
-      for (int x = 0; x < NS; x += 32) {
-        uint32_t hi[16], lo[16];
+        for (int x = 0; x < NS; x += 16) {
+          uint32_t hi[8], lo[8];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float s0 = S[x + 2 * i], s1 = S[x + 2 * i + 1];
-          ms = fmaxf(ms, fmaxf(fabsf(s0), fabsf(s1)));
-          split2(s0 * sdown, s1 * sdown, hi[i], lo[i]);
+          for (int i = 0; i < 8; ++i) {
+            const float s0 = S[x + 2 * i], s1 = S[x + 2 * i + 1];
+            ms = fmaxf(ms, fmaxf(fabsf(s0), fabsf(s1)));
+            split2(s0 * sdown, s1 * sdown, hi[i], lo[i]);
+          }
+          tmem_st8(base + SH + h * (NS / 2) + x / 2, hi);
+          tmem_st8(base + SL + h * (NS / 2) + x / 2, lo);
         }
-        tmem_st16(base + SH + h * (NS / 2) + x / 2, hi);
-        tmem_st16(base + SL + h * (NS / 2) + x / 2, lo);
       }
       tmem_wait_st();
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s_in[h]);
+      if (lane == 0) mbar_arrive(&s_in[h >> 1]);
       s_max[h][col] = ms;
       if (h == 0) s_exp[n & 1][col] = es;
 
       // this thread's values, and the largest of the column
       ok = wait_for(&full[n & 1], (n >> 1) & 1, failed) && ok;
-      const uint32_t counts = cok ? __float_as_uint(sc[3 * C + 16 + h]) : 0u;
-      const unsigned short* vs = (const unsigned short*)(st + G::V) + h * 32 * COLS + col;
-      uint32_t v[16];  // two tokens each
+      const uint32_t counts = cok ? __float_as_uint(sc[3 * C + 16 + (h >> 1)]) >> (16 * (h & 1)) : 0u;
+      const unsigned short* vs = (const unsigned short*)(st + G::V) + h * 16 * COLS + col;
+      uint32_t v[8];  // two tokens each
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; i < 8; ++i) {
         const uint32_t lo = (counts >> (2 * i)) & 1 ? vs[2 * i * COLS] : 0, hi = (counts >> (2 * i + 1)) & 1 ? vs[(2 * i + 1) * COLS] : 0;
         v[i] = lo | hi << 16;
       }
       __nv_bfloat162 mv = __float2bfloat162_rn(0.f);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mv = __hmax2_nan(mv, __habs2(*(const __nv_bfloat162*)&v[i]));
+      for (int i = 0; i < 8; ++i) mv = __hmax2_nan(mv, __habs2(*(const __nv_bfloat162*)&v[i]));
       const float2 mvf = __bfloat1622float2(mv);
       v_max[h][col] = fmaxf(mvf.x, mvf.y);
       meet();
       // |K S| <= |k|_2 sqrt(dk) |S|, where both factors' images are at most 2^13 and so is a key's norm
       const float ks_max = fmaxf(sc[3 * C + 12], sc[3 * C + 13]) * pow2(es) * (11.4f * 67108864.f);
-      const int er = scale_exp(fmaxf(v_max[0][col], v_max[1][col]) + ks_max);
-      const float both = fmaxf(s_max[0][col], s_max[1][col]);
+      const int er = scale_exp(most(v_max) + ks_max);
+      const float both = most(s_max);
       const float rdown = pow2(-er), wscale = pow2(es) * rdown;
 
       // R = V - diag(e^G) K S
       ok = wait_for(&ks_out, n & 1, failed) && ok;
       fence_after();
       {
-        uint32_t x[32], hi[16], lo[16];
-        tmem_ld32(base + KS + 32 * h, x);
-        tmem_wait_ld(x);
+        uint32_t x[16], hi[8], lo[8];
+        tmem_ld16(base + KS + 16 * h, x);
+        tmem_wait_ld16(x);
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const float4 w = *(const float4*)&sc[32 * h + 2 * i];
+        for (int i = 0; i < 8; i += 2) {
+          const float4 w = *(const float4*)&sc[16 * h + 2 * i];
           const float r0 = fmaf(-__uint_as_float(x[2 * i]), w.x * wscale, __uint_as_float(v[i] << 16) * rdown);
           const float r1 = fmaf(-__uint_as_float(x[2 * i + 1]), w.y * wscale, __uint_as_float(v[i] & 0xffff0000u) * rdown);
           const float r2 = fmaf(-__uint_as_float(x[2 * i + 2]), w.z * wscale, __uint_as_float(v[i + 1] << 16) * rdown);
@@ -154,8 +157,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
           split2(r0, r1, hi[i], lo[i]);
           split2(r2, r3, hi[i + 1], lo[i + 1]);
         }
-        tmem_st16(base + RH + 16 * h, hi);
-        tmem_st16(base + RL + 16 * h, lo);
+        tmem_st8(base + RH + 8 * h, hi);
+        tmem_st8(base + RL + 8 * h, lo);
       }
       tmem_wait_st();
       fence_before();
@@ -165,36 +168,35 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
       // V'
       ok = wait_for(&vp_out, n & 1, failed) && ok;
       fence_after();
-      float uup, decay = sc[3 * C];
+      float uup;
+      const float decay = sc[3 * C];
       {
-        uint32_t x[32], hi[16], lo[16];
-        tmem_ld32(base + VP + 32 * h, x);
-        tmem_wait_ld(x);
-        const float t0 = pow2(er) * sc[3 * C + 4 + 2 * h], t1 = pow2(er) * sc[3 * C + 5 + 2 * h];  // T is scaled per 16 rows
+        uint32_t x[16], hi[8], lo[8];
+        tmem_ld16(base + VP + 16 * h, x);
+        tmem_wait_ld16(x);
+        const float tscale = pow2(er) * sc[3 * C + 4 + h];  // T is scaled per 16 rows
         float m0 = 0.f, m1 = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) m0 = fmaxf(m0, fabsf(__uint_as_float(x[i]))), m1 = fmaxf(m1, fabsf(__uint_as_float(x[16 + i])));
-        const float mine = fmaxf(m0 * t0, m1 * t1);
-        vp_max[h][col] = mine;
+        for (int i = 0; i < 8; ++i) m0 = fmaxf(m0, fabsf(__uint_as_float(x[i]))), m1 = fmaxf(m1, fabsf(__uint_as_float(x[8 + i])));
+        vp_max[h][col] = fmaxf(m0, m1) * tscale;
         meet();
-        const float m = fmaxf(vp_max[0][col], vp_max[1][col]);
+        const float m = most(vp_max);
         const int ev = scale_exp(m), eu = scale_exp(m * fmaxf(sc[3 * C + 14], sc[3 * C + 15]));
         if (h == 0) v_exp[n & 1][col] = ev;
         uup = pow2(eu);
-        const float a0 = t0 * pow2(-ev), a1 = t1 * pow2(-ev), u0 = t0 * pow2(-eu), u1 = t1 * pow2(-eu);
+        const float a = tscale * pow2(-ev), u = tscale * pow2(-eu);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) hi[i] = h2(__uint_as_float(x[2 * i]) * (i < 8 ? a0 : a1), __uint_as_float(x[2 * i + 1]) * (i < 8 ? a0 : a1));
-        tmem_st16(base + VH + 16 * h, hi);
+        for (int i = 0; i < 8; ++i) hi[i] = h2(__uint_as_float(x[2 * i]) * a, __uint_as_float(x[2 * i + 1]) * a);
+        tmem_st8(base + VH + 8 * h, hi);
         if (!TREE) {
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const float4 w = *(const float4*)&sc[C + 32 * h + 2 * i];
-            const float u = i < 8 ? u0 : u1;
+          for (int i = 0; i < 8; i += 2) {
+            const float4 w = *(const float4*)&sc[C + 16 * h + 2 * i];
             split2(__uint_as_float(x[2 * i]) * (w.x * u), __uint_as_float(x[2 * i + 1]) * (w.y * u), hi[i], lo[i]);
             split2(__uint_as_float(x[2 * i + 2]) * (w.z * u), __uint_as_float(x[2 * i + 3]) * (w.w * u), hi[i + 1], lo[i + 1]);
           }
-          tmem_st16(base + RH + 16 * h, hi);
-          tmem_st16(base + RL + 16 * h, lo);
+          tmem_st8(base + RH + 8 * h, hi);
+          tmem_st8(base + RL + 8 * h, lo);
         }
       }
       tmem_wait_st();
@@ -204,15 +206,15 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
       if (TREE) break;
 
       // S: the update was accumulated apart and is added in fp32
-      ok = wait_for(&u_out[h], n & 1, failed) && ok;
+      ok = wait_for(&u_out[h >> 1], n & 1, failed) && ok;
       fence_after();
 #pragma unroll
-      for (int x = 0; x < NS; x += 32) {
-        uint32_t u[32];
-        tmem_ld32(base + UP + h * NS + x, u);
-        tmem_wait_ld(u);
+      for (int x = 0; x < NS; x += 16) {
+        uint32_t u[16];
+        tmem_ld16(base + UP + h * NS + x, u);
+        tmem_wait_ld16(u);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) S[x + i] = fmaf(__uint_as_float(u[i]), uup, S[x + i] * decay);
+        for (int i = 0; i < 16; ++i) S[x + i] = fmaf(__uint_as_float(u[i]), uup, S[x + i] * decay);
       }
       // the next S is at most decay |S| + |U|, the images of V' and K being at most 2^13 each
       es = scale_exp(fmaf(both, fabsf(decay), uup * (64.f * 67108864.f)));
@@ -225,58 +227,72 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
         if (cok && d < p.dk) So[(long)d * p.dv] = ok ? S[i] : __int_as_float(0x7fffffff);
       }
     }
-  } else if (warp < 12) {
-    // ---------------- output and loads ----------------
-    const int cols = min(COLS, p.dv - vb * COLS);
-    const long per = p.hk * (long)key_bytes(DKP) + p.hv * (long)HEAD_BYTES;
-    const unsigned char* src = p.scratch + (long)b * p.seg_chunks * per;
-    auto load = [&](int n) {  // by one lane
-      uint64_t* bar = &full[n & 1];
-      const uint32_t st = smem_u32(sm + (n & 1) * G::BYTES);
-      const int tok0 = (p.chunk0 + n) * C, rows = min(len - tok0, C);
-      mbar_expect_tx(bar, key_bytes(DKP) + HEAD_BYTES + rows * cols * 2);
-      bulk_copy(st, src + n * per + (long)hk * key_bytes(DKP), key_bytes(DKP), bar);
-      bulk_copy(st + G::T, src + n * per + p.hk * (long)key_bytes(DKP) + (long)hv * HEAD_BYTES, HEAD_BYTES, bar);
-      const bf16* v = p.v + b * p.v_stride[0] + (long)tok0 * p.v_stride[1] + hv * p.v_stride[2] + vb * COLS;
-      for (int i = 0; i < rows; ++i) bulk_copy(st + G::V + i * COLS * 2, v + i * p.v_stride[1], cols * 2, bar);
-    };
-    const bool loader = warp == 8 && elect_one();
-    if (loader)
-      for (int n = 0; n < min(2, nlive); ++n) load(n);
-    __syncwarp();
-    bf16* out = p.out + ((long)b * p.tokens * p.hv + hv) * p.dv + gcol;
+  } else if (warp < 20) {
+    // ---------------- output ----------------
+    bf16* rows_s = (bf16*)(sm + 2 * G::BYTES);  // a chunk's output rows on their way out
+    bf16* out = p.out + ((long)b * p.tokens * p.hv + hv) * p.dv + vb * COLS;
     const long orow = (long)p.hv * p.dv;
+    const int cols = min(COLS, p.dv - vb * COLS);
     for (int n = 0; n < nlive; ++n) {
       const float* sc = (const float*)(sm + (n & 1) * G::BYTES + G::SC);
       const int tok0 = (p.chunk0 + n) * C;
       ok = wait_for(&o_out, n & 1, failed) && ok;
       fence_after();
-      const float sup = pow2(s_exp[n & 1][col]), vup = pow2(v_exp[n & 1][col]);
+      const float sup = pow2(s_exp[n & 1][col]), vup = ok ? pow2(v_exp[n & 1][col]) : __int_as_float(0x7fffffff);
+      if (n > 0) {
+        bulk_stores_read();
+        asm volatile("bar.sync 5, 128;" ::: "memory");  // the rows of the chunk before have left
+      }
+#pragma unroll 1
+      for (int x = 0; x < C; x += 16) {
+        uint32_t a[16], z[16];
+        tmem_ld16(base + QS + x, a);
+        tmem_ld16(base + PV + x, z);
+        tmem_wait_ld16(a);
+        tmem_wait_ld16(z);
+        const float pscale = vup * sc[3 * C + 8 + x / 16];  // P is scaled per 16 rows
 #pragma unroll
-      for (int x = 0; x < C; x += 32) {
-        uint32_t a[32], z[32];
-        tmem_ld32(base + QS + x, a);
-        tmem_ld32(base + PV + x, z);
-        tmem_wait_ld(a);
-        tmem_wait_ld(z);
-        const float p0 = vup * sc[3 * C + 8 + x / 16], p1 = vup * sc[3 * C + 9 + x / 16];  // P is scaled per 16 rows
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float y = fmaf(__uint_as_float(a[i]), sc[2 * C + x + i] * sup, __uint_as_float(z[i]) * (i < 16 ? p0 : p1));
-          if (!ok) y = __int_as_float(0x7fffffff);
-          if (cok && tok0 + x + i < p.tokens) out[(long)(tok0 + x + i) * orow] = f2bf(y);
+        for (int i = 0; i < 16; i += 4) {
+          const float4 w = *(const float4*)&sc[2 * C + x + i];
+          rows_s[(x + i) * COLS + col] = f2bf(fmaf(__uint_as_float(a[i]), w.x * sup, __uint_as_float(z[i]) * pscale));
+          rows_s[(x + i + 1) * COLS + col] = f2bf(fmaf(__uint_as_float(a[i + 1]), w.y * sup, __uint_as_float(z[i + 1]) * pscale));
+          rows_s[(x + i + 2) * COLS + col] = f2bf(fmaf(__uint_as_float(a[i + 2]), w.z * sup, __uint_as_float(z[i + 2]) * pscale));
+          rows_s[(x + i + 3) * COLS + col] = f2bf(fmaf(__uint_as_float(a[i + 3]), w.w * sup, __uint_as_float(z[i + 3]) * pscale));
         }
       }
       fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&o_read);
-      if (loader && n + 2 < nlive && wait_for(&o_read, n & 1, failed)) load(n + 2);
-      __syncwarp();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      asm volatile("bar.sync 5, 128;" ::: "memory");
+      if (lane == 0) mbar_arrive(&o_read);  // TMEM and the scalars have been read
+      if (t - 16 * 32 < C && tok0 + t - 16 * 32 < p.tokens)
+        bulk_store(out + (tok0 + t - 16 * 32) * orow, smem_u32(rows_s + (t - 16 * 32) * COLS), cols * 2);
+      bulk_stores_commit();
     }
+    bulk_stores_done();
     // rows of tokens that no chunk covered: zeros
     const int from = (p.chunk0 + nlive) * C, to = min(p.tokens, (p.chunk0 + p.chunks) * C);
     for (int i = from; i < to; ++i)
-      if (cok) out[(long)i * orow] = f2bf(0.f);
+      if (cok) out[(long)i * orow + col] = f2bf(0.f);
+  } else if (warp == 20) {
+    // ---------------- loads ----------------
+    const int cols = min(COLS, p.dv - vb * COLS);
+    const long per = p.hk * (long)key_bytes(DKP) + p.hv * (long)HEAD_BYTES;
+    const unsigned char* src = p.scratch + (long)b * p.seg_chunks * per;
+    for (int n = 0; n < nlive; ++n) {
+      if (n >= 2) ok = wait_for(&o_read, n & 1, failed) && ok;  // chunk n - 2 has been used up
+      uint64_t* bar = &full[n & 1];
+      const uint32_t st = smem_u32(sm + (n & 1) * G::BYTES);
+      const int tok0 = (p.chunk0 + n) * C, rows = min(len - tok0, C);
+      if (!ok) continue;
+      if (lane == 0) {
+        mbar_expect_tx(bar, key_bytes(DKP) + HEAD_BYTES + rows * cols * 2);
+        bulk_copy(st, src + n * per + (long)hk * key_bytes(DKP), key_bytes(DKP), bar);
+        bulk_copy(st + G::T, src + n * per + p.hk * (long)key_bytes(DKP) + (long)hv * HEAD_BYTES, HEAD_BYTES, bar);
+      }
+      __syncwarp();  // the bytes are announced before any of them can arrive
+      const bf16* v = p.v + b * p.v_stride[0] + (long)tok0 * p.v_stride[1] + hv * p.v_stride[2] + vb * COLS;
+      for (int i = lane; i < rows; i += 32) bulk_copy(st + G::V + i * COLS * 2, v + i * p.v_stride[1], cols * 2, bar);
+    }
   } else {
     // ---------------- products ----------------
     if (elect_one()) {
@@ -343,7 +359,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
   }
   fence_before();
   __syncthreads();
-  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  if (warp == 21) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
 }
 
 template <int DKP, bool TREE>

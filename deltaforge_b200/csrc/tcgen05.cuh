@@ -121,6 +121,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
                DFB_IN8(v, 8)
                : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), DFB_IN8(v, 0) : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // bytes (a multiple of 16) from global to shared memory, both 16-byte aligned
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -128,6 +131,13 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
                "r"(smem_u32(bar))
                : "memory");
 }
+// the same the other way; the source may be written again after bulk_stores_read()
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_stores_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 // 2^x: one instruction, 2 ulp
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
