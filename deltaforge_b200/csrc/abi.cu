@@ -488,6 +488,8 @@ int dfb_delta_chunk(const dfb_delta_chunk_desc* d, void* stream) {
     return bad("dfb_delta_chunk: rows of q, k and v must start on 16-byte boundaries");
   const size_t need = delta_chunk_scratch_bytes(d->batch, d->tokens, d->hk, d->hv, d->dk, d->dv, tree);
   if (need && (!d->scratch || d->scratch_bytes < need || !aligned16(d->scratch))) return bad("dfb_delta_chunk: aligned scratch of %zu bytes required", need);
+  if ((d->hv > 1 && d->v_stride[2] <= 0) || (d->tokens > 1 && d->v_stride[1] <= 0) || (d->batch > 1 && d->v_stride[0] <= 0))
+    return bad("dfb_delta_chunk: v must not be an expanded view");
   DeltaChunkParams p = {};
   p.batch = d->batch;
   p.tokens = d->tokens;

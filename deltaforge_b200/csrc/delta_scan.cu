@@ -26,20 +26,22 @@ constexpr int COLS = 128;  // value columns per CTA
 constexpr int SCAN_WARPS = 22, SCAN_THREADS = SCAN_WARPS * 32;
 
 template <int DKP> struct Stage {
-  static constexpr int T = key_bytes(DKP), P = T + 2 * SQ, SC = P + SQ, V = SC + SCAL, BYTES = V + C * COLS * 2;
-  static constexpr int SMEM = 2 * BYTES + C * COLS * 2 + 1024;
+  static constexpr int T = key_bytes(DKP), P = T + 2 * SQ, V = P + SQ, BYTES = V + C * COLS * 2;
+  // two stages, the scalars of three chunks (the output reads them last), the output's rows, alignment
+  static constexpr int SC = 2 * BYTES, ROWS = SC + 3 * SCAL, SMEM = ROWS + C * COLS * 2 + 1024;
 };
-// TMEM columns. S, R and V' are A operands, two fp16 values per column; the others are accumulators. V' takes the place
-// of R, the product with P that of K S, the update that of T R.
-constexpr int SH = 0, SL = 64, KS = 128, QS = 192, RH = 256, RL = 288, VH = 320, VP = 352, UP = 352, PV = 128;
+// TMEM columns. S, R and V' are A operands, two fp16 values per column; the others are accumulators. V' (for the state) takes
+// the place of R, then the product with P does; the update takes that of T R.
+constexpr int SH = 0, SL = 64, KS = 128, QS = 192, RH = 256, RL = 288, VH = 320, VP = 352, UP = 352, PV = 256;
 
 template <int DKP, bool TREE>
-__global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const DeltaChunkParams p) {
+__global__ void __launch_bounds__(SCAN_THREADS, 1)
+    delta_scan_kernel(const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap omap, const DeltaChunkParams p) {
   using G = Stage<DKP>;
   constexpr int NS = DKP / 4;  // key rows per thread
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  __shared__ uint64_t full[2], s_in[2], ks_out, r_in, vp_out, u_in, u_out[2], o_out, o_read;
+  __shared__ uint64_t full[2], s_in[2], ks_out, r_in, vp_out, u_in, u_out[2], o_out[2], o_read;
   __shared__ float s_max[4][COLS], v_max[4][COLS], vp_max[4][COLS];
   __shared__ int s_exp[2][COLS], v_exp[2][COLS];  // by chunk parity, for the output
   __shared__ uint32_t tmem_slot;
@@ -51,8 +53,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.tokens) : p.tokens;
   const int nlive = min(max((len + C - 1) / C - p.chunk0, 0), p.chunks);  // chunks of this segment with tokens
   if (t == 0) {
-    for (int i = 0; i < 2; ++i) mbar_init(&full[i], 1), mbar_init(&s_in[i], 8), mbar_init(&u_out[i], 1);
-    mbar_init(&ks_out, 1), mbar_init(&vp_out, 1), mbar_init(&o_out, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&full[i], 1), mbar_init(&s_in[i], 8), mbar_init(&u_out[i], 1), mbar_init(&o_out[i], 1);
+    mbar_init(&ks_out, 1), mbar_init(&vp_out, 1);
     mbar_init(&r_in, 16), mbar_init(&u_in, 16), mbar_init(&o_read, 4);
     failed_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -77,14 +79,22 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
     const long sb = ((long)b * p.hv + hv) * p.dk * p.dv + gcol;
     auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + q) : "memory"); };  // the four warps of these columns
     auto most = [&](const float (&m)[4][COLS]) { return fmaxf(fmaxf(m[0][col], m[1][col]), fmaxf(m[2][col], m[3][col])); };
-    float S[NS];
+    // hi and lo of two values
+    auto split = [](F2 v, uint32_t& hi, uint32_t& lo) {
+      hi = h2(v.x, v.y);
+      const float2 f = __half22float2(*(const __half2*)&hi);
+      const F2 r = fma2({f.x, f.y}, {-1.f, -1.f}, v);
+      lo = h2(r.x, r.y);
+    };
+    F2 S[NS / 2];
     const float* Sin = p.first ? p.state + sb : p.state_out + sb;
     float ms = 0.f;
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       const int d = h * NS + i;
-      S[i] = cok && d < p.dk ? Sin[(long)d * p.dv] : 0.f;
-      ms = fmaxf(ms, fabsf(S[i]));
+      const float v = cok && d < p.dk ? Sin[(long)d * p.dv] : 0.f;
+      (i & 1 ? S[i / 2].y : S[i / 2].x) = v;
+      ms = fmaxf(ms, fabsf(v));
     }
     s_max[h][col] = ms;
     meet();
@@ -93,7 +103,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
 
     for (int n = 0; n < nlive; ++n) {
       const unsigned char* st = sm + (n & 1) * G::BYTES;
-      const float* sc = (const float*)(st + G::SC);
+      const float* sc = (const float*)(sm + G::SC + n % 3 * SCAL);
       // S in halves to TMEM; its largest on the side
       {
         const float sdown = pow2(-es);
@@ -103,9 +113,9 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
           uint32_t hi[8], lo[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float s0 = S[x + 2 * i], s1 = S[x + 2 * i + 1];
-            ms = fmaxf(ms, fmaxf(fabsf(s0), fabsf(s1)));
-            split2(s0 * sdown, s1 * sdown, hi[i], lo[i]);
+            const F2 s2 = S[x / 2 + i];
+            ms = fmaxf(fmaxf(ms, fabsf(s2.x)), fabsf(s2.y));
+            split(mul2(s2, {sdown, sdown}), hi[i], lo[i]);
           }
           tmem_st8(base + SH + h * (NS / 2) + x / 2, hi);
           tmem_st8(base + SL + h * (NS / 2) + x / 2, lo);
@@ -148,14 +158,14 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
         tmem_ld16(base + KS + 16 * h, x);
         tmem_wait_ld16(x);
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          const float4 w = *(const float4*)&sc[16 * h + 2 * i];
-          const float r0 = fmaf(-__uint_as_float(x[2 * i]), w.x * wscale, __uint_as_float(v[i] << 16) * rdown);
-          const float r1 = fmaf(-__uint_as_float(x[2 * i + 1]), w.y * wscale, __uint_as_float(v[i] & 0xffff0000u) * rdown);
-          const float r2 = fmaf(-__uint_as_float(x[2 * i + 2]), w.z * wscale, __uint_as_float(v[i + 1] << 16) * rdown);
-          const float r3 = fmaf(-__uint_as_float(x[2 * i + 3]), w.w * wscale, __uint_as_float(v[i + 1] & 0xffff0000u) * rdown);
-          split2(r0, r1, hi[i], lo[i]);
-          split2(r2, r3, hi[i + 1], lo[i + 1]);
+        for (int i = 0; i < 8; ++i) {
+          const float2 w = *(const float2*)&sc[16 * h + 2 * i];
+          const F2 vv = mul2({__uint_as_float(v[i] << 16), __uint_as_float(v[i] & 0xffff0000u)}, {rdown, rdown});
+          split(fma2({__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])}, mul2({w.x, w.y}, {-wscale, -wscale}), vv), hi[i], lo[i]);
+        }
+        if (n > 0) {  // Q S and P V' of the chunk before have been read
+          ok = wait_for(&o_read, (n & 1) ^ 1, failed) && ok;
+          fence_after();
         }
         tmem_st8(base + RH + 8 * h, hi);
         tmem_st8(base + RL + 8 * h, lo);
@@ -186,14 +196,16 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
         uup = pow2(eu);
         const float a = tscale * pow2(-ev), u = tscale * pow2(-eu);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) hi[i] = h2(__uint_as_float(x[2 * i]) * a, __uint_as_float(x[2 * i + 1]) * a);
+        for (int i = 0; i < 8; ++i) {
+          const F2 y = mul2({__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])}, {a, a});
+          hi[i] = h2(y.x, y.y);
+        }
         tmem_st8(base + VH + 8 * h, hi);
         if (!TREE) {
 #pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            const float4 w = *(const float4*)&sc[C + 16 * h + 2 * i];
-            split2(__uint_as_float(x[2 * i]) * (w.x * u), __uint_as_float(x[2 * i + 1]) * (w.y * u), hi[i], lo[i]);
-            split2(__uint_as_float(x[2 * i + 2]) * (w.z * u), __uint_as_float(x[2 * i + 3]) * (w.w * u), hi[i + 1], lo[i + 1]);
+          for (int i = 0; i < 8; ++i) {
+            const float2 w = *(const float2*)&sc[C + 16 * h + 2 * i];
+            split(mul2({__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])}, mul2({w.x, w.y}, {u, u})), hi[i], lo[i]);
           }
           tmem_st8(base + RH + 8 * h, hi);
           tmem_st8(base + RL + 8 * h, lo);
@@ -214,7 +226,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
         tmem_ld16(base + UP + h * NS + x, u);
         tmem_wait_ld16(u);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) S[x + i] = fmaf(__uint_as_float(u[i]), uup, S[x + i] * decay);
+        for (int i = 0; i < 8; ++i)
+          S[x / 2 + i] = fma2({__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])}, {uup, uup}, mul2(S[x / 2 + i], {decay, decay}));
       }
       // the next S is at most decay |S| + |U|, the images of V' and K being at most 2^13 each
       es = scale_exp(fmaf(both, fabsf(decay), uup * (64.f * 67108864.f)));
@@ -224,23 +237,22 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         const int d = h * NS + i;
-        if (cok && d < p.dk) So[(long)d * p.dv] = ok ? S[i] : __int_as_float(0x7fffffff);
+        if (cok && d < p.dk) So[(long)d * p.dv] = ok ? (i & 1 ? S[i / 2].y : S[i / 2].x) : __int_as_float(0x7fffffff);
       }
     }
   } else if (warp < 20) {
     // ---------------- output ----------------
-    bf16* rows_s = (bf16*)(sm + 2 * G::BYTES);  // a chunk's output rows on their way out
+    bf16* rows_s = (bf16*)(sm + G::ROWS);  // a chunk's output rows on their way out
     bf16* out = p.out + ((long)b * p.tokens * p.hv + hv) * p.dv + vb * COLS;
     const long orow = (long)p.hv * p.dv;
-    const int cols = min(COLS, p.dv - vb * COLS);
     for (int n = 0; n < nlive; ++n) {
-      const float* sc = (const float*)(sm + (n & 1) * G::BYTES + G::SC);
+      const float* sc = (const float*)(sm + G::SC + n % 3 * SCAL);
       const int tok0 = (p.chunk0 + n) * C;
-      ok = wait_for(&o_out, n & 1, failed) && ok;
+      ok = wait_for(&o_out[n & 1], (n >> 1) & 1, failed) && ok;
       fence_after();
       const float sup = pow2(s_exp[n & 1][col]), vup = ok ? pow2(v_exp[n & 1][col]) : __int_as_float(0x7fffffff);
       if (n > 0) {
-        bulk_stores_read();
+        if (warp == 16 && lane == 0) bulk_stores_read();
         asm volatile("bar.sync 5, 128;" ::: "memory");  // the rows of the chunk before have left
       }
 #pragma unroll 1
@@ -264,35 +276,36 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       asm volatile("bar.sync 5, 128;" ::: "memory");
       if (lane == 0) mbar_arrive(&o_read);  // TMEM and the scalars have been read
-      if (t - 16 * 32 < C && tok0 + t - 16 * 32 < p.tokens)
-        bulk_store(out + (tok0 + t - 16 * 32) * orow, smem_u32(rows_s + (t - 16 * 32) * COLS), cols * 2);
-      bulk_stores_commit();
+      if (warp == 16 && lane == 0) {  // (rows and columns past the ends are left out)
+        tma_store_box(&omap, smem_u32(rows_s), vb * COLS, hv, tok0, b);
+        bulk_stores_commit();
+      }
     }
-    bulk_stores_done();
+    if (warp == 16 && lane == 0) bulk_stores_done();
     // rows of tokens that no chunk covered: zeros
     const int from = (p.chunk0 + nlive) * C, to = min(p.tokens, (p.chunk0 + p.chunks) * C);
     for (int i = from; i < to; ++i)
       if (cok) out[(long)i * orow + col] = f2bf(0.f);
   } else if (warp == 20) {
     // ---------------- loads ----------------
-    const int cols = min(COLS, p.dv - vb * COLS);
-    const long per = p.hk * (long)key_bytes(DKP) + p.hv * (long)HEAD_BYTES;
-    const unsigned char* src = p.scratch + (long)b * p.seg_chunks * per;
-    for (int n = 0; n < nlive; ++n) {
-      if (n >= 2) ok = wait_for(&o_read, n & 1, failed) && ok;  // chunk n - 2 has been used up
-      uint64_t* bar = &full[n & 1];
-      const uint32_t st = smem_u32(sm + (n & 1) * G::BYTES);
-      const int tok0 = (p.chunk0 + n) * C, rows = min(len - tok0, C);
-      if (!ok) continue;
-      if (lane == 0) {
-        mbar_expect_tx(bar, key_bytes(DKP) + HEAD_BYTES + rows * cols * 2);
+    if (elect_one()) {
+      const long per = p.hk * (long)key_bytes(DKP) + p.hv * (long)HEAD_BYTES;
+      const unsigned char* src = p.scratch + (long)b * p.seg_chunks * per;
+      for (int n = 0; n < nlive; ++n) {
+        // the products of chunk n - 2 are done; they came after the output of chunk n - 3, whose scalars are replaced
+        if (n >= 2) ok = wait_for(&o_out[n & 1], (n >> 1) - 1 & 1, failed) && ok;
+        if (!ok) break;
+        uint64_t* bar = &full[n & 1];
+        const uint32_t st = smem_u32(sm + (n & 1) * G::BYTES);
+        mbar_expect_tx(bar, key_bytes(DKP) + HEAD_BYTES + C * COLS * 2);
         bulk_copy(st, src + n * per + (long)hk * key_bytes(DKP), key_bytes(DKP), bar);
-        bulk_copy(st + G::T, src + n * per + p.hk * (long)key_bytes(DKP) + (long)hv * HEAD_BYTES, HEAD_BYTES, bar);
+        const unsigned char* head = src + n * per + p.hk * (long)key_bytes(DKP) + (long)hv * HEAD_BYTES;
+        bulk_copy(st + G::T, head, 3 * SQ, bar);
+        bulk_copy(smem_u32(sm + G::SC + n % 3 * SCAL), head + 3 * SQ, SCAL, bar);
+        tma_box(st + G::V, &vmap, vb * COLS, hv, (p.chunk0 + n) * C, b, bar);  // (zeros past the ends)
       }
-      __syncwarp();  // the bytes are announced before any of them can arrive
-      const bf16* v = p.v + b * p.v_stride[0] + (long)tok0 * p.v_stride[1] + hv * p.v_stride[2] + vb * COLS;
-      for (int i = lane; i < rows; i += 32) bulk_copy(st + G::V + i * COLS * 2, v + i * p.v_stride[1], cols * 2, bar);
     }
+    __syncwarp();
   } else {
     // ---------------- products ----------------
     if (elect_one()) {
@@ -300,7 +313,6 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
       for (int n = 0; n < nlive; ++n) {
         const uint32_t st = smem_u32(sm + (n & 1) * G::BYTES), ph = n & 1;
         ok = wait_for(&full[n & 1], (n >> 1) & 1, failed) && ok;
-        if (n > 0) ok = wait_for(&o_read, ph ^ 1, failed) && ok;  // Q S and P V' of the chunk before have been read
         // K S, the key rows of each half as soon as they are there
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
@@ -315,11 +327,6 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
           }
         }
         if (ok) commit(&ks_out);
-        // Q S, in the shadow of what the threads do with K S
-        if (ok) {
-#pragma unroll
-          for (int k = 0; k < DKP / 16; ++k) mma_ts(tmem + QS, tmem + SH + k * 8, smem_desc(st + (k >> 2) * (2 * C * 128) + C * 128 + (k & 3) * 32, 0), i64, k != 0);
-        }
         // T R
         ok = wait_for(&r_in, ph, failed) && ok;
         fence_after();
@@ -332,6 +339,11 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
             mma_ts(tmem + VP, tmem + RH + k * 8, tl, i64, true);
           }
           commit(&vp_out);
+        }
+        // Q S, in the shadow of what the threads do with T R; they have waited for the output of the chunk before
+        if (ok) {
+#pragma unroll
+          for (int k = 0; k < DKP / 16; ++k) mma_ts(tmem + QS, tmem + SH + k * 8, smem_desc(st + (k >> 2) * (2 * C * 128) + C * 128 + (k & 3) * 32, 0), i64, k != 0);
         }
         // the update, 64 key dims at a time, then P V'
         ok = wait_for(&u_in, ph, failed) && ok;
@@ -352,7 +364,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1) delta_scan_kernel(const Delta
         }
 #pragma unroll
         for (int k = 0; k < C / 16; ++k) mma_ts(tmem + PV, tmem + VH + k * 8, smem_desc(st + G::P + k * 32, 0), i64, k != 0);
-        commit(&o_out);
+        commit(&o_out[n & 1]);
       }
     }
     __syncwarp();
@@ -382,12 +394,19 @@ int launch_delta_scan(const DeltaChunkParams& p, cudaStream_t stream) {
   static OncePerDevice once;
   const int rc = once.run(configure_all);
   if (rc) return rc;
+  CUtensorMap vmap, omap;
+  const long dims[4] = {p.dv, p.hv, p.tokens, p.batch};
+  if (!encode_map(&vmap, p.v, false, dims, {p.v_stride[2], p.v_stride[1], p.v_stride[0]}, {COLS, 1, C, 1}, false) ||
+      !encode_map(&omap, p.out, false, dims, {p.dv, (long)p.hv * p.dv, (long)p.tokens * p.hv * p.dv}, {COLS, 1, C, 1}, false)) {
+    set_error("delta rule scan: tensor map for the values or the output failed");
+    return 1;
+  }
   const dim3 grid((p.dv + COLS - 1) / COLS, p.hv, p.batch);
   const bool tree = p.parents != nullptr, wide = p.dk > 64;
-  if (tree && wide) delta_scan_kernel<128, true><<<grid, SCAN_THREADS, Stage<128>::SMEM, stream>>>(p);
-  else if (tree) delta_scan_kernel<64, true><<<grid, SCAN_THREADS, Stage<64>::SMEM, stream>>>(p);
-  else if (wide) delta_scan_kernel<128, false><<<grid, SCAN_THREADS, Stage<128>::SMEM, stream>>>(p);
-  else delta_scan_kernel<64, false><<<grid, SCAN_THREADS, Stage<64>::SMEM, stream>>>(p);
+  if (tree && wide) delta_scan_kernel<128, true><<<grid, SCAN_THREADS, Stage<128>::SMEM, stream>>>(vmap, omap, p);
+  else if (tree) delta_scan_kernel<64, true><<<grid, SCAN_THREADS, Stage<64>::SMEM, stream>>>(vmap, omap, p);
+  else if (wide) delta_scan_kernel<128, false><<<grid, SCAN_THREADS, Stage<128>::SMEM, stream>>>(vmap, omap, p);
+  else delta_scan_kernel<64, false><<<grid, SCAN_THREADS, Stage<64>::SMEM, stream>>>(vmap, omap, p);
   return check_launch("delta rule scan");
 }
 

@@ -58,6 +58,11 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
       "l"((uint64_t)map), "r"(dim), "r"(key), "r"(head), "r"(seq), "r"(smem_u32(bar))
       : "memory");
 }
+__device__ __forceinline__ void tma_store_box(const CUtensorMap* map, uint32_t src, int x, int head, int row, int seq) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"((uint64_t)map), "r"(x), "r"(head), "r"(row),
+               "r"(seq), "r"(src)
+               : "memory");
+}
 // Rows of one 128-byte swizzle span, 8-row groups 1024 bytes apart. `lead`: for an operand whose rows run along its
 // contraction (V: a row is a key), bytes from one block of 64 dims to the next; unused where rows run along M or N.
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead) {
@@ -131,10 +136,7 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
                "r"(smem_u32(bar))
                : "memory");
 }
-// the same the other way; the source may be written again after bulk_stores_read()
-__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
-  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
-}
+// stores: the source may be written again after bulk_stores_read()
 __device__ __forceinline__ void bulk_stores_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void bulk_stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
@@ -143,6 +145,59 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Pairs of fp32 in one instruction each
+struct F2 {
+  float x, y;
+};
+__device__ __forceinline__ unsigned long long f2_bits(F2 a) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+  return r;
+}
+__device__ __forceinline__ F2 f2_from(unsigned long long r) {
+  F2 a;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(r));
+  return a;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return f2_from(r);
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
+  return f2_from(r);
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+inline EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = []() -> EncodeTiledFn {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return nullptr;
+    return (EncodeTiledFn)ptr;
+  }();
+  return fn;
+}
+// A tensor of four dimensions of 16-bit elements, innermost first; stride[i] (elements) belongs to dimension i + 1, and that of
+// a dimension of one may be anything.
+inline bool encode_map(CUtensorMap* map, const void* base, bool fp16, const long (&dim)[4], const long (&stride)[3], const int (&box)[4], bool swizzle) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[4], strides[3];
+  cuuint32_t boxes[4], es[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) dims[i] = (cuuint64_t)dim[i], boxes[i] = (cuuint32_t)box[i];
+  for (int i = 0; i < 3; ++i) strides[i] = (cuuint64_t)(dim[i + 1] > 1 ? stride[i] : (dim[0] + 7) / 8 * 8) * 2;
+  return enc(map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void*)base, dims, strides, boxes, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace

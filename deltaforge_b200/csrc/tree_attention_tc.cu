@@ -588,32 +588,9 @@ __global__ void __launch_bounds__(256) tree_tc_merge_kernel(const TreeAttnParams
   *(uint2*)out = ok ? make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv)) : make_uint2(0u, 0u);
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = []() -> EncodeTiledFn {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      return nullptr;
-    return (EncodeTiledFn)ptr;
-  }();
-  return fn;
-}
-
 // The cache as [sequence][KV head][row][D] with the caller's strides; boxes of 64 dims x `rows` rows.
 bool encode_cache(CUtensorMap* map, const void* base, const long* stride, int rows, const TreeAttnParams& p) {
-  EncodeTiledFn enc = encode_fn();
-  if (!enc) return false;
-  const cuuint64_t dims[4] = {(cuuint64_t)p.d, (cuuint64_t)p.max_seq, (cuuint64_t)p.hkv, (cuuint64_t)p.batch};
-  const long row = p.max_seq > 1 ? stride[2] : p.d;  // (the stride of a dimension of one is never used and may be anything)
-  const cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)(p.hkv > 1 ? stride[1] : row) * 2, (cuuint64_t)(p.batch > 1 ? stride[0] : row) * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, es[4] = {1, 1, 1, 1};
-  return enc(map, p.is_fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void*)base, dims, strides, box, es,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_map(map, base, p.is_fp16, {p.d, p.max_seq, p.hkv, p.batch}, {stride[2], stride[1], stride[0]}, {64, rows, 1, 1}, true);
 }
 
 template <typename T, int D>

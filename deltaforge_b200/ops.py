@@ -1121,8 +1121,8 @@ def _delta_tokens(
     q_rows, k_rows, v_rows = _rows(op, "query", query), _rows(op, "key", key), _rows(op, "value", value)
     _same_device(op, state, query, key, value, g, beta, lengths, parents)
     qp, kp, vp = query.data_ptr(), key.data_ptr(), value.data_ptr()
-    if (q_rows[0] | q_rows[1] | q_rows[2] | k_rows[0] | k_rows[1] | k_rows[2] | v_rows[0] | v_rows[1] | v_rows[2]) % 8 or (qp | kp | vp) % 16:
-        query, key, value = _aligned_rows(query), _aligned_rows(key), _aligned_rows(value)
+    if 0 in v_rows or (q_rows[0] | q_rows[1] | q_rows[2] | k_rows[0] | k_rows[1] | k_rows[2] | v_rows[0] | v_rows[1] | v_rows[2]) % 8 or (qp | kp | vp) % 16:
+        query, key, value = _aligned_rows(query), _aligned_rows(key), _aligned_rows(value) if 0 not in v_rows else value.contiguous()
         q_rows, k_rows, v_rows = query.stride()[:3], key.stride()[:3], value.stride()[:3]
         qp, kp, vp = query.data_ptr(), key.data_ptr(), value.data_ptr()
     if not state.is_contiguous():

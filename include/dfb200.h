@@ -334,7 +334,7 @@ typedef struct dfb_delta_chunk_desc {
   int32_t batch, tokens, hk, hv, dk, dv; /* dk, dv multiples of 8, dk <= 128, hv a multiple of hk */
   const void* q;  /* bf16 [batch, tokens, hk, dk], strides batch, token, head (multiples of 8), 16-byte aligned */
   const void* k;
-  const void* v;  /* bf16 [batch, tokens, hv, dv] */
+  const void* v;  /* bf16 [batch, tokens, hv, dv], strides above 0 */
   int64_t q_stride[3], k_stride[3], v_stride[3];
   const float* g;    /* [batch, tokens, hv] log decay */
   const float* beta; /* [batch, tokens, hv] */
