@@ -10,12 +10,13 @@ namespace dfb {
 namespace {
 
 constexpr int C = 64;                // tokens per chunk
-constexpr int SQ = C * C * 2;        // bytes of one 64 x 64 fp16 image
-// Scalars of a (chunk, value head), floats: on K S, on V' into the state, on Q S per token; then at 3 C: decay of the state,
-// +4: scales of T per 16 rows, +8: scales of P likewise, +12, +13: the largest on K S per 32 tokens, +14, +15: the largest
-// on V' likewise, +16, +17: a bit per token that counts.
-constexpr int SCAL = 4 * C * 4;
-constexpr int HEAD_BYTES = 3 * SQ + SCAL;  // of a value head: T (hi, lo), P, scalars
+constexpr int SQ = C * C * 2;        // bytes of one 64 x 64 16-bit image
+// Scalars of a (chunk, value head), floats: on V' into the state, on Q S per token; then at 2 C: decay of the state, +4: scales
+// of W per 16 rows, +8: scales of P likewise, +12, +13: the largest on V' per 32 tokens, +14, +15: a bit per token that counts.
+constexpr int SCAL = 3 * C * 4;
+__host__ __device__ constexpr int w_bytes(int dkp) { return dkp / 64 * SQ; }  // of one half of W: per 64 key dims its 64 rows
+// of a value head: T (three bf16 parts), P, W (hi, lo), scalars
+__host__ __device__ constexpr int head_bytes(int dkp) { return 4 * SQ + 2 * (dkp / 64 * SQ) + SCAL; }
 // of a key head: per 64 key dims the 64 rows of k, then those of q
 __host__ __device__ constexpr int key_bytes(int dkp) { return dkp / 64 * 2 * C * 128; }
 

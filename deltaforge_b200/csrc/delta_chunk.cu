@@ -40,6 +40,22 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// (a, b) as three pairs of bf16 that add up to them: 24 bits
+__device__ __forceinline__ void split3(float a, float b, uint32_t& p0, uint32_t& p1, uint32_t& p2) {
+  const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+  const float2 xf = __bfloat1622float2(x);
+  const __nv_bfloat162 y = __floats2bfloat162_rn(a - xf.x, b - xf.y);
+  const float2 yf = __bfloat1622float2(y);
+  const __nv_bfloat162 z = __floats2bfloat162_rn(a - xf.x - yf.x, b - xf.y - yf.y);
+  p0 = *(const uint32_t*)&x, p1 = *(const uint32_t*)&y, p2 = *(const uint32_t*)&z;
+}
+
 constexpr int PREP_THREADS = 128;
 constexpr int TS = 68;  // row stride (floats) of the 64 x 64 fp32 matrices: 16-byte rows, neighbouring rows in other banks
 
@@ -79,10 +95,10 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
   extern __shared__ __align__(128) unsigned char smem[];
   unsigned char* kt = smem;                                  // bf16 [64][DKP]
   unsigned char* qt = smem + C * DKP * 2;
-  float* A = (float*)(smem + (2 * C * DKP * 2 > C * TS * 4 ? 2 * C * DKP * 2 : C * TS * 4));  // [64][TS]
-  float* T = (float*)smem;                                   // [64][TS], over the tiles once they have been read
+  float* T = (float*)qt;                                     // [64][TS], over the queries once they have been read
+  float* A = T + C * TS;                                     // [64][TS]
   __shared__ float4 col[C];                                  // per token: log2 decay sum (hi, lo), 1/|k|, beta
-  __shared__ float rq[C], sk[C], sq[C];
+  __shared__ float rq[C], sk[C], sq[C], on_w[C];
   __shared__ unsigned long long anc[C];
   __shared__ int up[C];
   __shared__ double gsum[C];
@@ -121,9 +137,11 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
     }
   }
 
-  const long sbase = ((long)b * p.seg_chunks + cl) * (p.hk * (long)key_bytes(DKP) + p.hv * (long)HEAD_BYTES);
+  const long sbase = ((long)b * p.seg_chunks + cl) * (p.hk * (long)key_bytes(DKP) + p.hv * (long)head_bytes(DKP));
   unsigned char* kimg = p.scratch + sbase + (long)hk * key_bytes(DKP);
-  unsigned char* himg = p.scratch + sbase + p.hk * (long)key_bytes(DKP) + (long)hv * HEAD_BYTES;
+  unsigned char* himg = p.scratch + sbase + p.hk * (long)key_bytes(DKP) + (long)hv * head_bytes(DKP);
+  unsigned char *pimg = himg + 3 * SQ, *wimg = himg + 4 * SQ;
+  float* sc = (float*)(wimg + 2 * w_bytes(DKP));
   const bool first = hv % group == 0;  // the first value head of a key head writes the key head's images
 
   // ---- 1 ----
@@ -283,10 +301,10 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
     const float down = pow2(-ep);
 #pragma unroll
     for (int nt = 0; nt < 8; ++nt) {
-      *(uint32_t*)(himg + 2 * SQ + img_off<C>(r0 + g, nt) + 4 * c) = h2(qk[nt][0] * down, qk[nt][1] * down);
-      *(uint32_t*)(himg + 2 * SQ + img_off<C>(r0 + g + 8, nt) + 4 * c) = h2(qk[nt][2] * down, qk[nt][3] * down);
+      *(uint32_t*)(pimg + img_off<C>(r0 + g, nt) + 4 * c) = h2(qk[nt][0] * down, qk[nt][1] * down);
+      *(uint32_t*)(pimg + img_off<C>(r0 + g + 8, nt) + 4 * c) = h2(qk[nt][2] * down, qk[nt][3] * down);
     }
-    if (lane == 0) ((float*)(himg + 3 * SQ))[3 * C + 8 + warp] = pow2(ep);
+    if (lane == 0) sc[2 * C + 8 + warp] = pow2(ep);
   }
   __syncwarp();
 
@@ -307,7 +325,11 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
       x[i] -= s0 + s1;
     }
   }
-  __syncthreads();  // A is complete, the tiles have been read
+  if (t < C) {
+    const float4 v = col[t];
+    on_w[t] = exp2_fast(v.x + v.y) * v.z * v.w;
+  }
+  __syncthreads();  // A is complete, the queries have been read
   if (lane < 16) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) T[(r0 + i) * TS + r0 + lane] = x[i];
@@ -349,45 +371,88 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
   }
   __syncthreads();
 
-  // ---- 5: this warp's 16 rows, eight columns per lane and pass ----
+  // ---- 5: W = T diag(beta e^G / |k|) K for this warp's 16 rows, the left factor in three bf16 parts (K is bf16) ----
   {
-    float tv[4][8], tm = 0.f;
+    float w[DKP / 8][4];
+#pragma unroll
+    for (int nt = 0; nt < DKP / 8; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[nt][e] = 0.f;
+    const uint32_t ks_s = smem_u32(kt);
+#pragma unroll 1
+    for (int ks = 0; ks <= warp; ++ks) {
+      uint32_t ta[3][4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // rows g, g + 8 of columns 2 c, then of columns 2 c + 8
+        const int row = r0 + g + 8 * (e & 1), j = 16 * ks + 2 * c + 8 * (e >> 1);
+        const float2 x = *(const float2*)&T[row * TS + j], f = *(const float2*)&on_w[j];
+        split3(x.x * f.x, x.y * f.y, ta[0][e], ta[1][e], ta[2][e]);
+      }
+#pragma unroll
+      for (int n2 = 0; n2 < DKP / 16; ++n2) {
+        uint32_t kb[4];
+        ldsm4_t(ks_s + img_off<DKP>(16 * ks + (lane & 15), 2 * n2 + (lane >> 4)), kb);
+#pragma unroll
+        for (int part = 2; part >= 0; --part) {
+          mma_bf16(w[2 * n2], ta[part], kb[0], kb[1]);
+          mma_bf16(w[2 * n2 + 1], ta[part], kb[2], kb[3]);
+        }
+      }
+    }
+    float wm = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < DKP / 8; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) wm = fmaxf(wm, fabsf(w[nt][e]));
+    const int ew = scale_exp(warp_max_abs(wm));
+    const float down = pow2(-ew);
+    if (lane == 0) sc[2 * C + 4 + warp] = pow2(ew);
+    // through this warp's rows of A, 64 key dims of one half at a time: 16 rows are 2 KB in a row of the image
+    unsigned char* stage = (unsigned char*)(A + r0 * TS);
+#pragma unroll
+    for (int x = 0; x < DKP / 64; ++x) {
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          uint32_t hi, lo;
+          split2(w[8 * x + nt][2 * r] * down, w[8 * x + nt][2 * r + 1] * down, hi, lo);
+          *(uint32_t*)(stage + img_off<64>(g + 8 * r, nt) + 4 * c) = hi;
+          *(uint32_t*)(stage + 2048 + img_off<64>(g + 8 * r, nt) + 4 * c) = lo;
+        }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        *(uint4*)(wimg + (i >> 2) * w_bytes(DKP) + x * SQ + r0 * 128 + (i & 3) * 512 + lane * 16) = *(const uint4*)(stage + i * 512 + lane * 16);
+      __syncwarp();
+    }
+  }
+
+  // ---- 6: T diag(beta), this warp's 16 rows, eight columns per lane and pass ----
+  {
     const int j0 = (lane & 7) * 8;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const float* src = &T[(r0 + 4 * k + (lane >> 3)) * TS + j0];
-      *(float4*)&tv[k][0] = *(const float4*)src;
-      *(float4*)&tv[k][4] = *(const float4*)(src + 4);
+      float tv[8];
+      *(float4*)&tv[0] = *(const float4*)src;
+      *(float4*)&tv[4] = *(const float4*)(src + 4);
+      uint32_t part[3][4];
 #pragma unroll
-      for (int y = 0; y < 8; ++y) {
-        tv[k][y] *= col[j0 + y].w;
-        tm = fmaxf(tm, fabsf(tv[k][y]));
-      }
-    }
-    const int et = scale_exp(warp_max_abs(tm));
-    const float down = pow2(-et);
+      for (int y = 0; y < 4; ++y) split3(tv[2 * y] * col[j0 + 2 * y].w, tv[2 * y + 1] * col[j0 + 2 * y + 1].w, part[0][y], part[1][y], part[2][y]);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      uint4 hi, lo;
-      split2(tv[k][0] * down, tv[k][1] * down, hi.x, lo.x);
-      split2(tv[k][2] * down, tv[k][3] * down, hi.y, lo.y);
-      split2(tv[k][4] * down, tv[k][5] * down, hi.z, lo.z);
-      split2(tv[k][6] * down, tv[k][7] * down, hi.w, lo.w);
-      *(uint4*)(himg + img_off<C>(r0 + 4 * k + (lane >> 3), lane & 7)) = hi;
-      *(uint4*)(himg + SQ + img_off<C>(r0 + 4 * k + (lane >> 3), lane & 7)) = lo;
+      for (int i = 0; i < 3; ++i)
+        *(uint4*)(himg + i * SQ + img_off<C>(r0 + 4 * k + (lane >> 3), lane & 7)) = make_uint4(part[i][0], part[i][1], part[i][2], part[i][3]);
     }
-    float* sc = (float*)(himg + 3 * SQ);
-    if (lane == 0) sc[3 * C + 4 + warp] = pow2(et);
     if (t < C) {
       const float4 v = col[t], e = col[C - 1];
-      const float eg = exp2_fast(v.x + v.y), on_ks = eg * sk[t], on_v = exp2_fast((e.x - v.x) + (e.y - v.y)) * sk[t];
-      sc[t] = on_ks;
-      sc[C + t] = on_v;
-      sc[2 * C + t] = eg * sq[t];
-      if (t == C - 1) sc[3 * C] = eg;
-      const float m0 = warp_max_abs(on_ks), m1 = warp_max_abs(on_v);
+      const float eg = exp2_fast(v.x + v.y), on_v = exp2_fast((e.x - v.x) + (e.y - v.y)) * sk[t];
+      sc[t] = on_v;
+      sc[C + t] = eg * sq[t];
+      if (t == C - 1) sc[2 * C] = eg;
+      const float m = warp_max_abs(on_v);
       const unsigned counts = __ballot_sync(0xffffffffu, t < live && (!TREE || anc[t] != 0));
-      if (lane == 0) sc[3 * C + 12 + warp] = m0, sc[3 * C + 14 + warp] = m1, sc[3 * C + 16 + warp] = __uint_as_float(counts);
+      if (lane == 0) sc[2 * C + 12 + warp] = m, sc[2 * C + 14 + warp] = __uint_as_float(counts);
     }
   }
   if (stays) pdl_wait();
@@ -484,10 +549,10 @@ __global__ void __launch_bounds__(FEW_THREADS) delta_few_kernel(const DeltaChunk
 }
 
 int pad_dk(int dk) { return dk <= 64 ? 64 : 128; }
-size_t chunk_bytes(int hk, int hv, int dk) { return (size_t)hk * key_bytes(pad_dk(dk)) + (size_t)hv * HEAD_BYTES; }
+size_t chunk_bytes(int hk, int hv, int dk) { return (size_t)hk * key_bytes(pad_dk(dk)) + (size_t)hv * head_bytes(pad_dk(dk)); }
 
 // How a prompt is walked through: in segments, each prepared by one kernel and scanned by the next. The scratch of a long prompt
-// so stays bounded, and in the L2 (1.3 MB per chunk at 16 key and 32 value heads).
+// so stays bounded, and in the L2 (2.6 MB per chunk at 16 key and 32 value heads).
 // Where the scan leaves most SMs idle (one CTA per head and sequence), the preparation of a segment runs beside the scan of the
 // one before, out of the other half of the scratch; only the first, short one is waited for.
 struct Walk {
@@ -497,7 +562,7 @@ struct Walk {
 Walk plan_walk(int batch, int tokens, int hk, int hv, int dk, int dv) {
   Walk w;
   const int chunks = (tokens + C - 1) / C;
-  const long fit = (long)((size_t)64 * 1024 * 1024 / (chunk_bytes(hk, hv, dk) * batch));
+  const long fit = (long)((size_t)128 * 1024 * 1024 / (chunk_bytes(hk, hv, dk) * batch));
   const long heads = (long)batch * hv, wave = 4 * 148 / heads;  // chunks whose preparation fills the SMs once
   w.beside = heads * ((dv + 127) / 128) <= 100 && chunks > wave;
   long seg = w.beside ? fit / 2 : fit;
@@ -509,7 +574,8 @@ Walk plan_walk(int batch, int tokens, int hk, int hv, int dk, int dv) {
   return w;
 }
 
-template <int DKP> constexpr int prep_smem() { return (2 * C * DKP * 2 > C * TS * 4 ? 2 * C * DKP * 2 : C * TS * 4) + C * TS * 4; }
+// keys, then T (or the queries, which need less), then A
+template <int DKP> constexpr int prep_smem() { return C * DKP * 2 + 2 * C * TS * 4; }
 
 template <int DKP, bool TREE>
 int configure() {

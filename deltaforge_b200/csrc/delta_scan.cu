@@ -26,13 +26,14 @@ constexpr int COLS = 128;  // value columns per CTA
 constexpr int SCAN_WARPS = 22, SCAN_THREADS = SCAN_WARPS * 32;
 
 template <int DKP> struct Stage {
-  static constexpr int T = key_bytes(DKP), P = T + 2 * SQ, V = P + SQ, BYTES = V + C * COLS * 2;
-  // two stages, the scalars of three chunks (the output reads them last), the output's rows, alignment
-  static constexpr int SC = 2 * BYTES, ROWS = SC + 3 * SCAL, SMEM = ROWS + C * COLS * 2 + 1024;
+  static constexpr int P = key_bytes(DKP), W = P + SQ, BYTES = W + 2 * w_bytes(DKP);
+  // two stages; T and the values, which one product reads; the scalars of three chunks (the output reads them last); the
+  // output's rows; alignment
+  static constexpr int T = 2 * BYTES, V = T + 3 * SQ, ROWS = V + C * COLS * 2, SC = ROWS + C * COLS * 2, SMEM = SC + 3 * SCAL + 1024;
 };
-// TMEM columns. S, R and V' are A operands, two fp16 values per column; the others are accumulators. V' (for the state) takes
-// the place of R, then the product with P does; the update takes that of T R.
-constexpr int SH = 0, SL = 64, KS = 128, QS = 192, RH = 256, RL = 288, VH = 320, VP = 352, UP = 352, PV = 256;
+// TMEM columns. S and V' are A operands, two fp16 values per column (V' twice: in halves with the decays into the state, and as
+// it is for the output); the others are accumulators. The update takes the place of W S, P V' that of the V' in halves.
+constexpr int SH = 0, SL = 64, WS = 128, UP = 128, QS = 256, TV = 320, RH = 384, RL = 416, PV = 384, VH = 448;
 
 template <int DKP, bool TREE>
 __global__ void __launch_bounds__(SCAN_THREADS, 1)
@@ -41,8 +42,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   constexpr int NS = DKP / 4;  // key rows per thread
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  __shared__ uint64_t full[2], s_in[2], ks_out, r_in, vp_out, u_in, u_out[2], o_out[2], o_read;
-  __shared__ float s_max[4][COLS], v_max[4][COLS], vp_max[4][COLS];
+  __shared__ uint64_t full[2], v_full, v_in, s_in[2], tv_out, ws_out, u_in, u_out[2], o_out[2], o_read;
+  __shared__ float s_max[4][COLS], vp_max[4][COLS];
   __shared__ int s_exp[2][COLS], v_exp[2][COLS];  // by chunk parity, for the output
   __shared__ uint32_t tmem_slot;
   __shared__ int failed_s;
@@ -54,8 +55,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   const int nlive = min(max((len + C - 1) / C - p.chunk0, 0), p.chunks);  // chunks of this segment with tokens
   if (t == 0) {
     for (int i = 0; i < 2; ++i) mbar_init(&full[i], 1), mbar_init(&s_in[i], 8), mbar_init(&u_out[i], 1), mbar_init(&o_out[i], 1);
-    mbar_init(&ks_out, 1), mbar_init(&vp_out, 1);
-    mbar_init(&r_in, 16), mbar_init(&u_in, 16), mbar_init(&o_read, 4);
+    mbar_init(&v_full, 1), mbar_init(&v_in, 1), mbar_init(&tv_out, 1), mbar_init(&ws_out, 1);
+    mbar_init(&u_in, 16), mbar_init(&o_read, 4);
     failed_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -102,7 +103,6 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
     meet();
 
     for (int n = 0; n < nlive; ++n) {
-      const unsigned char* st = sm + (n & 1) * G::BYTES;
       const float* sc = (const float*)(sm + G::SC + n % 3 * SCAL);
       // S in halves to TMEM; its largest on the side
       {
@@ -128,83 +128,53 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       s_max[h][col] = ms;
       if (h == 0) s_exp[n & 1][col] = es;
 
-      // this thread's values, and the largest of the column
+      // V' = T V - W S
       ok = wait_for(&full[n & 1], (n >> 1) & 1, failed) && ok;
-      const uint32_t counts = cok ? __float_as_uint(sc[3 * C + 16 + (h >> 1)]) >> (16 * (h & 1)) : 0u;
-      const unsigned short* vs = (const unsigned short*)(st + G::V) + h * 16 * COLS + col;
-      uint32_t v[8];  // two tokens each
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t lo = (counts >> (2 * i)) & 1 ? vs[2 * i * COLS] : 0, hi = (counts >> (2 * i + 1)) & 1 ? vs[(2 * i + 1) * COLS] : 0;
-        v[i] = lo | hi << 16;
-      }
-      __nv_bfloat162 mv = __float2bfloat162_rn(0.f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) mv = __hmax2_nan(mv, __habs2(*(const __nv_bfloat162*)&v[i]));
-      const float2 mvf = __bfloat1622float2(mv);
-      v_max[h][col] = fmaxf(mvf.x, mvf.y);
-      meet();
-      // |K S| <= |k|_2 sqrt(dk) |S|, where both factors' images are at most 2^13 and so is a key's norm
-      const float ks_max = fmaxf(sc[3 * C + 12], sc[3 * C + 13]) * pow2(es) * (11.4f * 67108864.f);
-      const int er = scale_exp(most(v_max) + ks_max);
-      const float both = most(s_max);
-      const float rdown = pow2(-er), wscale = pow2(es) * rdown;
-
-      // R = V - diag(e^G) K S
-      ok = wait_for(&ks_out, n & 1, failed) && ok;
+      const float wscale = pow2(es) * sc[2 * C + 4 + h], decay = sc[2 * C];  // W is scaled per 16 rows
+      ok = wait_for(&tv_out, n & 1, failed) && ok;
       fence_after();
+      float uup, both;
       {
         uint32_t x[16], hi[8], lo[8];
-        tmem_ld16(base + KS + 16 * h, x);
+        tmem_ld16(base + TV + 16 * h, x);
         tmem_wait_ld16(x);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 w = *(const float2*)&sc[16 * h + 2 * i];
-          const F2 vv = mul2({__uint_as_float(v[i] << 16), __uint_as_float(v[i] & 0xffff0000u)}, {rdown, rdown});
-          split(fma2({__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])}, mul2({w.x, w.y}, {-wscale, -wscale}), vv), hi[i], lo[i]);
-        }
-        if (n > 0) {  // Q S and P V' of the chunk before have been read
-          ok = wait_for(&o_read, (n & 1) ^ 1, failed) && ok;
-          fence_after();
-        }
-        tmem_st8(base + RH + 8 * h, hi);
-        tmem_st8(base + RL + 8 * h, lo);
-      }
-      tmem_wait_st();
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&r_in);
-
-      // V'
-      ok = wait_for(&vp_out, n & 1, failed) && ok;
-      fence_after();
-      float uup;
-      const float decay = sc[3 * C];
-      {
-        uint32_t x[16], hi[8], lo[8];
-        tmem_ld16(base + VP + 16 * h, x);
-        tmem_wait_ld16(x);
-        const float tscale = pow2(er) * sc[3 * C + 4 + h];  // T is scaled per 16 rows
+        ok = wait_for(&ws_out, n & 1, failed) && ok;
+        fence_after();
         float m0 = 0.f, m1 = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m0 = fmaxf(m0, fabsf(__uint_as_float(x[i]))), m1 = fmaxf(m1, fabsf(__uint_as_float(x[8 + i])));
-        vp_max[h][col] = fmaxf(m0, m1) * tscale;
+        for (int y = 0; y < 16; y += 8) {
+          uint32_t z[8];
+          tmem_ld8(base + WS + 16 * h + y, z);
+          tmem_wait_ld8(z);
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) {
+            const F2 r = fma2({__uint_as_float(z[i]), __uint_as_float(z[i + 1])}, {-wscale, -wscale}, {__uint_as_float(x[y + i]), __uint_as_float(x[y + i + 1])});
+            x[y + i] = __float_as_uint(r.x), x[y + i + 1] = __float_as_uint(r.y);
+            m0 = fmaxf(m0, fabsf(r.x)), m1 = fmaxf(m1, fabsf(r.y));
+          }
+        }
+        vp_max[h][col] = fmaxf(m0, m1);
         meet();
+        both = most(s_max);
         const float m = most(vp_max);
-        const int ev = scale_exp(m), eu = scale_exp(m * fmaxf(sc[3 * C + 14], sc[3 * C + 15]));
+        const int ev = scale_exp(m), eu = scale_exp(m * fmaxf(sc[2 * C + 12], sc[2 * C + 13]));
         if (h == 0) v_exp[n & 1][col] = ev;
         uup = pow2(eu);
-        const float a = tscale * pow2(-ev), u = tscale * pow2(-eu);
+        const float a = pow2(-ev), u = pow2(-eu);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const F2 y = mul2({__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])}, {a, a});
           hi[i] = h2(y.x, y.y);
         }
+        if (n > 0) {  // Q S and P V' of the chunk before have been read
+          ok = wait_for(&o_read, (n & 1) ^ 1, failed) && ok;
+          fence_after();
+        }
         tmem_st8(base + VH + 8 * h, hi);
         if (!TREE) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float2 w = *(const float2*)&sc[C + 16 * h + 2 * i];
+            const float2 w = *(const float2*)&sc[16 * h + 2 * i];
             split(mul2({__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])}, mul2({w.x, w.y}, {u, u})), hi[i], lo[i]);
           }
           tmem_st8(base + RH + 8 * h, hi);
@@ -262,10 +232,10 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
         tmem_ld16(base + PV + x, z);
         tmem_wait_ld16(a);
         tmem_wait_ld16(z);
-        const float pscale = vup * sc[3 * C + 8 + x / 16];  // P is scaled per 16 rows
+        const float pscale = vup * sc[2 * C + 8 + x / 16];  // P is scaled per 16 rows
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
-          const float4 w = *(const float4*)&sc[2 * C + x + i];
+          const float4 w = *(const float4*)&sc[C + x + i];
           rows_s[(x + i) * COLS + col] = f2bf(fmaf(__uint_as_float(a[i]), w.x * sup, __uint_as_float(z[i]) * pscale));
           rows_s[(x + i + 1) * COLS + col] = f2bf(fmaf(__uint_as_float(a[i + 1]), w.y * sup, __uint_as_float(z[i + 1]) * pscale));
           rows_s[(x + i + 2) * COLS + col] = f2bf(fmaf(__uint_as_float(a[i + 2]), w.z * sup, __uint_as_float(z[i + 2]) * pscale));
@@ -288,32 +258,72 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       if (cok) out[(long)i * orow + col] = f2bf(0.f);
   } else if (warp == 20) {
     // ---------------- loads ----------------
-    if (elect_one()) {
-      const long per = p.hk * (long)key_bytes(DKP) + p.hv * (long)HEAD_BYTES;
-      const unsigned char* src = p.scratch + (long)b * p.seg_chunks * per;
-      for (int n = 0; n < nlive; ++n) {
-        // the products of chunk n - 2 are done; they came after the output of chunk n - 3, whose scalars are replaced
-        if (n >= 2) ok = wait_for(&o_out[n & 1], (n >> 1) - 1 & 1, failed) && ok;
-        if (!ok) break;
+    const long per = p.hk * (long)key_bytes(DKP) + p.hv * (long)head_bytes(DKP);
+    const unsigned char* src = p.scratch + (long)b * p.seg_chunks * per;
+    for (int n = 0; n < nlive; ++n) {
+      // the products of chunk n - 2 are done; they came after the output of chunk n - 3, whose scalars are replaced
+      if (n >= 2) ok = wait_for(&o_out[n & 1], ((n >> 1) - 1) & 1, failed) && ok;
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const unsigned char* head = src + n * per + p.hk * (long)key_bytes(DKP) + (long)hv * head_bytes(DKP);
+      const uint32_t st = smem_u32(sm + (n & 1) * G::BYTES);
+      unsigned char* scn = sm + G::SC + n % 3 * SCAL;
+      if (elect_one()) {
         uint64_t* bar = &full[n & 1];
-        const uint32_t st = smem_u32(sm + (n & 1) * G::BYTES);
-        mbar_expect_tx(bar, key_bytes(DKP) + HEAD_BYTES + C * COLS * 2);
+        mbar_expect_tx(bar, G::BYTES + SCAL);
         bulk_copy(st, src + n * per + (long)hk * key_bytes(DKP), key_bytes(DKP), bar);
-        const unsigned char* head = src + n * per + p.hk * (long)key_bytes(DKP) + (long)hv * HEAD_BYTES;
-        bulk_copy(st + G::T, head, 3 * SQ, bar);
-        bulk_copy(smem_u32(sm + G::SC + n % 3 * SCAL), head + 3 * SQ, SCAL, bar);
-        tma_box(st + G::V, &vmap, vb * COLS, hv, (p.chunk0 + n) * C, b, bar);  // (zeros past the ends)
+        bulk_copy(st + G::P, head + 3 * SQ, SQ + 2 * w_bytes(DKP), bar);
+        bulk_copy(smem_u32(scn), head + 4 * SQ + 2 * w_bytes(DKP), SCAL, bar);
       }
+      __syncwarp();
+      if (n > 0) ok = wait_for(&tv_out, (n - 1) & 1, failed) && ok;
+      if (!__all_sync(0xffffffffu, ok)) break;
+      if (elect_one()) {
+        mbar_expect_tx(&v_full, 3 * SQ + C * COLS * 2);
+        bulk_copy(smem_u32(sm + G::T), head, 3 * SQ, &v_full);
+        for (int i = 0; i < 2; ++i)  // (zeros past the ends)
+          tma_box(smem_u32(sm + G::V + i * C * 128), &vmap, vb * COLS + 64 * i, hv, (p.chunk0 + n) * C, b, &v_full);
+      }
+      __syncwarp();
+      // values of tokens that do not count may be anything: zeros take their place
+      ok = wait_for(&full[n & 1], (n >> 1) & 1, failed) && ok;
+      ok = wait_for(&v_full, n & 1, failed) && ok;
+      if (!__all_sync(0xffffffffu, ok)) break;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t empty = ~__float_as_uint(((const float*)scn)[2 * C + 14 + i]);
+        if (empty) {
+          while (empty) {
+            const int row = 32 * i + __ffs(empty) - 1;
+            empty &= empty - 1;
+            *(uint2*)(sm + G::V + (lane >> 4) * C * 128 + row * 128 + (lane & 15) * 8) = make_uint2(0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_in);
     }
-    __syncwarp();
   } else {
     // ---------------- products ----------------
     if (elect_one()) {
       const uint32_t i64 = instr_desc<__half>(64, false), u64 = instr_desc<__half>(64, true);
+      const uint32_t t64 = instr_desc<bf16>(64, false) | 1u << 15;  // the values' rows run along the contraction
+      auto values = [&](int n) {  // T V of chunk n
+        ok = wait_for(&v_in, n & 1, failed) && ok;
+        fence_after();
+        if (!ok) return;
+        const uint32_t ts = smem_u32(sm + G::T), vs = smem_u32(sm + G::V);
+#pragma unroll
+        for (int k = 0; k < C / 16; ++k)
+#pragma unroll
+          for (int i = 2; i >= 0; --i) mma_ss(tmem + TV, smem_desc(vs + k * 2048, C * 128), smem_desc(ts + i * SQ + k * 32, 0), t64, k != 0 || i != 2);
+        commit(&tv_out);
+      };
+      if (nlive > 0) values(0);
       for (int n = 0; n < nlive; ++n) {
         const uint32_t st = smem_u32(sm + (n & 1) * G::BYTES), ph = n & 1;
         ok = wait_for(&full[n & 1], (n >> 1) & 1, failed) && ok;
-        // K S, the key rows of each half as soon as they are there
+        // W S, the key rows of each half as soon as they are there
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           ok = wait_for(&s_in[hh], ph, failed) && ok;
@@ -321,34 +331,26 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
           if (!ok) continue;
 #pragma unroll
           for (int k = hh * (DKP / 32); k < (hh + 1) * (DKP / 32); ++k) {
-            const uint64_t kd = smem_desc(st + (k >> 2) * (2 * C * 128) + (k & 3) * 32, 0);
-            mma_ts(tmem + KS, tmem + SH + k * 8, kd, i64, k != 0);
-            mma_ts(tmem + KS, tmem + SL + k * 8, kd, i64, true);
+            const uint32_t at = st + G::W + (k >> 2) * SQ + (k & 3) * 32;
+            const uint64_t wh = smem_desc(at, 0), wl = smem_desc(at + w_bytes(DKP), 0);
+            mma_ts(tmem + WS, tmem + SH + k * 8, wh, i64, k != 0);
+            mma_ts(tmem + WS, tmem + SL + k * 8, wh, i64, true);
+            mma_ts(tmem + WS, tmem + SH + k * 8, wl, i64, true);
           }
         }
-        if (ok) commit(&ks_out);
-        // T R
-        ok = wait_for(&r_in, ph, failed) && ok;
+        if (!ok) break;
+        commit(&ws_out);
+        // Q S, once the output of the chunk before has been read
+        if (n > 0) ok = wait_for(&o_read, ph ^ 1, failed) && ok;
         fence_after();
-        if (ok) {
-#pragma unroll
-          for (int k = 0; k < C / 16; ++k) {
-            const uint64_t th = smem_desc(st + G::T + k * 32, 0), tl = smem_desc(st + G::T + SQ + k * 32, 0);
-            mma_ts(tmem + VP, tmem + RH + k * 8, th, i64, k != 0);
-            mma_ts(tmem + VP, tmem + RL + k * 8, th, i64, true);
-            mma_ts(tmem + VP, tmem + RH + k * 8, tl, i64, true);
-          }
-          commit(&vp_out);
-        }
-        // Q S, in the shadow of what the threads do with T R; they have waited for the output of the chunk before
         if (ok) {
 #pragma unroll
           for (int k = 0; k < DKP / 16; ++k) mma_ts(tmem + QS, tmem + SH + k * 8, smem_desc(st + (k >> 2) * (2 * C * 128) + C * 128 + (k & 3) * 32, 0), i64, k != 0);
         }
-        // the update, 64 key dims at a time, then P V'
+        // the update, 64 key dims at a time, then P V' and the next chunk's T V
         ok = wait_for(&u_in, ph, failed) && ok;
         fence_after();
-        if (!ok) continue;
+        if (!ok) break;
         if (!TREE) {
 #pragma unroll
           for (int x = 0; x < DKP / 64; ++x) {
@@ -364,7 +366,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
         }
 #pragma unroll
         for (int k = 0; k < C / 16; ++k) mma_ts(tmem + PV, tmem + VH + k * 8, smem_desc(st + G::P + k * 32, 0), i64, k != 0);
-        commit(&o_out[n & 1]);
+        commit(&o_out[ph]);
+        if (n + 1 < nlive) values(n + 1);
       }
     }
     __syncwarp();
@@ -396,7 +399,7 @@ int launch_delta_scan(const DeltaChunkParams& p, cudaStream_t stream) {
   if (rc) return rc;
   CUtensorMap vmap, omap;
   const long dims[4] = {p.dv, p.hv, p.tokens, p.batch};
-  if (!encode_map(&vmap, p.v, false, dims, {p.v_stride[2], p.v_stride[1], p.v_stride[0]}, {COLS, 1, C, 1}, false) ||
+  if (!encode_map(&vmap, p.v, false, dims, {p.v_stride[2], p.v_stride[1], p.v_stride[0]}, {64, 1, C, 1}, true) ||
       !encode_map(&omap, p.out, false, dims, {p.dv, (long)p.hv * p.dv, (long)p.tokens * p.hv * p.dv}, {COLS, 1, C, 1}, false)) {
     set_error("delta rule scan: tensor map for the values or the output failed");
     return 1;
