@@ -562,7 +562,7 @@ struct Walk {
 Walk plan_walk(int batch, int tokens, int hk, int hv, int dk, int dv) {
   Walk w;
   const int chunks = (tokens + C - 1) / C;
-  const long fit = (long)((size_t)128 * 1024 * 1024 / (chunk_bytes(hk, hv, dk) * batch));
+  const long fit = (long)((size_t)256 * 1024 * 1024 / (chunk_bytes(hk, hv, dk) * batch));
   const long heads = (long)batch * hv, wave = 4 * 148 / heads;  // chunks whose preparation fills the SMs once
   w.beside = heads * ((dv + 127) / 128) <= 100 && chunks > wave;
   long seg = w.beside ? fit / 2 : fit;

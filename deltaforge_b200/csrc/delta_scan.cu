@@ -32,8 +32,8 @@ template <int DKP> struct Stage {
   static constexpr int T = 2 * BYTES, V = T + 3 * SQ, ROWS = V + C * COLS * 2, SC = ROWS + C * COLS * 2, SMEM = SC + 3 * SCAL + 1024;
 };
 // TMEM columns. S and V' are A operands, two fp16 values per column (V' twice: in halves with the decays into the state, and as
-// it is for the output); the others are accumulators. The update takes the place of W S, P V' that of the V' in halves.
-constexpr int SH = 0, SL = 64, WS = 128, UP = 128, QS = 256, TV = 320, RH = 384, RL = 416, PV = 384, VH = 448;
+// it is for the output); the others are accumulators. The update takes the place of W S, V' in halves that of the lower halves of S.
+constexpr int SH = 0, SL = 64, WS = 128, UP = 128, RH = 64, RL = 96, QS = 256, TV = 320, PV = 384, VH = 448;
 
 template <int DKP, bool TREE>
 __global__ void __launch_bounds__(SCAN_THREADS, 1)
@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   constexpr int NS = DKP / 4;  // key rows per thread
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  __shared__ uint64_t full[2], v_full, v_in, s_in[2], tv_out, ws_out, u_in, u_out[2], o_out[2], o_read;
+  __shared__ uint64_t full[2], v_full, v_in, s_in[2], tv_out, ws_out, u_in, p_in, u_out[2], o_out[2], o_read;
   __shared__ float s_max[4][COLS], vp_max[4][COLS];
   __shared__ int s_exp[2][COLS], v_exp[2][COLS];  // by chunk parity, for the output
   __shared__ uint32_t tmem_slot;
@@ -54,9 +54,9 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.tokens) : p.tokens;
   const int nlive = min(max((len + C - 1) / C - p.chunk0, 0), p.chunks);  // chunks of this segment with tokens
   if (t == 0) {
-    for (int i = 0; i < 2; ++i) mbar_init(&full[i], 1), mbar_init(&s_in[i], 8), mbar_init(&u_out[i], 1), mbar_init(&o_out[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&full[i], 1), mbar_init(&s_in[i], 16), mbar_init(&u_out[i], 1), mbar_init(&o_out[i], 1);
     mbar_init(&v_full, 1), mbar_init(&v_in, 1), mbar_init(&tv_out, 1), mbar_init(&ws_out, 1);
-    mbar_init(&u_in, 16), mbar_init(&o_read, 4);
+    mbar_init(&u_in, 16), mbar_init(&p_in, 16), mbar_init(&o_read, 4);
     failed_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -104,28 +104,32 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
 
     for (int n = 0; n < nlive; ++n) {
       const float* sc = (const float*)(sm + G::SC + n % 3 * SCAL);
-      // S in halves to TMEM; its largest on the side
+      // S in halves to TMEM, 16 key rows at a time; its largest on the side
       {
         const float sdown = pow2(-es);
-        ms = 0.f;
+        __half2 top = __float2half2_rn(0.f);
 #pragma unroll
         for (int x = 0; x < NS; x += 16) {
           uint32_t hi[8], lo[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const F2 s2 = S[x / 2 + i];
-            ms = fmaxf(fmaxf(ms, fabsf(s2.x)), fabsf(s2.y));
-            split(mul2(s2, {sdown, sdown}), hi[i], lo[i]);
+            split(mul2(S[x / 2 + i], {sdown, sdown}), hi[i], lo[i]);
+            top = __hmax2_nan(top, __habs2(*(const __half2*)&hi[i]));
+          }
+          if (x == 0 && n > 0 && h < 2 && DKP > 64) {  // the lower halves' place: all of the update before has read it
+            ok = wait_for(&u_out[1], (n & 1) ^ 1, failed) && ok;
+            fence_after();
           }
           tmem_st8(base + SH + h * (NS / 2) + x / 2, hi);
           tmem_st8(base + SL + h * (NS / 2) + x / 2, lo);
+          tmem_wait_st();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_in[x / 16]);
         }
+        ms = fmaxf(__low2float(top), __high2float(top));
       }
-      tmem_wait_st();
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_in[h >> 1]);
-      s_max[h][col] = ms;
+      s_max[h][col] = ms * pow2(es);
       if (h == 0) s_exp[n & 1][col] = es;
 
       // V' = T V - W S
@@ -166,10 +170,6 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
           const F2 y = mul2({__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])}, {a, a});
           hi[i] = h2(y.x, y.y);
         }
-        if (n > 0) {  // Q S and P V' of the chunk before have been read
-          ok = wait_for(&o_read, (n & 1) ^ 1, failed) && ok;
-          fence_after();
-        }
         tmem_st8(base + VH + 8 * h, hi);
         if (!TREE) {
 #pragma unroll
@@ -184,7 +184,10 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       tmem_wait_st();
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&u_in);
+      if (lane == 0) {
+        if (!TREE) mbar_arrive(&u_in);
+        mbar_arrive(&p_in);
+      }
       if (TREE) break;
 
       // S: the update was accumulated apart and is added in fp32
@@ -236,10 +239,14 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
           const float4 w = *(const float4*)&sc[C + x + i];
-          rows_s[(x + i) * COLS + col] = f2bf(fmaf(__uint_as_float(a[i]), w.x * sup, __uint_as_float(z[i]) * pscale));
-          rows_s[(x + i + 1) * COLS + col] = f2bf(fmaf(__uint_as_float(a[i + 1]), w.y * sup, __uint_as_float(z[i + 1]) * pscale));
-          rows_s[(x + i + 2) * COLS + col] = f2bf(fmaf(__uint_as_float(a[i + 2]), w.z * sup, __uint_as_float(z[i + 2]) * pscale));
-          rows_s[(x + i + 3) * COLS + col] = f2bf(fmaf(__uint_as_float(a[i + 3]), w.w * sup, __uint_as_float(z[i + 3]) * pscale));
+#pragma unroll
+          for (int y = 0; y < 4; y += 2) {
+            const F2 o = fma2({__uint_as_float(a[i + y]), __uint_as_float(a[i + y + 1])}, mul2(y ? F2{w.z, w.w} : F2{w.x, w.y}, {sup, sup}),
+                              mul2({__uint_as_float(z[i + y]), __uint_as_float(z[i + y + 1])}, {pscale, pscale}));
+            const __nv_bfloat162 r = __floats2bfloat162_rn(o.x, o.y);
+            rows_s[(x + i + y) * COLS + col] = r.x;
+            rows_s[(x + i + y + 1) * COLS + col] = r.y;
+          }
         }
       }
       fence_before();
@@ -323,14 +330,14 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       for (int n = 0; n < nlive; ++n) {
         const uint32_t st = smem_u32(sm + (n & 1) * G::BYTES), ph = n & 1;
         ok = wait_for(&full[n & 1], (n >> 1) & 1, failed) && ok;
-        // W S, the key rows of each half as soon as they are there
+        // W S, the key rows as they come: the first 16 of each quarter, then the others
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          ok = wait_for(&s_in[hh], ph, failed) && ok;
+        for (int x = 0; x < NS / 16; ++x) {
+          ok = wait_for(&s_in[x], ph, failed) && ok;
           fence_after();
           if (!ok) continue;
 #pragma unroll
-          for (int k = hh * (DKP / 32); k < (hh + 1) * (DKP / 32); ++k) {
+          for (int k = x; k < DKP / 16; k += NS / 16) {
             const uint32_t at = st + G::W + (k >> 2) * SQ + (k & 3) * 32;
             const uint64_t wh = smem_desc(at, 0), wl = smem_desc(at + w_bytes(DKP), 0);
             mma_ts(tmem + WS, tmem + SH + k * 8, wh, i64, k != 0);
@@ -348,10 +355,10 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
           for (int k = 0; k < DKP / 16; ++k) mma_ts(tmem + QS, tmem + SH + k * 8, smem_desc(st + (k >> 2) * (2 * C * 128) + C * 128 + (k & 3) * 32, 0), i64, k != 0);
         }
         // the update, 64 key dims at a time, then P V' and the next chunk's T V
-        ok = wait_for(&u_in, ph, failed) && ok;
-        fence_after();
-        if (!ok) break;
         if (!TREE) {
+          ok = wait_for(&u_in, ph, failed) && ok;
+          fence_after();
+          if (!ok) break;
 #pragma unroll
           for (int x = 0; x < DKP / 64; ++x) {
 #pragma unroll
@@ -364,6 +371,9 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
           }
           if (DKP == 64) commit(&u_out[1]);
         }
+        ok = wait_for(&p_in, ph, failed) && ok;
+        fence_after();
+        if (!ok) break;
 #pragma unroll
         for (int k = 0; k < C / 16; ++k) mma_ts(tmem + PV, tmem + VH + k * 8, smem_desc(st + G::P + k * 32, 0), i64, k != 0);
         commit(&o_out[ph]);
