@@ -111,6 +111,7 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
   // Launched beside the scan of the segment before: whatever follows this grid must find that scan done too, so one CTA stays
   // until it is.
   const bool stays = p.beside && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1;
+  pdl_launch_dependents();  // the scan may set itself up
   if (live <= 0) {
     if (stays) pdl_wait();
     return;

@@ -64,7 +64,6 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  pdl_launch_dependents();  // the preparation of the next segment may run beside this one
   fence_before();
   __syncthreads();
   fence_after();
@@ -88,6 +87,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       lo = h2(r.x, r.y);
     };
     F2 S[NS / 2];
+    // (The first segment's state is there before the preparation starts; nothing else here comes but through the loads.)
     const float* Sin = p.first ? p.state + sb : p.state_out + sb;
     float ms = 0.f;
 #pragma unroll
@@ -265,6 +265,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       if (cok) out[(long)i * orow + col] = f2bf(0.f);
   } else if (warp == 20) {
     // ---------------- loads ----------------
+    pdl_wait();
+    pdl_launch_dependents();  // the preparation of the next segment may run beside this scan, but not beside the one before
     const long per = p.hk * (long)key_bytes(DKP) + p.hv * (long)head_bytes(DKP);
     const unsigned char* src = p.scratch + (long)b * p.seg_chunks * per;
     for (int n = 0; n < nlive; ++n) {
@@ -401,6 +403,15 @@ int configure_all() {
   return rc;
 }
 
+template <int DKP, bool TREE>
+int launch_one(const CUtensorMap& vmap, const CUtensorMap& omap, const DeltaChunkParams& p, dim3 grid, cudaStream_t stream) {
+  // Set up beside the preparation (16 x 64 tree nodes: 57.0 -> 54.7 us); a later segment's has another scan to wait for, and
+  // its CTAs would only take room from the preparation (8192 tokens: 389 us, with it 407).
+  if (p.first) (void)launch_pdl(delta_scan_kernel<DKP, TREE>, grid, dim3(SCAN_THREADS), Stage<DKP>::SMEM, stream, vmap, omap, p);
+  else delta_scan_kernel<DKP, TREE><<<grid, SCAN_THREADS, Stage<DKP>::SMEM, stream>>>(vmap, omap, p);
+  return check_launch("delta rule scan");
+}
+
 }  // namespace
 
 int launch_delta_scan(const DeltaChunkParams& p, cudaStream_t stream) {
@@ -416,11 +427,8 @@ int launch_delta_scan(const DeltaChunkParams& p, cudaStream_t stream) {
   }
   const dim3 grid((p.dv + COLS - 1) / COLS, p.hv, p.batch);
   const bool tree = p.parents != nullptr, wide = p.dk > 64;
-  if (tree && wide) delta_scan_kernel<128, true><<<grid, SCAN_THREADS, Stage<128>::SMEM, stream>>>(vmap, omap, p);
-  else if (tree) delta_scan_kernel<64, true><<<grid, SCAN_THREADS, Stage<64>::SMEM, stream>>>(vmap, omap, p);
-  else if (wide) delta_scan_kernel<128, false><<<grid, SCAN_THREADS, Stage<128>::SMEM, stream>>>(vmap, omap, p);
-  else delta_scan_kernel<64, false><<<grid, SCAN_THREADS, Stage<64>::SMEM, stream>>>(vmap, omap, p);
-  return check_launch("delta rule scan");
+  if (tree) return wide ? launch_one<128, true>(vmap, omap, p, grid, stream) : launch_one<64, true>(vmap, omap, p, grid, stream);
+  return wide ? launch_one<128, false>(vmap, omap, p, grid, stream) : launch_one<64, false>(vmap, omap, p, grid, stream);
 }
 
 }  // namespace dfb
