@@ -461,14 +461,17 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
 
 // ---- a few tokens, one by one ---------------------------------------------------------------------------------------
 
-// One or a few tokens per sequence: the recurrence itself in fp32, bound by reading and writing the state once. A CTA owns 32
-// value columns of a head: lane = column, each of the eight warps holds 16 key rows of them in registers from the first
-// token to the last; the two sums over the key rows go through shared memory.
-constexpr int FEW = 4;  // most tokens (what the chunked form needs for one chunk is reached at about that many)
+// One or a few tokens per sequence: the recurrence itself in fp32. For one token it is bound by reading and writing the state
+// once (16 sequences x 32 heads of 128 x 128: 67 MB in 17 us; 19 without the streaming hints, 21 with four CTAs per SM instead of five), then by its two reductions per token. A CTA owns 32 value columns
+// of a head: lane = column, each of the eight warps holds 16 key rows of them in registers from the first token to the last;
+// the two sums over the key rows go through shared memory.
+constexpr int FEW = 24;  // most tokens
 constexpr int FEW_THREADS = 256, FEW_ROWS = 16;
 
-__global__ void __launch_bounds__(FEW_THREADS) delta_few_kernel(const DeltaChunkParams p) {
-  __shared__ float qn[FEW][128], kn[FEW][128], gate[FEW][2];
+__global__ void __launch_bounds__(FEW_THREADS, 5) delta_few_kernel(const DeltaChunkParams p) {
+  __shared__ __align__(16) float qn[FEW][128], kn[FEW][128];
+  __shared__ float gate[FEW][2];
+  __shared__ bf16 vs[FEW][32];
   __shared__ float red[2][8][32];
   const int vb = blockIdx.x, hv = blockIdx.y, b = blockIdx.z, hk = hv / (p.hv / p.hk);
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, col = vb * 32 + lane;
@@ -478,12 +481,12 @@ __global__ void __launch_bounds__(FEW_THREADS) delta_few_kernel(const DeltaChunk
 #pragma unroll
   for (int i = 0; i < FEW_ROWS; ++i) {
     const int k = warp * FEW_ROWS + i;
-    s[i] = cok && k < p.dk ? p.state[sb + (long)k * p.dv + col] : 0.f;
+    s[i] = cok && k < p.dk ? __ldcs(&p.state[sb + (long)k * p.dv + col]) : 0.f;
   }
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.tokens) : p.tokens;
-  // queries by warps 0 .. 3, keys by warps 4 .. 7, a token each
-  const int tok = warp & 3, is_k = warp >> 2;
-  if (tok < len) {
+  // queries by warps 0 .. 3, keys by warps 4 .. 7, every fourth token each
+  const bool is_k = warp >= 4;
+  for (int tok = warp & 3; tok < len; tok += 4) {
     const bf16* src = is_k ? p.k + b * p.k_stride[0] + tok * p.k_stride[1] + hk * p.k_stride[2] : p.q + b * p.q_stride[0] + tok * p.q_stride[1] + hk * p.q_stride[2];
     float x[4], ss = 0.f;
     uint2 raw = make_uint2(0u, 0u);
@@ -496,16 +499,13 @@ __global__ void __launch_bounds__(FEW_THREADS) delta_few_kernel(const DeltaChunk
       r = rsqrt_2step(__fadd_rn(warp_sum(ss), 1e-6f));
       if (!is_k) r = __fdiv_rn(r, sqrtf((float)p.dk));
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) (is_k ? kn : qn)[tok][4 * lane + i] = x[i] * r;
+    *(float4*)&(is_k ? kn : qn)[tok][4 * lane] = make_float4(x[0] * r, x[1] * r, x[2] * r, x[3] * r);
     if (is_k && lane == 0) {
       gate[tok][0] = expf(p.g[((long)b * p.tokens + tok) * p.hv + hv]);
       gate[tok][1] = p.beta[((long)b * p.tokens + tok) * p.hv + hv];
     }
+    if (!is_k) vs[tok][lane] = cok ? p.v[b * p.v_stride[0] + tok * p.v_stride[1] + hv * p.v_stride[2] + col] : f2bf(0.f);
   }
-  float v[FEW];
-#pragma unroll
-  for (int n = 0; n < FEW; ++n) v[n] = cok && n < len ? bf2f(p.v[b * p.v_stride[0] + n * p.v_stride[1] + hv * p.v_stride[2] + col]) : 0.f;
   __syncthreads();
 #pragma unroll 1
   for (int n = 0; n < len; ++n) {
@@ -521,10 +521,7 @@ __global__ void __launch_bounds__(FEW_THREADS) delta_few_kernel(const DeltaChunk
     r = 0.f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) r += red[0][w][lane];
-    float vn = v[0];
-#pragma unroll
-    for (int i = 1; i < FEW; ++i) vn = n == i ? v[i] : vn;
-    const float d = (vn - r) * gate[n][1];
+    const float d = (bf2f(vs[n][lane]) - r) * gate[n][1];
     float o = 0.f;
 #pragma unroll
     for (int i = 0; i < FEW_ROWS; ++i) {
@@ -543,10 +540,17 @@ __global__ void __launch_bounds__(FEW_THREADS) delta_few_kernel(const DeltaChunk
 #pragma unroll
   for (int i = 0; i < FEW_ROWS; ++i) {
     const int k = warp * FEW_ROWS + i;
-    if (cok && k < p.dk) p.state_out[sb + (long)k * p.dv + col] = s[i];
+    if (cok && k < p.dk) __stcs(&p.state_out[sb + (long)k * p.dv + col], s[i]);
   }
   for (int n = len + warp; n < p.tokens; n += 8)
     if (cok) p.out[(((long)b * p.tokens + n) * p.hv + hv) * p.dv + col] = f2bf(0.f);
+}
+
+// Where this form is taken. us, token by token / chunked, 32 heads of 128 x 128: one sequence 4 tokens 4.5 / 19, 12 tokens 9 / 18,
+// 24 tokens 13 / 18; two sequences 24 tokens 17 / 18; four 12 tokens 18 / 20, 16 tokens 23 / 20; 16 sequences 4 tokens 27 / 61, 12
+// tokens 51 / 61, 16 tokens 68 / 61.
+bool few_tokens(int batch, int tokens, int hv, int dv) {
+  return tokens <= ((long)batch * hv * ((dv + 31) / 32) <= 2 * 148 ? FEW : 12);
 }
 
 int pad_dk(int dk) { return dk <= 64 ? 64 : 128; }
@@ -603,7 +607,7 @@ int launch_prep(const DeltaChunkParams& p, cudaStream_t stream) {
 }  // namespace
 
 size_t delta_chunk_scratch_bytes(int batch, int tokens, int hk, int hv, int dk, int dv, bool tree) {
-  if (!tree && tokens <= FEW) return 0;
+  if (!tree && few_tokens(batch, tokens, hv, dv)) return 0;
   const Walk w = plan_walk(batch, tokens, hk, hv, dk, dv);
   return chunk_bytes(hk, hv, dk) * batch * (w.first > w.chunks ? w.first : w.chunks) * (w.beside ? 2 : 1);
 }
@@ -614,7 +618,7 @@ int launch_delta_chunk(const DeltaChunkParams& args, cudaStream_t stream) {
   if (rc) return rc;
   DeltaChunkParams p = args;
   const bool tree = p.parents != nullptr, wide = p.dk > 64;
-  if (!tree && p.tokens <= FEW) {
+  if (!tree && few_tokens(p.batch, p.tokens, p.hv, p.dv)) {
     delta_few_kernel<<<dim3((p.dv + 31) / 32, p.hv, p.batch), FEW_THREADS, 0, stream>>>(p);
     return check_launch("delta rule, few tokens");
   }

@@ -534,8 +534,15 @@ int launch_t(const TreeAttnParams& p, cudaStream_t stream) {
 TreePlan tree_plan(int batch, int nodes, int hq, int hkv, int d, int max_seq, bool tc_ok) {
   TreePlan pl = {};
   const int rows = nodes * (hq / hkv);
-  if (tc_ok && d >= 64 && rows > 16) {
-    const long row_tiles = (rows + 127) / 128, units = (long)batch * hkv, tiles = units * ((max_seq + 127) / 128);
+  // Which form (us, mma.sync / tcgen05; sequences x cache rows, 4 KV heads of 256 dims or 8 of 128): the products on tcgen05 are
+  // faster and read the cache once for up to 128 rows, but its pipeline takes 4 us more to fill and to merge.
+  // Many heads fill the SMs either way: 8 x 4096, 16 rows 37 / 31, 32 rows 41 / 32 (256 dims), 47 / 31 (128 dims); 8 x 512, 32 rows
+  // 15 / 14 and 13 / 14; only at 16 rows and long caches (8 x 32768: 165 / 169) does the other stay ahead.
+  // Few heads: one pass over 32 rows is enough for mma.sync, 1 x 32768: 34 / 42 and 31 / 38; 48 rows 52 / 43 and 43 / 38; unless
+  // there is little to do at all: 1 x 4096, 48 rows 18 / 17 and 14 / 20, 128 rows 24 / 22 and 19 / 23.
+  const long units = (long)batch * hkv;
+  if (tc_ok && d >= 64 && (units >= 32 ? rows > 16 : rows > 32 && (double)units * max_seq * rows * d > 5e8)) {
+    const long row_tiles = (rows + 127) / 128, tiles = units * ((max_seq + 127) / 128);
     const long most = row_tiles < 148 ? 148 / row_tiles : 1, groups = (tiles + TREE_TC_MIN_TILES - 1) / TREE_TC_MIN_TILES;
     pl.tc_groups = (int)(groups < most ? groups : most);
     pl.slots = (size_t)(pl.tc_groups + units) * row_tiles * 128;

@@ -173,7 +173,7 @@ def test_c_entries_refuse_before_any_launch():
     d.batch = d.tokens = d.hk = d.hv = 1
     d.dk, d.dv = 12, 16
     assert lib.dfb_delta_chunk(d, None) == 2 and b"unsupported" in lib.dfb_last_error()
-    d.dk, d.tokens = 16, 5
+    d.dk, d.tokens = 16, 64
     d.state = d.state_out = d.q = d.k = d.v = d.g = d.beta = d.out = 16
     assert lib.dfb_delta_chunk(d, None) == 2 and b"scratch" in lib.dfb_last_error()
     d.parents, d.lengths = 16, 16

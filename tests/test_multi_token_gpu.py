@@ -186,6 +186,12 @@ TREES = {
         (2, 64, 2, 1, 32, 4096, [4032, 17], "star"),
         (1, 5, 24, 2, 64, 8, [3], "random"),
         (2, 3, 3, 3, 32, 2, [0, 0], "chain"),  # more nodes than rows: keys past the cache are lost
+        # heads enough for the form that reads the cache once for 128 rows
+        (8, 12, 16, 4, 256, 300, [288, 0, 1, 127, 128, 129, 250, 90], "random"),
+        (9, 64, 12, 4, 128, 200, [136, 0, 63, 64, 65, 100, 1, 128, 31], "random"),
+        (16, 9, 8, 4, 64, 700, [691, 0, 5, 130, 600, 64, 63, 384] * 2, "chain"),
+        (11, 17, 3, 3, 256, 20, [3] * 11, "star"),
+        (1, 16, 16, 4, 128, 20000, [19984], "random"),
     ],
 )
 def test_tree_attention(b, n, hq, hkv, d, rows, lens, tree, dtype):
@@ -200,7 +206,7 @@ def test_tree_attention(b, n, hq, hkv, d, rows, lens, tree, dtype):
     within(got, want, tree_bound(want, size, q, kc, scale, rows))
 
 
-@pytest.mark.parametrize("hq,hkv,d", [(16, 4, 256), (4, 2, 64)])
+@pytest.mark.parametrize("hq,hkv,d", [(16, 4, 256), (4, 2, 64), (44, 11, 256), (32, 16, 64)])
 def test_tree_attention_rows_without_a_node_and_values_no_one_sees(hq, hkv, d):
     b, n, rows = 3, 12, 80
     q, kc, vc = rnd(21, b, n, hq, d, dtype=BF16), rnd(22, b, hkv, rows, d, dtype=BF16), rnd(23, b, hkv, rows, d, dtype=BF16)
@@ -230,8 +236,9 @@ def test_tree_attention_rows_without_a_node_and_values_no_one_sees(hq, hkv, d):
     assert torch.equal(ops.tree_attention(q, k2, v2, lt, pt, 0.1), got)
 
 
-def test_tree_attention_layouts_streams_and_graphs():
-    b, n, hq, hkv, d, rows = 2, 9, 8, 2, 128, 700
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (64, 16)])
+def test_tree_attention_layouts_streams_and_graphs(hq, hkv):
+    b, n, d, rows = 2, 9, 128, 700
     lens, parents = [600, 320], random_tree(5, n)
     q, kc, vc = rnd(31, b, n, hq, d, dtype=BF16), rnd(32, b, hkv, rows, d, dtype=BF16), rnd(33, b, hkv, rows, d, dtype=BF16)
     lt, pt = torch.tensor(lens, dtype=I32, device=DEV), torch.tensor(parents, dtype=I32, device=DEV)
@@ -320,7 +327,7 @@ def delta_state_bound(want, tokens):
 @pytest.mark.parametrize("l2norm", [False, True])
 @pytest.mark.parametrize(
     "b,t,hk,hv,dk,dv",
-    [(1, 1, 2, 4, 128, 128), (2, 3, 1, 1, 16, 16), (1, 64, 2, 4, 128, 128), (2, 65, 2, 2, 64, 128), (1, 200, 3, 9, 96, 80), (3, 129, 2, 4, 8, 8), (1, 17, 1, 2, 128, 264), (20, 70, 2, 8, 128, 64), (1, 1337, 16, 32, 64, 32)],
+    [(1, 1, 2, 4, 128, 128), (2, 3, 1, 1, 16, 16), (1, 64, 2, 4, 128, 128), (2, 65, 2, 2, 64, 128), (1, 200, 3, 9, 96, 80), (3, 129, 2, 4, 8, 8), (1, 17, 1, 2, 128, 264), (2, 24, 2, 6, 72, 104), (5, 12, 2, 32, 128, 128), (1, 25, 16, 32, 128, 128), (20, 70, 2, 8, 128, 64), (1, 1337, 16, 32, 64, 32)],
 )
 def test_delta_rule_chunk(b, t, hk, hv, dk, dv, l2norm):
     a = delta_inputs(41, b, t, hk, hv, dk, dv, l2norm)
