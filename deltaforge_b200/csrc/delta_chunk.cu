@@ -20,6 +20,7 @@
 //
 // delta_scan.cu has the scan.
 #include "delta.cuh"
+#include "tcgen05.cuh"
 
 namespace dfb {
 
@@ -27,7 +28,6 @@ namespace {
 
 constexpr float MIN_LOG_DECAY = -150.f;  // e^-150 is 0 in fp32: keeps sums finite when a log decay is -inf
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -56,15 +56,18 @@ __device__ __forceinline__ void split3(float a, float b, uint32_t& p0, uint32_t&
   p0 = *(const uint32_t*)&x, p1 = *(const uint32_t*)&y, p2 = *(const uint32_t*)&z;
 }
 
+// What the lanes of a warp wrote to shared memory goes to memory by itself; lane 0 has it to wait for
+__device__ __forceinline__ void send(unsigned char* dst, const unsigned char* src, uint32_t bytes) {
+  fence_async();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) {
+    bulk_store(dst, smem_u32(src), bytes);
+    bulk_stores_commit();
+  }
+}
+
 constexpr int PREP_THREADS = 128;
 constexpr int TS = 68;  // row stride (floats) of the 64 x 64 fp32 matrices: 16-byte rows, neighbouring rows in other banks
-
-// 2^x: one instruction, 2 ulp
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // z[r] = sum over m < M of a[4 r][m] y[m]: every fourth row of a (stride TS) against one column of y (stride TS). The four groups
 // of lanes take neighbouring rows, which lie in different banks.
@@ -88,7 +91,7 @@ __device__ __forceinline__ void block_product(float (&z)[R], const float* a, con
 //   2. K K^T and Q K^T rows by mma; decays; A to shared memory, P to its image
 //   3. the 16 x 16 diagonal blocks of (I + A)^-1 by substitution, a column per lane
 //   4. two doublings, 16 -> 32 -> 64
-//   5. T diag(beta) in halves to its images
+//   5. W by mma, T diag(beta) in parts and W in halves to their images
 // Bound by latency: three to four CTAs share an SM. Scales are per warp (16 rows), so no CTA-wide maximum is needed.
 template <int DKP, bool TREE>
 __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const DeltaChunkParams p) {
@@ -98,7 +101,8 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
   float* T = (float*)qt;                                     // [64][TS], over the queries once they have been read
   float* A = T + C * TS;                                     // [64][TS]
   __shared__ float4 col[C];                                  // per token: log2 decay sum (hi, lo), 1/|k|, beta
-  __shared__ float rq[C], sk[C], sq[C], on_w[C];
+  __shared__ float rq[C], sk[C], sq[C];
+  __shared__ __align__(16) float on_w[C], beta_s[C];
   __shared__ unsigned long long anc[C];
   __shared__ int up[C];
   __shared__ double gsum[C];
@@ -174,7 +178,7 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
         gv = gv < MIN_LOG_DECAY ? MIN_LOG_DECAY : gv;
       }
       gsum[t] = (double)gv * 1.4426950408889634074;  // log2(e)
-      col[t].w = bv;
+      col[t].w = beta_s[t] = bv;
     }
     __syncthreads();
     if (!TREE) {
@@ -300,11 +304,13 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
     }
     const int ep = scale_exp(warp_max_abs(pm));
     const float down = pow2(-ep);
+    unsigned char* stage = (unsigned char*)(T + r0 * TS);  // where this warp's rows of T will be; the queries have been read
 #pragma unroll
     for (int nt = 0; nt < 8; ++nt) {
-      *(uint32_t*)(pimg + img_off<C>(r0 + g, nt) + 4 * c) = h2(qk[nt][0] * down, qk[nt][1] * down);
-      *(uint32_t*)(pimg + img_off<C>(r0 + g + 8, nt) + 4 * c) = h2(qk[nt][2] * down, qk[nt][3] * down);
+      *(uint32_t*)(stage + img_off<C>(g, nt) + 4 * c) = h2(qk[nt][0] * down, qk[nt][1] * down);
+      *(uint32_t*)(stage + img_off<C>(g + 8, nt) + 4 * c) = h2(qk[nt][2] * down, qk[nt][3] * down);
     }
+    send(pimg + r0 * 128, stage, 2048);
     if (lane == 0) sc[2 * C + 8 + warp] = pow2(ep);
   }
   __syncwarp();
@@ -330,6 +336,7 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
     const float4 v = col[t];
     on_w[t] = exp2_fast(v.x + v.y) * v.z * v.w;
   }
+  if (lane == 0) bulk_stores_read();  // T may take the place of P's rows
   __syncthreads();  // A is complete, the queries have been read
   if (lane < 16) {
 #pragma unroll
@@ -408,10 +415,29 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
     const int ew = scale_exp(warp_max_abs(wm));
     const float down = pow2(-ew);
     if (lane == 0) sc[2 * C + 4 + warp] = pow2(ew);
-    // through this warp's rows of A, 64 key dims of one half at a time: 16 rows are 2 KB in a row of the image
-    unsigned char* stage = (unsigned char*)(A + r0 * TS);
+    // T diag(beta), this warp's 16 rows, eight columns per lane and pass
+    const int j0 = (lane & 7) * 8;
+    float bj[8];
+    *(float4*)&bj[0] = *(const float4*)&beta_s[j0];
+    *(float4*)&bj[4] = *(const float4*)&beta_s[j0 + 4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float* src = &T[(r0 + 4 * k + (lane >> 3)) * TS + j0];
+      float tv[8];
+      *(float4*)&tv[0] = *(const float4*)src;
+      *(float4*)&tv[4] = *(const float4*)(src + 4);
+      uint32_t part[3][4];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) split3(tv[2 * y] * bj[2 * y], tv[2 * y + 1] * bj[2 * y + 1], part[0][y], part[1][y], part[2][y]);
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        *(uint4*)(himg + i * SQ + img_off<C>(r0 + 4 * k + (lane >> 3), lane & 7)) = make_uint4(part[i][0], part[i][1], part[i][2], part[i][3]);
+    }
+    __syncwarp();
+    // W leaves through this warp's rows of A and then of T, 64 key dims each: 16 rows are 2 KB in a row of either half's image
 #pragma unroll
     for (int x = 0; x < DKP / 64; ++x) {
+      unsigned char* stage = (unsigned char*)((x ? T : A) + r0 * TS);
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
@@ -421,50 +447,31 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const Delta
           *(uint32_t*)(stage + img_off<64>(g + 8 * r, nt) + 4 * c) = hi;
           *(uint32_t*)(stage + 2048 + img_off<64>(g + 8 * r, nt) + 4 * c) = lo;
         }
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        *(uint4*)(wimg + (i >> 2) * w_bytes(DKP) + x * SQ + r0 * 128 + (i & 3) * 512 + lane * 16) = *(const uint4*)(stage + i * 512 + lane * 16);
-      __syncwarp();
+      send(wimg + x * SQ + r0 * 128, stage, 2048);
+      send(wimg + w_bytes(DKP) + x * SQ + r0 * 128, stage + 2048, 2048);
     }
   }
-
-  // ---- 6: T diag(beta), this warp's 16 rows, eight columns per lane and pass ----
-  {
-    const int j0 = (lane & 7) * 8;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float* src = &T[(r0 + 4 * k + (lane >> 3)) * TS + j0];
-      float tv[8];
-      *(float4*)&tv[0] = *(const float4*)src;
-      *(float4*)&tv[4] = *(const float4*)(src + 4);
-      uint32_t part[3][4];
-#pragma unroll
-      for (int y = 0; y < 4; ++y) split3(tv[2 * y] * col[j0 + 2 * y].w, tv[2 * y + 1] * col[j0 + 2 * y + 1].w, part[0][y], part[1][y], part[2][y]);
-#pragma unroll
-      for (int i = 0; i < 3; ++i)
-        *(uint4*)(himg + i * SQ + img_off<C>(r0 + 4 * k + (lane >> 3), lane & 7)) = make_uint4(part[i][0], part[i][1], part[i][2], part[i][3]);
-    }
-    if (t < C) {
-      const float4 v = col[t], e = col[C - 1];
-      const float eg = exp2_fast(v.x + v.y), on_v = exp2_fast((e.x - v.x) + (e.y - v.y)) * sk[t];
-      sc[t] = on_v;
-      sc[C + t] = eg * sq[t];
-      if (t == C - 1) sc[2 * C] = eg;
-      const float m = warp_max_abs(on_v);
-      const unsigned counts = __ballot_sync(0xffffffffu, t < live && (!TREE || anc[t] != 0));
-      if (lane == 0) sc[2 * C + 12 + warp] = m, sc[2 * C + 14 + warp] = __uint_as_float(counts);
-    }
+  if (t < C) {
+    const float4 v = col[t], e = col[C - 1];
+    const float eg = exp2_fast(v.x + v.y), on_v = exp2_fast((e.x - v.x) + (e.y - v.y)) * sk[t];
+    sc[t] = on_v;
+    sc[C + t] = eg * sq[t];
+    if (t == C - 1) sc[2 * C] = eg;
+    const float m = warp_max_abs(on_v);
+    const unsigned counts = __ballot_sync(0xffffffffu, t < live && (!TREE || anc[t] != 0));
+    if (lane == 0) sc[2 * C + 12 + warp] = m, sc[2 * C + 14 + warp] = __uint_as_float(counts);
   }
+  if (lane == 0) bulk_stores_done();
   if (stays) pdl_wait();
 }
 
 // ---- a few tokens, one by one ---------------------------------------------------------------------------------------
 
 // One or a few tokens per sequence: the recurrence itself in fp32. For one token it is bound by reading and writing the state
-// once (16 sequences x 32 heads of 128 x 128: 67 MB in 17 us; 19 without the streaming hints, 21 with four CTAs per SM instead of five), then by its two reductions per token. A CTA owns 32 value columns
-// of a head: lane = column, each of the eight warps holds 16 key rows of them in registers from the first token to the last;
-// the two sums over the key rows go through shared memory.
+// once (16 sequences x 32 heads of 128 x 128: 67 MB in 17 us; 19 without the streaming hints, 21 with four CTAs per SM instead
+// of five), then by its two reductions per token. A CTA owns 32 value columns of a head: lane = column, each of the eight
+// warps holds 16 key rows of them in registers from the first token to the last; the two sums over the key rows go through
+// shared memory.
 constexpr int FEW = 24;  // most tokens
 constexpr int FEW_THREADS = 256, FEW_ROWS = 16;
 

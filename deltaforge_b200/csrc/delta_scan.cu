@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
         }
       }
       fence_before();
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      fence_async();
       asm volatile("bar.sync 5, 128;" ::: "memory");
       if (lane == 0) mbar_arrive(&o_read);  // TMEM and the scalars have been read
       if (warp == 16 && lane == 0) {  // (rows and columns past the ends are left out)
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
             empty &= empty - 1;
             *(uint2*)(sm + G::V + (lane >> 4) * C * 128 + row * 128 + (lane & 15) * 8) = make_uint2(0, 0);
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          fence_async();
         }
       }
       __syncwarp();

@@ -140,7 +140,12 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
                "r"(smem_u32(bar))
                : "memory");
 }
-// stores: the source may be written again after bulk_stores_read()
+// the same the other way; the source may be written again after bulk_stores_read()
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+// before it, by the threads that wrote the source
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void bulk_stores_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void bulk_stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
