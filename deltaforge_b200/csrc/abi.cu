@@ -478,7 +478,7 @@ int dfb_delta_chunk(const dfb_delta_chunk_desc* d, void* stream) {
   const bool tree = d->parents != nullptr;
   if (tree && d->tokens > MAX_TREE_NODES) return bad("dfb_delta_chunk: a tree has at most %d nodes, got %d", MAX_TREE_NODES, d->tokens);
   if (tree && d->lengths) return bad("dfb_delta_chunk: a tree takes no lengths (rows without a node say so in parents)");
-  if (d->batch < 0 || d->tokens < 0 || d->batch > 65535 || d->hv > 65535) return bad("dfb_delta_chunk: bad shape batch=%d tokens=%d", d->batch, d->tokens);
+  if (d->batch < 0 || d->tokens < 0 || d->batch > 65535 || d->hv > 65535 || d->tokens > 0x7fffff00) return bad("dfb_delta_chunk: bad shape batch=%d tokens=%d", d->batch, d->tokens);
   if (d->batch == 0 || (tree && d->tokens == 0)) return DFB_OK;
   if (!d->state || (!tree && !d->state_out)) return bad("dfb_delta_chunk: null state pointer");
   if (d->tokens == 0) return bad("dfb_delta_chunk: no tokens");

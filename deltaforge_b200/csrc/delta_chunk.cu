@@ -4,18 +4,19 @@
 //   S <- e^g_t S;  r = S^T k_t;  d = beta_t (v_t - r);  S <- S + k_t d^T;  o_t = S^T q_t
 // Over a chunk of C = 64 tokens, with G_i = g_1 + .. + g_i, the same thing is
 //   A_ij = beta_i e^(G_i - G_j) k_i.k_j (j < i),  T = (I + A)^-1 diag(beta),  P_ij = e^(G_i - G_j) q_i.k_j (j <= i)
-//   R = V - diag(e^G) K S;  V' = T R;  O = diag(e^G) Q S + P V';  S <- e^G_C S + sum_j e^(G_C - G_j) k_j v'_j^T
-// T, P and the scalars do not depend on S: delta_prep_kernel makes them for all chunks at once. delta_scan_kernel then walks
+//   W = T diag(e^G) K;  V' = T V - W S;  O = diag(e^G) Q S + P V';  S <- e^G_C S + sum_j e^(G_C - G_j) k_j v'_j^T
+// T, W, P and the scalars do not depend on S: delta_prep_kernel makes them for all chunks at once. delta_scan_kernel then walks
 // through the chunks of a head; its work is matrix products with S.
 // For a tree, "j <= i" reads "j is i or an ancestor of i" and G_i is summed along the path of i; there is one chunk and no
 // new state (the accepted path is run through the prompt form afterwards).
 //
 // Precision. S is fp32 from end to end and so is the new state's bar: an operand rounded to 8 bits (bf16) would cost
-// 2e-3 per product. All matrix operands are therefore fp16 (11 bits), scaled by powers of two to the top of fp16's range
-// (per token for k and q, which are bf16 and stay exact; per 16 rows for T, P; per value column for S, R, V'), and S, T, R and
-// V' are split in two, hi + lo = 22 bits, wherever the product leads into the state: hi hi + hi lo + lo hi, fp32
-// accumulation. Products that lead into the bf16 output alone take hi (2^-12). The state's update is accumulated apart and
-// added in fp32 (the tensor core truncates what it adds to a large accumulator). Log decays are summed in fp64 and kept as
+// 2e-3 per product. Products with S or V' take fp16 operands (11 bits), scaled by powers of two to the top of fp16's range
+// (per token for k and q, which are bf16 and stay exact; per 16 rows for W, P; per value column for S, V'), and S, W and V'
+// are split in two, hi + lo = 22 bits, wherever the product leads into the state: hi hi + hi lo + lo hi, fp32 accumulation.
+// Products that lead into the bf16 output alone take hi (2^-12). T V is a product of bf16: the values as they are, T in three
+// parts (24 bits); so is W, the left factor in three parts and the keys as they are. The state's update is accumulated apart
+// and added in fp32 (the tensor core truncates what it adds to a large accumulator). Log decays are summed in fp64 and kept as
 // two floats, so that differences of large sums stay exact.
 //
 // delta_scan.cu has the scan.
@@ -92,7 +93,9 @@ __device__ __forceinline__ void block_product(float (&z)[R], const float* a, con
 //   3. the 16 x 16 diagonal blocks of (I + A)^-1 by substitution, a column per lane
 //   4. two doublings, 16 -> 32 -> 64
 //   5. W by mma, T diag(beta) in parts and W in halves to their images
-// Bound by latency: three to four CTAs share an SM. Scales are per warp (16 rows), so no CTA-wide maximum is needed.
+// Bound by latency: four CTAs of one warp per scheduler share an SM and issue in half of the cycles (six prompts of 1001 tokens
+// and 32 heads: 3072 CTAs, 73 us, 4400 shared-memory passes and 13000 warp instructions each). Scales are per warp (16 rows), so
+// no CTA-wide maximum is needed.
 template <int DKP, bool TREE>
 __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const DeltaChunkParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
@@ -564,9 +567,11 @@ int pad_dk(int dk) { return dk <= 64 ? 64 : 128; }
 size_t chunk_bytes(int hk, int hv, int dk) { return (size_t)hk * key_bytes(pad_dk(dk)) + (size_t)hv * head_bytes(pad_dk(dk)); }
 
 // How a prompt is walked through: in segments, each prepared by one kernel and scanned by the next. The scratch of a long prompt
-// so stays bounded, and in the L2 (2.6 MB per chunk at 16 key and 32 value heads).
+// so stays bounded: 256 MB, or four chunks of every sequence (2.6 MB per chunk at 16 key and 32 value heads. One prompt of 8192
+// tokens / six of 1001: 128 MB 402 / 179 us, 256 MB 390 / 161, 512 MB 404 / 160: fewer starts against a longer first wait).
 // Where the scan leaves most SMs idle (one CTA per head and sequence), the preparation of a segment runs beside the scan of the
-// one before, out of the other half of the scratch; only the first, short one is waited for.
+// one before, out of the other half of the scratch; only the first, short one is waited for. us, beside / one after the other,
+// 4096 tokens: 64 heads 291 / 334, 96 heads 393 / 412, 128 heads 516 / 509.
 struct Walk {
   int first, chunks;  // chunks of the first segment, and of the others at most
   bool beside;

@@ -1,20 +1,23 @@
 // The scan of the chunked delta rule on tcgen05 (sm_100a): the chunks of a head one after the other, the state in registers.
 //
-// The mathematics and the precision are those of delta_chunk.cu, which prepares k, q, T, P and the scalars of every chunk:
-//   R = V - diag(e^G) K S;  V' = T R;  O = diag(e^G) Q S + P V';  S <- e^G_C S + sum_j e^(G_C - G_j) k_j v'_j^T
+// The mathematics and the precision are those of delta_chunk.cu, which prepares k, q, T, W, P and the scalars of every chunk:
+//   V' = T V - W S;  O = diag(e^G) Q S + P V';  S <- e^G_C S + sum_j e^(G_C - G_j) k_j v'_j^T
 // Everything is done transposed: 128 value columns of a head are the M of the products, tokens or key dims the N. The left
-// operand then is always what was just computed (S^T, R^T, V'^T), written to TMEM by the threads that have it, a thread per
-// column, and the right one an image of the chunk in shared memory as it came. A column's scale belongs to its thread alone.
-// (mma.sync is no alternative on this GPU: its fp32 pipe does not run beside it. A product m16n8k16 and its eight
-// cycles add to the conversions instead of hiding them; that form took 4200 cycles per chunk on four times the SMs.)
+// operand then is always what was just computed (S^T, V'^T), written to TMEM by the threads that have it, a thread per column,
+// and the right one an image of the chunk in shared memory as it came. A column's scale belongs to its threads alone. T V does
+// not wait for the state: it is computed a chunk ahead from the values as they are (bf16 rows in shared memory).
 //
-// Warps 0-15: four threads per value column, a quarter of the key rows (of S) and of the tokens (of R, V') each; S stays
-// there in fp32 from the first chunk to the last. Warps 16-19: the output, a thread per column, from TMEM to memory, while the
-// others go on. Warp 20 fills the two stages of shared memory by bulk copies, warp 21 issues the products.
+// Warps 0-15: four threads per value column, a quarter of the key rows (of S) and of the tokens (of V') each; S stays there in
+// fp32 from the first chunk to the last. Warps 16-19: the output, a thread per column, from TMEM to memory, while the others go
+// on. Warp 20 fills the two stages of shared memory by bulk copies, warp 21 issues the products.
 //
-// Bound by the chain from chunk to chunk: 664 cycles of tensor time for K S, 500 for T R, 330 for half of the update, and
-// between them the conversions of 128 x 128 + 2 x 128 x 64 values on the threads (about 700 instructions each) and six
-// handovers.
+// Bound by the chain from chunk to chunk, 4800 cycles (one 8192-token prompt of 32 heads: 128 chunks, 388 us, of which the
+// preparation of the first chunks and the four segments' starts take 60): 1000 until S lies in halves in TMEM, 1000 of tensor
+// time for W S, 1400 until V' does, 330 for half of the update, 200 for the new S, and three handovers between threads and
+// tensor core of 300 each. The conversions, some 450 instructions per thread and chunk, fill half of all issue slots.
+// What it replaced: T R with R = V - diag(e^G) K S in place of W, a product and a handover more per chunk (490 us); and a scan by
+// mma.sync on four times the SMs, whose products share their issue slots with all other arithmetic (380 us for one prompt, but
+// 229 against 154 for six of 1001 tokens).
 #include "delta.cuh"
 #include "tcgen05.cuh"
 

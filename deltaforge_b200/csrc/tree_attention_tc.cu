@@ -1,6 +1,6 @@
-// Attention of a tree of drafted tokens over the KV cache on tcgen05 (sm_100a), for more than a few query rows.
+// Attention of a tree of drafted tokens over the KV cache on tcgen05 (sm_100a), for many heads or more than a few query rows.
 //
-// Same contract as tree_attention.cu, which serves the smallest trees. There the 16-row tiles of mma.sync read a key once per 64
+// Same contract as tree_attention.cu, which serves the others (tree_plan there has the rule). There the 16-row tiles of mma.sync read a key once per 64
 // rows and reach a quarter of the tensor rate; 64 nodes with 4 query heads per KV head (256 rows) were bound by that.
 // Here 128 rows (node * group + head) are the M of tcgen05.mma: S = Q K^T into TMEM, P = 2^(S - m) back into TMEM as the A
 // operand of O += P V, O in TMEM as well (S and its successor 128 columns each, O one column per dim: 512 at head dim 256).
@@ -19,9 +19,11 @@
 // the softmax of tile i. The maximum that P refers to is moved only when a row's true maximum is more than 2^8 above it,
 // so that O rarely has to be rescaled; sums stay exact because l refers to the same maximum.
 //
-// Bounds per tile of 128 keys at head dim 256: 2 x 1024 cycles of tensor time, 1024 of ex2, 128 KB of K and V from the L2. The
-// tensor time asks for wide products: with Q in TMEM (all of shared memory a ring) and tiles of 64 keys, an M 128 x N 64 x K 16
-// product took 75 cycles instead of 32, and 8 sequences x 64 nodes x 32K rows 247 us.
+// Bounds per tile of 128 keys at head dim 256: 1024 cycles of ex2, 128 KB of K and V from the L2, and of tensor time 16 products
+// Q K^T with both operands in shared memory (104 cycles each, measured, where the arithmetic takes 64) and 8 products P V with
+// P in TMEM and N = 256 (138): 2770 cycles, 161 of the 190 us that 8 sequences x 64 nodes x 32K rows take. (Q in TMEM would take
+// 74 cycles, but O, two S and Q are 640 columns; with tiles of 64 keys it was slower.) Run back to back for seconds, that case
+// draws 1000 W, the clock falls from 1965 to 1380 MHz and the call takes 240 us.
 //
 // Every wait is bounded; one that runs out makes the CTA leave NaN.
 #include <cuda.h>

@@ -18,8 +18,10 @@ this package                          reference op (file:line of its definition)
 ====================================  ===========================================================
 
 plus the fused forms the decode step is built from (``rmsnorm_int4_gemv``, ``int4_gemv_residual``,
-``silu_mul_int4_gemv_residual``, ``deltanet_step``, ``attn_prep``, ``attn_decode_gated``) and the two
-bit-exactness probes ``int4_unpack`` / ``int4_dequant``.
+``silu_mul_int4_gemv_residual``, ``deltanet_step``, ``attn_prep``, ``attn_decode_gated``), the two
+bit-exactness probes ``int4_unpack`` / ``int4_dequant``, and the ops that take several new tokens of a
+sequence at once, a prompt or a tree of drafted tokens: ``rotary_qk``, ``rotary_append`` (with
+``rope_frequencies``), ``tree_attention``, ``delta_rule_chunk``, ``delta_rule_tree``.
 
 Conventions kept from the reference: shape and dtype errors are ``ValueError`` and are raised before
 the device check, so they surface on any machine; a CPU tensor raises ``RuntimeError`` because there is

@@ -273,6 +273,43 @@ def test_tree_attention_layouts_streams_and_graphs(hq, hkv):
         assert torch.equal(out, ops.tree_attention(q, kc, vc, lt, pt, 0.09))
 
 
+@pytest.mark.parametrize("hq,hkv,n", [(4, 2, 5), (40, 20, 30)])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1.0])
+def test_tree_attention_scales(hq, hkv, n, scale):
+    b, d, rows = 2, 64, 200
+    q, kc, vc = rnd(35, b, n, hq, d, dtype=F16, scale=0.5), rnd(36, b, hkv, rows, d, dtype=F16, scale=0.5), rnd(37, b, hkv, rows, d, dtype=F16)
+    lens, parents = [150, 20], random_tree(9, n)
+    want, size = tree_ref(q, kc, vc, lens, [parents] * b, scale)
+    got = ops.tree_attention(q, kc, vc, torch.tensor(lens, dtype=I32, device=DEV), torch.tensor(parents, dtype=I32, device=DEV), scale)
+    within(got, want, tree_bound(want, size, q, kc, abs(scale), rows))
+
+
+@pytest.mark.parametrize("n,hq", [(3, 4), (20, 2)])
+def test_offsets_past_32_bits_in_a_long_cache(n, hq):
+    """One sequence of 9 million rows of 256: element offsets up to 2.3e9. All keys but a few are zero, so the scores are known."""
+    d, rows = 256, 9_000_000
+    kc, vc = torch.zeros(1, 1, rows, d, dtype=BF16, device=DEV), torch.zeros(1, 1, rows, d, dtype=BF16, device=DEV)
+    q, k, v = rnd(38, 1, n, hq, d, dtype=BF16), rnd(39, 1, n, 1, d, dtype=BF16), rnd(40, 1, n, 1, d, dtype=BF16)
+    at = [5, 8_388_609, 8_900_000]  # the second and the third lie past 2^31 elements
+    kc[0, 0, at], vc[0, 0, at] = rnd(41, 3, d, dtype=BF16), rnd(42, 3, d, dtype=BF16)
+    length = rows - n
+    lens = torch.tensor([length], dtype=I32, device=DEV)
+    inv, factor = ops.rope_frequencies(64, 1e6)
+    pos = (length + torch.arange(n, dtype=I32, device=DEV))[None]
+    tq = ops.rotary_append(q, k, v, pos, inv, factor, False, kc, vc, lens)
+    assert torch.equal(kc[0, 0, length:], ops.rotary_qk(q, k, pos, inv, factor, False)[1][0, :, 0]) and torch.equal(vc[0, 0, length:], v[0, :, 0])
+    scale = 0.25  # scores of about 4: the few rows and the millions of zeros both count
+    got = ops.tree_attention(tq, kc, vc, lens, torch.arange(-1, n - 1, dtype=I32, device=DEV), scale)
+    for i in range(n):
+        seen = at + [length + j for j in range(i + 1)]
+        s = torch.einsum("hd,kd->hk", tq[0, i].double(), kc[0, 0, seen].double()) * scale
+        w = s.exp() / (s.exp().sum(-1, keepdim=True) + rows - n - len(at))
+        want, size = w @ vc[0, 0, seen].double(), w @ vc[0, 0, seen].double().abs()
+        # as in tree_bound; the sum of 9 million ones is exact below 2^24 and grows in steps of a tile's sum
+        ds = 2 * d * half(F32) * scale * (tq.double().norm(dim=-1).max() * kc[0, 0, seen].double().norm(dim=-1).max()).item()
+        within(got[0, i], want, half(BF16) * want.abs() + (half(BF16) + 2 * ds + 2**-20 + rows / 128 * 2**-24) * size * (1 + 2**-6))
+
+
 # ---------------------------------------------------------------- the delta rule
 
 
@@ -478,6 +515,51 @@ def test_delta_rule_layouts_streams_and_graphs():
         assert torch.equal(out, want[0]) and torch.equal(state, want[1])
 
 
+def test_delta_rule_long_prompt_in_segments():
+    """Three segments, each prepared beside the scan of the one before: alone, on two streams at once, and replayed from a
+    graph with lengths that end in each of them."""
+    b, t, hk, hv, dk, dv = 1, 7000, 16, 32, 128, 8
+    a = delta_inputs(121, b, t, hk, hv, dk, dv, True)
+    out, state = ops.delta_rule_chunk(*a, None, True)
+    want, size, s = delta_ref(*a, None, True)
+    within(out, want, delta_out_bound(want, size))
+    within(state, s, delta_state_bound(s, t))
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        for x in (s1, s2):
+            with torch.cuda.stream(x):
+                got.append(ops.delta_rule_chunk(*a, None, True))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, out) and torch.equal(y, state) for x, y in got)
+    lens = torch.full((b,), t, dtype=I32, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, st = ops.delta_rule_chunk(*a, lens, True)
+    for n in (t, 0, 1152, 1153, 4000, 1, t):
+        lens.fill_(n)
+        graph.replay()
+        assert torch.equal(o[:, :n], out[:, :n]) and bool((o[:, n:] == 0).all())
+        if n == t:
+            assert torch.equal(st, state)
+        elif n == 0:
+            assert torch.equal(st, a[0])
+        else:
+            assert torch.equal(st, ops.delta_rule_chunk(*a, lens, True)[1])
+
+
+@pytest.mark.parametrize("t", [7, 100])
+def test_delta_rule_expanded_inputs(t):
+    b, hk, hv, dk, dv = 2, 4, 8, 64, 64
+    st, q, k, v, g, beta = delta_inputs(131, b, t, hk, hv, dk, dv, True)
+    q, k, v = q[:1].expand(b, t, hk, dk), k[:, :, :1].expand(b, t, hk, dk), v[:, :, :1].expand(b, t, hv, dv)
+    g, beta = g[:, :1].expand(b, t, hv), beta[:1].expand(b, t, hv)
+    got = ops.delta_rule_chunk(st[:1].expand(b, hv, dk, dv), q, k, v, g, beta, None, True)
+    want = ops.delta_rule_chunk(st[:1].repeat(b, 1, 1, 1), *(x.contiguous() for x in (q, k, v, g, beta)), None, True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_nothing_to_do():
     st, q, k, v, g, beta = delta_inputs(99, 2, 4, 1, 2, 16, 16, True)
     none = [x[:, :0] for x in (q, k, v, g, beta)]
@@ -514,6 +596,12 @@ def test_a_tree_is_verified_and_a_path_accepted():
     tq = ops.rotary_append(q[:, prompt:], k[:, prompt:], v[:, prompt:], pos, inv, factor, False, kc, vc, cached)
     attn = ops.tree_attention(tq, kc, vc, cached, parents, d**-0.5)
     lin = ops.delta_rule_tree(state, *(x[:, prompt:] for x in (dq, dkey, dval, g, beta)), parents, True)
+    want, size = tree_ref(tq, kc, vc, [prompt] * b, [tree] * b, d**-0.5)
+    within(attn, want, tree_bound(want, size, tq, kc, d**-0.5, rows))
+    want, size = tree_delta_ref(state, *(x[:, prompt:] for x in (dq, dkey, dval, g, beta)), [tree] * b, True)
+    within(lin, want, delta_out_bound(want, size))
+    # Against the single-token ops: each side rounds to bf16 once and its operands to 8 or 11 bits, together below
+    # 2^-7 |o| + 2^-7 sum |terms|, where the sums of this data's terms stay near 1
     for node, path in enumerate(paths(tree)):
         row = [prompt + j for j in path]
         keys = torch.cat((kc[:, :, :prompt], kc[:, :, row]), 2)
