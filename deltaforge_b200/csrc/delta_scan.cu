@@ -11,7 +11,10 @@
 // fp32 from the first chunk to the last. Warps 16-19: the output, a thread per column, from TMEM to memory, while the others go
 // on. Warp 20 fills the two stages of shared memory by bulk copies, warp 21 issues the products.
 //
-// Bound by the chain from chunk to chunk, 4800 cycles (one 8192-token prompt of 32 heads: 128 chunks, 388 us, of which the
+// Trees are one chunk each and leave no state: 148 CTAs walk through all of them, the next state on its way while the products
+// of this one run (16 trees x 32 heads: 53 us with a CTA for each, 42 so).
+//
+// Bound by the chain from chunk to chunk, 4800 cycles (one 8192-token prompt of 32 heads: 128 chunks, 381 us, of which the
 // preparation of the first chunks and the four segments' starts take 60): 1000 until S lies in halves in TMEM, 1000 of tensor
 // time for W S, 1400 until V' does, 330 for half of the update, 200 for the new S, and three handovers between threads and
 // tensor core of 300 each. The conversions, some 450 instructions per thread and chunk, fill half of all issue slots.
@@ -38,6 +41,10 @@ template <int DKP> struct Stage {
 // it is for the output); the others are accumulators. The update takes the place of W S, V' in halves that of the lower halves of S.
 constexpr int SH = 0, SL = 64, WS = 128, UP = 128, RH = 64, RL = 96, QS = 256, TV = 320, PV = 384, VH = 448;
 
+struct Unit {
+  int vb, hv, b;  // block of value columns, value head, sequence
+};
+
 template <int DKP, bool TREE>
 __global__ void __launch_bounds__(SCAN_THREADS, 1)
     delta_scan_kernel(const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap omap, const DeltaChunkParams p) {
@@ -53,9 +60,21 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   volatile int* failed = &failed_s;
 
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  const int vb = blockIdx.x, hv = blockIdx.y, b = blockIdx.z, hk = hv / (p.hv / p.hk);
-  const int len = p.lengths ? min(max(p.lengths[b], 0), p.tokens) : p.tokens;
-  const int nlive = min(max((len + C - 1) / C - p.chunk0, 0), p.chunks);  // chunks of this segment with tokens
+  // What is walked through: the chunks of one unit (value columns, head, sequence); for trees units, one chunk each.
+  const int wide = (p.dv + COLS - 1) / COLS;
+  auto nth = [&](unsigned u) {
+    const int rest = u / wide;
+    return Unit{(int)u - rest * wide, rest % p.hv, rest / p.hv};
+  };
+  const Unit here = nth(blockIdx.x);
+  auto unit = [&](int n) { return TREE && n > 0 ? nth(blockIdx.x + n * gridDim.x) : here; };
+  int nlive;
+  if (TREE) {
+    nlive = (wide * p.hv * p.batch - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+  } else {
+    const int len = p.lengths ? min(max(p.lengths[here.b], 0), p.tokens) : p.tokens;
+    nlive = min(max((len + C - 1) / C - p.chunk0, 0), p.chunks);  // chunks of this segment with tokens
+  }
   if (t == 0) {
     for (int i = 0; i < 2; ++i) mbar_init(&full[i], 1), mbar_init(&s_in[i], 16), mbar_init(&u_out[i], 1), mbar_init(&o_out[i], 1);
     mbar_init(&v_full, 1), mbar_init(&v_in, 1), mbar_init(&tv_out, 1), mbar_init(&ws_out, 1);
@@ -71,15 +90,13 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_slot;
-  const int q = warp & 3, col = q * 32 + lane, gcol = vb * COLS + col;
-  const bool cok = gcol < p.dv;
+  const int q = warp & 3, col = q * 32 + lane;
   const uint32_t base = tmem + ((uint32_t)(q * 32) << 16);
   bool ok = true;  // a wait that ran out lets everything run to its end on garbage; NaN is what is left then
 
   if (warp < 16) {
     // ---------------- the recurrence ----------------
     const int h = warp >> 2;
-    const long sb = ((long)b * p.hv + hv) * p.dk * p.dv + gcol;
     auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + q) : "memory"); };  // the four warps of these columns
     auto most = [&](const float (&m)[4][COLS]) { return fmaxf(fmaxf(m[0][col], m[1][col]), fmaxf(m[2][col], m[3][col])); };
     // hi and lo of two values
@@ -90,23 +107,44 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       lo = h2(r.x, r.y);
     };
     F2 S[NS / 2];
-    // (The first segment's state is there before the preparation starts; nothing else here comes but through the loads.)
-    const float* Sin = p.first ? p.state + sb : p.state_out + sb;
-    float ms = 0.f;
+    long sb = 0;  // this thread's column in the state
+    bool cok = false;
+    auto load = [&](int n) {
+      const Unit u = unit(n);
+      const int gcol = u.vb * COLS + col;
+      cok = gcol < p.dv;
+      sb = ((long)u.b * p.hv + u.hv) * p.dk * p.dv + gcol;
+      const float* Sin = p.first ? p.state + sb : p.state_out + sb;
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      const int d = h * NS + i;
-      const float v = cok && d < p.dk ? Sin[(long)d * p.dv] : 0.f;
-      (i & 1 ? S[i / 2].y : S[i / 2].x) = v;
-      ms = fmaxf(ms, fabsf(v));
-    }
-    s_max[h][col] = ms;
-    meet();
-    int es = scale_exp(most(s_max));
-    meet();
-
+      for (int i = 0; i < NS; ++i) {
+        const int d = h * NS + i;
+        const float v = cok && d < p.dk ? Sin[(long)d * p.dv] : 0.f;
+        (i & 1 ? S[i / 2].y : S[i / 2].x) = v;
+      }
+    };
+    // (The first segment's state is there before the preparation starts; nothing else here comes but through the loads.)
+    load(0);
+    float ms;
+    int es;
+    auto scale = [&]() {  // the columns' largest
+      ms = 0.f;
+#pragma unroll
+      for (int i = 0; i < NS / 2; ++i) ms = fmaxf(fmaxf(ms, fabsf(S[i].x)), fabsf(S[i].y));
+      s_max[h][col] = ms;
+      meet();
+      es = scale_exp(most(s_max));
+      meet();
+    };
+    if (!TREE) scale();
     for (int n = 0; n < nlive; ++n) {
       const float* sc = (const float*)(sm + G::SC + n % 3 * SCAL);
+      if (TREE) {
+        scale();
+        if (n > 0) {  // the products of the unit before have read its state
+          ok = wait_for(&o_out[(n - 1) & 1], ((n - 1) >> 1) & 1, failed) && ok;
+          fence_after();
+        }
+      }
       // S in halves to TMEM, 16 key rows at a time; its largest on the side
       {
         const float sdown = pow2(-es);
@@ -119,7 +157,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
             split(mul2(S[x / 2 + i], {sdown, sdown}), hi[i], lo[i]);
             top = __hmax2_nan(top, __habs2(*(const __half2*)&hi[i]));
           }
-          if (x == 0 && n > 0 && h < 2 && DKP > 64) {  // the lower halves' place: all of the update before has read it
+          if (!TREE && x == 0 && n > 0 && h < 2 && DKP > 64) {  // the lower halves' place: all of the update before has read it
             ok = wait_for(&u_out[1], (n & 1) ^ 1, failed) && ok;
             fence_after();
           }
@@ -134,6 +172,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       }
       s_max[h][col] = ms * pow2(es);
       if (h == 0) s_exp[n & 1][col] = es;
+      if (TREE && n + 1 < nlive) load(n + 1);
 
       // V' = T V - W S
       ok = wait_for(&full[n & 1], (n >> 1) & 1, failed) && ok;
@@ -191,7 +230,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
         if (!TREE) mbar_arrive(&u_in);
         mbar_arrive(&p_in);
       }
-      if (TREE) break;
+      if (TREE) continue;
 
       // S: the update was accumulated apart and is added in fp32
       ok = wait_for(&u_out[h >> 1], n & 1, failed) && ok;
@@ -219,11 +258,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   } else if (warp < 20) {
     // ---------------- output ----------------
     bf16* rows_s = (bf16*)(sm + G::ROWS);  // a chunk's output rows on their way out
-    bf16* out = p.out + ((long)b * p.tokens * p.hv + hv) * p.dv + vb * COLS;
-    const long orow = (long)p.hv * p.dv;
     for (int n = 0; n < nlive; ++n) {
       const float* sc = (const float*)(sm + G::SC + n % 3 * SCAL);
-      const int tok0 = (p.chunk0 + n) * C;
       ok = wait_for(&o_out[n & 1], (n >> 1) & 1, failed) && ok;
       fence_after();
       const float sup = pow2(s_exp[n & 1][col]), vup = ok ? pow2(v_exp[n & 1][col]) : __int_as_float(0x7fffffff);
@@ -257,32 +293,38 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       asm volatile("bar.sync 5, 128;" ::: "memory");
       if (lane == 0) mbar_arrive(&o_read);  // TMEM and the scalars have been read
       if (warp == 16 && lane == 0) {  // (rows and columns past the ends are left out)
-        tma_store_box(&omap, smem_u32(rows_s), vb * COLS, hv, tok0, b);
+        const Unit u = unit(n);
+        tma_store_box(&omap, smem_u32(rows_s), u.vb * COLS, u.hv, TREE ? 0 : (p.chunk0 + n) * C, u.b);
         bulk_stores_commit();
       }
     }
     if (warp == 16 && lane == 0) bulk_stores_done();
-    // rows of tokens that no chunk covered: zeros
-    const int from = (p.chunk0 + nlive) * C, to = min(p.tokens, (p.chunk0 + p.chunks) * C);
-    for (int i = from; i < to; ++i)
-      if (cok) out[(long)i * orow + col] = f2bf(0.f);
+    if (!TREE) {  // rows of tokens that no chunk covered: zeros
+      const Unit u = here;
+      const int from = (p.chunk0 + nlive) * C, to = min(p.tokens, (p.chunk0 + p.chunks) * C), gcol = u.vb * COLS + col;
+      const long orow = (long)p.hv * p.dv;
+      bf16* out = p.out + ((long)u.b * p.tokens * p.hv + u.hv) * p.dv + gcol;
+      for (int i = from; i < to; ++i)
+        if (gcol < p.dv) out[(long)i * orow] = f2bf(0.f);
+    }
   } else if (warp == 20) {
     // ---------------- loads ----------------
     pdl_wait();
     pdl_launch_dependents();  // the preparation of the next segment may run beside this scan, but not beside the one before
     const long per = p.hk * (long)key_bytes(DKP) + p.hv * (long)head_bytes(DKP);
-    const unsigned char* src = p.scratch + (long)b * p.seg_chunks * per;
     for (int n = 0; n < nlive; ++n) {
       // the products of chunk n - 2 are done; they came after the output of chunk n - 3, whose scalars are replaced
       if (n >= 2) ok = wait_for(&o_out[n & 1], ((n >> 1) - 1) & 1, failed) && ok;
       if (!__all_sync(0xffffffffu, ok)) break;
-      const unsigned char* head = src + n * per + p.hk * (long)key_bytes(DKP) + (long)hv * head_bytes(DKP);
+      const Unit u = unit(n);
+      const unsigned char* src = p.scratch + ((long)u.b * p.seg_chunks + (TREE ? 0 : n)) * per;
+      const unsigned char* head = src + p.hk * (long)key_bytes(DKP) + (long)u.hv * head_bytes(DKP);
       const uint32_t st = smem_u32(sm + (n & 1) * G::BYTES);
       unsigned char* scn = sm + G::SC + n % 3 * SCAL;
       if (elect_one()) {
         uint64_t* bar = &full[n & 1];
         mbar_expect_tx(bar, G::BYTES + SCAL);
-        bulk_copy(st, src + n * per + (long)hk * key_bytes(DKP), key_bytes(DKP), bar);
+        bulk_copy(st, src + (long)(u.hv / (p.hv / p.hk)) * key_bytes(DKP), key_bytes(DKP), bar);
         bulk_copy(st + G::P, head + 3 * SQ, SQ + 2 * w_bytes(DKP), bar);
         bulk_copy(smem_u32(scn), head + 4 * SQ + 2 * w_bytes(DKP), SCAL, bar);
       }
@@ -293,7 +335,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
         mbar_expect_tx(&v_full, 3 * SQ + C * COLS * 2);
         bulk_copy(smem_u32(sm + G::T), head, 3 * SQ, &v_full);
         for (int i = 0; i < 2; ++i)  // (zeros past the ends)
-          tma_box(smem_u32(sm + G::V + i * C * 128), &vmap, vb * COLS + 64 * i, hv, (p.chunk0 + n) * C, b, &v_full);
+          tma_box(smem_u32(sm + G::V + i * C * 128), &vmap, u.vb * COLS + 64 * i, u.hv, TREE ? 0 : (p.chunk0 + n) * C, u.b, &v_full);
       }
       __syncwarp();
       // values of tokens that do not count may be anything: zeros take their place
@@ -428,8 +470,13 @@ int launch_delta_scan(const DeltaChunkParams& p, cudaStream_t stream) {
     set_error("delta rule scan: tensor map for the values or the output failed");
     return 1;
   }
-  const dim3 grid((p.dv + COLS - 1) / COLS, p.hv, p.batch);
   const bool tree = p.parents != nullptr, wide = p.dk > 64;
+  const long units = (long)((p.dv + COLS - 1) / COLS) * p.hv * p.batch;
+  if (units > 0x7fffffff) {
+    set_error("delta rule scan: %d sequences of %d heads are too many", p.batch, p.hv);
+    return 2;
+  }
+  const dim3 grid((unsigned)(tree && units > 148 ? 148 : units));
   if (tree) return wide ? launch_one<128, true>(vmap, omap, p, grid, stream) : launch_one<64, true>(vmap, omap, p, grid, stream);
   return wide ? launch_one<128, false>(vmap, omap, p, grid, stream) : launch_one<64, false>(vmap, omap, p, grid, stream);
 }

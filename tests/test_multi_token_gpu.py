@@ -457,7 +457,7 @@ def tree_delta_ref(state, q, k, v, g, beta, parents, l2norm):
 
 
 @pytest.mark.parametrize("l2norm", [False, True])
-@pytest.mark.parametrize("b,n,hk,hv,dk,dv,tree", [(1, 1, 2, 4, 128, 128, "one"), (2, 16, 2, 4, 128, 128, "random"), (1, 64, 1, 3, 96, 80, "chain"), (3, 37, 2, 2, 64, 16, "random"), (1, 64, 1, 1, 128, 128, "star")])
+@pytest.mark.parametrize("b,n,hk,hv,dk,dv,tree", [(1, 1, 2, 4, 128, 128, "one"), (2, 16, 2, 4, 128, 128, "random"), (1, 64, 1, 3, 96, 80, "chain"), (3, 37, 2, 2, 64, 16, "random"), (1, 64, 1, 1, 128, 128, "star"), (20, 9, 4, 16, 64, 40, "random"), (12, 33, 8, 32, 128, 136, "random")])
 def test_delta_rule_tree(b, n, hk, hv, dk, dv, tree, l2norm):
     a = delta_inputs(91, b, n, hk, hv, dk, dv, l2norm)
     s0 = a[0].clone()
@@ -470,8 +470,9 @@ def test_delta_rule_tree(b, n, hk, hv, dk, dv, tree, l2norm):
         within(got, ops.delta_rule_chunk(*a, None, l2norm)[0].double(), 2 * delta_out_bound(want, size))
 
 
-def test_delta_rule_tree_rows_without_a_node():
-    b, n, hk, hv, dk, dv = 2, 12, 2, 4, 128, 128
+@pytest.mark.parametrize("hk,hv", [(2, 4), (40, 160)])
+def test_delta_rule_tree_rows_without_a_node(hk, hv):
+    b, n, dk, dv = 2, 12, 128, 128
     a = list(delta_inputs(95, b, n, hk, hv, dk, dv, True))
     parents = [[-1, 0, 7, 2, -5, 4, 5, 3, 99, 8, 9, 1], [-2] * n]
     want, size = tree_delta_ref(*a, parents, True)
