@@ -29,6 +29,7 @@ namespace dfb {
 namespace {
 
 constexpr int COLS = 128;  // value columns per CTA
+constexpr int BY_LENGTH = 256;  // sequences that are put in order (a comparison of each with each in every CTA)
 constexpr int SCAN_WARPS = 22, SCAN_THREADS = SCAN_WARPS * 32;
 
 template <int DKP> struct Stage {
@@ -56,7 +57,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   __shared__ float s_max[4][COLS], vp_max[4][COLS];
   __shared__ int s_exp[2][COLS], v_exp[2][COLS];  // by chunk parity, for the output
   __shared__ uint32_t tmem_slot;
-  __shared__ int failed_s;
+  __shared__ int failed_s, seq_s;
   volatile int* failed = &failed_s;
 
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
@@ -66,14 +67,18 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
     const int rest = u / wide;
     return Unit{(int)u - rest * wide, rest % p.hv, rest / p.hv};
   };
-  const Unit here = nth(blockIdx.x);
-  auto unit = [&](int n) { return TREE && n > 0 ? nth(blockIdx.x + n * gridDim.x) : here; };
-  int nlive;
-  if (TREE) {
-    nlive = (wide * p.hv * p.batch - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
-  } else {
-    const int len = p.lengths ? min(max(p.lengths[here.b], 0), p.tokens) : p.tokens;
-    nlive = min(max((len + C - 1) / C - p.chunk0, 0), p.chunks);  // chunks of this segment with tokens
+  Unit here = nth(blockIdx.x);
+  // The longest prompts first, where not all CTAs run at once (us, as they come / so, 32 heads: six drawn batches of 12 prompts
+  // of up to 2000 tokens 407 .. 528 / 390 .. 504, of 6 up to 1001 107 .. 166 / 105 .. 160)
+  const bool by_length = !TREE && p.lengths && gridDim.x > 148 && p.batch <= BY_LENGTH;
+  if (by_length && t < p.batch) {
+    const int mine = p.lengths[t];
+    int rank = 0;
+    for (int i = 0; i < p.batch; ++i) {
+      const int other = p.lengths[i];
+      rank += other > mine || (other == mine && i < t);
+    }
+    if (rank == here.b) seq_s = t;
   }
   if (t == 0) {
     for (int i = 0; i < 2; ++i) mbar_init(&full[i], 1), mbar_init(&s_in[i], 16), mbar_init(&u_out[i], 1), mbar_init(&o_out[i], 1);
@@ -89,6 +94,15 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   fence_before();
   __syncthreads();
   fence_after();
+  if (by_length) here.b = seq_s;
+  auto unit = [&](int n) { return TREE && n > 0 ? nth(blockIdx.x + n * gridDim.x) : here; };
+  int nlive;
+  if (TREE) {
+    nlive = (wide * p.hv * p.batch - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+  } else {
+    const int len = p.lengths ? min(max(p.lengths[here.b], 0), p.tokens) : p.tokens;
+    nlive = min(max((len + C - 1) / C - p.chunk0, 0), p.chunks);  // chunks of this segment with tokens
+  }
   const uint32_t tmem = tmem_slot;
   const int q = warp & 3, col = q * 32 + lane;
   const uint32_t base = tmem + ((uint32_t)(q * 32) << 16);

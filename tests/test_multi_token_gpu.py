@@ -376,9 +376,9 @@ def test_delta_rule_chunk(b, t, hk, hv, dk, dv, l2norm):
     assert torch.equal(a[0], s0)
 
 
-@pytest.mark.parametrize("t", [5, 150])
-def test_delta_rule_lengths_and_what_lies_behind_them(t):
-    b, hk, hv, dk, dv = 6, 2, 4, 128, 128
+@pytest.mark.parametrize("t,hv", [(5, 4), (150, 4), (150, 40)])  # (the last: more heads than run at once)
+def test_delta_rule_lengths_and_what_lies_behind_them(t, hv):
+    b, hk, dk, dv = 6, 2, 128, 128
     a = list(delta_inputs(51, b, t, hk, hv, dk, dv, True))
     lens = [t, 0, 1, t // 2, t + 7, -3]
     want, size, s = delta_ref(*a, lens, True)
