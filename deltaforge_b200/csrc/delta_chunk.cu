@@ -94,8 +94,9 @@ __device__ __forceinline__ void block_product(float (&z)[R], const float* a, con
 //   4. two doublings, 16 -> 32 -> 64
 //   5. W by mma, T diag(beta) in parts and W in halves to their images
 // Bound by latency: four CTAs of one warp per scheduler share an SM and issue in half of the cycles (six prompts of 1001 tokens
-// and 32 heads: 3072 CTAs, 73 us, 4400 shared-memory passes and 13000 warp instructions each). Scales are per warp (16 rows), so
-// no CTA-wide maximum is needed.
+// and 32 heads: 73 us, 4400 shared-memory passes and 13000 warp instructions per CTA; no single cause of waiting has a fifth).
+// Eight warps per CTA with half of the registers, and the doublings by mma in three parts, were not faster. Scales are per warp
+// (16 rows), so no CTA-wide maximum is needed.
 template <int DKP, bool TREE>
 __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prep_kernel(const DeltaChunkParams p) {
   extern __shared__ __align__(128) unsigned char smem[];

@@ -125,11 +125,6 @@ __device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t* v) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : DFB_OUT8(v, 0) : "r"(addr));
 }
 __device__ __forceinline__ void tmem_wait_ld8(uint32_t* v) { asm volatile("tcgen05.wait::ld.sync.aligned;" : DFB_TIE8(v, 0)::"memory"); }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), DFB_IN8(v, 0),
-               DFB_IN8(v, 8)
-               : "memory");
-}
 __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), DFB_IN8(v, 0) : "memory");
 }

@@ -20,7 +20,8 @@
 // Rounding: q, k, v as they are; scores, maximum, sum and accumulators in fp32; probabilities are rounded to the cache's
 // type for the second product (relative 2^-9 each in bf16, of random sign), the sum takes them unrounded.
 //
-// A row without a node (parent below -1 or not before the node) gets zeros. Splits leave (m, l, acc) in scratch and
+// A row without a node (parent below -1 or not before the node) gets zeros, and so does one that sees no key: without a
+// prefix, of a tree that reaches past the cache. Splits leave (m, l, acc) in scratch and
 // tree_merge_kernel adds them in split order: results do not depend on which CTA ends first.
 #include "common.cuh"
 #include "kernels.h"
@@ -417,7 +418,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_attention_kernel(const Tre
       const int node = gr / p.group;
       const int pa = p.parents[(long)b * p.parents_stride + node];
       const bool ok = pa >= -1 && pa < node;
-      const float inv = 1.f / l;
+      const float inv = l == 0.f ? 0.f : 1.f / l;  // 0: nothing seen
       T* out = (T*)p.out + (((long)b * p.nodes + node) * p.hq + hk * p.group + gr % p.group) * D + d2;
       *(uint32_t*)out = ok ? pack2<T>(a.x * inv, a.y * inv) : 0u;
     } else {
@@ -471,7 +472,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttnParams p)
     a.x += y.x, a.y += y.y, a.z += y.z, a.w += y.w;
     l += part_l[i];
   }
-  const float inv = 1.f / l;
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // 0: nothing seen
   T* out = (T*)p.out + (((long)b * p.nodes + node) * p.hq + hk * p.group + row % p.group) * D + 4 * li;
   uint2 v = make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
   if (!ok) v = make_uint2(0u, 0u);

@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
       const uint32_t o_base = lane_base + S_::O_COL;
       const long slot = (per_unit ? grp : grp + (long)b * upb + unit) * row_tiles + rt;
       const float2 ml = make_float2(row_m[r], row_l[r] + row_l[TM + r]);
-      const float w = whole ? 1.f / ml.y : 1.f;
+      const float w = !whole ? 1.f : ml.y == 0.f ? 0.f : 1.f / ml.y;  // (a sum of 0: nothing seen)
       float* stage = (float*)ring + warp * (32 * 36);  // the ring is idle: a row's 32 columns leave as whole lines
 #pragma unroll 1
       for (int x = (warp >> 2) * (D / 2); x < (warp >> 2) * (D / 2) + D / 2; x += 32) {
@@ -585,7 +585,7 @@ __global__ void __launch_bounds__(256) tree_tc_merge_kernel(const TreeAttnParams
       a.x = a.x * f + y[i].x * w, a.y = a.y * f + y[i].y * w, a.z = a.z * f + y[i].z * w, a.w = a.w * f + y[i].w * w;
     }
   }
-  const float inv = 1.f / l;
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // 0: nothing seen
   T* out = (T*)p.out + (((long)b * p.nodes + node) * p.hq + hk * p.group + row - node * p.group) * D + 4 * li;
   *(uint2*)out = ok ? make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv)) : make_uint2(0u, 0u);
 }

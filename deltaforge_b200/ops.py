@@ -1043,7 +1043,8 @@ def tree_attention(query: Tensor, key_cache: Tensor, value_cache: Tensor, cache_
     ``query`` is ``(batch, nodes, heads, head_dim)``; node ``i`` of sequence ``b`` holds cache row ``cache_len[b] + i`` and sees
     the rows before ``cache_len[b]``, its ancestors' and its own. ``parents (batch, nodes)``, or ``(nodes,)`` for one tree for
     all: the index of a node's parent, which comes before it; -1 where the parent is the last cached token. Any other
-    value marks a row without a node (a padded batch): its output is zero and no node sees it. One node is the decode
+    value marks a row without a node (a padded batch): its output is zero and no node sees it. Rows from ``max_seq`` on do
+    not exist: a node that reaches no other row gives zeros too. One node is the decode
     attention, a chain (``parents = [-1, 0, 1, ...]``) causal attention. bf16 or fp16, head dim 32, 64, 128 or 256."""
     op = "tree_attention"
     if query.dim() != 4:

@@ -327,7 +327,8 @@ size_t dfb_tree_attn_scratch_bytes(int batch, int nodes, int hq, int hkv, int d,
 
 /* Attention of a tree of drafted tokens over the KV cache that holds the accepted prefix and the tree's own rows: the
  * many-token form of split_kv_decode_attention (src/deltaforge/kernels/flash_decode_splitkv.py:177-256). Cache rows
- * past the tree are not read; a tree that reaches past max_seq loses the keys it has there. */
+ * past the tree are not read; a tree that reaches past max_seq loses the keys it has there, and a node that is left
+ * without any gives zeros. */
 int dfb_tree_attention(const dfb_tree_attn_desc* desc, void* stream);
 
 typedef struct dfb_delta_chunk_desc {

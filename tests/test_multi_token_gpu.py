@@ -186,11 +186,16 @@ TREES = {
         (2, 64, 2, 1, 32, 4096, [4032, 17], "star"),
         (1, 5, 24, 2, 64, 8, [3], "random"),
         (2, 3, 3, 3, 32, 2, [0, 0], "chain"),  # more nodes than rows: keys past the cache are lost
+        (3, 33, 2, 2, 64, 7, [0, 0, 7], "random"),  # and so do nodes whose whole path lies there: zeros
+        (2, 13, 2, 2, 32, 1, [0, 1], "one"),
+        (2, 40, 4, 1, 256, 5, [0, 2], "one"),
         # heads enough for the form that reads the cache once for 128 rows
         (8, 12, 16, 4, 256, 300, [288, 0, 1, 127, 128, 129, 250, 90], "random"),
         (9, 64, 12, 4, 128, 200, [136, 0, 63, 64, 65, 100, 1, 128, 31], "random"),
         (16, 9, 8, 4, 64, 700, [691, 0, 5, 130, 600, 64, 63, 384] * 2, "chain"),
         (11, 17, 3, 3, 256, 20, [3] * 11, "star"),
+        (9, 33, 8, 4, 64, 1, [1, 1, 1, 0, 0, 0, 0, 0, 0], "one"),
+        (4, 48, 16, 16, 128, 130, [0, 100, 130, 127], "one"),
         (1, 16, 16, 4, 128, 20000, [19984], "random"),
     ],
 )
