@@ -875,6 +875,11 @@ def _new_like(t: Tensor) -> Tensor:
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
+def _fresh(t: Tensor) -> Tensor:
+    """A contiguous copy (``contiguous`` would return a tensor that only starts at an odd offset as it is)."""
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _rows(op: str, name: str, t: Tensor) -> tuple[int, int, int]:
     """Strides of the three leading dimensions; the last one must be contiguous."""
     s = t.stride()
@@ -1067,7 +1072,7 @@ def tree_attention(query: Tensor, key_cache: Tensor, value_cache: Tensor, cache_
         raise ValueError(f"{op}: cache rows must start on 16-byte boundaries")
     _same_device(op, query, key_cache, value_cache, cache_len, parents)
     if (q_rows[0] | q_rows[1] | q_rows[2]) % 8 or query.data_ptr() % 16:
-        query = query.contiguous()
+        query = _fresh(query)
         q_rows = query.stride()[:3]
     out = _new_like(query)
     if batch == 0 or nodes == 0:
@@ -1089,10 +1094,10 @@ def _(query, key_cache, value_cache, cache_len, parents, scale):
     return query.new_empty(query.shape)
 
 
-def _aligned_rows(t: Tensor) -> Tensor:
-    """`t`, copied if its rows do not start on 16-byte boundaries."""
+def _aligned_rows(t: Tensor, expanded: bool = True) -> Tensor:
+    """`t`, copied if its rows do not start on 16-byte boundaries, or if it may not be `expanded` and is."""
     s = t.stride()
-    return t.contiguous() if (s[0] | s[1] | s[2]) % 8 or t.data_ptr() % 16 else t
+    return _fresh(t) if (s[0] | s[1] | s[2]) % 8 or t.data_ptr() % 16 or not (expanded or all(s)) else t
 
 
 def _delta_tokens(
@@ -1125,7 +1130,7 @@ def _delta_tokens(
     _same_device(op, state, query, key, value, g, beta, lengths, parents)
     qp, kp, vp = query.data_ptr(), key.data_ptr(), value.data_ptr()
     if 0 in v_rows or (q_rows[0] | q_rows[1] | q_rows[2] | k_rows[0] | k_rows[1] | k_rows[2] | v_rows[0] | v_rows[1] | v_rows[2]) % 8 or (qp | kp | vp) % 16:
-        query, key, value = _aligned_rows(query), _aligned_rows(key), _aligned_rows(value) if 0 not in v_rows else value.contiguous()
+        query, key, value = _aligned_rows(query), _aligned_rows(key), _aligned_rows(value, expanded=False)
         q_rows, k_rows, v_rows = query.stride()[:3], key.stride()[:3], value.stride()[:3]
         qp, kp, vp = query.data_ptr(), key.data_ptr(), value.data_ptr()
     if not state.is_contiguous():

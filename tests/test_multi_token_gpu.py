@@ -35,6 +35,11 @@ def rnd(seed, *shape, dtype=F32, scale=1.0):
     return (torch.randn(shape, generator=g) * scale).to(dtype).to(DEV)
 
 
+def at_odd_offset(x):
+    """The same tensor, contiguous, three elements into its storage."""
+    return torch.cat((x.new_zeros(3), x.flatten()))[3:].view(x.shape)
+
+
 def within(got, want, bound):
     assert got.shape == want.shape
     bad = int((~torch.isfinite(got.double())).sum())
@@ -259,6 +264,7 @@ def test_tree_attention_layouts_streams_and_graphs(hq, hkv):
     within(shared[:1], want[:1], tree_bound(want, size, q, kc, 0.09, rows)[:1])  # (an expanded cache takes the other kernel)
     odd = rnd(31, b, n, hq, d + 1, dtype=BF16)[..., :d]  # rows on odd elements: copied
     assert torch.equal(ops.tree_attention(odd, kc, vc, lt, pt, 0.09), ops.tree_attention(odd.contiguous(), kc, vc, lt, pt, 0.09))
+    assert torch.equal(ops.tree_attention(at_odd_offset(q), kc, vc, lt, pt, 0.09), base)
     # two streams at once, and a captured graph whose lengths change between replays
     s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
     torch.cuda.synchronize()
@@ -498,7 +504,7 @@ def test_delta_rule_layouts_streams_and_graphs():
     odd = torch.cat([rnd(1, b, t, 1, dtype=BF16), row], -1)[..., 1:]  # rows on odd elements: copied
     cut2 = [x.unflatten(-1, (h, 128)) for x, h in zip(odd.split([hk * dk, hk * dk, hv * dv], -1), (hk, hk, hv))]
     heads_first = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v)]
-    for x in (cut, cut2, heads_first):
+    for x in (cut, cut2, heads_first, [at_odd_offset(x) for x in (q, k, v)], [q, k, at_odd_offset(v)]):
         got = ops.delta_rule_chunk(st.transpose(2, 3).contiguous().transpose(2, 3), *x, g.transpose(1, 2).contiguous().transpose(1, 2), beta, None, True)
         assert torch.equal(got[0], base[0]) and torch.equal(got[1], base[1])
     s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
