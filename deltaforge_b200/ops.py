@@ -35,6 +35,7 @@ import ctypes as C
 import functools
 import inspect
 import math
+import operator
 
 import torch
 from torch import Tensor
@@ -826,25 +827,29 @@ def _eager(op):
     """The function of a custom op, called directly where the dispatcher has nothing to add: plain tensors, no tracing or
     dispatch mode, no gradient asked for. The dispatcher's 20 us are more than the smallest of these calls takes. Everything
     else goes through the op (and meets its errors there)."""
-    run, mutated = op._init_fn, [i for i, name in enumerate(inspect.signature(op._init_fn).parameters) if name in ("key_cache", "value_cache")]
-    if not op._opoverload._schema.is_mutable:
-        mutated = []
+    run, mutates = op._init_fn, op._opoverload._schema.is_mutable
+    params = list(inspect.signature(run).parameters.values())
+    count = len(params)
+    tensors = operator.itemgetter(*(i for i, x in enumerate(params) if "Tensor" in str(x.annotation)))
+    caches = operator.itemgetter(*(i for i, x in enumerate(params) if x.name in ("key_cache", "value_cache"))) if mutates else None
 
     @functools.wraps(run)
     def call(*args, **kwargs):
-        if kwargs or _dispatch_modes() or _transforms() is not None or torch.compiler.is_compiling():
+        if kwargs or len(args) != count or _dispatch_modes() or _transforms() is not None or torch.compiler.is_compiling():
             return op(*args, **kwargs)
-        for x in args:
+        grad = torch.is_grad_enabled()
+        for x in tensors(args):
             kind = type(x)
             if kind is Tensor or kind is torch.nn.Parameter:
-                if x.requires_grad and torch.is_grad_enabled():
+                if grad and x.requires_grad:
                     return op(*args)
-            elif isinstance(x, Tensor):
+            elif x is not None:
                 return op(*args)
         out = run(*args)
-        for i in mutated:
-            if not args[i].is_inference():  # (inference tensors have no version)
-                torch.autograd.graph.increment_version(args[i])
+        if mutates:
+            for x in caches(args):
+                if not x.is_inference():  # (inference tensors have no version)
+                    torch._C._increment_version((x,))
         return out
 
     call.op = op
