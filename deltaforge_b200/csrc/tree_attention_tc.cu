@@ -558,13 +558,13 @@ __global__ void __launch_bounds__(256) tree_tc_merge_kernel(const TreeAttnParams
   }
   __syncthreads();
   const int count = count_s;
+  pdl_wait();  // by every thread, with or without work here: what follows this grid may rely on the attention grid's end
   if (count == 1 || row >= p.rows) return;  // one part: finished by the CTA that had all of it
   const int node = row / p.group, pa = p.parents[(long)b * p.parents_stride + node];
   const bool ok = pa >= -1 && pa < node;
   const long step = (long)row_tiles * TM, at = (first_s * row_tiles + row / TM) * TM + row % TM;  // rows from one part to the next
   const float2* ml = (const float2*)p.part_ml + at;
   const float* acc = p.part_acc + at * D + 4 * li;
-  pdl_wait();
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   float m = -INFINITY, l = 0.f;
   for (int s0 = 0; s0 < count; s0 += AHEAD) {

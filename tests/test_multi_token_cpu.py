@@ -219,3 +219,14 @@ def test_fake_kernels_give_shapes():
         d = {n: torch.empty(x.shape, dtype=x.dtype) if isinstance(x, torch.Tensor) else x for n, x in delta_args().items()}
         out, state = torch.ops.dfb200.delta_rule_chunk(**d)
         assert out.shape == (2, 5, 4, 24) and out.dtype == BF16 and state.shape == (2, 4, 16, 24) and state.dtype == F32
+
+
+@pytest.mark.parametrize("source,kernel", [("tree_attention.cu", "tree_merge_kernel"), ("tree_attention_tc.cu", "tree_tc_merge_kernel")])
+def test_merge_kernels_wait_before_any_return(source, kernel):
+    """They are launched while the attention grid still runs, and what follows in the stream is ordered behind them alone: a
+    thread that returned before the wait could let it read an output that is still being written."""
+    text = (_lib._build.CSRC / source).read_text()
+    body = text[text.index(f" {kernel}(const") :]
+    body = body[: body.index("\n}\n")]
+    assert body.count("pdl_wait();") == 1
+    assert "return" not in body[: body.index("pdl_wait();")]

@@ -629,3 +629,35 @@ def test_a_tree_is_verified_and_a_path_accepted():
     whole = ops.delta_rule_chunk(st, *(torch.cat((x[:, :prompt], x[:, row]), 1) for x in (dq, dkey, dval, g, beta)), None, True)[1]
     assert torch.equal(after[1], state[1])
     within(after[0], whole[0].double(), 4 * delta_state_bound(whole[0].double(), prompt + n))
+
+
+# ---------------------------------------------------------------- what follows a call in its stream
+
+
+@pytest.mark.parametrize("b,hq,hkv,d,n,rows,lens", [(16, 16, 8, 128, 17, 1500, 1400), (16, 16, 8, 64, 9, 128, 100), (9, 16, 4, 256, 5, 128, 123)])
+def test_tree_attention_has_ended_before_the_next_kernel_reads(b, hq, hkv, d, n, rows, lens):
+    """Every unit is one part here, so the merge has nothing to do. The queries change from call to call: an output read too early
+    would be that of another call. Eager and in a captured graph."""
+    kc, vc = rnd(141, b, hkv, rows, d, dtype=BF16), rnd(142, b, hkv, rows, d, dtype=BF16)
+    lt, pt = torch.full((b,), lens, dtype=I32, device=DEV), torch.tensor(random_tree(7, n), dtype=I32, device=DEV)
+    qs = [rnd(143 + i, b, n, hq, d, dtype=BF16) for i in range(3)]
+    base = []
+    for q in qs:
+        o = ops.tree_attention(q, kc, vc, lt, pt, d**-0.5)
+        torch.cuda.synchronize()
+        base.append(o.clone())
+    want, size = tree_ref(qs[0][:1], kc[:1], vc[:1], [lens], [pt.tolist()], d**-0.5)
+    within(base[0][:1], want, tree_bound(want, size, qs[0], kc, d**-0.5, rows))
+    got = []
+    for i in range(30):
+        got.append(ops.tree_attention(qs[i % 3], kc, vc, lt, pt, d**-0.5).clone())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, base[i % 3]) for i, x in enumerate(got))
+    q = qs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        copy = ops.tree_attention(q, kc, vc, lt, pt, d**-0.5).clone()
+    for i in range(9):
+        q.copy_(qs[i % 3])
+        graph.replay()
+        assert torch.equal(copy, base[i % 3])
