@@ -513,6 +513,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
       }
       if (warp < 4 && row < p.rows && !whole) *(float2*)(p.part_ml + (slot * TM + r) * 2) = ml;
     }
+    fence_async();  // the ring was written by ordinary stores (row sums, the result's rows): the next unit's copies come after them
     fence_before();
     __syncthreads();  // queries, O and the flags may be written again
     fence_after();

@@ -230,3 +230,13 @@ def test_merge_kernels_wait_before_any_return(source, kernel):
     body = body[: body.index("\n}\n")]
     assert body.count("pdl_wait();") == 1
     assert "return" not in body[: body.index("pdl_wait();")]
+
+
+def test_tree_attention_orders_its_stores_before_the_next_units_copies():
+    """A unit's end writes the ring by ordinary stores, and the next unit's copies go to the same bytes through the async proxy:
+    the writers' fence stands before the barrier that lets the loading warp go on."""
+    text = (_lib._build.CSRC / "tree_attention_tc.cu").read_text()
+    end = text.index("queries, O and the flags may be written again")
+    written = text.rindex("*(float4*)(stage", 0, end)
+    barrier = text.rindex("__syncthreads();", 0, end)
+    assert "fence_async();" in text[written:barrier]

@@ -661,3 +661,20 @@ def test_tree_attention_has_ended_before_the_next_kernel_reads(b, hq, hkv, d, n,
         q.copy_(qs[i % 3])
         graph.replay()
         assert torch.equal(copy, base[i % 3])
+
+
+@pytest.mark.parametrize("b,hq,hkv,d,n", [(40, 16, 4, 256, 6), (60, 20, 4, 128, 7), (37, 12, 6, 64, 31)])
+def test_tree_attention_of_many_ragged_units_repeats_itself(b, hq, hkv, d, n):
+    """Each CTA walks through several units of different lengths, whose copies follow the stores of the unit before."""
+    rows = 1500
+    g = torch.Generator().manual_seed(b)
+    lens = [0, 1, rows - n, 128 - n, 127] + torch.randint(0, rows - n, (b - 5,), generator=g).tolist()
+    q = rnd(151, b, n, hq, d, dtype=BF16)
+    kc, vc = rnd(152, b, hkv, rows, d, dtype=BF16), rnd(153, b, hkv, rows, d, dtype=BF16)
+    parents = [random_tree(i, n) for i in range(b)]
+    lt, pt = torch.tensor(lens, dtype=I32, device=DEV), torch.tensor(parents, dtype=I32, device=DEV)
+    base = ops.tree_attention(q, kc, vc, lt, pt, d**-0.5)
+    want, size = tree_ref(q, kc, vc, lens, parents, d**-0.5)
+    within(base, want, tree_bound(want, size, q, kc, d**-0.5, rows))
+    for _ in range(20):
+        assert torch.equal(ops.tree_attention(q, kc, vc, lt, pt, d**-0.5), base)
