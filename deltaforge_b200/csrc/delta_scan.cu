@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   constexpr int NS = DKP / 4;  // key rows per thread
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  __shared__ uint64_t full[2], v_full, v_in, s_in[2], tv_out, ws_out, u_in, p_in, u_out[2], o_out[2], o_read;
+  __shared__ uint64_t full[2], v_full, v_in, s_in[2], tv_out, ws_out, u_in, p_in, u_out[2], o_out[2], o_read, drained;
   __shared__ float s_max[4][COLS], vp_max[4][COLS];
   __shared__ int s_exp[2][COLS], v_exp[2][COLS];  // by chunk parity, for the output
   __shared__ uint32_t tmem_slot;
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   if (t == 0) {
     for (int i = 0; i < 2; ++i) mbar_init(&full[i], 1), mbar_init(&s_in[i], 16), mbar_init(&u_out[i], 1), mbar_init(&o_out[i], 1);
     mbar_init(&v_full, 1), mbar_init(&v_in, 1), mbar_init(&tv_out, 1), mbar_init(&ws_out, 1);
-    mbar_init(&u_in, 16), mbar_init(&p_in, 16), mbar_init(&o_read, 4);
+    mbar_init(&u_in, 16), mbar_init(&p_in, 16), mbar_init(&o_read, 4), mbar_init(&drained, 1);
     failed_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -326,6 +326,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
     pdl_wait();
     pdl_launch_dependents();  // the preparation of the next segment may run beside this scan, but not beside the one before
     const long per = p.hk * (long)key_bytes(DKP) + p.hv * (long)head_bytes(DKP);
+    int sent = 0, v_sent = 0;  // chunks and values asked for
     for (int n = 0; n < nlive; ++n) {
       // the products of chunk n - 2 are done; they came after the output of chunk n - 3, whose scalars are replaced
       if (n >= 2) ok = wait_for(&o_out[n & 1], ((n >> 1) - 1) & 1, failed) && ok;
@@ -343,6 +344,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
         bulk_copy(smem_u32(scn), head + 4 * SQ + 2 * w_bytes(DKP), SCAL, bar);
       }
       __syncwarp();
+      sent = n + 1;
       if (n > 0) ok = wait_for(&tv_out, (n - 1) & 1, failed) && ok;
       if (!__all_sync(0xffffffffu, ok)) break;
       if (elect_one()) {
@@ -352,6 +354,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
           tma_box(smem_u32(sm + G::V + i * C * 128), &vmap, u.vb * COLS + 64 * i, u.hv, TREE ? 0 : (p.chunk0 + n) * C, u.b, &v_full);
       }
       __syncwarp();
+      v_sent = n + 1;
       // values of tokens that do not count may be anything: zeros take their place
       ok = wait_for(&full[n & 1], (n >> 1) & 1, failed) && ok;
       ok = wait_for(&v_full, n & 1, failed) && ok;
@@ -370,6 +373,10 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&v_in);
+    }
+    if (!__all_sync(0xffffffffu, ok)) {  // a wait ran out (else all that was asked for has been waited for)
+      for (int n = max(sent - 2, 0); n < sent; ++n) wait_out(&full[n & 1], (n >> 1) & 1);
+      if (v_sent > 0) wait_out(&v_full, (v_sent - 1) & 1);
     }
   } else {
     // ---------------- products ----------------
@@ -445,6 +452,13 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   }
   fence_before();
   __syncthreads();
+  if (*failed) {  // products that are still under way end before their memory is given back
+    if (warp == 21 && elect_one()) {
+      commit(&drained);
+      wait_out(&drained, 0);
+    }
+    __syncthreads();
+  }
   if (warp == 21) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
 }
 

@@ -52,6 +52,12 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatil
     }
   }
 }
+// The same after a failure, for what the CTA has under way itself: bounded, whatever the flag says.
+__device__ __forceinline__ void wait_out(uint64_t* bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity))
+    if (clock64() - t0 > WAIT_CYCLES) return;
+}
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int dim, int key, int head, int seq, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),

@@ -25,7 +25,8 @@
 // 74 cycles, but O, two S and Q are 640 columns; with tiles of 64 keys it was slower.) Run back to back for seconds, that case
 // draws 1000 W, the clock falls from 1965 to 1380 MHz and the call takes 240 us.
 //
-// Every wait is bounded; one that runs out makes the CTA leave NaN.
+// Every wait is bounded; one that runs out makes the CTA leave NaN, wait (again with a limit) for its own copies and products, and
+// return.
 #include <cuda.h>
 
 #include "common.cuh"
@@ -112,13 +113,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   unsigned char* ring = sm + S_::Q_BYTES;
-  __shared__ uint64_t full[S_::RING], freed[S_::RING], s_full[2], p_full[2], pv_done[2], at_tree, v_fixed;
+  __shared__ uint64_t full[S_::RING], freed[S_::RING], s_full[2], p_full[2], pv_done[2], at_tree, v_fixed, drained;
   __shared__ bf16 part_m[2][2][TM];  // by turns: the largest score of each half of a row, rounded (any reference will do, if both use the same)
   float *row_l = (float*)(ring + 40960), *row_m = row_l + 2 * TM;  // at a unit's end, when the ring is idle: [2][TM] sums, [TM] maxima
   __shared__ unsigned long long anc[MAX_TREE_NODES];
   __shared__ unsigned char up[MAX_TREE_NODES];
   __shared__ uint32_t tmem_slot;
-  __shared__ int failed_s, odd_s, where[5];
+  __shared__ int failed_s, odd_s, where[5], sent_s;  // sent_s: ring pieces asked for
   volatile int* failed = &failed_s;
 
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
@@ -127,7 +128,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 8), mbar_init(&pv_done[i], 1);
     mbar_init(&at_tree, 8);
     mbar_init(&v_fixed, 2);
-    failed_s = 0;
+    mbar_init(&drained, 1);
+    failed_s = sent_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -246,7 +248,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
         auto slot = [&]() {  // the next slot, once it is free
           const int s = c % S_::RING;
           if (c >= S_::RING) ok = ok && wait_for(&freed[s], (c / S_::RING - 1) & 1, failed);
-          if (ok) mbar_expect_tx(&full[s], S_::PIECE);
+          if (ok) mbar_expect_tx(&full[s], S_::PIECE), sent_s = c + 1;
           ++c;
           return s;
         };
@@ -525,6 +527,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     if (tile == tiles) {
       tile = 0;
       if (++unit == upb) unit = 0, ++b;
+    }
+  }
+  if (*failed) {  // a wait ran out: what is still under way ends before its memory is given back
+    if (warp == 0 && elect_one()) {
+      for (int c = max(sent_s - S_::RING, 0); c < sent_s; ++c) wait_out(&full[c % S_::RING], (c / S_::RING) & 1);
+    }
+    if (warp == 1 && elect_one()) {
+      commit(&drained);
+      wait_out(&drained, 0);
     }
   }
   __syncthreads();

@@ -240,3 +240,15 @@ def test_tree_attention_orders_its_stores_before_the_next_units_copies():
     written = text.rindex("*(float4*)(stage", 0, end)
     barrier = text.rindex("__syncthreads();", 0, end)
     assert "fence_async();" in text[written:barrier]
+
+
+@pytest.mark.parametrize("source,kernel", [("tree_attention_tc.cu", "tree_attention_tc_kernel"), ("delta_scan.cu", "delta_scan_kernel")])
+def test_a_wait_that_ran_out_leaves_nothing_under_way(source, kernel):
+    """Copies into shared memory and products in tensor memory that a kernel has started end before it gives that memory back."""
+    text = (_lib._build.CSRC / source).read_text()
+    body = text[text.index(f" {kernel}(const") :]
+    body = body[: body.index("\n}\n")]
+    assert "wait_out(&full[" in body
+    end = body[body.rindex("if (*failed)") : body.index("tcgen05.dealloc")]
+    assert "commit(&drained);" in end and "wait_out(&drained, 0);" in end
+    assert "__syncthreads();" in end[end.index("wait_out(&drained") :]
