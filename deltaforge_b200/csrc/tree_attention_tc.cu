@@ -114,7 +114,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
   unsigned char* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   unsigned char* ring = sm + S_::Q_BYTES;
   __shared__ uint64_t full[S_::RING], freed[S_::RING], s_full[2], p_full[2], pv_done[2], at_tree, v_fixed, drained;
-  __shared__ bf16 part_m[2][2][TM];  // by turns: the largest score of each half of a row, rounded (any reference will do, if both use the same)
+  // The largest score of each half of a row, in fp32: it is the reference of the exponentials, and rounded to eight bits it was off by
+  // 16 at a score of 4096, which is the whole range of an fp16 probability.
+  __shared__ float part_m[2][TM];
   float *row_l = (float*)(ring + 40960), *row_m = row_l + 2 * TM;  // at a unit's end, when the ring is idle: [2][TM] sums, [TM] maxima
   __shared__ unsigned long long anc[MAX_TREE_NODES];
   __shared__ unsigned char up[MAX_TREE_NODES];
@@ -362,8 +364,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
 #pragma unroll
         for (int x = 0; x < 64; ++x) m4[x & 3] = fmaxf(m4[x & 3], __uint_as_float(v[x]));
         float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl;
-        const bf16 mine = f2bf(top);
-        part_m[gi & 1][half][r] = mine;
+        asm volatile("bar.sync %0, 64;" ::"r"(4 + (warp & 3)) : "memory");  // the tile before's have been read
+        part_m[half][r] = top;
         {  // the two warps of these rows meet: both have read S, and both go on or both give up
           uint32_t go;
           asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
@@ -373,7 +375,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
           ok = go != 0;
         }
         if (!ok) break;
-        top = fmaxf(bf2f(mine), bf2f(part_m[gi & 1][half ^ 1][r]));
+        top = fmaxf(top, part_m[half ^ 1][r]);
         if (i == 0) {
           mref = top;
         } else {

@@ -678,3 +678,28 @@ def test_tree_attention_of_many_ragged_units_repeats_itself(b, hq, hkv, d, n):
     within(base, want, tree_bound(want, size, q, kc, d**-0.5, rows))
     for _ in range(20):
         assert torch.equal(ops.tree_attention(q, kc, vc, lt, pt, d**-0.5), base)
+
+
+# ---------------------------------------------------------------- scores of any size
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("b,hq,hkv,n,d", [(2, 4, 2, 5, 64), (2, 40, 20, 30, 64), (3, 4, 2, 40, 256), (8, 16, 4, 17, 256)])
+@pytest.mark.parametrize("size_of_scores", [2850, 5710, 10_000, 23_000, 100_000, -2870, -5700, -23_000, -100_000])
+def test_tree_attention_with_large_scores(size_of_scores, b, hq, hkv, n, d, dtype):
+    """All scores lie near one large number, whose place against a coarse grid must not matter; differences between them are
+    ordinary. Queries and keys are whole numbers, so that every score is exact in fp32; what remains of the error ds of
+    `tree_bound` is scale log2(e) (two roundings), its product with the score and the difference to the maximum: 4 h(fp32) |score|."""
+    rows, scale = 700, 0.25
+    g = torch.Generator().manual_seed(n)
+    q = torch.randint(-2, 3, (b, n, hq, d), generator=g).to(dtype).to(DEV)
+    kc = torch.randint(-1, 2, (b, hkv, rows, d), generator=g).to(dtype).to(DEV)
+    vc = rnd(161, b, hkv, rows, d, dtype=dtype)
+    q[..., 0], kc[..., 0] = 256, round(size_of_scores / (256 * scale))
+    q[..., 1], kc[..., 1] = 8, (torch.arange(rows, device=DEV) // 128 - 3).to(dtype)  # the maximum moves from tile to tile
+    lens = [rows - n] + [int(torch.randint(0, rows - n, (1,), generator=g)) for _ in range(b - 1)]
+    parents = [random_tree(i, n) for i in range(b)]
+    want, size = tree_ref(q, kc, vc, lens, parents, scale)
+    got = ops.tree_attention(q, kc, vc, torch.tensor(lens, dtype=I32, device=DEV), torch.tensor(parents, dtype=I32, device=DEV), scale)
+    ds = 4 * half(F32) * (abs(size_of_scores) * 1.01 + 1000)
+    within(got, want, half(dtype) * want.abs() + (half(dtype) + 2 * ds + 2**-20 + rows * 2**-24) * size * (1 + 2**-6))
