@@ -18,7 +18,11 @@
 // row, for the nodes that do see them (no cost when there are none but the look itself).
 //
 // Rounding: q, k, v as they are; scores, maximum, sum and accumulators in fp32; probabilities are rounded to the cache's
-// type for the second product (relative 2^-9 each in bf16, of random sign), the sum takes them unrounded.
+// type for the second product (relative 2^-9 each in bf16, of random sign), the sum takes them unrounded. fp16 has five bits of
+// exponent: relative to the largest of a row, probabilities below 2^-14 would lose bits there and those below 2^-25 vanish, and
+// behind one dominant key (an attention sink) they are the output. So for fp16 the reference of the exponentials lies 2^15 below
+// the maximum; sums and accumulators refer to it alike, and the factor goes out in the division. 17 e-folds below the
+// dominant key the output was off by 7 %.
 //
 // A row without a node (parent below -1 or not before the node) gets zeros, and so does one that sees no key: without a
 // prefix, of a tree that reaches past the cache. Splits leave (m, l, acc) in scratch and
@@ -81,6 +85,11 @@ template <> __device__ __forceinline__ float elem_f(bf16 v) { return __bfloat162
 template <> __device__ __forceinline__ float elem_f(__half v) { return __half2float(v); }
 template <typename T> __device__ __forceinline__ uint16_t exp_mask() { return 0x7f80; }  // all ones: infinity or NaN
 template <> __device__ __forceinline__ uint16_t exp_mask<__half>() { return 0x7c00; }
+
+// How far the reference of the exponentials lies below the maximum, in powers of two: probabilities are at most 2^this. The
+// subtraction rounds upwards, which keeps that true for scores of any size.
+template <typename T> __device__ __forceinline__ float headroom() { return 0.f; }
+template <> __device__ __forceinline__ float headroom<__half>() { return 15.f; }
 
 // One row of a tile is D elements; its 16-byte chunks are permuted within 128-byte lines so that the eight rows an 8x8
 // matrix load touches lie in different banks.
@@ -305,7 +314,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_attention_kernel(const Tre
       for (int nt = 0; nt < TK / 8; ++nt) mx = fmaxf(mx, fmaxf(s[nt][2 * r], s[nt][2 * r + 1]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mn = fmaxf(mrun[r], mx);
+      const float mn = fmaxf(mrun[r], __fadd_ru(mx, -headroom<T>()));
       const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: every probability is 2^-inf = 0
       corr[r] = exp2_fast(mrun[r] - ref);
       float sum = 0.f;

@@ -16,8 +16,8 @@
 // Roles: warp 0 loads (TMA boxes 64 dims wide, 128-byte swizzle; a ring of K and V pieces), warp 1 issues the products, warps
 // 2 and 3 look after values that must not meet a zero probability, warps 4-11 have two threads per row, half of a tile's
 // keys each: scores out of TMEM, masks, maximum, exponentials, P into the columns of S. The product of tile i + 1 runs under
-// the softmax of tile i. The maximum that P refers to is moved only when a row's true maximum is more than 2^8 above it,
-// so that O rarely has to be rescaled; sums stay exact because l refers to the same maximum.
+// the softmax of tile i. The maximum that P refers to is moved only when a row's true maximum is more than 2^8 (fp16: 2^4) above
+// it, so that O rarely has to be rescaled; sums stay exact because l refers to the same maximum.
 //
 // Bounds per tile of 128 keys at head dim 256: 1024 cycles of ex2, 128 KB of K and V from the L2, and of tensor time 16 products
 // Q K^T with both operands in shared memory (104 cycles each, measured, where the arithmetic takes 64) and 8 products P V with
@@ -41,7 +41,13 @@ constexpr int TM = 128;          // query rows per tile
 constexpr int TN = 128;          // keys per tile
 constexpr int TC_WARPS = 12, TC_THREADS = TC_WARPS * 32;
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LAZY = 8.f;      // rescale O when the maximum has grown by more than this (in powers of two)
+
+// In powers of two: how far the reference of the exponentials lies below the maximum it was taken from, and by how much the
+// maximum may grow before O is rescaled. Probabilities are at most 2^(HEADROOM + LAZY): for fp16, 2^15, so that its five bits of
+// exponent begin at 2^-25 of the largest and not at 2^-14 (see tree_attention.cu). Roundings go the way that keeps this true for
+// scores of any size.
+template <typename T> struct Range { static constexpr float HEADROOM = 0.f, LAZY = 8.f; };
+template <> struct Range<__half> { static constexpr float HEADROOM = 11.f, LAZY = 4.f; };
 
 template <int D> struct Tc {
   static constexpr int BLOCKS = D / 64;                          // 64-dim blocks of a row
@@ -363,7 +369,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int x = 0; x < 64; ++x) m4[x & 3] = fmaxf(m4[x & 3], __uint_as_float(v[x]));
-        float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl;
+        float top = __fmul_ru(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), sl);
         asm volatile("bar.sync %0, 64;" ::"r"(4 + (warp & 3)) : "memory");  // the tile before's have been read
         part_m[half][r] = top;
         {  // the two warps of these rows meet: both have read S, and both go on or both give up
@@ -375,11 +381,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
           ok = go != 0;
         }
         if (!ok) break;
-        top = fmaxf(top, part_m[half ^ 1][r]);
+        top = __fadd_ru(fmaxf(top, part_m[half ^ 1][r]), -Range<T>::HEADROOM);
         if (i == 0) {
           mref = top;
         } else {
-          const bool move = top > mref + LAZY;
+          const bool move = top > __fadd_rd(mref, Range<T>::LAZY);
           if (__any_sync(0xffffffffu, move)) {  // (the same in both warps)
             ok = wait_for(&pv_done[(gi - 1) & 1], ((gi - 1) >> 1) & 1, failed);
             fence_after();

@@ -703,3 +703,22 @@ def test_tree_attention_with_large_scores(size_of_scores, b, hq, hkv, n, d, dtyp
     got = ops.tree_attention(q, kc, vc, torch.tensor(lens, dtype=I32, device=DEV), torch.tensor(parents, dtype=I32, device=DEV), scale)
     ds = 4 * half(F32) * (abs(size_of_scores) * 1.01 + 1000)
     within(got, want, half(dtype) * want.abs() + (half(dtype) + 2 * ds + 2**-20 + rows * 2**-24) * size * (1 + 2**-6))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("b,hq,hkv,n,d", [(2, 4, 2, 5, 64), (2, 40, 20, 30, 64), (1, 8, 2, 12, 256), (8, 16, 4, 17, 256)])
+@pytest.mark.parametrize("gap", [9.0, 14.0, 17.0])
+def test_tree_attention_behind_one_dominant_key(gap, b, hq, hkv, n, d, dtype):
+    """One key takes nearly all of the weight and has a value of zero (an attention sink): the output is the sum over the others,
+    whose probabilities lie e^-gap below the largest one, in fp16's subnormal range if they were held relative to it."""
+    rows = 3000
+    q, kc = torch.zeros(b, n, hq, d, dtype=dtype, device=DEV), torch.zeros(b, hkv, rows, d, dtype=dtype, device=DEV)
+    q[..., 3], kc[:, :, 1, 3] = 1.0, gap
+    kc[..., 5], q[..., 5] = rnd(171, b, hkv, rows, dtype=dtype), 0.25
+    kc[:, :, 1, 5] = 0.0
+    vc = rnd(172, b, hkv, rows, d, dtype=dtype, scale=64.0) + 64.0
+    vc[:, :, 1] = 0.0
+    lens, parents = [rows - n] * b, [random_tree(i, n) for i in range(b)]
+    want, size = tree_ref(q, kc, vc, lens, parents, 1.0)
+    got = ops.tree_attention(q, kc, vc, torch.tensor(lens, dtype=I32, device=DEV), torch.tensor(parents, dtype=I32, device=DEV), 1.0)
+    within(got, want, tree_bound(want, size, q, kc, 1.0, rows))
