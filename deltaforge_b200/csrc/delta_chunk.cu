@@ -14,6 +14,8 @@
 // 2e-3 per product. Products with S or V' take fp16 operands (11 bits), scaled by powers of two to the top of fp16's range
 // (per token for k and q, which are bf16 and stay exact; per 16 rows for W, P; per value column for S, V'), and S, W and V'
 // are split in two, hi + lo = 22 bits, wherever the product leads into the state: hi hi + hi lo + lo hi, fp32 accumulation.
+// (The update's V' are scaled by the larger of the two halves of a chunk, each its largest V' times its largest weight: values
+// 2^13 times above what the half leaves in the state begin to cost the update bits.)
 // Products that lead into the bf16 output alone take hi (2^-12). T V is a product of bf16: the values as they are, T in three
 // parts (24 bits); so is W, the left factor in three parts and the keys as they are. The state's update is accumulated apart
 // and added in fp32 (the tensor core truncates what it adds to a large accumulator). Log decays are summed in fp64 and kept as

@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ uint64_t full[2], v_full, v_in, s_in[2], tv_out, ws_out, u_in, p_in, u_out[2], o_out[2], o_read, drained;
-  __shared__ float s_max[4][COLS], vp_max[4][COLS];
+  __shared__ float s_max[4][COLS], vp_max[4][COLS], r_max[4][COLS];  // of S, V', and the images of V' on their way into S
   __shared__ int s_exp[2][COLS], v_exp[2][COLS];  // by chunk parity, for the output
   __shared__ uint32_t tmem_slot;
   __shared__ int failed_s, seq_s;
@@ -193,9 +193,10 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       const float wscale = pow2(es) * sc[2 * C + 4 + h], decay = sc[2 * C];  // W is scaled per 16 rows
       ok = wait_for(&tv_out, n & 1, failed) && ok;
       fence_after();
-      float uup, both;
+      float uup;
+      uint32_t hi[8];
       {
-        uint32_t x[16], hi[8], lo[8];
+        uint32_t x[16], lo[8];
         tmem_ld16(base + TV + 16 * h, x);
         tmem_wait_ld16(x);
         ok = wait_for(&ws_out, n & 1, failed) && ok;
@@ -215,9 +216,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
         }
         vp_max[h][col] = fmaxf(m0, m1);
         meet();
-        both = most(s_max);
         const float m = most(vp_max);
-        const int ev = scale_exp(m), eu = scale_exp(m * fmaxf(sc[2 * C + 12], sc[2 * C + 13]));
+        const int ev = scale_exp(m), eu = scale_exp(fmaxf(fmaxf(vp_max[0][col], vp_max[1][col]) * sc[2 * C + 12], fmaxf(vp_max[2][col], vp_max[3][col]) * sc[2 * C + 13]));
         if (h == 0) v_exp[n & 1][col] = ev;
         uup = pow2(eu);
         const float a = pow2(-ev), u = pow2(-eu);
@@ -245,6 +245,19 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
         mbar_arrive(&p_in);
       }
       if (TREE) continue;
+      {
+        __half2 top = __habs2(*(const __half2*)&hi[0]);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) top = __hmax2(top, __habs2(*(const __half2*)&hi[i]));
+        r_max[h][col] = fmaxf(__low2float(top), __high2float(top));
+        // The next S is at most decay |S| + |U|, and U is a sum of 64 products of an image of V', as large as these really are, with one
+        // of K, at most 2^13. (An update may be nothing at all, or its largest values forgotten within the chunk: a bound from
+        // 2^13, or from a scale that stands for "nothing", pushes S down into fp16's subnormal numbers. Found out here, under the
+        // products, it costs nothing; a maximum of V' times its weight per token before them cost 20 to 30 of 382 us.)
+        const float both = most(s_max);
+        meet();
+        es = scale_exp(fmaf(both, fabsf(decay), uup * most(r_max) * (64.f * 8192.f)));
+      }
 
       // S: the update was accumulated apart and is added in fp32
       ok = wait_for(&u_out[h >> 1], n & 1, failed) && ok;
@@ -258,8 +271,6 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
         for (int i = 0; i < 8; ++i)
           S[x / 2 + i] = fma2({__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])}, {uup, uup}, mul2(S[x / 2 + i], {decay, decay}));
       }
-      // the next S is at most decay |S| + |U|, the images of V' and K being at most 2^13 each
-      es = scale_exp(fmaf(both, fabsf(decay), uup * (64.f * 67108864.f)));
     }
     if (!TREE) {
       float* So = p.state_out + sb;

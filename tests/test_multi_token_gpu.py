@@ -722,3 +722,43 @@ def test_tree_attention_behind_one_dominant_key(gap, b, hq, hkv, n, d, dtype):
     want, size = tree_ref(q, kc, vc, lens, parents, 1.0)
     got = ops.tree_attention(q, kc, vc, torch.tensor(lens, dtype=I32, device=DEV), torch.tensor(parents, dtype=I32, device=DEV), 1.0)
     within(got, want, tree_bound(want, size, q, kc, 1.0, rows))
+
+
+# ---------------------------------------------------------------- chunks whose update is nothing, or small beside a bound on it
+
+
+@pytest.mark.parametrize("l2norm", [False, True])
+@pytest.mark.parametrize("dk,dv,hv", [(128, 128, 4), (64, 40, 2)])
+@pytest.mark.parametrize("kind", ["beta 0", "keys and values 0", "beta 0 and no decay", "forgotten", "forgotten by all", "small"])
+def test_delta_rule_state_after_a_chunk_that_adds_little(kind, dk, dv, hv, l2norm):
+    """The state's scale in the next chunk follows from a bound on this chunk's update. Tokens 64 .. 127 add nothing at all, or the
+    largest values of theirs are forgotten within the chunk, or are far below the state."""
+    t = 260
+    st, q, k, v, g, beta = delta_inputs(181, 1, t, 2, hv, dk, dv, l2norm)
+    mid = slice(64, 128)
+    if kind.startswith("beta 0"):
+        beta[:, mid] = 0.0
+        if kind != "beta 0":
+            g[:, mid] = 0.0
+    elif kind == "keys and values 0":
+        k[:, mid], v[:, mid] = 0.0, 0.0
+    elif kind == "small":
+        v[:, mid] *= 2.0**-40
+        st, beta[:, 64:65] = st * 0.0, 1.0
+        v[:, :64] *= 2.0**-40
+    else:
+        v[:, 64:68] *= 2.0**18
+        g[:, 70] = -40.0  # e^-40 of 2^18 is 1e-12
+        if kind == "forgotten by all":
+            g[:, 127] = -60.0
+    want, size, s = delta_ref(st, q, k, v, g, beta, None, l2norm)
+    out, state = ops.delta_rule_chunk(st, q, k, v, g, beta, None, l2norm)
+    within(out, want, delta_out_bound(want, size))
+    within(state, s, delta_state_bound(s, t))
+    # the outputs of the chunk behind it hold to the bound of the state, up to their own rounding to 11 and 8 bits; with a query that
+    # reads the state alone (beta 0 from there on) no product of new terms covers an error of it
+    beta[:, 128:], g[:, 128:] = 0.0, 0.0
+    want, size, s = delta_ref(st, q, k, v, g, beta, None, l2norm)
+    out, state = ops.delta_rule_chunk(st, q, k, v, g, beta, None, l2norm)
+    within(out, want, delta_out_bound(want, size))
+    within(state, s, delta_state_bound(s, t))
