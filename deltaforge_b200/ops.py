@@ -813,7 +813,8 @@ _DTYPES = {BF16: 0, torch.float16: 1, torch.float32: 2}
 _ROTARY, _TREE, _DELTA = (_lib.packer(d) for d in (_lib.RotaryDesc, _lib.TreeAttnDesc, _lib.DeltaChunkDesc))
 
 
-_dispatch_modes, _transforms = torch._C._len_torch_dispatch_stack, torch._C._functorch.peek_interpreter_stack
+_dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+_transforms, _tracing = torch._C._functorch.peek_interpreter_stack, torch._C._is_tracing
 _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
@@ -824,32 +825,46 @@ def _scratch_bytes(query: str, *sizes: int) -> int:
 
 
 def _eager(op):
-    """The function of a custom op, called directly where the dispatcher has nothing to add: plain tensors, no tracing or
-    dispatch mode, no gradient asked for. The dispatcher's 20 us are more than the smallest of these calls takes. Everything
-    else goes through the op (and meets its errors there)."""
+    """The function of a custom op, called directly where the dispatcher has nothing to add: plain tensors whose memory holds
+    their values, nothing that compiles, traces or transforms, no dispatch or function mode, no gradient asked for. The
+    dispatcher's 20 us are more than the smallest of these calls takes. Everything else goes through the op (and meets its
+    errors there)."""
     run, mutates = op._init_fn, op._opoverload._schema.is_mutable
     params = list(inspect.signature(run).parameters.values())
     count = len(params)
-    tensors = operator.itemgetter(*(i for i, x in enumerate(params) if "Tensor" in str(x.annotation)))
+    # activations, states and caches; and whole numbers, which have no gradients and no negative views
+    counts = ("positions", "cache_len", "parents", "lengths")
+    tensors = [i for i, x in enumerate(params) if "Tensor" in str(x.annotation)]
+    values = operator.itemgetter(*(i for i in tensors if params[i].name not in counts))
+    numbers = tuple(i for i in tensors if params[i].name in counts)
     caches = operator.itemgetter(*(i for i, x in enumerate(params) if x.name in ("key_cache", "value_cache"))) if mutates else None
 
     @functools.wraps(run)
     def call(*args, **kwargs):
-        if kwargs or len(args) != count or _dispatch_modes() or _transforms() is not None or torch.compiler.is_compiling():
+        # (compiling first: the compiler follows this function, and stops at the other questions)
+        if torch.compiler.is_dynamo_compiling() or kwargs or len(args) != count:
             return op(*args, **kwargs)
+        if _dispatch_modes() or _function_modes() or _transforms() is not None or _tracing():
+            return op(*args)
         grad = torch.is_grad_enabled()
-        for x in tensors(args):
+        for x in values(args):
             kind = type(x)
-            if kind is Tensor or kind is torch.nn.Parameter:
-                if grad and x.requires_grad:
-                    return op(*args)
-            elif x is not None:
+            if kind is not Tensor and kind is not torch.nn.Parameter:
                 return op(*args)
+            if x.is_neg() or (grad and x.requires_grad):  # (a negative view's memory holds the opposite of its values)
+                return op(*args)
+        for i in numbers:
+            x = args[i]
+            if type(x) is not Tensor and x is not None:
+                return op(*args)
+        if args[0].is_meta:
+            return op(*args)
         out = run(*args)
         if mutates:
-            for x in caches(args):
-                if not x.is_inference():  # (inference tensors have no version)
-                    torch._C._increment_version((x,))
+            written = caches(args)
+            if written[0].is_inference() or written[1].is_inference():  # (inference tensors have no version)
+                written = tuple(x for x in written if not x.is_inference())
+            torch._C._increment_version(written)
         return out
 
     call.op = op

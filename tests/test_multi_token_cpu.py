@@ -252,3 +252,120 @@ def test_a_wait_that_ran_out_leaves_nothing_under_way(source, kernel):
     end = body[body.rindex("if (*failed)") : body.index("tcgen05.dealloc")]
     assert "commit(&drained);" in end and "wait_out(&drained, 0);" in end
     assert "__syncthreads();" in end[end.index("wait_out(&drained") :]
+
+
+# ---------------------------------------------------------------- the wrapper that passes the dispatcher by
+
+
+def _read(x):
+    import ctypes
+
+    return list((ctypes.c_float * x.numel()).from_address(x.data_ptr()))
+
+
+@ops._eager
+@torch.library.custom_op("dfb200_test::weighted", mutates_args=())
+def weighted(query: torch.Tensor, key: torch.Tensor, factor: float, lengths: torch.Tensor | None) -> torch.Tensor:
+    """An op under the wrapper that runs here, and that like those of the package reads memory."""
+    return torch.tensor([factor * a + b for a, b in zip(_read(query), _read(key))]).view(query.shape)
+
+
+@weighted.op.register_fake
+def _(query, key, factor, lengths):
+    return query.new_empty(query.shape)
+
+
+@ops._eager
+@torch.library.custom_op("dfb200_test::append_one", mutates_args=("key_cache", "value_cache"))
+def append_one(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor) -> torch.Tensor:
+    key_cache.data.add_(1.0)  # (past the version counter, as a kernel writes)
+    value_cache.data.add_(1.0)
+    return query.clone()
+
+
+@append_one.op.register_fake
+def _(query, key_cache, value_cache):
+    return query.new_empty(query.shape)
+
+
+def call_weighted(a, b):
+    return weighted(a, b, 2.0, None)
+
+
+def pair(seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(3, 4, generator=g), torch.randn(3, 4, generator=g)
+
+
+def test_wrapper_calls_the_function_itself_for_plain_tensors(monkeypatch):
+    a, b = pair()
+    with monkeypatch.context() as m:  # the op is not called
+        m.setattr(type(weighted.op), "__call__", lambda *x: pytest.fail("went through the dispatcher"))
+        assert torch.equal(call_weighted(a, b), 2 * a + b)
+        assert torch.equal(weighted(torch.nn.Parameter(a, requires_grad=False), b, 2.0, None), 2 * a + b)
+        with torch.no_grad():
+            assert torch.equal(weighted(a.clone().requires_grad_(), b, 2.0, None), 2 * a + b)
+    assert torch.equal(weighted(a, key=b, factor=2.0, lengths=None), 2 * a + b)
+
+
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
+def test_wrapper_under_a_jit_trace():
+    a, b = pair()
+    traced = torch.jit.trace(call_weighted, (a, b))
+    a, b = pair(1)
+    assert torch.equal(traced(a, b), 2 * a + b)
+    assert "dfb200_test::weighted" in str(traced.graph)
+
+
+def test_wrapper_under_compilation():
+    a, b = pair()
+    compiled = torch.compile(call_weighted, fullgraph=True, backend="eager")
+    assert torch.equal(compiled(a, b), 2 * a + b)
+
+
+def test_wrapper_sees_negative_views():
+    a, b = pair()
+    for x, y in ((torch._neg_view(a), b), (a, torch._neg_view(b)), (torch.complex(b, a).conj().imag.view(-1)[:1], b[0, :1])):
+        assert x.is_neg() or y.is_neg()
+        assert torch.equal(call_weighted(x, y), 2 * x + y)
+
+
+def test_wrapper_under_a_function_mode():
+    class Seen(torch.overrides.TorchFunctionMode):
+        def __init__(self):
+            super().__init__()
+            self.names = []
+
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            self.names.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    a, b = pair()
+    with Seen() as seen:
+        out = call_weighted(a, b)
+    assert torch.equal(out, 2 * a + b) and any("weighted" in x for x in seen.names)
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_wrapper_under_vmap_and_with_gradients_meta_and_fake_tensors():
+    a, b = pair()
+    assert torch.equal(torch.func.vmap(call_weighted)(a, b), 2 * a + b)
+    x = a.clone().requires_grad_()
+    y = call_weighted(x, b)
+    assert y.requires_grad and y.grad_fn is not None  # the op: it says at the backward pass that it has none
+    with pytest.raises(Exception, match="autograd|backward|Autograd"):
+        y.sum().backward()
+    assert call_weighted(a.to("meta"), b.to("meta")).is_meta
+    with torch._subclasses.fake_tensor.FakeTensorMode() as mode:
+        assert call_weighted(mode.from_tensor(a), mode.from_tensor(b)).shape == a.shape
+
+
+def test_wrapper_moves_the_version_counters_of_what_an_op_writes():
+    q, kc, vc = torch.zeros(2), torch.zeros(3), torch.zeros(3)
+    for n in range(1, 4):
+        append_one(q, kc, vc)
+        assert kc._version == vc._version == n and q._version == 0 and kc[0] == n
+    with torch.inference_mode():
+        inner = torch.zeros(3)
+        append_one(q, kc, inner)  # (an inference tensor has no version)
+    assert kc._version == 4 and inner[0] == 1

@@ -762,3 +762,56 @@ def test_delta_rule_state_after_a_chunk_that_adds_little(kind, dk, dv, hv, l2nor
     out, state = ops.delta_rule_chunk(st, q, k, v, g, beta, None, l2norm)
     within(out, want, delta_out_bound(want, size))
     within(state, s, delta_state_bound(s, t))
+
+
+# ---------------------------------------------------------------- the ops as a compiled, traced or plain call
+
+
+def small_calls():
+    """(name, function of its tensors alone, tensors) of each of the five ops"""
+    b, t, hq, hkv, d = 2, 5, 4, 2, 64
+    q, k, v = rnd(191, b, t, hq, d, dtype=BF16), rnd(192, b, t, hkv, d, dtype=BF16), rnd(193, b, t, hkv, d, dtype=BF16)
+    kc, vc = rnd(194, b, hkv, 40, d, dtype=BF16), rnd(195, b, hkv, 40, d, dtype=BF16)
+    pos = torch.arange(b * t, dtype=I32, device=DEV).view(b, t)
+    inv, factor = ops.rope_frequencies(32, 1e4)
+    lens, parents = torch.tensor([30, 7], dtype=I32, device=DEV), torch.tensor(random_tree(2, t), dtype=I32, device=DEV)
+    st, dq, dk, dv, g, beta = delta_inputs(196, b, t, 2, 4, 64, 32, True)
+    return [
+        ("rotary_qk", lambda q, k, pos, inv: ops.rotary_qk(q, k, pos, inv, factor, True), (q, k, pos, inv)),
+        ("rotary_append", lambda q, k, v, pos, inv, kc, vc, n: (ops.rotary_append(q, k, v, pos, inv, factor, False, kc, vc, n), kc, vc), (q, k, v, pos, inv, kc, vc, lens)),
+        ("tree_attention", lambda q, kc, vc, n, p: ops.tree_attention(q, kc, vc, n, p, 0.125), (q, kc, vc, lens, parents)),
+        ("delta_rule_chunk", lambda s, q, k, v, g, b: ops.delta_rule_chunk(s, q, k, v, g, b, None, True), (st, dq, dk, dv, g, beta)),
+        ("delta_rule_tree", lambda s, q, k, v, g, b, p: ops.delta_rule_tree(s, q, k, v, g, b, p, True), (st, dq, dk, dv, g, beta, parents)),
+    ]
+
+
+def same(x, y):
+    x, y = (z if isinstance(z, tuple) else (z,) for z in (x, y))
+    return len(x) == len(y) and all(torch.equal(u, w) for u, w in zip(x, y))
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_compiled_and_dispatched_calls_equal_plain_ones(which):
+    name, call, tensors = small_calls()[which]
+    want = call(*(x.clone() for x in tensors))
+    torch._dynamo.reset()
+    assert same(torch.compile(call, fullgraph=True, backend="aot_eager")(*(x.clone() for x in tensors)), want)
+    traced = torch.jit.trace(call, tuple(x.clone() for x in tensors), check_trace=False)
+    assert same(traced(*(x.clone() for x in tensors)), want)
+
+
+def test_negative_views_are_read_as_what_they_stand_for():
+    _, call, (st, q, k, v, g, beta) = small_calls()[3]
+    want = call(-st, -q, k, v, g, -beta)
+    assert same(call(torch._neg_view(st), torch._neg_view(q), k, v, g, torch._neg_view(beta)), want)
+    q, pos = rnd(197, 1, 3, 2, 16), torch.arange(3, dtype=I32, device=DEV)[None]
+    inv, factor = ops.rope_frequencies(16, 1e4)
+    assert same(ops.rotary_qk(torch._neg_view(q), q, pos, inv, factor, False), ops.rotary_qk(-q, q, pos, inv, factor, False))
+
+
+def test_the_caches_versions_move_with_an_append():
+    _, call, tensors = small_calls()[1]
+    before = [x._version for x in tensors]
+    call(*tensors)
+    moved = [x._version - y for x, y in zip(tensors, before)]
+    assert moved == [0, 0, 0, 0, 0, 1, 1, 0]
