@@ -818,9 +818,10 @@ _transforms, _tracing = torch._C._functorch.peek_interpreter_stack, torch._C._is
 _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-@functools.cache
+@functools.lru_cache(maxsize=4096)
 def _scratch_bytes(query: str, *sizes: int) -> int:
-    """What a scratch-size query of the library says; it depends on the sizes alone."""
+    """What a scratch-size query of the library says; it depends on the sizes alone. (Bounded: a server meets prompts of every
+    length.)"""
     return getattr(_lib.load(), query)(*sizes)
 
 

@@ -369,3 +369,11 @@ def test_wrapper_moves_the_version_counters_of_what_an_op_writes():
         inner = torch.zeros(3)
         append_one(q, kc, inner)  # (an inference tensor has no version)
     assert kc._version == 4 and inner[0] == 1
+
+
+def test_remembered_scratch_sizes_are_bounded():
+    assert ops._scratch_bytes.cache_info().maxsize is not None
+    for tokens in range(65, 65 + 2 * ops._scratch_bytes.cache_info().maxsize):
+        ops._scratch_bytes("dfb_delta_chunk_scratch_bytes", 1, tokens, 2, 4, 128, 128, 0)
+    assert ops._scratch_bytes.cache_info().currsize <= ops._scratch_bytes.cache_info().maxsize
+    assert ops._scratch_bytes("dfb_delta_chunk_scratch_bytes", 1, 64, 16, 32, 128, 128, 0) == _lib.load().dfb_delta_chunk_scratch_bytes(1, 64, 16, 32, 128, 128, 0)
