@@ -909,6 +909,11 @@ def _rows(op: str, name: str, t: Tensor) -> tuple[int, int, int]:
     return s[:3]
 
 
+def _steps(t: Tensor) -> tuple[int, int, int]:
+    """Strides of the three leading dimensions, 0 for one of size one: no address depends on it, and it may be anything."""
+    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape))
+
+
 def _check_cache(op: str, batch: int, heads: int, dim: int, dtype: torch.dtype, key_cache: Tensor, value_cache: Tensor, cache_len: Tensor) -> int:
     shape = key_cache.shape
     if len(shape) != 4 or shape != value_cache.shape:
@@ -1090,11 +1095,13 @@ def tree_attention(query: Tensor, key_cache: Tensor, value_cache: Tensor, cache_
     q_rows, k_rows, v_rows = _rows(op, "query", query), _rows(op, "key_cache", key_cache), _rows(op, "value_cache", value_cache)
     kp, vp = key_cache.data_ptr(), value_cache.data_ptr()
     if (k_rows[0] | k_rows[1] | k_rows[2] | v_rows[0] | v_rows[1] | v_rows[2]) % 8 or (kp | vp) % 16:
-        raise ValueError(f"{op}: cache rows must start on 16-byte boundaries")
+        k_rows, v_rows = _steps(key_cache), _steps(value_cache)
+        if (k_rows[0] | k_rows[1] | k_rows[2] | v_rows[0] | v_rows[1] | v_rows[2]) % 8 or (kp | vp) % 16:
+            raise ValueError(f"{op}: cache rows must start on 16-byte boundaries")
     _same_device(op, query, key_cache, value_cache, cache_len, parents)
     if (q_rows[0] | q_rows[1] | q_rows[2]) % 8 or query.data_ptr() % 16:
-        query = _fresh(query)
-        q_rows = query.stride()[:3]
+        query = _aligned_rows(query)
+        q_rows = _steps(query)
     out = _new_like(query)
     if batch == 0 or nodes == 0:
         return out
@@ -1117,8 +1124,8 @@ def _(query, key_cache, value_cache, cache_len, parents, scale):
 
 def _aligned_rows(t: Tensor, expanded: bool = True) -> Tensor:
     """`t`, copied if its rows do not start on 16-byte boundaries, or if it may not be `expanded` and is."""
-    s = t.stride()
-    return _fresh(t) if (s[0] | s[1] | s[2]) % 8 or t.data_ptr() % 16 or not (expanded or all(s)) else t
+    s = _steps(t)
+    return _fresh(t) if (s[0] | s[1] | s[2]) % 8 or t.data_ptr() % 16 or not (expanded or all(x for x, n in zip(s, t.shape) if n > 1)) else t
 
 
 def _delta_tokens(
@@ -1152,7 +1159,7 @@ def _delta_tokens(
     qp, kp, vp = query.data_ptr(), key.data_ptr(), value.data_ptr()
     if 0 in v_rows or (q_rows[0] | q_rows[1] | q_rows[2] | k_rows[0] | k_rows[1] | k_rows[2] | v_rows[0] | v_rows[1] | v_rows[2]) % 8 or (qp | kp | vp) % 16:
         query, key, value = _aligned_rows(query), _aligned_rows(key), _aligned_rows(value, expanded=False)
-        q_rows, k_rows, v_rows = query.stride()[:3], key.stride()[:3], value.stride()[:3]
+        q_rows, k_rows, v_rows = _steps(query), _steps(key), _steps(value)
         qp, kp, vp = query.data_ptr(), key.data_ptr(), value.data_ptr()
     if not state.is_contiguous():
         state = state.contiguous()

@@ -377,3 +377,20 @@ def test_remembered_scratch_sizes_are_bounded():
         ops._scratch_bytes("dfb_delta_chunk_scratch_bytes", 1, tokens, 2, 4, 128, 128, 0)
     assert ops._scratch_bytes.cache_info().currsize <= ops._scratch_bytes.cache_info().maxsize
     assert ops._scratch_bytes("dfb_delta_chunk_scratch_bytes", 1, 64, 16, 32, 128, 128, 0) == _lib.load().dfb_delta_chunk_scratch_bytes(1, 64, 16, 32, 128, 128, 0)
+
+
+def test_strides_of_dimensions_of_one_may_be_anything():
+    """A cache of one sequence, of one head or of one row, cut out of a buffer whose other strides are odd."""
+    for shape, stride in (((1, 2, 16, 64), (4097, 1024, 64, 1)), ((2, 1, 16, 64), (1024, 33, 64, 1)), ((2, 2, 1, 64), (128, 64, 65, 1))):
+        cache = torch.empty_strided(shape, stride, dtype=BF16).zero_()
+        n, hkv, _, _ = shape
+        a = tree_args(query=z(n, 5, 4, 64), key_cache=cache, value_cache=cache, cache_len=z(n, dtype=torch.int32), parents=z(n, 5, dtype=torch.int32))
+        with pytest.raises(RuntimeError, match="no PyTorch fallback"):  # past all that is checked before the device
+            ops.tree_attention(**a)
+    one = torch.empty_strided((1, 1, 4, 64), (3, 5, 64, 1), dtype=BF16)
+    assert ops._aligned_rows(one) is one and ops._aligned_rows(one, expanded=False) is one
+    assert ops._aligned_rows(z(1, 1, 4, 72)[..., 4:68]) is not one
+    wide = z(2, 1, 1, 64).expand(2, 3, 4, 64)
+    assert ops._aligned_rows(wide) is wide and ops._aligned_rows(wide, expanded=False).is_contiguous()
+    odd = torch.zeros(2, 3, 4, 68, dtype=BF16)[..., :64]
+    assert ops._aligned_rows(odd) is not odd

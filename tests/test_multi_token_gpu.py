@@ -815,3 +815,30 @@ def test_the_caches_versions_move_with_an_append():
     call(*tensors)
     moved = [x._version - y for x, y in zip(tensors, before)]
     assert moved == [0, 0, 0, 0, 0, 1, 1, 0]
+
+
+# ---------------------------------------------------------------- strides that no address depends on
+
+
+@pytest.mark.parametrize("b,hkv,rows,n,group", [(1, 2, 300, 7, 2), (3, 1, 300, 33, 4), (33, 1, 200, 20, 2), (2, 2, 1, 3, 2), (1, 40, 150, 30, 1)])
+def test_tree_attention_with_odd_strides_of_dimensions_of_one(b, hkv, rows, n, group):
+    d = 64
+    q = rnd(201, b, n, hkv * group, d, dtype=BF16)
+    kc, vc = rnd(202, b, hkv, rows, d, dtype=BF16), rnd(203, b, hkv, rows, d, dtype=BF16)
+    lt, pt = torch.full((b,), max(0, rows - n), dtype=I32, device=DEV), torch.tensor(random_tree(3, n), dtype=I32, device=DEV)
+
+    def odd(x):
+        y = x.as_strided(x.shape, tuple(s if m > 1 else 2 * s + 5 for s, m in zip(x.stride()[:3], x.shape)) + (1,))
+        assert torch.equal(x, y) and any(s % 8 for s in y.stride()[:3])
+        return y
+
+    want = ops.tree_attention(q, kc, vc, lt, pt, 0.125)
+    assert torch.equal(ops.tree_attention(q, odd(kc), odd(vc), lt, pt, 0.125), want)
+
+
+def test_delta_rule_with_odd_strides_of_dimensions_of_one():
+    st, q, k, v, g, beta = delta_inputs(205, 1, 70, 1, 1, 64, 64, True)
+    want = ops.delta_rule_chunk(st, q, k, v, g, beta, None, True)
+    cut = [x.as_strided(x.shape, (3, x.stride(1), 7, 1)) for x in (q, k, v)]
+    got = ops.delta_rule_chunk(st, *cut, g, beta, None, True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
