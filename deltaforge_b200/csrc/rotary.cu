@@ -159,10 +159,22 @@ int launch_rotary_t(RotaryParams p, cudaStream_t stream) {
   const int v = vec ? V : 1;
   p.turn_units = p.interleaved ? p.rotary_dim / (v == 1 ? 2 : v) : p.rotary_dim / 2 / v;
   p.pass_units = (p.d - p.rotary_dim) / v;
-  auto mul = [](int n) { return n > 0 ? ((1ull << 32) + n - 1) / n : 0ull; };  // x / n = x * mul >> 32 for x below 2^32 / n
-  p.turn_mul = mul(p.turn_units);
-  p.pass_mul = mul(p.pass_units);
-  p.value_mul = mul(p.d / v);
+  // x / n = x * mul >> 32 with mul = 2^32 / n rounded up by e / n, for all x with x e < 2^32: any x where n is a power of two, and
+  // below 2^32 / n always. Heads of many thousand dims can go beyond that, and a wrong quotient is another head's address.
+  bool exact = true;
+  auto mul = [&exact](int n, long heads) {
+    if (n <= 0) return 0ull;
+    const unsigned long long m = ((1ull << 32) + n - 1) / n, e = m * n - (1ull << 32), most = (unsigned long long)heads * n;
+    if (most > 0x7fffffff || (most - 1) * e >= 1ull << 32) exact = false;
+    return m;
+  };
+  p.turn_mul = mul(p.turn_units, (long)p.hq + p.hkv);
+  p.pass_mul = mul(p.pass_units, (long)p.hq + p.hkv);
+  p.value_mul = mul(p.d / v, p.hkv);
+  if (!exact) {
+    set_error("rotary positions: %d + %d heads of %d dims are too many for one call", p.hq, p.hkv, p.d);
+    return 2;
+  }
   const dim3 grid((unsigned)((long)p.batch * p.tokens)), block(ROT_THREADS);
   if (vec && p.interleaved) rotary_kernel<T, V, true><<<grid, block, 0, stream>>>(p);
   else if (vec) rotary_kernel<T, V, false><<<grid, block, 0, stream>>>(p);

@@ -394,3 +394,32 @@ def test_strides_of_dimensions_of_one_may_be_anything():
     assert ops._aligned_rows(wide) is wide and ops._aligned_rows(wide, expanded=False).is_contiguous()
     odd = torch.zeros(2, 3, 4, 68, dtype=BF16)[..., :64]
     assert ops._aligned_rows(odd) is not odd
+
+
+def rotary_desc(hq, hkv, d, rotary_dim, dtype=2):
+    r = _lib.RotaryDesc()
+    r.batch = r.tokens = 1
+    r.hq, r.hkv, r.d, r.rotary_dim, r.dtype = hq, hkv, d, rotary_dim, dtype
+    r.q = r.k = r.pos = r.inv_freq = r.q_out = r.k_out = 16  # never dereferenced: there is no device, or the check comes first
+    for s in (r.q_stride, r.k_stride):
+        s[0], s[1], s[2] = hq * d, hq * d, d
+    return r
+
+
+def wrong_quotients(n, heads):
+    """Whether some x below heads * n has x * ceil(2^32 / n) >> 32 != x / n: the kernel's division, tried at the ends of all heads"""
+    m = -(-(1 << 32) // n)
+    return any(x * m >> 32 != x // n for h in range(heads) for x in (h * n, h * n + n - 1))
+
+
+@pytest.mark.parametrize("hq,hkv,d,rotary_dim", [(16, 4, 256, 64), (60, 4, 12011, 8), (40, 40, 8192 + 512, 512), (1, 1, 70001, 2), (32, 32, 4096, 4096 // 8), (200, 8, 6000, 6)])
+def test_rotary_refuses_heads_whose_division_is_not_exact(hq, hkv, d, rotary_dim):
+    if torch.cuda.is_available():
+        pytest.skip("descriptors without memory behind them are for machines without a device")
+    lib = _lib.load()
+    vec = 4 if d % 4 == 0 and rotary_dim % 8 == 0 else 1  # fp32 vectors of 16 bytes
+    n = (d - rotary_dim) // vec
+    if not wrong_quotients(n, hq + hkv):
+        assert lib.dfb_rotary(rotary_desc(hq, hkv, d, rotary_dim), None) != 2
+        return
+    assert lib.dfb_rotary(rotary_desc(hq, hkv, d, rotary_dim), None) == 2 and b"too many" in lib.dfb_last_error()
