@@ -14,7 +14,7 @@
 // Trees are one chunk each and leave no state: 148 CTAs walk through all of them, the next state on its way while the products
 // of this one run (16 trees x 32 heads: 53 us with a CTA for each, 42 so).
 //
-// Bound by the chain from chunk to chunk, 4800 cycles (one 8192-token prompt of 32 heads: 128 chunks, 381 us, of which the
+// Bound by the chain from chunk to chunk, 4800 cycles (one 8192-token prompt of 32 heads: 128 chunks, 383 us, of which the
 // preparation of the first chunks and the four segments' starts take 60): 1000 until S lies in halves in TMEM, 1000 of tensor
 // time for W S, 1400 until V' does, 330 for half of the update, 200 for the new S, and three handovers between threads and
 // tensor core of 300 each. The conversions, some 450 instructions per thread and chunk, fill half of all issue slots.

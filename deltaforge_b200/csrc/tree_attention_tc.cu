@@ -21,9 +21,9 @@
 //
 // Bounds per tile of 128 keys at head dim 256: 1024 cycles of ex2, 128 KB of K and V from the L2, and of tensor time 16 products
 // Q K^T with both operands in shared memory (104 cycles each, measured, where the arithmetic takes 64) and 8 products P V with
-// P in TMEM and N = 256 (138): 2770 cycles, 161 of the 190 us that 8 sequences x 64 nodes x 32K rows take. (Q in TMEM would take
+// P in TMEM and N = 256 (138): 2770 cycles, 161 of the 188 us that 8 sequences x 64 nodes x 32K rows take. (Q in TMEM would take
 // 74 cycles, but O, two S and Q are 640 columns; with tiles of 64 keys it was slower.) Run back to back for seconds, that case
-// draws 1000 W, the clock falls from 1965 to 1380 MHz and the call takes 240 us.
+// draws 1000 W, the clock falls from 1965 to 1380 MHz and the call takes 215 to 240 us.
 //
 // Every wait is bounded; one that runs out makes the CTA leave NaN, wait (again with a limit) for its own copies and products, and
 // return.
@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
 }
 
 // D / 4 lanes per output row, as many rows per CTA as 256 threads hold: the parts of the row's unit in the order of the groups
-// that left them, with a running maximum; the loads of four parts are under way at once (8 x 64 nodes: 186 us, with eight 188).
+// that left them, with a running maximum; the loads of four parts are under way at once (8 x 64 nodes, measured side by side: 186 us, with eight 188).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tree_tc_merge_kernel(const TreeAttnParams p) {
   constexpr int LANES = D / 4, ROWS = 256 / LANES, AHEAD = 4;

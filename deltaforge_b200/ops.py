@@ -936,7 +936,9 @@ def rope_frequencies(
     ``stretch`` > 1 scales them for a context that many times ``trained_len``: ``"linear"`` divides every frequency by
     it; ``"base"`` raises ``theta`` so that the slowest frequency is divided by it and the fastest stays; ``"by_parts"``
     divides those that turn less than ``slow_turns`` times over ``trained_len``, keeps those that turn more than ``fast_turns``
-    times, goes linearly in between, and scales cos and sin by ``0.1 ln(stretch) + 1``.
+    times, goes linearly in between, and scales cos and sin by ``0.1 ln(stretch) + 1``. The ramp is linear in the number of turns.
+    Checkpoints whose configuration means a ramp that is linear in the index of the frequency, between two rounded indices, want
+    other frequencies (64 dims, theta 1e7, stretch 4: six of 32 differ, by up to 41 %): compute those and pass them.
     """
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and at least 2, got {rotary_dim}")
@@ -1021,7 +1023,7 @@ def rotary_append(
 ) -> Tensor:  # fmt: skip
     """``rotary_qk``, with the rotated keys and the values written into the caches ``(batch, kv_heads, max_seq, head_dim)``
     instead of returned: token ``t`` of sequence ``b`` becomes row ``cache_len[b] + t`` (int32, on the device). Rows below 0 or
-    from ``max_seq`` on are not written. Returns the rotated query."""
+    from ``max_seq`` on are not written. The inputs must not overlap the rows that are. Returns the rotated query."""
     op = "rotary_append"
     rd = _check_rotary(op, query, key, positions, inv_freq)
     dtype, (batch, tokens, hq, d) = query.dtype, query.shape
@@ -1196,7 +1198,8 @@ def delta_rule_chunk(
     over the key dim and scales q by ``key_dim ** -0.5``; without it they are used as they are. With ``lengths (batch,)``
     int32, only the first ``lengths[b]`` tokens of a sequence count: later rows give zeros and leave its state as it is
     (a padded batch of prompts, or the accepted tokens of a draft). Returns ``(output bf16, new_state)``. Inputs that
-    count are finite: a NaN or an infinity reaches the outputs of its chunk."""
+    count are finite: a NaN or an infinity reaches the outputs of its chunk, and so does, with ``qk_l2norm``, a query or key whose
+    sum of squares is beyond fp32."""
     return _delta_tokens("delta_rule_chunk", state, query, key, value, g, beta, lengths, None, qk_l2norm)
 
 

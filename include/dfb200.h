@@ -303,7 +303,8 @@ typedef struct dfb_rotary_desc {
 
 /* Rotary positions of several tokens, angles formed in 64 bits from integer positions; in the appending form rotated
  * keys and the values are written into the KV cache. The many-token counterpart of GatedAttention.forward's RoPE and
- * cache update (src/deltaforge/reference.py:638-650); rotary_dim even and at most 512. Outputs must not overlap inputs. */
+ * cache update (src/deltaforge/reference.py:638-650); rotary_dim even and at most 512; heads of many
+ * thousand dims are refused where (hq + hkv) of them are too many. Outputs must not overlap inputs. */
 int dfb_rotary(const dfb_rotary_desc* desc, void* stream);
 
 typedef struct dfb_tree_attn_desc {
