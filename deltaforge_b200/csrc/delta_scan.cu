@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
         // The next S is at most decay |S| + |U|, and U is a sum of 64 products of an image of V', as large as these really are, with one
         // of K, at most 2^13. (An update may be nothing at all, or its largest values forgotten within the chunk: a bound from
         // 2^13, or from a scale that stands for "nothing", pushes S down into fp16's subnormal numbers. Found out here, under the
-        // products, it costs nothing; a maximum of V' times its weight per token before them cost 20 to 30 of 382 us.)
+        // products, it costs nothing; a maximum of V' times its weight per token before them cost 15 to 40 of 382 us.)
         const float both = most(s_max);
         meet();
         es = scale_exp(fmaf(both, fabsf(decay), uup * most(r_max) * (64.f * 8192.f)));
